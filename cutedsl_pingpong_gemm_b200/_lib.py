@@ -25,9 +25,18 @@ CPG_ERR_NULL = -10
 CPG_DTYPE_BF16 = 0
 CPG_DTYPE_E4M3 = 1
 CPG_DTYPE_F32 = 2
+CPG_DTYPE_I8 = 3
 
 CPG_SCALE_TENSOR = 0
 CPG_SCALE_BLOCK = 1
+CPG_SCALE_ROWS_A = 2
+CPG_SCALE_ROWS_B = 4
+
+CPG_ROUTE_MAX_EXPERTS = 1024
+CPG_ROUTE_MAX_K = 32
+CPG_ROUTE_MAX_GROUPS = 32
+ROUTE_SCORINGS = {"softmax": 0, "sigmoid": 1}
+ROUTE_GROUP_SCORES = {"max": 0, "top2": 1}
 
 CPG_INJECT_SKIP_LOADS = 1
 CPG_SPLIT_K_STREAM = -1
@@ -42,7 +51,7 @@ CPG_ACT_GELU_TANH = 4
 ACTIVATIONS = {None: CPG_ACT_NONE, "none": CPG_ACT_NONE, "relu": CPG_ACT_RELU,
                "silu": CPG_ACT_SILU, "gelu": CPG_ACT_GELU, "gelu_tanh": CPG_ACT_GELU_TANH}
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 
 class CpgError(RuntimeError):
@@ -109,6 +118,13 @@ class EpilogueC(ctypes.Structure):
                 ("batch_stride_source", ctypes.c_int64)]
 
 
+class RouteConfigC(ctypes.Structure):
+    _fields_ = [("experts", ctypes.c_int32), ("k", ctypes.c_int32), ("scoring", ctypes.c_int32),
+                ("groups", ctypes.c_int32), ("kept_groups", ctypes.c_int32),
+                ("group_score", ctypes.c_int32), ("renormalize", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
 CPG_MAX_PEERS = 8
 
 
@@ -153,6 +169,17 @@ SIGNATURES = {
     "cpg_max_active_clusters": (ctypes.c_int, [_i32, _P(_i32)]),
     "cpg_quantize_e4m3": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _i32,
                                          _vp]),
+    "cpg_quantize_int8": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "cpg_route": (ctypes.c_int, [_P(RouteConfigC), _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "cpg_route_backward": (ctypes.c_int, [_P(RouteConfigC), _vp, _vp, _i32, _i64, _i64, _vp, _vp,
+                                          _i64, _vp]),
+    "cpg_expert_order": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "cpg_dispatch_rows": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i64,
+                                         _i64, _vp, _vp]),
+    "cpg_combine_rows": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp,
+                                        _i64, _vp, _i64, _vp]),
+    "cpg_combine_rows_backward": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64,
+                                                 _vp, _vp, _i32, _vp, _i64, _vp, _vp]),
     "cpg_cast_f32_bf16": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "cpg_gemm_splitk_static": (ctypes.c_int, [_P(GemmConfigC), _P(GemmProblemC), _vp, _vp, _vp,
                                               _P(EpilogueC), _vp]),

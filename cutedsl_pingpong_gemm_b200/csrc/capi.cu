@@ -5,13 +5,11 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <cstdarg>
-#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
-#include <string>
 
+#include "capi_common.h"
 #include "cpgemm.h"
 #include "gemm_decode.cuh"
 #include "gemm_fp8_block.cuh"
@@ -19,24 +17,11 @@
 #include "peer_kernels.cuh"
 #include "quant_kernels.cuh"
 
+using cpg_capi::cuda_fail;
+using cpg_capi::fail;
+using cpg_capi::g_last_error;
+
 namespace {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-int cuda_fail(cudaError_t e, const char* what) {
-  return fail(CPG_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-}
 
 // Restores the caller's current device on scope exit.
 struct DeviceGuard {
@@ -131,6 +116,8 @@ template <>
 constexpr int dtype_code<cpg::e4m3_t>() { return CPG_DTYPE_E4M3; }
 template <>
 constexpr int dtype_code<float>() { return CPG_DTYPE_F32; }
+template <>
+constexpr int dtype_code<int8_t>() { return CPG_DTYPE_I8; }
 
 template <int BN, int CG, typename AB, typename OutT>
 Variant make_variant() {
@@ -169,7 +156,7 @@ void add_variants(Variant* t, int& n) {
 
 bool find_variant(int bn, int cta_group, int dtype_ab, int dtype_d, int scale_mode,
                   Variant* out) {
-  static Variant table[36];
+  static Variant table[52];
   static int count = 0;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -177,6 +164,8 @@ bool find_variant(int bn, int cta_group, int dtype_ab, int dtype_d, int scale_mo
     add_variants<__nv_bfloat16, float>(table, count);
     add_variants<cpg::e4m3_t, __nv_bfloat16>(table, count);
     add_variants<cpg::e4m3_t, float>(table, count);
+    add_variants<int8_t, __nv_bfloat16>(table, count);
+    add_variants<int8_t, float>(table, count);
     table[count++] = make_block_variant<128, 1>();
     table[count++] = make_block_variant<128, 2>();
     table[count++] = make_block_variant<256, 1>();
@@ -194,7 +183,18 @@ bool find_variant(int bn, int cta_group, int dtype_ab, int dtype_d, int scale_mo
   return false;
 }
 
-int elem_bytes(int dtype) { return dtype == CPG_DTYPE_E4M3 ? 1 : (dtype == CPG_DTYPE_F32 ? 4 : 2); }
+int elem_bytes(int dtype) {
+  return dtype == CPG_DTYPE_E4M3 || dtype == CPG_DTYPE_I8 ? 1 : (dtype == CPG_DTYPE_F32 ? 4 : 2);
+}
+
+bool operand_dtype(int dtype) {
+  return dtype == CPG_DTYPE_BF16 || dtype == CPG_DTYPE_E4M3 || dtype == CPG_DTYPE_I8;
+}
+
+// Scale modes of INT8 operands: a scale per row of A and / or per row of B, or (TENSOR) one value.
+bool int8_scale_mode(int mode) {
+  return (mode & ~(CPG_SCALE_ROWS_A | CPG_SCALE_ROWS_B)) == 0;
+}
 
 // Raster group size of a plan whose K ranges hold k_iters k-blocks.  The dynamic schedule starts
 // clusters in id order, so the clusters running at any time hold about consecutive ids: a
@@ -217,7 +217,8 @@ int32_t plan_group_size(const cpg_gemm_config* cfg, int64_t k_iters) {
 
 CUtensorMapDataType tma_dtype(int dtype) {
   switch (dtype) {
-    case CPG_DTYPE_E4M3: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    case CPG_DTYPE_E4M3:
+    case CPG_DTYPE_I8: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
     case CPG_DTYPE_F32: return CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     default: return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   }
@@ -380,7 +381,7 @@ struct cpg_gemm {
 
 extern "C" {
 
-int cpg_abi_version(void) { return 14; }
+int cpg_abi_version(void) { return 15; }
 
 const char* cpg_strerror(int code) {
   switch (code) {
@@ -472,7 +473,10 @@ using DecodeFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMa
 static const void* decode_kernel(int dtype_ab, int dtype_d, int cta_group) {
   const bool fp8 = dtype_ab == CPG_DTYPE_E4M3, f32 = dtype_d == CPG_DTYPE_F32;
   DecodeFn fn;
-  if (cta_group == 2) {
+  if (dtype_ab == CPG_DTYPE_I8) {
+    fn = f32 ? &cpg::gemm_decode_kernel<int8_t, float, 1>
+             : &cpg::gemm_decode_kernel<int8_t, __nv_bfloat16, 1>;
+  } else if (cta_group == 2) {
     fn = fp8 ? (f32 ? &cpg::gemm_decode_kernel<cpg::e4m3_t, float, 2>
                     : &cpg::gemm_decode_kernel<cpg::e4m3_t, __nv_bfloat16, 2>)
              : (f32 ? &cpg::gemm_decode_kernel<__nv_bfloat16, float, 2>
@@ -498,7 +502,9 @@ static int create_decode_plan(const cpg_gemm_config* cfg, const cpg_gemm_problem
   if (prob->m < 1 || prob->m > cpg::kDecodeMaxM)
     return fail(CPG_ERR_INVALID_SHAPE, "the small-M kernel takes 1 <= M <= %d, got %lld",
                 cpg::kDecodeMaxM, static_cast<long long>(prob->m));
-  if (prob->scale_mode != CPG_SCALE_TENSOR || prob->gated || prob->grouped || prob->l > 1)
+  const bool int8 = prob->dtype_ab == CPG_DTYPE_I8;
+  if ((int8 ? !int8_scale_mode(prob->scale_mode) : prob->scale_mode != CPG_SCALE_TENSOR) ||
+      prob->gated || prob->grouped || prob->l > 1)
     return fail(CPG_ERR_UNSUPPORTED,
                 "the small-M kernel has no block scales, gating, batches or groups");
   const int64_t bk = cpg::kRowBytes / elem_bytes(prob->dtype_ab);
@@ -511,7 +517,7 @@ static int create_decode_plan(const cpg_gemm_config* cfg, const cpg_gemm_problem
   const char* env_pair = std::getenv("CPG_DECODE_PAIR");
   const char* env_s = std::getenv("CPG_DECODE_SPLITS");
   const char* env_st = std::getenv("CPG_DECODE_STAGES");
-  const int cg = (env_pair != nullptr && std::atoi(env_pair) == 1) ? 2 : 1;
+  const int cg = (env_pair != nullptr && std::atoi(env_pair) == 1 && !int8) ? 2 : 1;
   const int64_t tile_rows = int64_t(cg) * cpg::kDecodeTileN;
   const int64_t tiles = (prob->n + tile_rows - 1) / tile_rows;
   if (tiles > 65535)
@@ -668,8 +674,10 @@ static int run_decode(cpg_gemm* g, const void* a, const void* b, void* d, const 
   p.st_async = g->dec_st_async;
   p.stages = g->dec_stages;
   p.alpha = epi != nullptr ? epi->alpha : 1.0f;
-  p.scale_a = epi != nullptr ? epi->scale_a : nullptr;
-  p.scale_b = epi != nullptr ? epi->scale_b : nullptr;
+  const float* sa = epi != nullptr ? epi->scale_a : nullptr;
+  const float* sb = epi != nullptr ? epi->scale_b : nullptr;
+  ((pr.scale_mode & CPG_SCALE_ROWS_A) ? p.row_scale : p.scale_a) = sa;
+  ((pr.scale_mode & CPG_SCALE_ROWS_B) ? p.col_scale : p.scale_b) = sb;
   p.bias = epi != nullptr ? static_cast<const __nv_bfloat16*>(epi->bias) : nullptr;
   p.d = d;
   p.ldd = pr.ldd;
@@ -732,10 +740,15 @@ int cpg_gemm_create(const cpg_gemm_config* cfg, const cpg_gemm_problem* prob, in
     return fail(CPG_ERR_INVALID_CONFIG, "gemm_n_prologue must be below ab_stage");
 
   // Problem checks.
-  if (prob->dtype_ab != CPG_DTYPE_BF16 && prob->dtype_ab != CPG_DTYPE_E4M3)
-    return fail(CPG_ERR_DTYPE, "A and B must be BF16 or FP8 E4M3");
+  if (!operand_dtype(prob->dtype_ab))
+    return fail(CPG_ERR_DTYPE, "A and B must be BF16, FP8 E4M3 or INT8");
   if (prob->dtype_d != CPG_DTYPE_BF16 && prob->dtype_d != CPG_DTYPE_F32)
     return fail(CPG_ERR_DTYPE, "D must be BF16 or FP32");
+  const bool int8 = prob->dtype_ab == CPG_DTYPE_I8;
+  if (int8 && prob->k > cpg::kInt8MaxK)
+    return fail(CPG_ERR_INVALID_SHAPE,
+                "INT8 operands: K must be at most %lld (32-bit integer sums), got %lld",
+                static_cast<long long>(cpg::kInt8MaxK), static_cast<long long>(prob->k));
   const int64_t lim = (int64_t(1) << 31) - 1;
   if (prob->m < 0 || prob->n < 0 || prob->k < 0 || prob->m > lim || prob->n > lim || prob->k > lim)
     return fail(CPG_ERR_INVALID_SHAPE, "M, N, K must be in [0, 2^31)");
@@ -759,8 +772,11 @@ int cpg_gemm_create(const cpg_gemm_config* cfg, const cpg_gemm_problem* prob, in
 
   Variant v;
   const int cta_group = cfg->cluster_m == 2 ? 2 : 1;
-  if (prob->scale_mode != CPG_SCALE_TENSOR && prob->scale_mode != CPG_SCALE_BLOCK)
-    return fail(CPG_ERR_INVALID_CONFIG, "scale_mode must be 0 (none / per tensor) or 1 (block)");
+  if (int8 ? !int8_scale_mode(prob->scale_mode)
+           : prob->scale_mode != CPG_SCALE_TENSOR && prob->scale_mode != CPG_SCALE_BLOCK)
+    return fail(CPG_ERR_INVALID_CONFIG,
+                "scale_mode must be 0 (none / per tensor), 1 (block, E4M3) or of "
+                "CPG_SCALE_ROWS_A | CPG_SCALE_ROWS_B (INT8)");
   if (prob->scale_mode == CPG_SCALE_BLOCK &&
       (prob->dtype_ab != CPG_DTYPE_E4M3 || prob->dtype_d != CPG_DTYPE_BF16 ||
        (cfg->tile_n != 128 && cfg->tile_n != 256)))
@@ -1218,8 +1234,11 @@ static int run_impl(cpg_gemm* g, const void* a, const void* b, void* d, const cp
     bs.sa = epi->scale_a;
     bs.sb = epi->scale_b;
   } else {
-    p.scale_a = epi != nullptr ? epi->scale_a : nullptr;
-    p.scale_b = epi != nullptr ? epi->scale_b : nullptr;
+    const float* sa = epi != nullptr ? epi->scale_a : nullptr;
+    const float* sb = epi != nullptr ? epi->scale_b : nullptr;
+    ((pr.scale_mode & CPG_SCALE_ROWS_A) ? p.row_scale : p.scale_a) = sa;
+    ((pr.scale_mode & CPG_SCALE_ROWS_B) ? p.col_scale : p.scale_b) = sb;
+    p.col_scale_len = static_cast<int32_t>(pr.gated ? 2 * pr.n : pr.n);
   }
   p.bias = static_cast<const __nv_bfloat16*>(bias);
   p.tile_trace = g->trace;
@@ -1350,8 +1369,8 @@ int cpg_sched_plan_group_size(const cpg_gemm_config* cfg, int64_t k, int32_t dty
   if (cfg == nullptr || out == nullptr) return fail(CPG_ERR_NULL, "NULL argument");
   const int rc = cpg_config_validate(cfg);
   if (rc != CPG_OK) return rc;
-  if (dtype_ab != CPG_DTYPE_BF16 && dtype_ab != CPG_DTYPE_E4M3)
-    return fail(CPG_ERR_DTYPE, "dtype_ab must be BF16 or E4M3, got %d", dtype_ab);
+  if (!operand_dtype(dtype_ab))
+    return fail(CPG_ERR_DTYPE, "dtype_ab must be BF16, E4M3 or I8, got %d", dtype_ab);
   if (k < 0) return fail(CPG_ERR_INVALID_SHAPE, "k must be >= 0, got %lld", (long long)k);
   const int64_t bk = cpg::kRowBytes / elem_bytes(dtype_ab);
   *out = plan_group_size(cfg, (k + bk - 1) / bk);
@@ -1555,10 +1574,11 @@ static int check_reduce_scatter(const cpg_gemm* g, const cpg_reduce_scatter* rs)
   if (g == nullptr || rs == nullptr) return fail(CPG_ERR_NULL, "plan and rs must be non-NULL");
   const cpg_gemm_problem& pr = g->prob;
   if (pr.dtype_d != CPG_DTYPE_F32 || g->stream_k || g->groups > 0 || g->batches > 1 ||
-      pr.gated || g->v.scale_mode != CPG_SCALE_TENSOR || g->decode)
+      pr.gated || g->v.scale_mode != CPG_SCALE_TENSOR || g->decode ||
+      pr.dtype_ab == CPG_DTYPE_I8)
     return fail(CPG_ERR_UNSUPPORTED,
-                "the peer reduce-scatter needs an FP32-output plan without Stream-K, batches, "
-                "groups, gating or block scales");
+                "the peer reduce-scatter needs an FP32-output plan of BF16 or E4M3 operands "
+                "without Stream-K, batches, groups, gating or block scales");
   if (rs->ranks < 1 || rs->ranks > CPG_MAX_PEERS || rs->rank < 0 || rs->rank >= rs->ranks)
     return fail(CPG_ERR_INVALID_CONFIG, "rank %d of %d ranks (at most %d)", rs->rank, rs->ranks,
                 CPG_MAX_PEERS);

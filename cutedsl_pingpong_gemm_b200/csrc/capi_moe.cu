@@ -1,0 +1,313 @@
+// C ABI of the INT8 row quantiser and of the operators around the experts' products: routing,
+// expert order, dispatch and combine, and their gradients (include/cpgemm.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "capi_common.h"
+#include "cpgemm.h"
+#include "expert_route.cuh"
+#include "expert_rows.cuh"
+
+using cpg_capi::cuda_fail;
+using cpg_capi::fail;
+
+namespace {
+
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;  // rows and pairs are counted in int32
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CPG_OK : cuda_fail(e, what);
+}
+
+bool float_dtype(int32_t dtype) { return dtype == CPG_DTYPE_BF16 || dtype == CPG_DTYPE_F32; }
+int bytes_of(int32_t dtype) { return dtype == CPG_DTYPE_F32 ? 4 : (dtype == CPG_DTYPE_I8 ? 1 : 2); }
+
+bool misaligned(const void* p, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) != 0;
+}
+
+unsigned row_grid(int64_t rows) { return static_cast<unsigned>(std::min<int64_t>(rows, kMaxRows)); }
+
+// rows x cols of a row-major matrix with row stride ld: sizes and stride make sense.
+int check_matrix(const char* name, int64_t rows, int64_t cols, int64_t ld) {
+  if (rows < 0 || rows > kMaxRows || cols < 0 || cols > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: %lld x %lld is not within [0, 2^31)", name,
+                static_cast<long long>(rows), static_cast<long long>(cols));
+  if (ld < cols)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: row stride %lld below the row length %lld", name,
+                static_cast<long long>(ld), static_cast<long long>(cols));
+  return CPG_OK;
+}
+
+int check_pairs(int64_t tokens, int32_t k) {
+  if (tokens < 0 || tokens > kMaxRows || k < 1 || k > CPG_ROUTE_MAX_K || tokens * k > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE,
+                "%lld tokens x %d choices: 1 <= k <= %d and at most 2^31 - 1 pairs",
+                static_cast<long long>(tokens), k, CPG_ROUTE_MAX_K);
+  return CPG_OK;
+}
+
+int launch_rows(const cpg::RowsParams& p, int32_t dtype_x, bool int8, cudaStream_t st) {
+  const unsigned grid = row_grid(p.tokens);
+  if (dtype_x == CPG_DTYPE_BF16) {
+    if (int8)
+      cpg::rows_kernel<__nv_bfloat16, int8_t><<<grid, 256, 0, st>>>(p);
+    else
+      cpg::rows_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (int8)
+      cpg::rows_kernel<float, int8_t><<<grid, 256, 0, st>>>(p);
+    else
+      cpg::rows_kernel<float, float><<<grid, 256, 0, st>>>(p);
+  }
+  return launched("row kernel launch");
+}
+
+int check_route(const cpg_route_config* c, int64_t tokens) {
+  if (c == nullptr) return fail(CPG_ERR_NULL, "route config is NULL");
+  if (c->experts < 1 || c->experts > CPG_ROUTE_MAX_EXPERTS)
+    return fail(CPG_ERR_INVALID_SHAPE, "1 <= experts <= %d, got %d", CPG_ROUTE_MAX_EXPERTS,
+                c->experts);
+  if (c->k > c->experts)
+    return fail(CPG_ERR_INVALID_SHAPE, "k = %d choices of %d experts", c->k, c->experts);
+  if (c->scoring != CPG_ROUTE_SOFTMAX && c->scoring != CPG_ROUTE_SIGMOID)
+    return fail(CPG_ERR_INVALID_CONFIG, "scoring %d is not one of CPG_ROUTE_*", c->scoring);
+  if (c->groups < 1 || c->groups > CPG_ROUTE_MAX_GROUPS || c->experts % c->groups != 0)
+    return fail(CPG_ERR_INVALID_CONFIG, "%d groups must divide %d experts and be at most %d",
+                c->groups, c->experts, CPG_ROUTE_MAX_GROUPS);
+  if (c->kept_groups < 1 || c->kept_groups > c->groups ||
+      c->k > c->kept_groups * (c->experts / c->groups))
+    return fail(CPG_ERR_INVALID_CONFIG, "%d of %d groups cannot hold %d choices", c->kept_groups,
+                c->groups, c->k);
+  if (c->group_score != CPG_GROUP_MAX && c->group_score != CPG_GROUP_TOP2)
+    return fail(CPG_ERR_INVALID_CONFIG, "group_score %d is not one of CPG_GROUP_*",
+                c->group_score);
+  return check_pairs(tokens, c->k);
+}
+
+// Calls f(std::integral_constant<int, V>) with the smallest V whose 32 lanes hold `experts`.
+template <typename F>
+void by_lane_values(int32_t experts, F&& f) {
+  if (experts <= 32) f(std::integral_constant<int, 1>{});
+  else if (experts <= 64) f(std::integral_constant<int, 2>{});
+  else if (experts <= 128) f(std::integral_constant<int, 4>{});
+  else if (experts <= 256) f(std::integral_constant<int, 8>{});
+  else if (experts <= 512) f(std::integral_constant<int, 16>{});
+  else f(std::integral_constant<int, 32>{});
+}
+
+unsigned route_grid(int64_t tokens) {
+  return static_cast<unsigned>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps);
+}
+
+static_assert(CPG_ROUTE_MAX_EXPERTS == cpg::kRouteMaxExperts &&
+                  CPG_ROUTE_MAX_K == cpg::kRouteMaxK &&
+                  CPG_ROUTE_MAX_GROUPS == cpg::kRouteMaxGroups,
+              "routing limits");
+static_assert(CPG_ROUTE_SOFTMAX == cpg::kRouteSoftmax && CPG_ROUTE_SIGMOID == cpg::kRouteSigmoid &&
+                  CPG_GROUP_MAX == cpg::kRouteGroupMax && CPG_GROUP_TOP2 == cpg::kRouteGroupTop2,
+              "routing codes");
+
+}  // namespace
+
+extern "C" {
+
+int cpg_quantize_int8(const void* x, int32_t dtype_x, int64_t rows, int64_t cols, int64_t ldx,
+                      void* q, int64_t ldq, float* scales, void* stream) {
+  if (!float_dtype(dtype_x)) return fail(CPG_ERR_DTYPE, "x must be BF16 or FP32");
+  int rc = check_matrix("x", rows, cols, ldx);
+  if (rc == CPG_OK) rc = check_matrix("q", rows, cols, ldq);
+  if (rc != CPG_OK) return rc;
+  if (rows == 0) return CPG_OK;
+  if (scales == nullptr || (cols > 0 && (x == nullptr || q == nullptr)))
+    return fail(CPG_ERR_NULL, "x, q and scales must be non-NULL");
+  if (misaligned(x, bytes_of(dtype_x)) || misaligned(scales, 4))
+    return fail(CPG_ERR_ALIGNMENT, "x and scales must be aligned to their elements");
+  const cpg::RowsParams p{x, rows, cols, ldx, nullptr, 1, q, rows, ldq, scales};
+  return launch_rows(p, dtype_x, true, static_cast<cudaStream_t>(stream));
+}
+
+int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int64_t tokens,
+              int64_t ld, const float* bias, int32_t* ids, float* weights, void* stream) {
+  int rc = check_route(c, tokens);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype)) return fail(CPG_ERR_DTYPE, "logits must be BF16 or FP32");
+  rc = check_matrix("logits", tokens, c->experts, ld);
+  if (rc != CPG_OK) return rc;
+  if (tokens == 0) return CPG_OK;
+  if (logits == nullptr || ids == nullptr || weights == nullptr)
+    return fail(CPG_ERR_NULL, "logits, ids and weights must be non-NULL");
+  if (misaligned(logits, bytes_of(dtype)) || misaligned(bias, 4) || misaligned(ids, 4) ||
+      misaligned(weights, 4))
+    return fail(CPG_ERR_ALIGNMENT, "logits, bias, ids and weights must be aligned to their elements");
+  const cpg::RouteParams p{logits,    tokens,  ld,        bias,           ids,
+                           weights,   c->experts, c->k,   c->scoring,     c->groups,
+                           c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, c->scale};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  by_lane_values(c->experts, [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    const size_t smem = c->groups > 1 ? sizeof(double) * 32 * V * cpg::kRouteWarps : 0;
+    if (dtype == CPG_DTYPE_BF16)
+      cpg::route_kernel<__nv_bfloat16, V>
+          <<<route_grid(tokens), 32 * cpg::kRouteWarps, smem, st>>>(p);
+    else
+      cpg::route_kernel<float, V><<<route_grid(tokens), 32 * cpg::kRouteWarps, smem, st>>>(p);
+  });
+  return launched("route kernel launch");
+}
+
+int cpg_route_backward(const cpg_route_config* c, const float* dweights, const void* logits,
+                       int32_t dtype, int64_t tokens, int64_t ld, const int32_t* ids,
+                       void* dlogits, int64_t ldd, void* stream) {
+  int rc = check_route(c, tokens);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype)) return fail(CPG_ERR_DTYPE, "logits must be BF16 or FP32");
+  rc = check_matrix("logits", tokens, c->experts, ld);
+  if (rc == CPG_OK) rc = check_matrix("dlogits", tokens, c->experts, ldd);
+  if (rc != CPG_OK) return rc;
+  if (tokens == 0) return CPG_OK;
+  if (dweights == nullptr || logits == nullptr || ids == nullptr || dlogits == nullptr)
+    return fail(CPG_ERR_NULL, "dweights, logits, ids and dlogits must be non-NULL");
+  if (misaligned(logits, bytes_of(dtype)) || misaligned(dlogits, bytes_of(dtype)) ||
+      misaligned(dweights, 4) || misaligned(ids, 4))
+    return fail(CPG_ERR_ALIGNMENT,
+                "dweights, logits, ids and dlogits must be aligned to their elements");
+  const cpg::RouteGradParams p{dweights, logits,     tokens, ld,         ids,
+                               dlogits,  ldd,        c->experts, c->k,   c->scoring,
+                               c->renormalize != 0 ? 1 : 0, c->scale};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  by_lane_values(c->experts, [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    if (dtype == CPG_DTYPE_BF16)
+      cpg::route_grad_kernel<__nv_bfloat16, V>
+          <<<route_grid(tokens), 32 * cpg::kRouteWarps, 0, st>>>(p);
+    else
+      cpg::route_grad_kernel<float, V><<<route_grid(tokens), 32 * cpg::kRouteWarps, 0, st>>>(p);
+  });
+  return launched("route gradient kernel launch");
+}
+
+int cpg_expert_order(const int32_t* ids, int64_t tokens, int32_t k, int32_t experts,
+                     int32_t* offsets, int32_t* slots, void* stream) {
+  int rc = check_pairs(tokens, k);
+  if (rc != CPG_OK) return rc;
+  if (experts < 1 || experts > CPG_ROUTE_MAX_EXPERTS)
+    return fail(CPG_ERR_INVALID_SHAPE, "1 <= experts <= %d, got %d", CPG_ROUTE_MAX_EXPERTS,
+                experts);
+  const int64_t pairs = tokens * k;
+  if (offsets == nullptr || (pairs > 0 && (ids == nullptr || slots == nullptr)))
+    return fail(CPG_ERR_NULL, "ids, offsets and slots must be non-NULL");
+  if (misaligned(ids, 4) || misaligned(offsets, 4) || misaligned(slots, 4))
+    return fail(CPG_ERR_ALIGNMENT, "ids, offsets and slots must be 4-byte aligned");
+  // One block while its 32 warps have at most 64 pairs each, then up to 8 blocks of one cluster.
+  int blocks = 1;
+  while (blocks < cpg::kOrderMaxCluster && pairs > int64_t(blocks) * cpg::kOrderWarps * 64)
+    blocks *= 2;
+  const int smem = static_cast<int>(sizeof(uint32_t)) * (cpg::kOrderWarps + 1) * experts;
+  const void* fn = reinterpret_cast<const void*>(&cpg::expert_order_kernel);
+  // Always the limit of the largest call: a smaller later call must not lower it.
+  cudaError_t e = cudaFuncSetAttribute(
+      fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      static_cast<int>(sizeof(uint32_t)) * (cpg::kOrderWarps + 1) * CPG_ROUTE_MAX_EXPERTS);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(expert order)");
+  cpg::OrderParams p{ids, pairs, experts, offsets, slots};
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  lc.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  lc.blockDim = dim3(cpg::kOrderThreads, 1, 1);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem);
+  lc.stream = static_cast<cudaStream_t>(stream);
+  lc.attrs = attr;
+  lc.numAttrs = blocks > 1 ? 1 : 0;
+  void* args[] = {&p};
+  e = cudaLaunchKernelExC(&lc, fn, args);
+  return e == cudaSuccess ? CPG_OK : cuda_fail(e, "expert order launch");
+}
+
+int cpg_dispatch_rows(const void* x, int32_t dtype_x, int64_t tokens, int64_t cols, int64_t ldx,
+                      const int32_t* slots, int32_t k, void* rows, int32_t dtype_rows,
+                      int64_t num_rows, int64_t ldr, float* scales, void* stream) {
+  int rc = check_pairs(tokens, k);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype_x) || (dtype_rows != dtype_x && dtype_rows != CPG_DTYPE_I8))
+    return fail(CPG_ERR_DTYPE, "x must be BF16 or FP32 and rows of the same type or INT8");
+  rc = check_matrix("x", tokens, cols, ldx);
+  if (rc == CPG_OK) rc = check_matrix("rows", num_rows, cols, ldr);
+  if (rc != CPG_OK) return rc;
+  const bool int8 = dtype_rows == CPG_DTYPE_I8;
+  if (tokens == 0 || num_rows == 0 || (cols == 0 && !int8)) return CPG_OK;
+  if (slots == nullptr || (int8 && scales == nullptr) ||
+      (cols > 0 && (x == nullptr || rows == nullptr)))
+    return fail(CPG_ERR_NULL, "x, slots, rows (and scales with INT8) must be non-NULL");
+  if (misaligned(x, bytes_of(dtype_x)) || misaligned(rows, bytes_of(dtype_rows)) ||
+      misaligned(slots, 4) || misaligned(scales, 4))
+    return fail(CPG_ERR_ALIGNMENT, "x, rows, slots and scales must be aligned to their elements");
+  const cpg::RowsParams p{x, tokens, cols, ldx, slots, k, rows, num_rows, ldr, scales};
+  return launch_rows(p, dtype_x, int8, static_cast<cudaStream_t>(stream));
+}
+
+int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
+                     const int32_t* slots, const float* weights, int64_t tokens, int32_t k,
+                     const void* source, int64_t ld_source, void* y, int64_t ldy, void* stream) {
+  int rc = check_pairs(tokens, k);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype)) return fail(CPG_ERR_DTYPE, "rows must be BF16 or FP32");
+  rc = check_matrix("rows", num_rows, cols, ldr);
+  if (rc == CPG_OK) rc = check_matrix("y", tokens, cols, ldy);
+  if (rc == CPG_OK && source != nullptr) rc = check_matrix("source", tokens, cols, ld_source);
+  if (rc != CPG_OK) return rc;
+  if (tokens == 0 || cols == 0) return CPG_OK;
+  if ((num_rows > 0 && rows == nullptr) || slots == nullptr || y == nullptr)
+    return fail(CPG_ERR_NULL, "rows, slots and y must be non-NULL");
+  const int es = bytes_of(dtype);
+  if (misaligned(rows, es) || misaligned(source, es) || misaligned(y, es) ||
+      misaligned(slots, 4) || misaligned(weights, 4))
+    return fail(CPG_ERR_ALIGNMENT, "rows, slots, weights, source and y must be aligned to their elements");
+  const cpg::CombineParams p{rows,   num_rows, cols,   ldr,       slots, weights,
+                             tokens, k,        source, ld_source, y,     ldy};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == CPG_DTYPE_BF16)
+    cpg::combine_kernel<__nv_bfloat16><<<row_grid(tokens), 256, 0, st>>>(p);
+  else
+    cpg::combine_kernel<float><<<row_grid(tokens), 256, 0, st>>>(p);
+  return launched("combine kernel launch");
+}
+
+int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int64_t cols,
+                              int64_t lddy, const void* rows, int64_t num_rows, int64_t ldr,
+                              const int32_t* slots, const float* weights, int32_t k, void* drows,
+                              int64_t lddr, float* dweights, void* stream) {
+  int rc = check_pairs(tokens, k);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype)) return fail(CPG_ERR_DTYPE, "dy and rows must be BF16 or FP32");
+  rc = check_matrix("dy", tokens, cols, lddy);
+  if (rc == CPG_OK) rc = check_matrix("rows", num_rows, cols, ldr);
+  if (rc == CPG_OK) rc = check_matrix("drows", num_rows, cols, lddr);
+  if (rc != CPG_OK) return rc;
+  if (tokens == 0) return CPG_OK;
+  if (slots == nullptr || weights == nullptr || dweights == nullptr ||
+      (cols > 0 && dy == nullptr) ||
+      (cols > 0 && num_rows > 0 && (rows == nullptr || drows == nullptr)))
+    return fail(CPG_ERR_NULL, "dy, rows, slots, weights, drows and dweights must be non-NULL");
+  const int es = bytes_of(dtype);
+  if (misaligned(dy, es) || misaligned(rows, es) || misaligned(drows, es) ||
+      misaligned(slots, 4) || misaligned(weights, 4) || misaligned(dweights, 4))
+    return fail(CPG_ERR_ALIGNMENT, "every argument must be aligned to its elements");
+  const cpg::CombineGradParams p{dy,    tokens,  cols, lddy,  rows, num_rows, ldr,
+                                 slots, weights, k,    drows, lddr, dweights};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = row_grid((tokens * k + 7) / 8);
+  if (dtype == CPG_DTYPE_BF16)
+    cpg::combine_grad_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  else
+    cpg::combine_grad_kernel<float><<<grid, 256, 0, st>>>(p);
+  return launched("combine gradient kernel launch");
+}
+
+}  // extern "C"

@@ -1,6 +1,7 @@
 // Small-M ("decode") GEMM for sm_100a: D[M, N] = alpha * s_a * s_b * A[M, K] . B[N, K]^T + bias
 // for M <= 128, the decode-like shapes where B (the weight, N x K) is read from HBM once and A
-// holds a few token rows.
+// holds a few token rows.  INT8 operands take a scale per row of A and per row of B; their partial
+// sums are exchanged and added as 32-bit integers, exactly.
 //
 // The tile is transposed with respect to the plain kernel: the MMA computes D^T, B's rows on its
 // M side (one TMEM lane each) and the M token rows of A on its N side (rounded up to 16; rows
@@ -67,6 +68,8 @@ struct DecodeParams {
   float alpha;
   const float* scale_a;  // optional per-tensor FP8 scales (device scalars)
   const float* scale_b;
+  const float* row_scale;  // INT8: optional scale per row of A (length M) ...
+  const float* col_scale;  // ... and per row of B (length N), instead of the scalars
   const __nv_bfloat16* bias;  // optional, length N
   void* d;
   int64_t ldd;
@@ -128,6 +131,26 @@ __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ float to_out<float>(float x) {
   return x;
+}
+
+// The type partial sums are added in, and an accumulator word as that type.
+template <bool Int8>
+struct DecodeAcc {
+  using T = float;
+};
+template <>
+struct DecodeAcc<true> {
+  using T = uint32_t;  // wraps like the signed sum, without signed overflow
+};
+template <typename Acc>
+__device__ __forceinline__ Acc acc_word(uint32_t w);
+template <>
+__device__ __forceinline__ float acc_word<float>(uint32_t w) {
+  return __uint_as_float(w);
+}
+template <>
+__device__ __forceinline__ uint32_t acc_word<uint32_t>(uint32_t w) {
+  return w;
 }
 
 template <typename AB, typename OutT, int CG>
@@ -297,8 +320,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer (leader)
     if (lane == 0 && leader) {
-      const uint32_t idesc = OT::kFp8 ? ptx::make_idesc_e4m3_f32(CG * kDecodeTileN, p.mma_n)
-                                      : ptx::make_idesc_bf16_f32(CG * kDecodeTileN, p.mma_n);
+      const uint32_t idesc = OT::kInt8  ? ptx::make_idesc_s8_s32(CG * kDecodeTileN, p.mma_n)
+                             : OT::kFp8 ? ptx::make_idesc_e4m3_f32(CG * kDecodeTileN, p.mma_n)
+                                        : ptx::make_idesc_bf16_f32(CG * kDecodeTileN, p.mma_n);
       // Descriptors as 32-bit low halves: stage s's B rows start at b_lo0 + s * stage_step,
       // its A rows at a_lo0 + s * stage_step.
       const uint32_t hi = ptx::sw128_desc_hi();
@@ -316,9 +340,16 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
         // The stage's bytes arrived through the async proxy (TMA) and are read through it (the
         // MMA): the completed barrier phase orders them; no tcgen05 fence is needed here.
 #pragma unroll
-        for (int k = 0; k < kBK / kUmmaK; ++k)
-          ptx::umma_ss_lohi<CG, OT::kFp8>(tmem_base, b_lo + 2u * k, a_lo + 2u * k, hi, idesc,
-                                          (i > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kBK / kUmmaK; ++k) {
+          if constexpr (OT::kInt8) {
+            static_assert(CG == 1, "INT8 runs on single CTAs");
+            ptx::umma_i8_ss_lohi(tmem_base, b_lo + 2u * k, a_lo + 2u * k, hi, idesc,
+                                 (i > 0 || k > 0) ? 1u : 0u);
+          } else {
+            ptx::umma_ss_lohi<CG, OT::kFp8>(tmem_base, b_lo + 2u * k, a_lo + 2u * k, hi, idesc,
+                                            (i > 0 || k > 0) ? 1u : 0u);
+          }
+        }
         if constexpr (CG == 1) {
           ptx::umma_commit<1>(empty_bar + 8u * stage);
         } else {
@@ -448,6 +479,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
         float scale = p.alpha;
         if (p.scale_a != nullptr) scale *= *p.scale_a;
         if (p.scale_b != nullptr) scale *= *p.scale_b;
+        if (OT::kInt8 && p.col_scale != nullptr)
+          scale *= n < p.n ? __ldg(p.col_scale + n) : 0.f;
         const float bias = (p.bias != nullptr && n < p.n) ? __bfloat162float(p.bias[n]) : 0.f;
         // The quadrant's box of D (mma_n token rows x its 32 columns, unswizzled): lane l holds
         // column l of every row, so each row of the box is one conflict-free warp store; each
@@ -458,9 +491,11 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
         for (int j = 0; j < 4; ++j) {
           const int c = static_cast<int>(half) + 2 * j;
           if (c < chunks) {
-            float acc[16];
+            // fp32 sums, or the words of 32-bit integer sums (INT8).
+            using Acc = typename DecodeAcc<OT::kInt8>::T;
+            Acc acc[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[i] = __uint_as_float(v[j][i]);
+            for (int i = 0; i < 16; ++i) acc[i] = acc_word<Acc>(v[j][i]);
             for (int sidx = 0; sidx < S - 1; ++sidx) {
               const uint32_t r_addr =
                   base + lay.recv_off +
@@ -469,15 +504,27 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint4 w = ptx::ld_shared_v4(r_addr + 16u * i);
-                acc[4 * i] += __uint_as_float(w.x);
-                acc[4 * i + 1] += __uint_as_float(w.y);
-                acc[4 * i + 2] += __uint_as_float(w.z);
-                acc[4 * i + 3] += __uint_as_float(w.w);
+                acc[4 * i] += acc_word<Acc>(w.x);
+                acc[4 * i + 1] += acc_word<Acc>(w.y);
+                acc[4 * i + 2] += acc_word<Acc>(w.z);
+                acc[4 * i + 3] += acc_word<Acc>(w.w);
               }
             }
+            if constexpr (OT::kInt8) {
+              // Token rows 16 c + i: one scale each, the same for the whole warp.
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              box[(16 * c + i) * 32 + static_cast<int>(lane)] = to_out<OutT>(acc[i] * scale + bias);
+              for (int i = 0; i < 16; ++i) {
+                const int32_t r = 16 * c + i;
+                float x = __int2float_rn(static_cast<int32_t>(acc[i])) * scale;
+                if (p.row_scale != nullptr) x *= r < p.m ? __ldg(p.row_scale + r) : 0.f;
+                box[r * 32 + static_cast<int>(lane)] = to_out<OutT>(x + bias);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                box[(16 * c + i) * 32 + static_cast<int>(lane)] =
+                    to_out<OutT>(acc[i] * scale + bias);
+            }
           }
         }
         ptx::fence_proxy_async_shared();  // the box's generic stores before the TMA stores

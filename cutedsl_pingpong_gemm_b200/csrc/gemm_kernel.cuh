@@ -1,5 +1,6 @@
-// Warp-specialised persistent GEMM for sm_100a (BF16 or FP8 E4M3 operands, BF16 or FP32 D):
+// Warp-specialised persistent GEMM for sm_100a (BF16, FP8 E4M3 or INT8 operands, BF16 or FP32 D):
 //   D[M,N] = act(alpha * s_a * s_b * A[M,K] . B[N,K]^T + bias[N] + beta * C)
+// with scalar scales, or for INT8 operands s_a per row and s_b per column.
 //
 // Role of each warp (192 threads per CTA; 512-wide tiles: 384, see EpiShape):
 //   warp 0     TMA producer: one lane streams A/B k-blocks into an `ab_stages`-deep ring of
@@ -85,13 +86,35 @@ struct OperandTraits<__nv_bfloat16> {
   static constexpr int kBK = 64;     // elements per 128-byte row
   static constexpr int kUmmaK = 16;  // K per tcgen05.mma kind::f16
   static constexpr bool kFp8 = false;
+  static constexpr bool kInt8 = false;
 };
 template <>
 struct OperandTraits<e4m3_t> {
   static constexpr int kBK = 128;
   static constexpr int kUmmaK = 32;  // K per tcgen05.mma kind::f8f6f4
   static constexpr bool kFp8 = true;
+  static constexpr bool kInt8 = false;
 };
+// INT8: the sums are exact in the 32-bit integer accumulator for K <= kInt8MaxK (two's
+// complement operands, |a b| <= 2^14); the epilogue's conversion to fp32 rounds them once.
+constexpr int64_t kInt8MaxK = 131071;
+template <>
+struct OperandTraits<int8_t> {
+  static constexpr int kBK = 128;
+  static constexpr int kUmmaK = 32;  // K per tcgen05.mma kind::i8
+  static constexpr bool kFp8 = false;
+  static constexpr bool kInt8 = true;
+};
+
+// A TMEM accumulator word as fp32.
+template <typename AB>
+__device__ __forceinline__ float acc_f32(uint32_t w) {
+  if constexpr (OperandTraits<AB>::kInt8) {
+    return __int2float_rn(static_cast<int32_t>(w));
+  } else {
+    return __uint_as_float(w);
+  }
+}
 
 // Output element type -> columns per 128-byte staging row.
 template <typename T>
@@ -138,6 +161,11 @@ struct GemmParams {
   float alpha;
   const float* scale_a;   // optional device scalar (FP8 per-tensor scale of A); D *= *scale_a
   const float* scale_b;   // optional device scalar (FP8 per-tensor scale of B)
+  // INT8 operands: optional scale per row of A ([batches][M]) and per row of B, i.e. per column
+  // of the product ([batches or groups][N, or 2N when gated]), instead of the scalars.
+  const float* row_scale;
+  const float* col_scale;
+  int32_t col_scale_len;  // entries of one batch's or group's col_scale
   const __nv_bfloat16* bias;  // optional per-column bias, length N
   int32_t* tile_trace;    // optional: (pid_m, pid_n) per CTA per tile, trace_stride tiles per CTA
   int32_t trace_stride;
@@ -896,8 +924,9 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
   constexpr int kBK = OT::kBK;
   constexpr int kUmmaK = OT::kUmmaK;
   constexpr int kStoreCols = OutputTraits<OutT>::kStoreCols;
-  constexpr uint32_t kIdesc = OT::kFp8 ? ptx::make_idesc_e4m3_f32(kBM * CtaGroup, L::kMmaN)
-                                       : ptx::make_idesc_bf16_f32(kBM * CtaGroup, L::kMmaN);
+  constexpr uint32_t kIdesc = OT::kInt8  ? ptx::make_idesc_s8_s32(kBM * CtaGroup, L::kMmaN)
+                              : OT::kFp8 ? ptx::make_idesc_e4m3_f32(kBM * CtaGroup, L::kMmaN)
+                                         : ptx::make_idesc_bf16_f32(kBM * CtaGroup, L::kMmaN);
   constexpr int kAccStages = L::kAccStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
@@ -1037,7 +1066,10 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
             for (int j = 0; j < L::kNumMma; ++j) {
               const uint64_t dbj = db + static_cast<uint64_t>(2 * k + j * L::kBRowsPerMma * 8);
               const uint32_t dj = d_tmem + static_cast<uint32_t>(j * L::kMmaN);
-              if constexpr (OT::kFp8) {
+              if constexpr (OT::kInt8) {
+                ptx::umma_i8_ss<CtaGroup>(dj, da + static_cast<uint64_t>(2 * k), dbj, kIdesc,
+                                          (kb > kb0 || k > 0) ? 1u : 0u);
+              } else if constexpr (OT::kFp8) {
                 ptx::umma_f8_ss<CtaGroup>(dj, da + static_cast<uint64_t>(2 * k), dbj, kIdesc,
                                           (kb > kb0 || k > 0) ? 1u : 0u);
               } else {
@@ -1271,6 +1303,38 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
         __syncwarp();
         if (lane == 0) ptx::red_release_sys_add_u32(p.rs_count[rs_owner], 1u);
       };
+      // INT8: this row's scale (with alpha), and the columns' scales of the tile's batch or group.
+      // Rows outside the problem are not stored; they take the scale 0 without reading it.
+      float row_alpha = alpha;
+      const float* col_scale = nullptr;
+      if constexpr (OT::kInt8) {
+        if (p.row_scale != nullptr)
+          row_alpha *= my_row < row_end
+                           ? __ldg(p.row_scale + static_cast<int64_t>(sg.ab_batch) * p.m + my_row)
+                           : 0.f;
+        if (p.col_scale != nullptr)
+          col_scale = p.col_scale + static_cast<int64_t>(sg.batch) * p.col_scale_len;
+      }
+      // v[j] *= col_scale[col0 + j] for 32 columns of this row, of which those below `limit`
+      // exist.  Every lane needs the same values: 16-byte loads broadcast to the warp where they
+      // are aligned, else one coalesced load and shuffles (as the bias row below).
+      auto scale_cols = [&](float* v, int32_t col0, int32_t limit) {
+        const float* sp0 = col_scale + col0;
+        if (col0 + 32 <= limit && (reinterpret_cast<uintptr_t>(sp0) & 15u) == 0) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint4 w = ptx::ld_global_nc_v4(sp0 + 4 * q);
+            v[4 * q] *= __uint_as_float(w.x);
+            v[4 * q + 1] *= __uint_as_float(w.y);
+            v[4 * q + 2] *= __uint_as_float(w.z);
+            v[4 * q + 3] *= __uint_as_float(w.w);
+          }
+          return;
+        }
+        const float sl = col0 + static_cast<int32_t>(lane) < limit ? __ldg(sp0 + lane) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= __shfl_sync(0xffffffffu, sl, j);
+      };
       auto add_bias_row = [&](float (&x)[kStoreCols], int32_t col0) {
         if (bias_vec && col0 + kStoreCols <= p.n) {
           // Every row needs the same kStoreCols values: all lanes load them with the same
@@ -1318,7 +1382,14 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
           ptx::tmem_ld_wait();
           if (c == c_end - 1) release_tmem(acc);
 #pragma unroll
-          for (int j = 0; j < kStoreCols; ++j) x[j] = __uint_as_float(v[j]) * alpha;
+          for (int j = 0; j < kStoreCols; ++j) x[j] = acc_f32<AB>(v[j]) * row_alpha;
+          if constexpr (OT::kInt8) {
+            if (col_scale != nullptr) {
+#pragma unroll
+              for (int h = 0; h < kStoreCols / 32; ++h)
+                scale_cols(&x[32 * h], col0 + 32 * h, p.n);
+            }
+          }
         } else {
           // 32 gate and 32 up columns per TMEM round trip.
 #pragma unroll
@@ -1331,10 +1402,19 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
             if (c == c_end - 1 && h == kStoreCols / 32 - 1) release_tmem(acc);
             float gv[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) gv[j] = __uint_as_float(vg[j]) * alpha;
+            for (int j = 0; j < 32; ++j) gv[j] = acc_f32<AB>(vg[j]) * row_alpha;
+            if constexpr (OT::kInt8) {
+              if (col_scale != nullptr) scale_cols(gv, col0 + 32 * h, p.n);
+            }
             act_inplace(p.act, gv);
+            float uv[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[32 * h + j] = gv[j] * (__uint_as_float(vu[j]) * alpha);
+            for (int j = 0; j < 32; ++j) uv[j] = acc_f32<AB>(vu[j]) * row_alpha;
+            if constexpr (OT::kInt8) {
+              if (col_scale != nullptr) scale_cols(uv, p.n + col0 + 32 * h, 2 * p.n);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[32 * h + j] = gv[j] * uv[j];
           }
         }
         if (partial) {

@@ -141,7 +141,7 @@ enum : int32_t {
   kStatusTimeoutBase = 0x100,
 };
 
-__device__ __noinline__ void record_timeout(const WaitCtx& ctx, int32_t site) {
+inline __device__ __noinline__ void record_timeout(const WaitCtx& ctx, int32_t site) {
   *ctx.abort_flag = 1;
   if (ctx.status != nullptr) atomicCAS(ctx.status, 0, kStatusTimeoutBase | site);
 }
@@ -395,6 +395,15 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3_f32(int M, int N) {
          | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Instruction descriptor for kind::i8 with signed 8-bit A/B, S32 accumulate (wrapping, not
+// saturating), both K-major.
+__host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
+  return (2u << 4)                                   // c_format = S32
+         | (1u << 7)                                 // a_format = signed 8-bit
+         | (1u << 10)                                // b_format = signed 8-bit
+         | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, issued by one thread.
 template <int CtaGroup>
 __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -431,6 +440,26 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uin
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+template <int CtaGroup>
+__device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CtaGroup == 1) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
   }
@@ -486,6 +515,20 @@ __device__ __forceinline__ void umma_ss_lohi(uint32_t d_tmem, uint32_t a_lo, uin
         "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
   }
+}
+
+// The single-CTA kind::i8 form of umma_ss_lohi.
+__device__ __forceinline__ void umma_i8_ss_lohi(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                                uint32_t hi, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 // Arrive once on `bar` when all previously issued tcgen05 async operations of this thread

@@ -13,9 +13,12 @@ Drop-in surface (adelmuursepp/cutedsl_pingpong_gemm, gemm_base.py):
 ``a`` is [M, K], ``b`` is [N, K] and ``c`` is [M, N], all BF16 CUDA tensors with unit stride in
 the last dimension (the reference's harness layout, gemm_base.py:587-590).  Beyond the reference,
 ``a``/``b`` may be FP8 E4M3 (``torch.float8_e4m3fn``, with per-tensor ``scale_a``/``scale_b``
-device scalars) and ``c`` may be FP32 (split-K partials); ``bias`` adds a BF16 per-column vector.  Underneath, every call
-goes through the C ABI of ``libcpgemm.so`` into hand-written sm_100a kernels (tcgen05 MMA into
-TMEM, TMA loads/stores, persistent grouped tile scheduler); there is no other execution path.
+device scalars) or INT8 (``torch.int8``, with scales per tensor, or per row of ``a`` and per row of
+``b``: FP32 [M] and [N], of a batched call [L, M] and [L, N]) and ``c`` may be FP32 (split-K
+partials); ``bias`` adds a BF16 per-column vector.  INT8 sums are exact 32-bit integers (K <=
+131071), rounded once before the scales.  Underneath, every call goes through the C ABI of
+``libcpgemm.so`` into hand-written sm_100a kernels (tcgen05 MMA into TMEM, TMA loads/stores,
+persistent grouped tile scheduler); there is no other execution path.
 
 Argument meaning on sm_100a:
 
@@ -50,7 +53,8 @@ THREADS_PER_CTA_SM100_WIDE = 384
 def _dtype_tables():
     """(A/B dtype -> CPG code, D dtype -> CPG code)."""
     import torch
-    ab = {torch.bfloat16: _lib.CPG_DTYPE_BF16, torch.float8_e4m3fn: _lib.CPG_DTYPE_E4M3}
+    ab = {torch.bfloat16: _lib.CPG_DTYPE_BF16, torch.float8_e4m3fn: _lib.CPG_DTYPE_E4M3,
+          torch.int8: _lib.CPG_DTYPE_I8}
     d = {torch.bfloat16: _lib.CPG_DTYPE_BF16, torch.float32: _lib.CPG_DTYPE_F32}
     return ab, d
 
@@ -68,6 +72,21 @@ def _stream_handle(stream, device) -> int:
     if get_ptr is not None:
         return int(get_ptr())
     return int(stream)
+
+
+def _scale_mode(a, scale_a, scale_b) -> int:
+    """CPG scale mode of a call.  INT8: a scale of other than one element is one per row of its
+    operand (tokens of A, output channels of B).  E4M3: more than one element of ``scale_a`` selects
+    the block-scaled kernel (A: 1 x 128, B: 128 x 128 blocks, layouts of cpgemm.h).  One element
+    each is a per-tensor scale."""
+    import torch
+    if a.dtype == torch.int8:
+        rows_a = scale_a is not None and scale_a.numel() != 1
+        rows_b = scale_b is not None and scale_b.numel() != 1
+        return ((_lib.CPG_SCALE_ROWS_A if rows_a else 0)
+                | (_lib.CPG_SCALE_ROWS_B if rows_b else 0))
+    block = scale_a is not None and scale_a.numel() > 1
+    return _lib.CPG_SCALE_BLOCK if block else _lib.CPG_SCALE_TENSOR
 
 
 class CompiledGemm:
@@ -95,7 +114,7 @@ class CompiledGemm:
         ab_codes, d_codes = _dtype_tables()
         # gemm_base.py:514 requires BF16 everywhere; sm_100a adds FP8 E4M3 operands and FP32 D.
         assert a.dtype == b.dtype and a.dtype in ab_codes and c.dtype in d_codes, \
-            "A, B and D must be BF16 (gemm_base.py:514), or FP8 E4M3 A/B, or FP32 D"
+            "A, B and D must be BF16 (gemm_base.py:514), or FP8 E4M3 or INT8 A/B, or FP32 D"
         nd = a.dim()
         if nd not in (2, 3) or b.dim() != nd or c.dim() != nd:
             raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
@@ -172,10 +191,8 @@ class CompiledGemm:
             raise _lib.CpgError(_lib.CPG_ERR_INVALID_CONFIG, f"unknown activation {activation!r}")
         act = _lib.ACTIVATIONS[activation]
         fused = act != _lib.CPG_ACT_NONE or source is not None or gated
-        # More than one scale per operand selects the block-scaled FP8 kernel (A: 1 x 128,
-        # B: 128 x 128 blocks, layouts of cpgemm.h); one value each is a per-tensor scale.
-        block = scale_a is not None and scale_a.numel() > 1
-        mode = _lib.CPG_SCALE_BLOCK if block else _lib.CPG_SCALE_TENSOR
+        mode = _scale_mode(a, scale_a, scale_b)
+        block = mode == _lib.CPG_SCALE_BLOCK
         if a.dim() == 3 and a.shape[0] == 0:
             return None  # no batches: nothing to compute
         if split_k == 0:
@@ -210,7 +227,8 @@ class CompiledGemm:
         [G, 2N, K] with ``gated``), ``c`` [T, N]; ``group_offsets`` is an int32 CUDA tensor of
         G + 1 non-decreasing offsets within [0, T] (read on the device: no host synchronisation);
         rows outside every group are not written.  Epilogue options as in ``__call__``; no
-        split-K and no block scales.  The reference has no grouped form (its kernel fixes the L
+        split-K and no block scales; INT8 operands take ``scale_a`` [T] and ``scale_b`` [G, N]
+        (or [G, 2N]).  The reference has no grouped form (its kernel fixes the L
         mode at one, gemm_base.py:221)."""
         import torch
         if activation not in _lib.ACTIVATIONS:
@@ -226,17 +244,19 @@ class CompiledGemm:
                                 "group_offsets must be a contiguous int32 CUDA tensor of G + 1")
         if groups == 0 or a.shape[0] == 0:
             return None
-        plan = self._grouped_plan(a, b, c, gated)
+        mode = _scale_mode(a, scale_a, scale_b)
+        plan = self._grouped_plan(a, b, c, gated,
+                                  mode if a.dtype == torch.int8 else _lib.CPG_SCALE_TENSOR)
         plan.run(a, b, c, stream, bias=bias, alpha=alpha, scale_a=scale_a, scale_b=scale_b,
                  activation=_lib.ACTIVATIONS[activation], source=source, beta=beta,
                  group_offsets=group_offsets)
         return None
 
-    def _grouped_plan(self, a, b, c, gated):
+    def _grouped_plan(self, a, b, c, gated, scale_mode=0):
         import torch
         ab_codes, d_codes = _dtype_tables()
         assert a.dtype == b.dtype and a.dtype in ab_codes and c.dtype in d_codes, \
-            "A, B and D must be BF16 (gemm_base.py:514), or FP8 E4M3 A/B, or FP32 D"
+            "A, B and D must be BF16 (gemm_base.py:514), or FP8 E4M3 or INT8 A/B, or FP32 D"
         t, k = a.shape
         groups, b_rows, kb = b.shape
         n = b_rows // 2 if gated else b_rows
@@ -254,11 +274,12 @@ class CompiledGemm:
         ldd = c.stride(0) if t > 1 else max(16 // c.element_size(), n)
         dev = c.device.index
         dt_ab, dt_d = ab_codes[a.dtype], d_codes[c.dtype]
-        key = ("grouped", t, n, k, groups, lda, ldb, ldd, b.stride(0), dev, dt_ab, dt_d, bool(gated))
+        key = ("grouped", t, n, k, groups, lda, ldb, ldd, b.stride(0), dev, dt_ab, dt_d,
+               bool(gated), scale_mode)
         plan = self._plans.get(key)
         if plan is None:
-            plan = _Plan(self.gemm, t, n, k, lda, ldb, ldd, dev, dt_ab, dt_d, 0, 1, gated, groups,
-                         0, b.stride(0), 0, grouped=True)
+            plan = _Plan(self.gemm, t, n, k, lda, ldb, ldd, dev, dt_ab, dt_d, scale_mode, 1, gated,
+                         groups, 0, b.stride(0), 0, grouped=True)
             self._plans[key] = plan
         return plan
 
@@ -346,6 +367,7 @@ class _Plan:
         self.lib = _lib.load()
         self.m, self.n, self.k = m, n, k
         self.l = l
+        self.gated = bool(gated)
         self.device = device
         self.scale_mode = scale_mode
         cfg = gemm._config_c()
@@ -416,7 +438,12 @@ class _Plan:
             nkb, nnb = -(-self.k // 128), -(-self.n // 128)
             want = {"scale_a": (nkb, self.m), "scale_b": (nnb, nkb)}
         else:
-            want = {"scale_a": (1,), "scale_b": (1,)}
+            # One value, or (INT8) one per row of A and of B, of every batch or group.
+            b_rows = 2 * self.n if self.gated else self.n
+            rows_a = (self.l, self.m) if self.l and not self.grouped else (self.m,)
+            rows_b = (self.l, b_rows) if self.l or self.grouped else (b_rows,)
+            want = {"scale_a": rows_a if self.scale_mode & _lib.CPG_SCALE_ROWS_A else (1,),
+                    "scale_b": rows_b if self.scale_mode & _lib.CPG_SCALE_ROWS_B else (1,)}
         for name, sc in (("scale_a", scale_a), ("scale_b", scale_b)):
             if sc is not None and not (sc.is_cuda and sc.dtype == torch.float32 and sc.is_contiguous()
                                        and sc.numel() == math.prod(want[name])):
@@ -521,9 +548,9 @@ class GemmSM90:
     @staticmethod
     def cta_tile_k(dtype) -> int:
         """K extent of one pipeline stage: a 128-byte swizzled row of the operand type (64 BF16
-        elements, 128 FP8 E4M3)."""
+        elements, 128 FP8 E4M3 or INT8)."""
         import torch
-        return 128 if dtype == torch.float8_e4m3fn else 64
+        return 128 if dtype in (torch.float8_e4m3fn, torch.int8) else 64
 
     @property
     def max_active_clusters(self) -> int:
@@ -556,9 +583,7 @@ class GemmSM90:
         ``gated`` plans the gated FFN form (B = [W_gate; W_up])."""
         compiled = CompiledGemm(self)
         self.cta_tile_shape_mnk = (*self.cta_tile_shape_mnk[:2], self.cta_tile_k(a.dtype))
-        block = scale_a is not None and scale_a.numel() > 1
-        compiled.plan_for(a, b, c, _lib.CPG_SCALE_BLOCK if block else _lib.CPG_SCALE_TENSOR,
-                          gated=gated)
+        compiled.plan_for(a, b, c, _scale_mode(a, scale_a, scale_b), gated=gated)
         self._compiled = compiled
         return compiled
 

@@ -1,0 +1,268 @@
+"""What surrounds the experts' products of an MoE layer (``GemmSM90.grouped``), on the GPU alone (C
+ABI: cpg_route, cpg_expert_order, cpg_dispatch_rows, cpg_combine_rows and their gradients).
+
+    ids, weights = route(logits, k)                      # experts and weights of every token
+    d = dispatch(x, ids, experts, quantize="int8")       # rows in expert order, group offsets
+    gemm.grouped(d.rows, w_up, h, d.offsets, scale_a=d.scales, scale_b=s_up, ...)
+    ...
+    y = combine(out, d.slots, weights)                   # weighted sum back per token
+
+Nothing synchronises with the host: offsets and slots stay on the device.  Every function runs on
+the current stream of its tensors' device and keeps nothing between calls, so calls on several
+streams and captured graphs are independent.  Gradients: ``route_backward``, ``combine_backward``;
+the gradient of ``dispatch`` is ``combine`` of the rows' gradients without weights (a quantised
+dispatch: of the rows it stands for, rounding ignored).  The reference has no such operators.
+"""
+import contextlib
+import ctypes
+from collections import namedtuple
+from typing import Optional
+
+from . import _lib
+from .quant import alloc_int8_rows
+
+Dispatched = namedtuple("Dispatched", "rows offsets slots scales")
+
+
+def _error(code, message):
+    return _lib.CpgError(code, message)
+
+
+def _float_code(name, t):
+    import torch
+    codes = {torch.bfloat16: _lib.CPG_DTYPE_BF16, torch.float32: _lib.CPG_DTYPE_F32}
+    if t.dtype not in codes:
+        raise _error(_lib.CPG_ERR_DTYPE, f"{name} must be BF16 or FP32, got {t.dtype}")
+    return codes[t.dtype]
+
+
+def _matrix(name, t, shape=None, device=None):
+    """A 2-D CUDA tensor with unit column stride (of ``shape``, on ``device``); its row stride."""
+    if not t.is_cuda:
+        raise _error(_lib.CPG_ERR_NO_DEVICE, f"{name} must be a CUDA tensor")
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
+                     f"{name} must be 2-D{'' if shape is None else ' of shape ' + str(tuple(shape))}"
+                     f", got {tuple(t.shape)}")
+    if t.numel() and t.shape[1] > 1 and t.stride(1) != 1:
+        raise _error(_lib.CPG_ERR_UNSUPPORTED, f"{name} must have unit column stride")
+    _same_device(name, t, device)
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _same_device(name, t, device):
+    if device is not None and t.device != device:
+        raise _error(_lib.CPG_ERR_NO_DEVICE, f"{name} is on {t.device}, the others on {device}")
+
+
+def _output(name, t, shape, device):
+    """As ``_matrix`` for a tensor that is written: its rows must not overlap."""
+    ld = _matrix(name, t, shape, device)
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"{name}'s rows overlap (row stride {ld})")
+    return ld
+
+
+def _vector(name, t, shape, dtype, device):
+    if t is None:
+        raise _error(_lib.CPG_ERR_NULL, f"{name} must be given")
+    if not (t.is_cuda and t.dtype == dtype and tuple(t.shape) == tuple(shape)
+            and t.is_contiguous()):
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
+                     f"{name} must be a contiguous {dtype} CUDA tensor of shape {tuple(shape)}, "
+                     f"got {t.dtype} {tuple(t.shape)}")
+    _same_device(name, t, device)
+
+
+def _ptr(t):
+    return None if t is None or t.numel() == 0 else t.data_ptr()
+
+
+def _call(fn, what, device, *args):
+    """Call a C entry point on the current stream of ``device`` (made current for the call)."""
+    import torch
+    here = torch.cuda.current_device() == device.index
+    with contextlib.nullcontext() if here else torch.cuda.device(device):
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, what)
+
+
+def _route_config(experts, k, scoring, groups, kept_groups, group_score, renormalize, scale):
+    if scoring not in _lib.ROUTE_SCORINGS:
+        raise _error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown scoring {scoring!r}")
+    if group_score not in _lib.ROUTE_GROUP_SCORES:
+        raise _error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown group_score {group_score!r}")
+    return _lib.RouteConfigC(experts, k, _lib.ROUTE_SCORINGS[scoring], groups, kept_groups,
+                             _lib.ROUTE_GROUP_SCORES[group_score], 1 if renormalize else 0,
+                             float(scale))
+
+
+def route(logits, k: int, *, scoring: str = "softmax", bias=None, groups: int = 1,
+          kept_groups: Optional[int] = None, group_score: Optional[str] = None,
+          renormalize: bool = True, scale: float = 1.0, ids=None, weights=None):
+    """Choose ``k`` of the E experts for every row of ``logits`` [T, E] (BF16 or FP32).
+
+    Returns ``(ids, weights)``, int32 and FP32 [T, k], best first: the experts with the largest
+    ``scoring(logits) + bias`` ("softmax" over all experts, or "sigmoid"; ties to the lowest index)
+    and ``scale * score``, over the sum of the chosen scores when ``renormalize``.  ``bias`` (FP32
+    [E]) only ranks.  ``groups`` > 1 first keeps the best ``kept_groups`` groups of E / groups
+    consecutive experts, a group counting as its best expert ("max") or its two best ("top2";
+    the default with a bias).  A logit of -inf masks an expert; where fewer than k are left the
+    last ids are -1 with weight 0.  A NaN logit makes the row's weights NaN (under the softmax
+    +inf too).  E <= 1024, k and groups <= 32.  ``ids`` / ``weights`` may be given as outputs."""
+    import torch
+    ld = _matrix("logits", logits)
+    code = _float_code("logits", logits)
+    t, e = logits.shape
+    dev = logits.device
+    if group_score is None:
+        group_score = "top2" if bias is not None else "max"
+    cfg = _route_config(e, k, scoring, groups, groups if kept_groups is None else kept_groups,
+                        group_score, renormalize, scale)
+    if bias is not None:
+        _vector("bias", bias, (e,), torch.float32, dev)
+    if ids is None:
+        ids = torch.empty(t, max(k, 0), dtype=torch.int32, device=dev)
+    if weights is None:
+        weights = torch.empty(t, max(k, 0), dtype=torch.float32, device=dev)
+    _vector("ids", ids, (t, max(k, 0)), torch.int32, dev)
+    _vector("weights", weights, (t, max(k, 0)), torch.float32, dev)
+    _call(_lib.load().cpg_route, "route", dev, ctypes.byref(cfg), _ptr(logits), code, t, ld,
+          _ptr(bias), _ptr(ids), _ptr(weights))
+    return ids, weights
+
+
+def route_backward(dweights, logits, ids, *, scoring: str = "softmax", renormalize: bool = True,
+                   scale: float = 1.0, out=None):
+    """Gradient of ``route``'s weights: ``dlogits`` [T, E] in the logits' type from ``dweights``
+    (FP32 [T, k]) for the choices ``ids`` of the forward call (same scoring, renormalize, scale).
+    Entries of ``ids`` that are no expert take no part; an expert given twice counts twice."""
+    import torch
+    ld = _matrix("logits", logits)
+    code = _float_code("logits", logits)
+    t, e = logits.shape
+    dev = logits.device
+    if ids.dim() != 2:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"ids must be [T, k], got {tuple(ids.shape)}")
+    k = ids.shape[1]
+    _vector("ids", ids, (t, k), torch.int32, dev)
+    _vector("dweights", dweights, (t, k), torch.float32, dev)
+    cfg = _route_config(e, k, scoring, 1, 1, "max", renormalize, scale)
+    if out is None:
+        out = torch.empty(t, e, dtype=logits.dtype, device=dev)
+    ldd = _output("out", out, (t, e), dev)
+    if out.dtype != logits.dtype:
+        raise _error(_lib.CPG_ERR_DTYPE, f"out must be {logits.dtype} like logits")
+    _call(_lib.load().cpg_route_backward, "route_backward", dev, ctypes.byref(cfg), _ptr(dweights),
+          _ptr(logits), code, t, ld, _ptr(ids), _ptr(out), ldd)
+    return out
+
+
+def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, scales=None):
+    """Rows of ``x`` [T, D] (BF16 or FP32) in expert order, for ``GemmSM90.grouped``.
+
+    ``ids`` int32 [T, k] gives each token's experts (entries outside [0, experts) are skipped).
+    Returns ``Dispatched(rows, offsets, slots, scales)``: ``rows`` [T * k, D] holds the rows of
+    expert e at ``offsets[e] <= r < offsets[e + 1]`` (int32 [experts + 1]) in token order, ``slots``
+    int32 [T, k] the row of every (token, choice), -1 if skipped.  Rows from ``offsets[experts]``
+    on are not written.  ``quantize="int8"`` makes ``rows`` the int8 rows and ``scales`` (FP32
+    [T * k]) the scales of ``quant.quantize_int8``; otherwise ``scales`` is None.  ``out`` /
+    ``scales`` may be given as outputs.  experts <= 1024, k <= 32."""
+    import torch
+    ldx = _matrix("x", x)
+    code = _float_code("x", x)
+    t, d = x.shape
+    dev = x.device
+    if quantize not in (None, "int8"):
+        raise _error(_lib.CPG_ERR_UNSUPPORTED, f"quantize must be None or 'int8', got {quantize!r}")
+    if ids.dim() != 2:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"ids must be [T, k], got {tuple(ids.shape)}")
+    k = ids.shape[1]
+    _vector("ids", ids, (t, k), torch.int32, dev)
+    if experts < 1 or experts > _lib.CPG_ROUTE_MAX_EXPERTS:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
+                     f"1 <= experts <= {_lib.CPG_ROUTE_MAX_EXPERTS}, got {experts}")
+    int8 = quantize == "int8"
+    dtype = torch.int8 if int8 else x.dtype
+    if out is None:
+        out = (alloc_int8_rows(t * k, d, dev) if int8
+               else torch.empty(t * k, d, dtype=dtype, device=dev))
+    ldr = _output("out", out, (t * k, d), dev)
+    if out.dtype != dtype:
+        raise _error(_lib.CPG_ERR_DTYPE, f"out must be {dtype}, got {out.dtype}")
+    if int8:
+        if scales is None:
+            scales = torch.empty(t * k, dtype=torch.float32, device=dev)
+        _vector("scales", scales, (t * k,), torch.float32, dev)
+    elif scales is not None:
+        raise _error(_lib.CPG_ERR_UNSUPPORTED, "scales only with quantize='int8'")
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(t, k, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    _call(lib.cpg_expert_order, "dispatch", dev, _ptr(ids), t, k, experts, _ptr(offsets),
+          _ptr(slots))
+    _call(lib.cpg_dispatch_rows, "dispatch", dev, _ptr(x), code, t, d, ldx, _ptr(slots), k,
+          _ptr(out), _lib.CPG_DTYPE_I8 if int8 else code, t * k, ldr, _ptr(scales))
+    return Dispatched(out, offsets, slots, scales)
+
+
+def combine(rows, slots, weights=None, *, source=None, out=None):
+    """``y[t] = source[t] + sum_j weights[t, j] * rows[slots[t, j]]`` (FP32 sums, rounded once).
+
+    ``rows`` [R, D] BF16 or FP32, ``slots`` int32 [T, k] (entries outside [0, R) are not read),
+    ``weights`` FP32 [T, k] or None for ones, ``source`` an optional [T, D] of the rows' type
+    (it may be ``out``), such as a shared expert's output."""
+    import torch
+    ldr = _matrix("rows", rows)
+    code = _float_code("rows", rows)
+    r, d = rows.shape
+    dev = rows.device
+    if slots.dim() != 2:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"slots must be [T, k], got {tuple(slots.shape)}")
+    t, k = slots.shape
+    _vector("slots", slots, (t, k), torch.int32, dev)
+    if weights is not None:
+        _vector("weights", weights, (t, k), torch.float32, dev)
+    lds = 0
+    if source is not None:
+        lds = _matrix("source", source, (t, d), dev)
+    if out is None:
+        out = torch.empty(t, d, dtype=rows.dtype, device=dev)
+    ldy = _output("out", out, (t, d), dev)
+    if out.dtype != rows.dtype or (source is not None and source.dtype != rows.dtype):
+        raise _error(_lib.CPG_ERR_DTYPE, f"source and out must be {rows.dtype} like rows")
+    _call(_lib.load().cpg_combine_rows, "combine", dev, _ptr(rows), code, r, d, ldr, _ptr(slots),
+          _ptr(weights), t, k, _ptr(source), lds, _ptr(out), ldy)
+    return out
+
+
+def combine_backward(dy, rows, slots, weights, *, drows=None, dweights=None):
+    """Gradients of ``combine``: ``drows[slots[t, j]] = weights[t, j] * dy[t]`` [R, D] (rows that
+    no slot names are left as they were) and ``dweights[t, j] = <dy[t], rows[slots[t, j]]>`` FP32
+    [T, k].  No two slots may be the same row (``dispatch`` makes none).  ``drows`` / ``dweights``
+    may be given as outputs."""
+    import torch
+    lddy = _matrix("dy", dy)
+    code = _float_code("dy", dy)
+    t, d = dy.shape
+    dev = dy.device
+    ldr = _matrix("rows", rows, (rows.shape[0], d) if rows.dim() == 2 else None, dev)
+    r = rows.shape[0]
+    if slots.dim() != 2:
+        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"slots must be [T, k], got {tuple(slots.shape)}")
+    k = slots.shape[1]
+    _vector("slots", slots, (t, k), torch.int32, dev)
+    _vector("weights", weights, (t, k), torch.float32, dev)
+    if drows is None:
+        drows = torch.empty(r, d, dtype=rows.dtype, device=dev)
+    if dweights is None:
+        dweights = torch.empty(t, k, dtype=torch.float32, device=dev)
+    lddr = _output("drows", drows, (r, d), dev)
+    _vector("dweights", dweights, (t, k), torch.float32, dev)
+    if not (dy.dtype == rows.dtype == drows.dtype):
+        raise _error(_lib.CPG_ERR_DTYPE, f"dy, rows and drows must share one type, got {dy.dtype}, "
+                                         f"{rows.dtype}, {drows.dtype}")
+    _call(_lib.load().cpg_combine_rows_backward, "combine_backward", dev, _ptr(dy), code, t, d,
+          lddy, _ptr(rows), r, ldr, _ptr(slots), _ptr(weights), k, _ptr(drows), lddr,
+          _ptr(dweights))
+    return drows, dweights

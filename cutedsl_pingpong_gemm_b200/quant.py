@@ -1,10 +1,13 @@
-"""FP8 E4M3 quantisation and FP32 -> BF16 cast on the GPU (C ABI: cpg_quantize_e4m3,
-cpg_cast_f32_bf16).
+"""FP8 E4M3 and INT8 quantisation and FP32 -> BF16 cast on the GPU (C ABI: cpg_quantize_e4m3,
+cpg_quantize_int8, cpg_cast_f32_bf16).
 
 ``quantize_e4m3(x, block=None)`` returns ``(q, scales)`` with ``s = amax(|x|) / 448`` per tensor
 (``block=None``), per 1 x 128 block (``block=(1, 128)``, the A operand of block-scaled FP8
 GEMM) or per 128 x 128 block (``block=(128, 128)``, the B operand), and ``q = e4m3(x / s)``.
 Scale layouts are described in ``include/cpgemm.h``.
+
+``quantize_int8(x)`` returns ``(q, scales)`` with one scale per row, ``s = amax(|x|) / 127``, and
+``q = rint(x / s)``: the scales of the tokens of A, or of the output channels of a weight B.
 """
 from typing import Optional, Tuple
 
@@ -40,6 +43,44 @@ def quantize_e4m3(x, block: Optional[Tuple[int, int]] = None):
                                      q.data_ptr() if q.numel() else None, cols, scales.data_ptr(),
                                      br, bc, _stream(x)), "quantize_e4m3")
     return q, scales
+
+
+def alloc_int8_rows(rows: int, cols: int, device):
+    """int8 [rows, cols] whose rows start on 16 bytes, as the GEMM's loads need."""
+    import torch
+    return torch.empty(rows, -(-cols // 16) * 16, dtype=torch.int8, device=device)[:, :cols]
+
+
+def quantize_int8(x, out=None, scales=None):
+    """INT8 rows of a 2-D BF16 or FP32 CUDA tensor and their FP32 scales [rows], on the current
+    stream.  ``q`` has rows padded to 16 bytes, ready for the GEMM; ``out`` (int8, x's shape, unit
+    column stride) and ``scales`` may be given as outputs.  Rows of zeros get q = 0 and a tiny
+    scale; a row that holds an infinity or NaN gets q = 0 and the scale NaN."""
+    import torch
+    if not x.is_cuda or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise _lib.CpgError(_lib.CPG_ERR_DTYPE, "x must be a 2-D BF16 or FP32 CUDA tensor")
+    if x.numel() and x.shape[1] > 1 and x.stride(1) != 1:
+        raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED, "x must have unit column stride")
+    rows, cols = x.shape
+    if out is None:
+        out = alloc_int8_rows(rows, cols, x.device)
+    if scales is None:
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if (out.dtype != torch.int8 or out.shape != x.shape or out.device != x.device
+            or (out.numel() and ((cols > 1 and out.stride(1) != 1)
+                                 or (rows > 1 and out.stride(0) < cols)))):
+        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
+                            "out must be an int8 tensor of x's shape with unit column stride")
+    if (scales.dtype != torch.float32 or tuple(scales.shape) != (rows,)
+            or scales.device != x.device or not scales.is_contiguous()):
+        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE, "scales must be contiguous FP32 [rows]")
+    dt = _lib.CPG_DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.CPG_DTYPE_F32
+    from .moe import _call
+    _call(_lib.load().cpg_quantize_int8, "quantize_int8", x.device,
+          x.data_ptr() if x.numel() else None, dt, rows, cols, x.stride(0) if rows > 1 else cols,
+          out.data_ptr() if out.numel() else None, out.stride(0) if rows > 1 else cols,
+          scales.data_ptr() if rows else None)
+    return out, scales
 
 
 def cast_f32_bf16(x, bias=None, out=None, stream=None):

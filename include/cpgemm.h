@@ -54,6 +54,7 @@ extern "C" {
 #define CPG_DTYPE_BF16 0
 #define CPG_DTYPE_E4M3 1
 #define CPG_DTYPE_F32 2
+#define CPG_DTYPE_I8 3 /* signed 8-bit integers (A and B only) */
 
 /* FP8 scale modes.  TENSOR: optional per-tensor scales (cpg_epilogue.scale_a / scale_b point to
  * one fp32 each).  BLOCK: scale_a points to A's 1 x 128 scales laid out [ceil(K/128)][M] and
@@ -61,6 +62,14 @@ extern "C" {
  * tile_n = 128 or 256 and BF16 output. */
 #define CPG_SCALE_TENSOR 0
 #define CPG_SCALE_BLOCK 1
+/* Scales of INT8 operands (CPG_SCALE_TENSOR, either flag, or both): with ROWS_A scale_a points to
+ * one fp32 per row of A ([batches][M]; the scale of a token), with ROWS_B scale_b to one per row of
+ * B, i.e. per column of the product ([batches or groups][N], or [..][2N] when gated; the scale of
+ * an output channel); an operand without its flag has one value, and a NULL pointer means 1.  Each
+ * batch's or group's scales follow the previous one's without a gap.  The sum over k is exact in
+ * 32-bit integers (K <= 131071) and is rounded once to fp32 before the scales. */
+#define CPG_SCALE_ROWS_A 2
+#define CPG_SCALE_ROWS_B 4
 
 /* Raster order of the tile scheduler (tile_scheduler.py:24-27). */
 #define CPG_RASTER_ALONG_M 0
@@ -112,9 +121,10 @@ typedef struct cpg_gemm_config {
 typedef struct cpg_gemm_problem {
   int64_t m, n, k;
   int64_t lda, ldb, ldd; /* row strides in elements */
-  int32_t dtype_ab;      /* CPG_DTYPE_BF16 or CPG_DTYPE_E4M3 (A and B share one type) */
+  int32_t dtype_ab;      /* CPG_DTYPE_BF16, _E4M3 or _I8 (A and B share one type) */
   int32_t dtype_d;       /* CPG_DTYPE_BF16, or CPG_DTYPE_F32 for split-K partials */
-  int32_t scale_mode;    /* CPG_SCALE_TENSOR, or CPG_SCALE_BLOCK for block-scaled E4M3 */
+  int32_t scale_mode;    /* CPG_SCALE_TENSOR, CPG_SCALE_BLOCK for block-scaled E4M3, or
+                            CPG_SCALE_ROWS_A | CPG_SCALE_ROWS_B (either, both) for INT8 */
   int32_t split_k;       /* 0 or 1: none; S > 1: K is cut into S ranges scheduled as the L
                             dimension, and the ranges add their FP32 partial sums into D
                             (dtype_d must be CPG_DTYPE_F32; D is cleared by cpg_gemm_run);
@@ -152,7 +162,7 @@ typedef struct cpg_gemm_problem {
 /* Small-M (decode-like) kernel, for 1 <= M <= 128: each CTA computes D^T for 128 rows of B (B's
  * rows on the MMA's M side, the M rows of A on its N side, rounded up to 16), the K range of a
  * tile is split over a cluster of 1, 2 or 4 CTAs and the partial sums are added in distributed
- * shared memory, in one launch with no workspace.  BF16 or E4M3 operands (per-tensor scales),
+ * shared memory, in one launch with no workspace.  BF16, E4M3 (per-tensor scales) or INT8 operands,
  * BF16 or FP32 D, alpha and bias; no activation, C, gating, batches or groups.  The tile, cluster
  * and stage settings of the config do not apply (the kernel picks its own).  It is launched as a
  * programmatic dependent of the stream's previous kernel (environment CPG_DECODE_PDL=0 at plan
@@ -165,7 +175,8 @@ typedef struct cpg_gemm_problem {
 /* Per-call epilogue options:
  *   D = act(alpha * s_a * s_b * (A . B^T) + bias + beta * C), rounded to D's type.
  * alpha scales the fp32 accumulator; scale_a / scale_b (optional device pointers to one fp32
- * value each) are the per-tensor dequantisation scales of FP8 operands; bias (optional device
+ * value each) are the per-tensor dequantisation scales of FP8 or INT8 operands, or vectors as the
+ * plan's scale_mode says; bias (optional device
  * pointer, BF16, length N) is added per column; source (optional device pointer to C, same type
  * and M x N shape as D, row stride ld_source elements, 16-byte aligned rows; it may be D itself)
  * is added times beta; activation is one of CPG_ACT_*.  The reference has none of these
@@ -285,6 +296,85 @@ int cpg_max_active_clusters(int32_t cluster_size, int32_t* out);
 int cpg_quantize_e4m3(const void* x, int32_t dtype_x, int64_t rows, int64_t cols, int64_t ldx,
                       void* q, int64_t ldq, float* scales, int32_t block_rows, int32_t block_cols,
                       void* stream);
+
+/* INT8 quantisation of x [rows, cols] (BF16 or FP32, row stride ldx) into q (row stride ldq), one
+ * scale per row (the scale of a token, or of an output channel of a weight):
+ * scales[r] = max(max|x[r]|, 1e-12) / 127 in fp32, q = x / scales[r] (fp32 quotient) rounded to
+ * the nearest integer, ties to even.  A row that holds an infinity or a NaN gets q = 0 and the
+ * scale NaN, so every product of it is NaN.  Produces the INT8 operands of the GEMM. */
+int cpg_quantize_int8(const void* x, int32_t dtype_x, int64_t rows, int64_t cols, int64_t ldx,
+                      void* q, int64_t ldq, float* scales, void* stream);
+
+/* ---- Around the experts' products (grouped GEMM) -------------------------------------------
+ * cpg_route chooses k experts per token and their weights; cpg_expert_order gives the group offsets
+ * of cpg_gemm_run_grouped and the row of every (token, choice); cpg_dispatch_rows copies (or
+ * quantises) token rows into that order; cpg_combine_rows adds the experts' output rows back.
+ * All are stream-ordered, run on the current device, keep no state and never synchronise; ids,
+ * weights, slots and their gradients are contiguous [tokens][k].  The reference has no such
+ * operators. */
+#define CPG_ROUTE_MAX_EXPERTS 1024
+#define CPG_ROUTE_MAX_K 32
+#define CPG_ROUTE_MAX_GROUPS 32
+#define CPG_ROUTE_SOFTMAX 0
+#define CPG_ROUTE_SIGMOID 1
+#define CPG_GROUP_MAX 0  /* a group counts as its best expert */
+#define CPG_GROUP_TOP2 1 /* ... as the sum of its two best (its one, if only one can be chosen) */
+
+typedef struct cpg_route_config {
+  int32_t experts;     /* 1..CPG_ROUTE_MAX_EXPERTS */
+  int32_t k;           /* choices per token, 1..min(experts, CPG_ROUTE_MAX_K) */
+  int32_t scoring;     /* CPG_ROUTE_SOFTMAX (over all experts) or CPG_ROUTE_SIGMOID */
+  int32_t groups;      /* groups of experts / groups consecutive experts; 1: none */
+  int32_t kept_groups; /* experts are chosen from the best kept_groups groups */
+  int32_t group_score; /* CPG_GROUP_MAX or CPG_GROUP_TOP2 */
+  int32_t renormalize; /* nonzero: the weights of a token are divided by their sum */
+  float scale;         /* factor of every weight */
+} cpg_route_config;
+
+/* s = scoring(logits), c = s + bias (bias optional, FP32 [experts]; it ranks and does not enter
+ * the weights), ids = the k largest c of the kept groups in falling order, ties to the lowest
+ * index; weights = scale * s[ids] (/ sum of s[ids]).  c is ranked in 64 bits; without a bias (and
+ * with CPG_GROUP_MAX) the logits themselves rank.  A logit of -inf (a masked expert) or a c of
+ * -inf or NaN is never chosen; where fewer than k can be chosen the last ids are -1 with weight 0.
+ * A NaN logit, and under the softmax +inf, is not chosen either and makes the token's weights
+ * NaN.  logits [tokens, experts] BF16 or FP32 with row stride ld. */
+int cpg_route(const cpg_route_config* cfg, const void* logits, int32_t dtype, int64_t tokens,
+              int64_t ld, const float* bias, int32_t* ids, float* weights, void* stream);
+
+/* dlogits (logits' type, row stride ldd, every entry written) from dweights, with the experts
+ * fixed at ids (entries outside [0, experts) take no part; an expert given twice counts twice).
+ * groups, kept_groups and group_score are checked and not used.  A row that cpg_route would give
+ * NaN weights gets a NaN gradient. */
+int cpg_route_backward(const cpg_route_config* cfg, const float* dweights, const void* logits,
+                       int32_t dtype, int64_t tokens, int64_t ld, const int32_t* ids,
+                       void* dlogits, int64_t ldd, void* stream);
+
+/* Rows in expert order: offsets[0..experts] (device int32, offsets[0] = 0) and, for every pair, its
+ * row slots[t * k + j] = offsets[id] + the number of pairs of that expert before it; -1 for ids
+ * outside [0, experts).  The same order in every run. */
+int cpg_expert_order(const int32_t* ids, int64_t tokens, int32_t k, int32_t experts,
+                     int32_t* offsets, int32_t* slots, void* stream);
+
+/* rows[slots[t * k + j]] = x[t] for every token and choice whose slot is within [0, num_rows)
+ * (no two may be equal); other rows are left as they were.  dtype_rows is x's type, or CPG_DTYPE_I8:
+ * rows and scales[slot] are then the token's cpg_quantize_int8. */
+int cpg_dispatch_rows(const void* x, int32_t dtype_x, int64_t tokens, int64_t cols, int64_t ldx,
+                      const int32_t* slots, int32_t k, void* rows, int32_t dtype_rows,
+                      int64_t num_rows, int64_t ldr, float* scales, void* stream);
+
+/* y[t] = source[t] + sum over j of weights[t * k + j] * rows[slots[t * k + j]], summed in fp32 in
+ * the order of j and rounded once; slots outside [0, num_rows) are not read and add nothing;
+ * weights NULL: ones (the gradient of cpg_dispatch_rows); source optional (it may be y). */
+int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
+                     const int32_t* slots, const float* weights, int64_t tokens, int32_t k,
+                     const void* source, int64_t ld_source, void* y, int64_t ldy, void* stream);
+
+/* drows[slot] = weights * dy[t] and dweights = <dy[t], rows[slot]> (0 for slots outside
+ * [0, num_rows)); rows of drows that no slot names are left as they were. */
+int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int64_t cols,
+                              int64_t lddy, const void* rows, int64_t num_rows, int64_t ldr,
+                              const int32_t* slots, const float* weights, int32_t k, void* drows,
+                              int64_t lddr, float* dweights, void* stream);
 
 /* y = bf16(x + bias) for x FP32 [rows, cols]: the last step of split-K after the reduction.
  * bias is optional (BF16, length cols). */
