@@ -49,8 +49,60 @@ int check_pairs(int64_t tokens, int32_t k) {
   return CPG_OK;
 }
 
+// Rows that start on 16 bytes (the vector kernels, whose column arithmetic is 32-bit).
+bool vector_rows(const void* p, int64_t cols, int64_t ld, int elem) {
+  return !misaligned(p, 16) && (ld * elem) % 16 == 0 && cols < (int64_t(1) << 30);
+}
+
+template <typename T>
+void launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
+  // A warp per row up to 64 registers of packed row a lane, then a block per row.
+  constexpr int kWarpVecs = sizeof(T) == 2 ? 8 : 4;
+  const int64_t units = (p.cols + 15) / 16;
+  if (units <= 32 * kWarpVecs)
+    cpg::rows_int8_vec_kernel<T, 32, kWarpVecs, true>
+        <<<row_grid((p.tokens + 7) / 8), 256, 0, st>>>(p);
+  else if (units <= 512)
+    cpg::rows_int8_vec_kernel<T, 256, 2, true><<<row_grid(p.tokens), 256, 0, st>>>(p);
+  else if (units <= 1024)
+    cpg::rows_int8_vec_kernel<T, 256, 4, true><<<row_grid(p.tokens), 256, 0, st>>>(p);
+  else
+    cpg::rows_int8_vec_kernel<T, 256, 4, false><<<row_grid(p.tokens), 256, 0, st>>>(p);
+}
+
+// Warps of work and blocks of 8 warps for rows cut into chunks of `vecs` vectors a lane.
+template <typename T>
+int32_t row_chunks(int64_t cols, int vecs) {
+  const int64_t per = int64_t(32) * vecs * cpg::RowVec<T>::kElems;
+  return static_cast<int32_t>((cols + per - 1) / per);
+}
+unsigned warp_grid(int64_t warps) { return row_grid((warps + 7) / 8); }
+
+template <typename T>
+void launch_copy_vec(const cpg::RowsParams& p, cudaStream_t st) {
+  const int32_t chunks = row_chunks<T>(p.cols, cpg::kCopyVecs);
+  cpg::rows_copy_vec_kernel<T><<<warp_grid(p.tokens * chunks), 256, 0, st>>>(p, chunks);
+}
+
+template <typename T>
+void launch_combine_vec(const cpg::CombineParams& p, cudaStream_t st) {
+  const int32_t chunks = row_chunks<T>(p.cols, cpg::kCombineVecs);
+  cpg::combine_vec_kernel<T><<<warp_grid(p.tokens * chunks), 256, 0, st>>>(p, chunks);
+}
+
 int launch_rows(const cpg::RowsParams& p, int32_t dtype_x, bool int8, cudaStream_t st) {
   const unsigned grid = row_grid(p.tokens);
+  if (vector_rows(p.x, p.cols, p.ldx, bytes_of(dtype_x)) &&
+      vector_rows(p.rows, p.cols, p.ldr, int8 ? 1 : bytes_of(dtype_x))) {
+    if (dtype_x == CPG_DTYPE_BF16) {
+      if (int8) launch_int8_vec<__nv_bfloat16>(p, st);
+      else launch_copy_vec<__nv_bfloat16>(p, st);
+    } else {
+      if (int8) launch_int8_vec<float>(p, st);
+      else launch_copy_vec<float>(p, st);
+    }
+    return launched("row kernel launch");
+  }
   if (dtype_x == CPG_DTYPE_BF16) {
     if (int8)
       cpg::rows_kernel<__nv_bfloat16, int8_t><<<grid, 256, 0, st>>>(p);
@@ -272,6 +324,12 @@ int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t 
   const cpg::CombineParams p{rows,   num_rows, cols,   ldr,       slots, weights,
                              tokens, k,        source, ld_source, y,     ldy};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (vector_rows(rows, cols, ldr, es) && vector_rows(y, cols, ldy, es) &&
+      (source == nullptr || vector_rows(source, cols, ld_source, es))) {
+    if (dtype == CPG_DTYPE_BF16) launch_combine_vec<__nv_bfloat16>(p, st);
+    else launch_combine_vec<float>(p, st);
+    return launched("combine kernel launch");
+  }
   if (dtype == CPG_DTYPE_BF16)
     cpg::combine_kernel<__nv_bfloat16><<<row_grid(tokens), 256, 0, st>>>(p);
   else
@@ -302,7 +360,12 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
   const cpg::CombineGradParams p{dy,    tokens,  cols, lddy,  rows, num_rows, ldr,
                                  slots, weights, k,    drows, lddr, dweights};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = row_grid((tokens * k + 7) / 8);
+  const unsigned grid = warp_grid(tokens * k);
+  if (vector_rows(dy, cols, lddy, es) && vector_rows(rows, cols, ldr, es) && vector_rows(drows, cols, lddr, es)) {
+    if (dtype == CPG_DTYPE_BF16) cpg::combine_grad_vec_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+    else cpg::combine_grad_vec_kernel<float><<<grid, 256, 0, st>>>(p);
+    return launched("combine gradient kernel launch");
+  }
   if (dtype == CPG_DTYPE_BF16)
     cpg::combine_grad_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
   else

@@ -70,6 +70,120 @@ __device__ __forceinline__ uint32_t int8_quotient(float x, float s) {
   return s == s ? static_cast<uint32_t>(__float2int_rn(__fdiv_rn(x, s))) & 0xffu : 0u;
 }
 
+// ---------------------------------------------------------------- rows of whole vectors
+// The vector kernels need rows that start on 16 bytes (input and output) and fewer than 2^30
+// columns; the last vector of a row may be partial.  Loads bypass L1 (every row is read once).
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// The first n elements (any n) at p as a vector, zeros after them.
+template <typename T>
+__device__ __forceinline__ uint4 ld_tail_v4(const T* p, int32_t n) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) w[j >> 1] |= static_cast<uint32_t>(__bfloat16_as_ushort(p[j])) << (16 * (j & 1));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) w[j] = __float_as_uint(p[j]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Elements [c, c + kElems) of a row of `cols` elements, zeros past its end.
+template <typename T>
+__device__ __forceinline__ uint4 ld_row_vec(const T* row, int32_t c, int32_t cols) {
+  if (c + RowVec<T>::kElems <= cols) return ld_stream_v4(row + c);
+  return ld_tail_v4(row + c, cols - c);
+}
+
+template <typename T>
+__device__ __forceinline__ void st_row_vec(T* row, int32_t c, int32_t cols, const uint4& v) {
+  if (c + RowVec<T>::kElems <= cols) {
+    ptx::st_global_v4(row + c, v.x, v.y, v.z, v.w);
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < RowVec<T>::kElems; ++j) {
+    if (c + j < cols) {
+      if constexpr (sizeof(T) == 2)
+        row[c + j] = __ushort_as_bfloat16(static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))));
+      else
+        row[c + j] = __uint_as_float(w[j]);
+    }
+  }
+}
+
+// Bits of the largest |value| of a vector, given the largest so far.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max_vec(const uint4& v, uint32_t m) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      m = max(m, (w[i] << 16) & 0x7fffffffu);
+      m = max(m, w[i] & 0x7fff0000u);
+    } else {
+      m = max(m, w[i] & 0x7fffffffu);
+    }
+  }
+  return m;
+}
+
+// Four quotients x / s rounded to integers, as the bytes of a word, without a division per
+// element.  With y = RN(1 / s), q = RN(x y) is within 127 * 1.5 * 2^-23 < 2.3e-5 of x / s, and the
+// fp32 quotient within 127 * 2^-24 < 7.6e-6 of it; so where q is farther than 4e-5 from a
+// half-integer both round to the same integer, and elsewhere the word takes the division.
+// Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte.
+__device__ __forceinline__ uint32_t int8_word(const float* x, float s, float y) {
+  constexpr float kRound = 12582912.f;
+  uint32_t b[4];
+  bool risky = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float q = __fmul_rn(x[i], y);
+    const float r = __fadd_rn(q, kRound);
+    risky |= fabsf(q - __fsub_rn(r, kRound)) > 0.5f - 4e-5f;
+    b[i] = __float_as_uint(r);
+  }
+  if (risky) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = int8_quotient(x[i], s);
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// Sixteen consecutive elements as INT8 (rows of a NaN scale: zeros).
+template <typename T>
+__device__ __forceinline__ uint4 int8_vec(const uint4* raw, float s, float y) {
+  constexpr int kVecs = 16 / RowVec<T>::kElems;
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) RowVec<T>::unpack(raw[i], f + i * RowVec<T>::kElems);
+  if (s != s) return make_uint4(0u, 0u, 0u, 0u);
+  return make_uint4(int8_word(f, s, y), int8_word(f + 4, s, y), int8_word(f + 8, s, y),
+                    int8_word(f + 12, s, y));
+}
+
+__device__ __forceinline__ void st_int8_vec(int8_t* row, int32_t c, int32_t cols, const uint4& v) {
+  if (c + 16 <= cols) {
+    ptx::st_global_v4(row + c, v.x, v.y, v.z, v.w);
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (c + j < cols) row[c + j] = static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3)));
+}
+
 struct RowsParams {
   const void* x;
   int64_t tokens, cols, ldx;
@@ -116,6 +230,117 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
   }
 }
 
+// Quantised rows of whole vectors: G threads per token (a warp, or the block) hold the row packed
+// in registers, NV times 16 elements each, between its maximum and the quantisation, so the row is
+// read once however many copies of it are written.  Longer rows (Resident false) are read a second
+// time, from L2.
+template <typename T, int G, int NV, bool Resident>
+__global__ void __launch_bounds__(256, 2) rows_int8_vec_kernel(const RowsParams p) {
+  constexpr int kVecs = 16 / RowVec<T>::kElems;
+  constexpr int kE = RowVec<T>::kElems;
+  constexpr int kRowsPerBlock = 256 / G;
+  constexpr int kPass = G * NV * 16;  // elements per pass over a row
+  __shared__ uint32_t red[2][8];
+  const int lane = threadIdx.x & 31;
+  const int li = threadIdx.x % G;
+  const int32_t cols = static_cast<int32_t>(p.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRowsPerBlock;
+  int parity = 0;
+  for (int64_t t = blockIdx.x * static_cast<int64_t>(kRowsPerBlock) + threadIdx.x / G;
+       t < p.tokens; t += step) {
+    const T* x = static_cast<const T*>(p.x) + t * p.ldx;
+    uint4 raw[NV][kVecs];
+    auto load = [&](int32_t c0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int32_t c = c0 + (i * G + li) * 16;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          raw[i][v] = make_uint4(0u, 0u, 0u, 0u);
+          if (c + v * kE < cols) raw[i][v] = ld_row_vec(x, c + v * kE, cols);
+        }
+      }
+    };
+    uint32_t m = 0u;
+    for (int32_t c0 = 0; c0 < cols; c0 += kPass) {
+      load(c0);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) m = abs_max_vec<T>(raw[i][v], m);
+      if constexpr (Resident) break;
+    }
+    // Slots of this token: lane j of every warp holds choice j.
+    int32_t my_slot = -1;
+    if (lane < p.k) my_slot = p.slots != nullptr ? p.slots[t * p.k + lane] : static_cast<int32_t>(t);
+    if (my_slot >= p.num_rows) my_slot = -1;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (G > 32) {
+      // The parity keeps the next row's writes off the words a slow warp still reads.
+      if (lane == 0) red[parity][threadIdx.x >> 5] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = max(m, red[parity][w]);
+      parity ^= 1;
+    }
+    const float s = int8_scale(m);
+    const float y = __frcp_rn(s);
+    for (int32_t c0 = 0; c0 < cols; c0 += kPass) {
+      if constexpr (!Resident) load(c0);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) raw[i][0] = int8_vec<T>(raw[i], s, y);
+      for (int32_t j = 0; j < p.k; ++j) {
+        const int32_t slot = __shfl_sync(0xffffffffu, my_slot, j);
+        if (slot < 0) continue;
+        int8_t* out = static_cast<int8_t*>(p.rows) + slot * p.ldr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int32_t c = c0 + (i * G + li) * 16;
+          if (c < cols) st_int8_vec(out, c, cols, raw[i][0]);
+        }
+      }
+      if constexpr (Resident) break;
+    }
+    if (li < p.k && my_slot >= 0) p.scales[my_slot] = s;
+  }
+}
+
+// Copied rows of whole vectors: a warp takes 32 * kCopyVecs vectors of one token and writes them
+// k times.
+constexpr int kCopyVecs = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256) rows_copy_vec_kernel(const RowsParams p, int32_t chunks) {
+  constexpr int kE = RowVec<T>::kElems;
+  const int lane = threadIdx.x & 31;
+  const int32_t cols = static_cast<int32_t>(p.cols);
+  const int64_t units = p.tokens * chunks;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+  for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < units; u += step) {
+    const int64_t t = u / chunks;
+    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kCopyVecs + lane) * kE;
+    int64_t my_slot = -1;
+    if (lane < p.k) my_slot = p.slots[t * p.k + lane];
+    const T* x = static_cast<const T*>(p.x) + t * p.ldx;
+    uint4 raw[kCopyVecs];
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i) {
+      const int32_t c = c0 + i * 32 * kE;
+      if (c < cols) raw[i] = ld_row_vec(x, c, cols);
+    }
+    for (int32_t j = 0; j < p.k; ++j) {
+      const int64_t slot = __shfl_sync(0xffffffffu, my_slot, j);
+      if (slot < 0 || slot >= p.num_rows) continue;
+      T* out = static_cast<T*>(p.rows) + slot * p.ldr;
+#pragma unroll
+      for (int i = 0; i < kCopyVecs; ++i) {
+        const int32_t c = c0 + i * 32 * kE;
+        if (c < cols) st_row_vec(out, c, cols, raw[i]);
+      }
+    }
+  }
+}
+
 struct CombineParams {
   const void* rows;
   int64_t num_rows, cols, ldr;
@@ -144,6 +369,79 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
         acc = fmaf(w, RowVec<T>::load(static_cast<const T*>(p.rows) + slot * p.ldr + c), acc);
       }
       RowVec<T>::store(static_cast<T*>(p.y) + t * p.ldy + c, acc);
+    }
+  }
+}
+
+// As combine_kernel for rows of whole vectors: a warp takes 32 * kCombineVecs vectors of one token
+// and keeps the loads of four choices in flight.  Every output element sums its choices in the
+// same order as combine_kernel.
+constexpr int kCombineVecs = 2;
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p, int32_t chunks) {
+  constexpr int kE = RowVec<T>::kElems;
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 31;
+  const int32_t cols = static_cast<int32_t>(p.cols);
+  const int64_t units = p.tokens * chunks;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+  for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < units; u += step) {
+    const int64_t t = u / chunks;
+    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kCombineVecs + lane) * kE;
+    int64_t my_slot = -1;
+    float my_w = 1.f;
+    if (lane < p.k) {
+      my_slot = p.slots[t * p.k + lane];
+      if (p.weights != nullptr) my_w = p.weights[t * p.k + lane];
+    }
+    if (my_slot >= p.num_rows) my_slot = -1;
+    float acc[kCombineVecs][kE];
+#pragma unroll
+    for (int i = 0; i < kCombineVecs; ++i) {
+      const int32_t c = c0 + i * 32 * kE;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (p.source != nullptr && c < cols) {
+        // The source may be y itself, so it is not a read-only load.
+        const T* src = static_cast<const T*>(p.source) + t * p.lds + c;
+        v = c + kE <= cols ? *reinterpret_cast<const uint4*>(src)
+                             : ld_tail_v4(src, cols - c);
+      }
+      RowVec<T>::unpack(v, acc[i]);
+    }
+    for (int32_t j0 = 0; j0 < p.k; j0 += kBatch) {
+      uint4 raw[kBatch][kCombineVecs];
+      int64_t slot[kBatch];
+      float w[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        // Lanes past k hold slot -1.
+        slot[b] = __shfl_sync(0xffffffffu, my_slot, (j0 + b) & 31);
+        w[b] = __shfl_sync(0xffffffffu, my_w, (j0 + b) & 31);
+        const T* row = static_cast<const T*>(p.rows) + slot[b] * p.ldr;
+#pragma unroll
+        for (int i = 0; i < kCombineVecs; ++i) {
+          const int32_t c = c0 + i * 32 * kE;
+          if (slot[b] >= 0 && c < cols) raw[b][i] = ld_row_vec(row, c, cols);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (slot[b] < 0) continue;
+#pragma unroll
+        for (int i = 0; i < kCombineVecs; ++i) {
+          float f[kE];
+          RowVec<T>::unpack(raw[b][i], f);
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[i][e] = fmaf(w[b], f[e], acc[i][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCombineVecs; ++i) {
+      const int32_t c = c0 + i * 32 * kE;
+      if (c < cols)
+        st_row_vec(static_cast<T*>(p.y) + t * p.ldy, c, cols, RowVec<T>::pack(acc[i]));
     }
   }
 }
@@ -185,6 +483,55 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineGradPara
       for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     }
     if (lane == 0) p.dweights[i] = dot;
+  }
+}
+
+// As combine_grad_kernel for rows of whole vectors, four vectors of dy and of the row in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_grad_vec_kernel(const CombineGradParams p) {
+  constexpr int kE = RowVec<T>::kElems;
+  constexpr int kVecs = 4;
+  const int lane = threadIdx.x & 31;
+  const int32_t cols = static_cast<int32_t>(p.cols);
+  const int64_t pairs = p.tokens * p.k;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+  for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < pairs; u += step) {
+    const int64_t slot = p.slots[u];
+    float dot = 0.f;
+    if (slot >= 0 && slot < p.num_rows) {
+      const float w = p.weights[u];
+      const T* dy = static_cast<const T*>(p.dy) + (u / p.k) * p.lddy;
+      const T* row = static_cast<const T*>(p.rows) + slot * p.ldr;
+      T* out = static_cast<T*>(p.drows) + slot * p.lddr;
+      for (int32_t c0 = lane * kE; c0 < cols; c0 += 32 * kE * kVecs) {
+        uint4 g[kVecs], r[kVecs];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const int32_t c = c0 + i * 32 * kE;
+          g[i] = r[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (c < cols) {
+            g[i] = ld_row_vec(dy, c, cols);
+            r[i] = ld_row_vec(row, c, cols);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const int32_t c = c0 + i * 32 * kE;
+          float gf[kE], rf[kE];
+          RowVec<T>::unpack(g[i], gf);
+          RowVec<T>::unpack(r[i], rf);
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            dot = fmaf(gf[e], rf[e], dot);
+            gf[e] *= w;
+          }
+          if (c < cols) st_row_vec(out, c, cols, RowVec<T>::pack(gf));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    }
+    if (lane == 0) p.dweights[u] = dot;
   }
 }
 
