@@ -14,6 +14,7 @@ using cpg_capi::fail;
 
 namespace {
 
+constexpr int64_t kFewThreads = 148 * 1024;  // half of the threads that fit on the SMs
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;  // rows and pairs are counted in int32
 
 int launched(const char* what) {
@@ -54,20 +55,25 @@ bool vector_rows(const void* p, int64_t cols, int64_t ld, int elem) {
   return !misaligned(p, 16) && (ld * elem) % 16 == 0 && cols < (int64_t(1) << 30);
 }
 
+template <typename T, int G, bool Resident>
+void launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
+  constexpr int kRows = 256 / G;
+  cpg::rows_int8_vec_kernel<T, G, Resident>
+      <<<row_grid((p.tokens + kRows - 1) / kRows), 256, 0, st>>>(p);
+}
+
 template <typename T>
 void launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
-  // A warp per row up to 64 registers of packed row a lane, then a block per row.
-  constexpr int kWarpVecs = sizeof(T) == 2 ? 8 : 4;
-  const int64_t units = (p.cols + 15) / 16;
-  if (units <= 32 * kWarpVecs)
-    cpg::rows_int8_vec_kernel<T, 32, kWarpVecs, true>
-        <<<row_grid((p.tokens + 7) / 8), 256, 0, st>>>(p);
-  else if (units <= 512)
-    cpg::rows_int8_vec_kernel<T, 256, 2, true><<<row_grid(p.tokens), 256, 0, st>>>(p);
-  else if (units <= 1024)
-    cpg::rows_int8_vec_kernel<T, 256, 4, true><<<row_grid(p.tokens), 256, 0, st>>>(p);
-  else
-    cpg::rows_int8_vec_kernel<T, 256, 4, false><<<row_grid(p.tokens), 256, 0, st>>>(p);
+  // The fewest threads that hold a row; more while the tokens leave most of the GPU idle (each
+  // then has less of a row to wait for).
+  int threads = 32;
+  while (threads < 256 && p.cols > int64_t(threads) * cpg::kInt8Vecs * 16) threads *= 2;
+  while (threads < 256 && p.tokens * threads < kFewThreads && p.cols > threads * 16) threads *= 2;
+  if (p.cols > int64_t(256) * cpg::kInt8Vecs * 16) launch_int8_vec<T, 256, false>(p, st);
+  else if (threads == 256) launch_int8_vec<T, 256, true>(p, st);
+  else if (threads == 128) launch_int8_vec<T, 128, true>(p, st);
+  else if (threads == 64) launch_int8_vec<T, 64, true>(p, st);
+  else launch_int8_vec<T, 32, true>(p, st);
 }
 
 // Warps of work and blocks of 8 warps for rows cut into chunks of `vecs` vectors a lane.
@@ -150,6 +156,15 @@ void by_lane_values(int32_t experts, F&& f) {
   else f(std::integral_constant<int, 32>{});
 }
 
+// Whether every lane's run of V elements of every row starts on its vectors.
+template <int V>
+int32_t run_vectors(const void* p, int64_t ld, int32_t dtype) {
+  const int es = bytes_of(dtype);
+  const int bytes = dtype == CPG_DTYPE_BF16 ? cpg::run_vector_bytes<__nv_bfloat16, V>()
+                                            : cpg::run_vector_bytes<float, V>();
+  return !misaligned(p, bytes) && (ld * es) % bytes == 0 ? 1 : 0;
+}
+
 unsigned route_grid(int64_t tokens) {
   return static_cast<unsigned>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps);
 }
@@ -194,13 +209,14 @@ int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int6
   if (misaligned(logits, bytes_of(dtype)) || misaligned(bias, 4) || misaligned(ids, 4) ||
       misaligned(weights, 4))
     return fail(CPG_ERR_ALIGNMENT, "logits, bias, ids and weights must be aligned to their elements");
-  const cpg::RouteParams p{logits,    tokens,  ld,        bias,           ids,
-                           weights,   c->experts, c->k,   c->scoring,     c->groups,
-                           c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, c->scale};
+  cpg::RouteParams p{logits,         tokens,         ld,         bias,      ids,
+                     weights,        c->experts,     c->k,       c->scoring, c->groups,
+                     c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, 0, c->scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_lane_values(c->experts, [&](auto v) {
     constexpr int V = decltype(v)::value;
     const size_t smem = c->groups > 1 ? sizeof(double) * 32 * V * cpg::kRouteWarps : 0;
+    p.vec = run_vectors<V>(logits, ld, dtype);
     if (dtype == CPG_DTYPE_BF16)
       cpg::route_kernel<__nv_bfloat16, V>
           <<<route_grid(tokens), 32 * cpg::kRouteWarps, smem, st>>>(p);
@@ -226,12 +242,14 @@ int cpg_route_backward(const cpg_route_config* c, const float* dweights, const v
       misaligned(dweights, 4) || misaligned(ids, 4))
     return fail(CPG_ERR_ALIGNMENT,
                 "dweights, logits, ids and dlogits must be aligned to their elements");
-  const cpg::RouteGradParams p{dweights, logits,     tokens, ld,         ids,
-                               dlogits,  ldd,        c->experts, c->k,   c->scoring,
-                               c->renormalize != 0 ? 1 : 0, c->scale};
+  cpg::RouteGradParams p{dweights, logits, tokens,     ld,   ids,
+                         dlogits,  ldd,    c->experts, c->k, c->scoring,
+                         c->renormalize != 0 ? 1 : 0, 0, 0, c->scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_lane_values(c->experts, [&](auto v) {
     constexpr int V = decltype(v)::value;
+    p.vec = run_vectors<V>(logits, ld, dtype);
+    p.vec_out = run_vectors<V>(dlogits, ldd, dtype);
     if (dtype == CPG_DTYPE_BF16)
       cpg::route_grad_kernel<__nv_bfloat16, V>
           <<<route_grid(tokens), 32 * cpg::kRouteWarps, 0, st>>>(p);

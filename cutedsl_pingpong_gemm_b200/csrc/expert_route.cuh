@@ -4,9 +4,10 @@
 //   s = softmax(l) or sigmoid(l);  c = s + bias (what is ranked);  ids = the k largest c among the
 //   kept groups, ties to the lowest index;  w = scale * s[ids], over the sum of s[ids] if renormalised.
 //
-// c is ranked in 64 bits: two 32-bit scores may round to one value, or to the wrong order, where
-// their logits do not.  Without a bias and with group score "max" c is not formed: s grows with l,
-// so the logits rank, exactly.
+// c is ranked as its 64-bit value: two 32-bit scores may round to one value, or to the wrong order,
+// where their logits do not.  Without a bias and with group score "max" c is not formed: s grows
+// with l, so the logits rank, exactly.  Otherwise a row is ranked in 32 bits with a bound on their
+// error, and again in 64 bits if two candidates that matter are nearer than the bound allows.
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -30,6 +31,7 @@ struct RouteParams {
   int32_t* ids;       // [tokens][k]
   float* weights;     // [tokens][k]
   int32_t experts, k, scoring, groups, kept_groups, group_score, renormalize;
+  int32_t vec;  // a lane's run of logits may be read by vectors (run_vectors)
   float scale;
 };
 
@@ -42,10 +44,86 @@ __device__ __forceinline__ void route_store(__nv_bfloat16* p, float v) {
   *p = __float2bfloat16_rn(v);
 }
 
+// A lane's run of V consecutive logits: bytes of one vector access to it (at most 16).
+template <typename T, int V>
+__host__ __device__ constexpr int run_vector_bytes() {
+  return V * static_cast<int>(sizeof(T)) < 16 ? V * static_cast<int>(sizeof(T)) : 16;
+}
+
+// l[i] = row[e0 + i] for those below `experts`, -inf after them.
+template <typename T, int V>
+__device__ __forceinline__ void load_run(const T* row, int e0, int experts, bool vec,
+                                         float (&l)[V]) {
+  constexpr int kBytes = run_vector_bytes<T, V>();
+  if (kBytes >= 4 && vec && e0 + V <= experts) {
+    constexpr int kWords = V * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords > 0 ? kWords : 1];
+    if constexpr (kBytes == 16) {
+#pragma unroll
+      for (int q = 0; q < kWords / 4; ++q) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + e0 + q * (16 / sizeof(T)));
+        w[4 * q] = v.x;
+        w[4 * q + 1] = v.y;
+        w[4 * q + 2] = v.z;
+        w[4 * q + 3] = v.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(row + e0);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(row + e0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4)
+        l[i] = __uint_as_float(w[i]);
+      else
+        l[i] = __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) l[i] = e0 + i < experts ? route_load(row + e0 + i) : -INFINITY;
+}
+
+// row[e0 + i] = v[i] for those below `experts`.
+template <typename T, int V>
+__device__ __forceinline__ void store_run(T* row, int e0, int experts, bool vec,
+                                          const float (&v)[V]) {
+  constexpr int kBytes = run_vector_bytes<T, V>();
+  if (kBytes >= 4 && vec && e0 + V <= experts) {
+    constexpr int kWords = V * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords > 0 ? kWords : 1];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4)
+        w[i] = __float_as_uint(v[i]);
+      else
+        w[i] = ptx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    }
+    if constexpr (kBytes == 16) {
+#pragma unroll
+      for (int q = 0; q < kWords / 4; ++q)
+        *reinterpret_cast<uint4*>(row + e0 + q * (16 / sizeof(T))) =
+            make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(row + e0) = make_uint2(w[0], w[1]);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(row + e0) = w[0];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e0 + i < experts) route_store(row + e0 + i, v[i]);
+}
+
 __device__ __forceinline__ double neg_inf() { return __longlong_as_double(0xfff0000000000000ll); }
 __device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fc00000u); }
 
-__device__ __forceinline__ double warp_sum(double v) {
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -56,156 +134,331 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
+// Unsigned keys that order like the floats (no NaN; -0 as +0).  Every key of a number above -inf
+// exceeds kNoKey.
+constexpr uint32_t kNoKey = 0u;
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ float warp_max(float v) {
+  return key_value(__reduce_max_sync(0xffffffffu, order_key(v)));
+}
+
 __device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
+__device__ __forceinline__ float sigmoid32(float l) { return 1.f / (1.f + expf(-l)); }
 
 // A logit that cannot be chosen and spoils its row's weights: NaN, and +inf under the softmax.
 __device__ __forceinline__ bool route_bad(float l, int32_t scoring) {
   return l != l || (scoring == kRouteSoftmax && l == __uint_as_float(0x7f800000u));
 }
 
-// Weights of the chosen experts: lane j holds choice j's logit and (softmax over all experts) its
-// probability.  Renormalised softmax weights are the softmax of the chosen logits alone;
-// renormalised sigmoid weights of logits all below -60, where sigmoid(l) = e^l, likewise (the
-// sum of the scores would underflow).  Lanes without a choice get 0.
-__device__ __forceinline__ double route_part(int32_t scoring, int32_t renormalize, bool has,
-                                             double l, double p) {
-  if (!renormalize) return has ? (scoring == kRouteSoftmax ? p : sigmoid64(l)) : 0.0;
-  const double top = warp_max(has ? l : neg_inf());
-  double v;
-  if (scoring == kRouteSoftmax || top < -60.0)
-    v = has ? exp(l - top) : 0.0;
-  else
-    v = has ? sigmoid64(l) : 0.0;
-  const double sum = warp_sum(v);
-  return sum > 0.0 ? v / sum : 0.0;
+// Shares of the chosen experts: lane j holds choice j's logit and (softmax over all experts) its
+// probability.  Renormalised softmax shares are the softmax of the chosen logits alone;
+// renormalised sigmoid shares of logits all below -60, where sigmoid(l) = e^l, likewise (the sum
+// of the scores would underflow).  Lanes without a choice get 0.
+__device__ __forceinline__ float route_share(int32_t scoring, int32_t renormalize, bool has, float l,
+                                             float prob) {
+  if (!renormalize) return has ? (scoring == kRouteSoftmax ? prob : sigmoid32(l)) : 0.f;
+  const float top = warp_max(has ? l : -INFINITY);
+  float v = 0.f;
+  if (has) v = scoring == kRouteSoftmax || top < -60.f ? expf(l - top) : sigmoid32(l);
+  const float sum = warp_sum(v);
+  return sum > 0.f ? v / sum : 0.f;
+}
+
+// The k best experts of a row with c in 64 bits: lane j returns choice j, or -1.  l holds the
+// lane's run of logits, -inf where an expert cannot be chosen.  c_sh: 32 * V words of the warp's
+// own shared memory (groups > 1).
+template <int V>
+__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (&l)[V],
+                                             double* c_sh) {
+  const int lane = threadIdx.x & 31;
+  double c[V];
+  double top = neg_inf(), sum = 0.0;
+  if (p.scoring == kRouteSoftmax) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = fmax(top, static_cast<double>(l[i]));
+    top = warp_max(top);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    c[i] = 0.0;
+    if (l[i] > -INFINITY)
+      c[i] = p.scoring == kRouteSoftmax ? exp(static_cast<double>(l[i]) - top)
+                                        : sigmoid64(static_cast<double>(l[i]));
+    sum += c[i];
+  }
+  if (p.scoring == kRouteSoftmax) sum = warp_sum(sum);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane * V + i;
+    if (p.scoring == kRouteSoftmax) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
+    if (p.bias != nullptr && e < p.experts) c[i] += static_cast<double>(p.bias[e]);
+    if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = neg_inf();
+  }
+  if (p.groups > 1) {
+    // Lane g scores group g, ranks it among the others and keeps it if fewer than kept_groups are
+    // better (a higher score, or the same and a lower index).
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
+    __syncwarp();
+    const int per = p.experts / p.groups;
+    double a = neg_inf(), b = neg_inf();
+    if (lane < p.groups) {
+      for (int i = 0; i < per; ++i) {
+        const double v = c_sh[lane * per + i];
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
+      }
+      if (p.group_score == kRouteGroupTop2 && b > neg_inf()) a += b;
+    }
+    int better = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double v = __shfl_sync(0xffffffffu, a, g);
+      better += (v > a || (v == a && g < lane)) ? 1 : 0;
+    }
+    const uint32_t keep = __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int g = (lane * V + i) / per;
+      if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = neg_inf();
+    }
+    __syncwarp();
+  }
+  int32_t my_id = -1;
+  for (int j = 0; j < p.k; ++j) {
+    double best = neg_inf();
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (c[i] > best) {
+        best = c[i];
+        at = i;
+      }
+    }
+    const double all = warp_max(best);
+    if (!(all > neg_inf())) break;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
+    const int id = __shfl_sync(0xffffffffu, lane * V + at, owner);
+    if (lane == j) my_id = id;
+    if (lane == owner) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == at) c[i] = neg_inf();
+    }
+  }
+  return my_id;
 }
 
 // One warp per token; lane l holds experts l * V .. l * V + V - 1.
+//
+// Error of the 32-bit scores (ulp bounds of __expf and __fdividef, 2^-23 = one ulp of 1):
+//   sigmoid: e^-l is off by (2 + 1.173 |l|) ulp, which s (1 - s) turns into at most 0.57 ulp of s;
+//            the sum 1 + e^-l and the quotient add 2.5: below 2^-21 altogether.
+//   softmax: p = e^(l - top) inv with inv <= 1 the common factor.  Each exponential is off by at most
+//            (2.9 ulp) inv absolutely; inv by (10.2 + 18.5 + 1) ulp relatively (the terms' errors
+//            weighted by p, whose mean |l - top| is at most ln 1024; 37 additions; the quotient),
+//            which the largest p <= inv carries: below 2^-18 inv altogether.
+// c = s + bias adds half an ulp of c.  Two c nearer than twice the bound are ranked in 64 bits,
+// unless logit and bias are the same: such c are equal, and the lower index goes first.
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   double* c_sh = route_smem + warp * (32 * V);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kRouteWarps;
   const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_score == kRouteGroupMax);
+  const int e0 = lane * V;
   for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
        t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
     float l[V];
+    load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
     bool bad = false;
-    double top = neg_inf();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      l[i] = e < p.experts ? route_load(row + e) : -INFINITY;
       if (route_bad(l[i], p.scoring)) {
         bad = true;
         l[i] = -INFINITY;
       }
-      top = fmax(top, static_cast<double>(l[i]));
     }
     bad = __any_sync(0xffffffffu, bad);
-    top = warp_max(top);
-    double s[V], c[V];
-    double sum = 0.0;
-    const bool scores = !by_logit || (p.scoring == kRouteSoftmax && !p.renormalize);
+    float top = -INFINITY, inv = 1.f;
+    float c[V];
+    if (p.scoring == kRouteSoftmax && (!by_logit || !p.renormalize)) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[i] = 0.0;
-      if (scores && l[i] > -INFINITY)
-        s[i] = p.scoring == kRouteSoftmax ? exp(static_cast<double>(l[i]) - top)
-                                          : sigmoid64(static_cast<double>(l[i]));
-      sum += s[i];
-    }
-    if (scores && p.scoring == kRouteSoftmax) {
+      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+      top = warp_max(top);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[i] = l[i] > -INFINITY ? __expf(l[i] - top) : 0.f;
+        sum += c[i];
+      }
       sum = warp_sum(sum);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
+      inv = sum > 0.f ? 1.f / sum : 0.f;
     }
+    uint32_t key[V];
+    float near = 0.f;  // c nearer than this (plus 2^-21 |c|) may be in another order
+    if (by_logit) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      if (by_logit) {
-        c[i] = static_cast<double>(l[i]);
-      } else {
-        c[i] = s[i] + (p.bias != nullptr && e < p.experts ? static_cast<double>(p.bias[e]) : 0.0);
-        if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = neg_inf();
+      for (int i = 0; i < V; ++i) c[i] = l[i];
+    } else {
+      near = 2.f * (p.scoring == kRouteSoftmax ? 0x1p-18f * inv : 0x1p-21f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = e0 + i;
+        c[i] = p.scoring == kRouteSoftmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-l[i]));
+        if (p.bias != nullptr && e < p.experts) c[i] += __ldg(p.bias + e);
+        if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = -INFINITY;
       }
     }
+    bool close = false;  // the 32-bit order cannot be trusted
     if (p.groups > 1) {
-      // Lane g scores group g, ranks it among the others and keeps it if fewer than kept_groups
-      // are better (a higher score, or the same and a lower index).
-#pragma unroll
-      for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
-      __syncwarp();
       const int per = p.experts / p.groups;
-      double a = neg_inf(), b = neg_inf();
-      if (lane < p.groups) {
-        for (int i = 0; i < per; ++i) {
-          const double v = c_sh[lane * per + i];
-          if (v > a) {
-            b = a;
-            a = v;
-          } else if (v > b) {
-            b = v;
+      const int lanes = per / V;  // lanes of a group, when that is a whole power of two
+      const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
+      float a = -INFINITY, b = -INFINITY;  // the group's two best
+      int group;
+      if (whole) {
+        group = lane / lanes;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          b = fmaxf(b, fminf(a, c[i]));
+          a = fmaxf(a, c[i]);
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+          const float a2 = __shfl_xor_sync(0xffffffffu, a, o);
+          const float b2 = __shfl_xor_sync(0xffffffffu, b, o);
+          b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+          a = fmaxf(a, a2);
+        }
+      } else {
+        group = lane;
+        float* f_sh = reinterpret_cast<float*>(c_sh);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < V; ++i) f_sh[e0 + i] = c[i];
+        __syncwarp();
+        if (lane < p.groups) {
+          for (int i = 0; i < per; ++i) {
+            const float v = f_sh[lane * per + i];
+            b = fmaxf(b, fminf(a, v));
+            a = fmaxf(a, v);
           }
         }
-        if (p.group_score == kRouteGroupTop2 && b > neg_inf()) a += b;
+        __syncwarp();
+      }
+      const bool real = group < p.groups;
+      float slack = near + 0x1p-21f * fabsf(a);
+      if (p.group_score == kRouteGroupTop2 && b > -INFINITY) {
+        slack = 2.f * near + 0x1p-21f * (fabsf(a) + fabsf(b));
+        a += b;
       }
       int better = 0;
       for (int g = 0; g < p.groups; ++g) {
-        const double v = __shfl_sync(0xffffffffu, a, g);
-        better += (v > a || (v == a && g < lane)) ? 1 : 0;
+        const float v = __shfl_sync(0xffffffffu, a, whole ? g * lanes : g);
+        better += (v > a || (v == a && g < group)) ? 1 : 0;
       }
-      const uint32_t keep =
-          __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int g = (lane * V + i) / per;
-        if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = neg_inf();
+      const bool kept = real && better < p.kept_groups;
+      if (!by_logit) {
+        const bool some = real && a > -INFINITY;
+        const uint32_t worst_kept =
+            __reduce_min_sync(0xffffffffu, kept && some ? order_key(a - slack) : 0xffffffffu);
+        const uint32_t best_left =
+            __reduce_max_sync(0xffffffffu, !kept && some ? order_key(a + slack) : kNoKey);
+        close = best_left >= worst_kept;
       }
-      __syncwarp();
-    }
-    // k times: the largest c of the row, the lowest lane (so the lowest index) among equals.
-    int my_id = -1;
-    float my_l = 0.f;
-    double my_s = 0.0;
-    for (int j = 0; j < p.k; ++j) {
-      double best = neg_inf();
-      int at = 0;
-      float lb = 0.f;
-      double sb = 0.0;
+      if (whole) {
+        if (!kept) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (c[i] > best) {
-          best = c[i];
-          at = i;
-          lb = l[i];
-          sb = s[i];
+          for (int i = 0; i < V; ++i) c[i] = -INFINITY;
+        }
+      } else {
+        const uint32_t keep = __ballot_sync(0xffffffffu, kept);
+        int g = e0 / per, left = per - (e0 - g * per);  // group of the next element, its rest
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = -INFINITY;
+          if (--left == 0) {
+            left = per;
+            ++g;
+          }
         }
       }
-      const double all = warp_max(best);
-      if (!(all > neg_inf())) break;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = c[i] > -INFINITY ? order_key(c[i]) : kNoKey;
+    // k times: the largest key of the row, the lowest lane (so the lowest index) among equals.
+    int32_t my_id = -1;
+    uint32_t my_key = kNoKey, last_key = kNoKey;
+    int found = 0;
+    for (; found < p.k; ++found) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i]);
+      const uint32_t all = __reduce_max_sync(0xffffffffu, best);
+      if (all == kNoKey) break;
       const int owner = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
-      const int id = __shfl_sync(0xffffffffu, lane * V + at, owner);
-      const float lw = __shfl_sync(0xffffffffu, lb, owner);
-      const double sw = __shfl_sync(0xffffffffu, sb, owner);
-      if (lane == j) {
-        my_id = id;
-        my_l = lw;
-        my_s = sw;
-      }
+      int at = 0;
+#pragma unroll
+      for (int i = V - 1; i >= 0; --i)
+        if (key[i] == all) at = i;
       if (lane == owner) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (i == at) c[i] = neg_inf();
+          if (i == at) key[i] = kNoKey;
+      }
+      const int id = __shfl_sync(0xffffffffu, e0 + at, owner);
+      if (lane == found) {
+        my_id = id;
+        my_key = all;
+      }
+      last_key = all;
+    }
+    float my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
+    if (!by_logit && !close) {
+      // Neighbours in the order, and the last choice against everything left.
+      const float my_c = key_value(my_key);
+      const float my_b = my_id >= 0 && p.bias != nullptr ? __ldg(p.bias + my_id) : 0.f;
+      const float next_c = __shfl_down_sync(0xffffffffu, my_c, 1);
+      const float next_l = __shfl_down_sync(0xffffffffu, my_l, 1);
+      const float next_b = __shfl_down_sync(0xffffffffu, my_b, 1);
+      close = lane + 1 < found && my_c - next_c <= near + 0x1p-21f * fabsf(my_c) &&
+              !(my_l == next_l && my_b == next_b);
+      if (found == p.k) {
+        const float last_c = key_value(last_key);
+        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
+        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
+        const float limit = last_c - (near + 0x1p-21f * fabsf(last_c));
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (key[i] != kNoKey && c[i] >= limit)
+            close |= !(l[i] == last_l &&
+                       (p.bias == nullptr || __ldg(p.bias + e0 + i) == last_b));
+        }
       }
     }
-    const double w = route_part(p.scoring, p.renormalize, my_id >= 0, my_l, my_s);
+    if (__any_sync(0xffffffffu, close)) {
+      float l64[V];  // a copy, so that l itself stays in registers
+#pragma unroll
+      for (int i = 0; i < V; ++i) l64[i] = l[i];
+      my_id = route_rank64<V>(p, l64, c_sh);
+      my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
+    }
+    const bool has = my_id >= 0;
+    const float prob = has && p.scoring == kRouteSoftmax && !p.renormalize
+                           ? expf(my_l - top) * inv : 0.f;
+    const float w = route_share(p.scoring, p.renormalize, has, my_l, prob);
     if (lane < p.k) {
       p.ids[t * p.k + lane] = my_id;
-      p.weights[t * p.k + lane] = bad ? nan_f32() : static_cast<float>(w * p.scale);
+      p.weights[t * p.k + lane] = bad ? nan_f32() : w * p.scale;
     }
   }
 }
@@ -218,6 +471,7 @@ struct RouteGradParams {
   void* dlogits;
   int64_t ldd;
   int32_t experts, k, scoring, renormalize;
+  int32_t vec, vec_out;  // runs of logits and of dlogits may be accessed by vectors
   float scale;
 };
 
@@ -232,75 +486,67 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kRouteWarps;
+  const int e0 = lane * V;
+  const bool dense = p.scoring == kRouteSoftmax && !p.renormalize;
   for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
        t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    float l[V];
-    bool bad = false;
-    double top = neg_inf();
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      l[i] = e < p.experts ? route_load(row + e) : -INFINITY;
-      bad |= route_bad(l[i], p.scoring);
-      top = fmax(top, static_cast<double>(l[i]));
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    top = warp_max(top);
-    const bool dense = p.scoring == kRouteSoftmax && !p.renormalize;
-    double sum = 1.0;
-    if (dense) {
-      sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (l[i] > -INFINITY) sum += exp(static_cast<double>(l[i]) - top);
-      sum = warp_sum(sum);
-    }
     int id = -1;
-    double g = 0.0, lj = 0.0;
+    float g = 0.f;
     if (lane < p.k) {
       id = p.ids[t * p.k + lane];
-      if (id < 0 || id >= p.experts) id = -1;
-      if (id >= 0) {
-        g = static_cast<double>(p.dweights[t * p.k + lane]);
-        lj = static_cast<double>(route_load(row + id));
-        if (!(lj > neg_inf())) id = -1;  // a masked expert: its score is 0 whatever the logit does
-      }
+      g = p.dweights[t * p.k + lane];
     }
-    const bool has = id >= 0 && !bad;
-    double pj = 0.0;
-    if (dense && has) pj = exp(lj - top) / sum;
-    const double r = route_part(p.scoring, p.renormalize, has, lj, pj);
-    const double mean = warp_sum(has ? g * r : 0.0);
-    double add;  // the choice's own term
-    if (dense)
-      add = g * r;
-    else if (p.renormalize)
-      add = r * (g - mean);
-    else
-      add = g * r;
-    if (p.scoring == kRouteSigmoid) add *= sigmoid64(-lj);
-    if (!has) add = 0.0;
-    double out[V];
+    float l[V];
+    load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      out[i] = dense && l[i] > -INFINITY
-                   ? -exp(static_cast<double>(l[i]) - top) / sum * mean
-                   : 0.0;
+    for (int i = 0; i < V; ++i) bad |= route_bad(l[i], p.scoring);
+    bad = __any_sync(0xffffffffu, bad);
+    float top = -INFINITY, inv = 0.f;
+    float out[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = 0.f;
+    if (dense) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+      top = warp_max(top);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        out[i] = l[i] > -INFINITY ? expf(l[i] - top) : 0.f;
+        sum += out[i];
+      }
+      sum = warp_sum(sum);
+      inv = sum > 0.f ? 1.f / sum : 0.f;
+    }
+    // A masked expert (logit -inf) scores 0 whatever its logit does: it takes no part.
+    float lj = -INFINITY;
+    if (id >= 0 && id < p.experts) lj = route_load(row + id);
+    const bool has = lj > -INFINITY && !bad;
+    const float prob = dense && has ? expf(lj - top) * inv : 0.f;
+    const float r = route_share(p.scoring, p.renormalize, has, lj, prob);
+    const float mean = warp_sum(has ? g * r : 0.f);
+    float add = 0.f;  // the choice's own term
+    if (has) {
+      add = dense || !p.renormalize ? g * r : r * (g - mean);
+      if (p.scoring == kRouteSigmoid) add *= 1.f / (1.f + expf(lj));
+    }
+    const int at = has ? id : -1;
+    if (dense) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] *= -inv * mean;
+    }
     for (int j = 0; j < p.k; ++j) {
-      const int ej = __shfl_sync(0xffffffffu, has ? id : -1, j);
-      const double aj = __shfl_sync(0xffffffffu, add, j);
+      const int ej = __shfl_sync(0xffffffffu, at, j) - e0;
+      const float aj = __shfl_sync(0xffffffffu, add, j);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (ej == lane * V + i) out[i] += aj;
+        if (ej == i) out[i] += aj;
     }
-    T* drow = static_cast<T*>(p.dlogits) + t * p.ldd;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      if (e < p.experts)
-        route_store(drow + e, bad ? nan_f32() : static_cast<float>(out[i] * p.scale));
-    }
+    for (int i = 0; i < V; ++i) out[i] = bad ? nan_f32() : out[i] * p.scale;
+    store_run<T, V>(static_cast<T*>(p.dlogits) + t * p.ldd, e0, p.experts, p.vec_out != 0, out);
   }
 }
 
@@ -313,6 +559,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kOrderMaxCluster = 8;
+constexpr int kOrderHold = 16;  // pairs a lane loads at a time
 
 struct OrderParams {
   const int32_t* ids;
@@ -346,15 +593,31 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
   const int64_t run = (p.pairs + warps * 32 - 1) / (warps * 32) * 32;
   const int64_t first = (static_cast<int64_t>(rank) * kOrderWarps + warp) * run;
   const int64_t last = first + run < p.pairs ? first + run : p.pairs;
-  for (int64_t i = first + lane; i < last; i += 32) {
-    const int32_t e = p.ids[i];
-    if (e >= 0 && e < E) atomicAdd(mine + e, 1u);  // counts only: any order gives the same sum
+  // kOrderHold pairs per lane at a time, all loaded before the first is used; a run of one such
+  // chunk keeps them for the second walk.
+  int32_t held[kOrderHold];
+  auto load = [&](int64_t i0) {
+#pragma unroll
+    for (int u = 0; u < kOrderHold; ++u) {
+      const int64_t i = i0 + u * 32 + lane;
+      held[u] = i < last ? p.ids[i] : -1;
+    }
+  };
+  constexpr int kChunk = 32 * kOrderHold;
+  for (int64_t i0 = first; i0 < last; i0 += kChunk) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < kOrderHold; ++u) {
+      // Counts only: any order of the additions gives the same sum.
+      if (held[u] >= 0 && held[u] < E) atomicAdd(mine + held[u], 1u);
+    }
   }
   __syncthreads();
   // Exclusive sums over the warps; the block's counts.
   const int e = threadIdx.x;
   if (e < E) {
     uint32_t s = 0u;
+#pragma unroll 8
     for (int w = 0; w < kOrderWarps; ++w) {
       const uint32_t v = order_smem[w * E + e];
       order_smem[w * E + e] = s;
@@ -394,21 +657,25 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
       p.offsets[e] = static_cast<int32_t>(start);
       if (e == E - 1) p.offsets[E] = static_cast<int32_t>(start + all);
     }
+#pragma unroll 8
     for (int w = 0; w < kOrderWarps; ++w) order_smem[w * E + e] += start + before;
   }
   __syncthreads();
-  for (int64_t i0 = first; i0 < last; i0 += 32) {
-    const int64_t i = i0 + lane;
-    int32_t id = i < last ? p.ids[i] : -1;
-    if (id >= E) id = -1;
-    const uint32_t peers = __match_any_sync(0xffffffffu, id);
-    const uint32_t before_me = __popc(peers & ((1u << lane) - 1u));
-    uint32_t slot = 0u;
-    if (id >= 0) slot = mine[id] + before_me;
-    __syncwarp();
-    if (id >= 0 && before_me == 0u) mine[id] += __popc(peers);
-    __syncwarp();
-    if (i < last) p.slots[i] = id >= 0 ? static_cast<int32_t>(slot) : -1;
+  for (int64_t i0 = first; i0 < last; i0 += kChunk) {
+    if (run > kChunk) load(i0);
+#pragma unroll
+    for (int u = 0; u < kOrderHold; ++u) {
+      const int64_t i = i0 + u * 32 + lane;
+      const int32_t id = held[u] < E ? held[u] : -1;  // lanes past the run hold -1
+      const uint32_t peers = __match_any_sync(0xffffffffu, id);
+      const uint32_t before_me = __popc(peers & ((1u << lane) - 1u));
+      uint32_t slot = 0u;
+      if (id >= 0) slot = mine[id] + before_me;
+      __syncwarp();
+      if (id >= 0 && before_me == 0u) mine[id] += __popc(peers);
+      __syncwarp();
+      if (i < last) p.slots[i] = id >= 0 ? static_cast<int32_t>(slot) : -1;
+    }
   }
   if (blocks > 1) ptx::cluster_sync();  // no block leaves while another may read its totals
 }

@@ -138,26 +138,29 @@ __device__ __forceinline__ uint32_t abs_max_vec(const uint4& v, uint32_t m) {
   return m;
 }
 
-// Four quotients x / s rounded to integers, as the bytes of a word, without a division per
-// element.  With y = RN(1 / s), q = RN(x y) is within 127 * 1.5 * 2^-23 < 2.3e-5 of x / s, and the
-// fp32 quotient within 127 * 2^-24 < 7.6e-6 of it; so where q is farther than 4e-5 from a
-// half-integer both round to the same integer, and elsewhere the word takes the division.
-// Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte.
+// Four quotients x / s by IEEE division, rounded to integers, as the bytes of a word.
+__device__ __noinline__ uint32_t int8_word_div(float x0, float x1, float x2, float x3, float s) {
+  return int8_quotient(x0, s) | (int8_quotient(x1, s) << 8) | (int8_quotient(x2, s) << 16) |
+         (int8_quotient(x3, s) << 24);
+}
+
+// The same without a division per element.  With y = RN(1 / s), q = RN(x y) is within
+// 127 * 1.5 * 2^-23 < 2.3e-5 of x / s, and the fp32 quotient within 127 * 2^-24 < 7.6e-6 of it; so
+// where q is farther than 4e-5 from a half-integer both round to the same integer, and elsewhere
+// (about 2e-4 of the elements) the word takes the division.  Adding 1.5 * 2^23 rounds to the nearest
+// even integer and leaves it in the low byte.
 __device__ __forceinline__ uint32_t int8_word(const float* x, float s, float y) {
   constexpr float kRound = 12582912.f;
   uint32_t b[4];
-  bool risky = false;
+  float worst = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float q = __fmul_rn(x[i], y);
     const float r = __fadd_rn(q, kRound);
-    risky |= fabsf(q - __fsub_rn(r, kRound)) > 0.5f - 4e-5f;
+    worst = fmaxf(worst, fabsf(q - __fsub_rn(r, kRound)));
     b[i] = __float_as_uint(r);
   }
-  if (risky) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = int8_quotient(x[i], s);
-  }
+  if (worst > 0.5f - 4e-5f) return int8_word_div(x[0], x[1], x[2], x[3], s);
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
@@ -230,12 +233,14 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
   }
 }
 
-// Quantised rows of whole vectors: G threads per token (a warp, or the block) hold the row packed
-// in registers, NV times 16 elements each, between its maximum and the quantisation, so the row is
-// read once however many copies of it are written.  Longer rows (Resident false) are read a second
-// time, from L2.
-template <typename T, int G, int NV, bool Resident>
-__global__ void __launch_bounds__(256, 2) rows_int8_vec_kernel(const RowsParams p) {
+// Quantised rows of whole vectors: G threads per token hold the row packed in registers, kInt8Vecs
+// times 16 elements each, between its maximum and the quantisation, so the row is read once however
+// many copies of it are written.  Longer rows (Resident false) are read a second time, from L2.
+constexpr int kInt8Vecs = 4;
+
+template <typename T, int G, bool Resident>
+__global__ void __launch_bounds__(256, 16 / sizeof(T) / 2) rows_int8_vec_kernel(const RowsParams p) {
+  constexpr int NV = kInt8Vecs;
   constexpr int kVecs = 16 / RowVec<T>::kElems;
   constexpr int kE = RowVec<T>::kElems;
   constexpr int kRowsPerBlock = 256 / G;
@@ -277,10 +282,12 @@ __global__ void __launch_bounds__(256, 2) rows_int8_vec_kernel(const RowsParams 
     m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (G > 32) {
       // The parity keeps the next row's writes off the words a slow warp still reads.
+      constexpr int kWarps = G / 32;
+      const int first = (threadIdx.x / G) * kWarps;
       if (lane == 0) red[parity][threadIdx.x >> 5] = m;
-      __syncthreads();
+      ptx::named_barrier_sync(1u + threadIdx.x / G, G);
 #pragma unroll
-      for (int w = 0; w < 8; ++w) m = max(m, red[parity][w]);
+      for (int w = 0; w < kWarps; ++w) m = max(m, red[parity][first + w]);
       parity ^= 1;
     }
     const float s = int8_scale(m);
