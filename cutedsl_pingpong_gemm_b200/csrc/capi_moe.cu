@@ -169,6 +169,23 @@ unsigned route_grid(int64_t tokens) {
   return static_cast<unsigned>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps);
 }
 
+template <int L, int V>
+void launch_route_grad(cpg::RouteGradParams& p, int32_t dtype, cudaStream_t st) {
+  const int64_t per = 32 / L * cpg::kRouteWarps;
+  const unsigned grid = static_cast<unsigned>((p.tokens + per - 1) / per);
+  // Vectors of as many logits as 16 bytes or V hold.
+  if (dtype == CPG_DTYPE_BF16) {
+    constexpr int kPer = V < 8 ? V : 8;
+    p.vec = run_vectors<kPer>(p.logits, p.ld, dtype);
+    p.vec_out = run_vectors<kPer>(p.dlogits, p.ldd, dtype);
+    cpg::route_grad_kernel<__nv_bfloat16, L, V><<<grid, 32 * cpg::kRouteWarps, 0, st>>>(p);
+  } else {
+    p.vec = run_vectors<4>(p.logits, p.ld, dtype);
+    p.vec_out = run_vectors<4>(p.dlogits, p.ldd, dtype);
+    cpg::route_grad_kernel<float, L, V><<<grid, 32 * cpg::kRouteWarps, 0, st>>>(p);
+  }
+}
+
 static_assert(CPG_ROUTE_MAX_EXPERTS == cpg::kRouteMaxExperts &&
                   CPG_ROUTE_MAX_K == cpg::kRouteMaxK &&
                   CPG_ROUTE_MAX_GROUPS == cpg::kRouteMaxGroups,
@@ -211,12 +228,13 @@ int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int6
     return fail(CPG_ERR_ALIGNMENT, "logits, bias, ids and weights must be aligned to their elements");
   cpg::RouteParams p{logits,         tokens,         ld,         bias,      ids,
                      weights,        c->experts,     c->k,       c->scoring, c->groups,
-                     c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, 0, c->scale};
+                     c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, 0, 0, c->scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_lane_values(c->experts, [&](auto v) {
     constexpr int V = decltype(v)::value;
     const size_t smem = c->groups > 1 ? sizeof(double) * 32 * V * cpg::kRouteWarps : 0;
     p.vec = run_vectors<V>(logits, ld, dtype);
+    p.vec_bias = run_vectors<V>(bias, 0, CPG_DTYPE_F32);
     if (dtype == CPG_DTYPE_BF16)
       cpg::route_kernel<__nv_bfloat16, V>
           <<<route_grid(tokens), 32 * cpg::kRouteWarps, smem, st>>>(p);
@@ -246,16 +264,18 @@ int cpg_route_backward(const cpg_route_config* c, const float* dweights, const v
                          dlogits,  ldd,    c->experts, c->k, c->scoring,
                          c->renormalize != 0 ? 1 : 0, 0, 0, c->scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  by_lane_values(c->experts, [&](auto v) {
-    constexpr int V = decltype(v)::value;
-    p.vec = run_vectors<V>(logits, ld, dtype);
-    p.vec_out = run_vectors<V>(dlogits, ldd, dtype);
-    if (dtype == CPG_DTYPE_BF16)
-      cpg::route_grad_kernel<__nv_bfloat16, V>
-          <<<route_grid(tokens), 32 * cpg::kRouteWarps, 0, st>>>(p);
-    else
-      cpg::route_grad_kernel<float, V><<<route_grid(tokens), 32 * cpg::kRouteWarps, 0, st>>>(p);
-  });
+  // The fewest lanes per token that hold its choices and at most 16 of its logits each.
+  const int32_t e = c->experts, k = c->k;
+  if (k <= 8 && e <= 32) launch_route_grad<8, 4>(p, dtype, st);
+  else if (k <= 8 && e <= 64) launch_route_grad<8, 8>(p, dtype, st);
+  else if (k <= 8 && e <= 128) launch_route_grad<8, 16>(p, dtype, st);
+  else if (k <= 16 && e <= 64) launch_route_grad<16, 4>(p, dtype, st);
+  else if (k <= 16 && e <= 128) launch_route_grad<16, 8>(p, dtype, st);
+  else if (k <= 16 && e <= 256) launch_route_grad<16, 16>(p, dtype, st);
+  else if (e <= 128) launch_route_grad<32, 4>(p, dtype, st);
+  else if (e <= 256) launch_route_grad<32, 8>(p, dtype, st);
+  else if (e <= 512) launch_route_grad<32, 16>(p, dtype, st);
+  else launch_route_grad<32, 32>(p, dtype, st);
   return launched("route gradient kernel launch");
 }
 

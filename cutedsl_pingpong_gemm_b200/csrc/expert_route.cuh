@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 
 namespace cpg {
@@ -31,7 +33,7 @@ struct RouteParams {
   int32_t* ids;       // [tokens][k]
   float* weights;     // [tokens][k]
   int32_t experts, k, scoring, groups, kept_groups, group_score, renormalize;
-  int32_t vec;  // a lane's run of logits may be read by vectors (run_vectors)
+  int32_t vec, vec_bias;  // a lane's run of logits, of biases may be read by vectors
   float scale;
 };
 
@@ -170,16 +172,16 @@ __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormaliz
   return sum > 0.f ? v / sum : 0.f;
 }
 
-// The k best experts of a row with c in 64 bits: lane j returns choice j, or -1.  l holds the
-// lane's run of logits, -inf where an expert cannot be chosen.  c_sh: 32 * V words of the warp's
-// own shared memory (groups > 1).
+// The k best experts of a row with c (by_logit: l) in 64 bits: lane j returns choice j, or -1.  l
+// holds the lane's run of logits, -inf where an expert cannot be chosen.  c_sh: 32 * V words of the
+// warp's own shared memory (groups > 1).
 template <int V>
 __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (&l)[V],
-                                             double* c_sh) {
+                                             double* c_sh, bool by_logit) {
   const int lane = threadIdx.x & 31;
   double c[V];
   double top = neg_inf(), sum = 0.0;
-  if (p.scoring == kRouteSoftmax) {
+  if (p.scoring == kRouteSoftmax && !by_logit) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmax(top, static_cast<double>(l[i]));
     top = warp_max(top);
@@ -187,16 +189,18 @@ __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     c[i] = 0.0;
-    if (l[i] > -INFINITY)
+    if (by_logit)
+      c[i] = static_cast<double>(l[i]);
+    else if (l[i] > -INFINITY)
       c[i] = p.scoring == kRouteSoftmax ? exp(static_cast<double>(l[i]) - top)
                                         : sigmoid64(static_cast<double>(l[i]));
     sum += c[i];
   }
-  if (p.scoring == kRouteSoftmax) sum = warp_sum(sum);
+  if (p.scoring == kRouteSoftmax && !by_logit) sum = warp_sum(sum);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = lane * V + i;
-    if (p.scoring == kRouteSoftmax) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
+    if (p.scoring == kRouteSoftmax && !by_logit) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
     if (p.bias != nullptr && e < p.experts) c[i] += static_cast<double>(p.bias[e]);
     if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = neg_inf();
   }
@@ -255,7 +259,33 @@ __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (
   return my_id;
 }
 
-// One warp per token; lane l holds experts l * V .. l * V + V - 1.
+// Sorts a lane's N keys, the largest first (odd-even merge network).
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2) {
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2) {
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k) {
+#pragma unroll
+        for (int i = 0; i < k; ++i) {
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t hi = max(a[i + j], a[i + j + k]);
+            a[i + j + k] = min(a[i + j], a[i + j + k]);
+            a[i + j] = hi;
+          }
+        }
+      }
+    }
+  }
+}
+
+// One warp per token; lane l holds experts l * V .. l * V + V - 1.  Each lane sorts the keys of its
+// run; the choices are then k warp-wide maxima of the lanes' first keys, the lane that holds the
+// maximum moving up by one.  The low log2 V bits of a key hold the place in the run (lower places
+// first), so a key names its expert in the run; what they cost in precision is part of the bound
+// below.
 //
 // Error of the 32-bit scores (ulp bounds of __expf and __fdividef, 2^-23 = one ulp of 1):
 //   sigmoid: e^-l is off by (2 + 1.173 |l|) ulp, which s (1 - s) turns into at most 0.57 ulp of s;
@@ -264,80 +294,107 @@ __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (
 //            (2.9 ulp) inv absolutely; inv by (10.2 + 18.5 + 1) ulp relatively (the terms' errors
 //            weighted by p, whose mean |l - top| is at most ln 1024; 37 additions; the quotient),
 //            which the largest p <= inv carries: below 2^-18 inv altogether.
-// c = s + bias adds half an ulp of c.  Two c nearer than twice the bound are ranked in 64 bits,
-// unless logit and bias are the same: such c are equal, and the lower index goes first.
+// c = s + bias adds half an ulp of c, a key's lost bits less than V ulp.  Two c nearer than twice the
+// bound are ranked in 64 bits, unless logit and bias are the same: such c are equal, and the lower
+// index goes first.  Measured with 256 experts in 8 groups: about one row in 200.
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(32 * kRouteWarps)
+    route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
+  constexpr uint32_t kPlace = V - 1;  // bits of a key that hold the place in the run
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   double* c_sh = route_smem + warp * (32 * V);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kRouteWarps;
   const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_score == kRouteGroupMax);
+  const bool softmax = p.scoring == kRouteSoftmax;
   const int e0 = lane * V;
+  const bool off = e0 >= p.experts;  // a lane without experts
   for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
        t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    float l[V];
+    float l[V], c[V], b[V];
     load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
-    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = 0.f;
+    if (p.bias != nullptr) load_run<float, V>(p.bias, e0, p.experts, p.vec_bias != 0, b);
+    float top = -INFINITY, inv = 1.f;
+    // c of the run.  `all` assumes finite values; otherwise what cannot be chosen becomes -inf.
+    auto score = [&](auto all) {
+      constexpr bool kAll = decltype(all)::value;
+      top = -INFINITY;
+      inv = 1.f;
+      if (softmax && (!by_logit || !p.renormalize)) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+        if (kAll && off) top = -INFINITY;
+        top = warp_max(top);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          c[i] = kAll || l[i] > -INFINITY ? __expf(l[i] - top) : 0.f;
+          sum += c[i];
+        }
+        if (kAll && off) sum = 0.f;
+        sum = warp_sum(sum);
+        inv = sum > 0.f ? 1.f / sum : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (by_logit)
+          c[i] = l[i];
+        else
+          c[i] = (softmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-l[i]))) + b[i];
+        if (!kAll && (!(l[i] > -INFINITY) || c[i] != c[i])) c[i] = -INFINITY;
+      }
+    };
+    if (off) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) l[i] = b[i] = 0.f;
+    }
+    score(std::true_type{});
+    // 0 x l is NaN where l is not finite; a bias that is not finite makes c so.
+    float finite = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (route_bad(l[i], p.scoring)) {
-        bad = true;
-        l[i] = -INFINITY;
-      }
+      finite = fmaf(l[i], 0.f, finite);
+      finite = fmaf(c[i], 0.f, finite);
     }
-    bad = __any_sync(0xffffffffu, bad);
-    float top = -INFINITY, inv = 1.f;
-    float c[V];
-    if (p.scoring == kRouteSoftmax && (!by_logit || !p.renormalize)) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-      top = warp_max(top);
-      float sum = 0.f;
+    bool bad = false;
+    if (__any_sync(0xffffffffu, finite != finite)) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        c[i] = l[i] > -INFINITY ? __expf(l[i] - top) : 0.f;
-        sum += c[i];
+        if (route_bad(l[i], p.scoring)) {
+          bad = true;
+          l[i] = -INFINITY;
+        }
+        if (off) l[i] = -INFINITY;
       }
-      sum = warp_sum(sum);
-      inv = sum > 0.f ? 1.f / sum : 0.f;
+      bad = __any_sync(0xffffffffu, bad);
+      score(std::false_type{});
     }
-    uint32_t key[V];
-    float near = 0.f;  // c nearer than this (plus 2^-21 |c|) may be in another order
-    if (by_logit) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = l[i];
-    } else {
-      near = 2.f * (p.scoring == kRouteSoftmax ? 0x1p-18f * inv : 0x1p-21f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = e0 + i;
-        c[i] = p.scoring == kRouteSoftmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-l[i]));
-        if (p.bias != nullptr && e < p.experts) c[i] += __ldg(p.bias + e);
-        if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = -INFINITY;
-      }
-    }
-    bool close = false;  // the 32-bit order cannot be trusted
+    // Two c whose difference is at most near + rel (|c1| + |c2|) may be in another order.
+    const float near = by_logit ? 0.f : 2.f * (softmax ? 0x1p-18f * inv : 0x1p-21f);
+    const float rel = 0x1p-22f + V * 0x1p-23f;
+    bool close = false;
     if (p.groups > 1) {
       const int per = p.experts / p.groups;
       const int lanes = per / V;  // lanes of a group, when that is a whole power of two
       const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
-      float a = -INFINITY, b = -INFINITY;  // the group's two best
+      float a = -INFINITY, a2 = -INFINITY;  // the group's two best
       int group;
       if (whole) {
         group = lane / lanes;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          b = fmaxf(b, fminf(a, c[i]));
+          a2 = fmaxf(a2, fminf(a, c[i]));
           a = fmaxf(a, c[i]);
         }
         for (int o = 1; o < lanes; o <<= 1) {
-          const float a2 = __shfl_xor_sync(0xffffffffu, a, o);
-          const float b2 = __shfl_xor_sync(0xffffffffu, b, o);
-          b = fmaxf(fminf(a, a2), fmaxf(b, b2));
-          a = fmaxf(a, a2);
+          const float u = __shfl_xor_sync(0xffffffffu, a, o);
+          const float u2 = __shfl_xor_sync(0xffffffffu, a2, o);
+          a2 = fmaxf(fminf(a, u), fmaxf(a2, u2));
+          a = fmaxf(a, u);
         }
       } else {
         group = lane;
@@ -349,17 +406,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_co
         if (lane < p.groups) {
           for (int i = 0; i < per; ++i) {
             const float v = f_sh[lane * per + i];
-            b = fmaxf(b, fminf(a, v));
+            a2 = fmaxf(a2, fminf(a, v));
             a = fmaxf(a, v);
           }
         }
         __syncwarp();
       }
       const bool real = group < p.groups;
-      float slack = near + 0x1p-21f * fabsf(a);
-      if (p.group_score == kRouteGroupTop2 && b > -INFINITY) {
-        slack = 2.f * near + 0x1p-21f * (fabsf(a) + fabsf(b));
-        a += b;
+      float slack = near + rel * fabsf(a);
+      if (p.group_score == kRouteGroupTop2 && a2 > -INFINITY) {
+        slack = 2.f * near + rel * (fabsf(a) + fabsf(a2));
+        a += a2;
       }
       int better = 0;
       for (int g = 0; g < p.groups; ++g) {
@@ -393,29 +450,31 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_co
         }
       }
     }
+    uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = c[i] > -INFINITY ? order_key(c[i]) : kNoKey;
-    // k times: the largest key of the row, the lowest lane (so the lowest index) among equals.
+    for (int i = 0; i < V; ++i)
+      key[i] = c[i] > -INFINITY && !off ? (order_key(c[i]) & ~kPlace) | (kPlace - i) : kNoKey;
+    sort_keys(key);
+    // The row's largest key without its place bits (all ones), at most kPlace if none is left.
+    auto largest = [&]() { return __reduce_max_sync(0xffffffffu, key[0] | kPlace); };
+    // Takes that key away from its lane, the lowest among equals, and returns its expert.
+    auto take = [&](uint32_t all) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, (key[0] | kPlace) == all)) - 1;
+      const uint32_t taken = __shfl_sync(0xffffffffu, key[0], owner);
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+        key[V - 1] = kNoKey;
+      }
+      return owner * V + static_cast<int>(kPlace - (taken & kPlace));
+    };
     int32_t my_id = -1;
     uint32_t my_key = kNoKey, last_key = kNoKey;
     int found = 0;
     for (; found < p.k; ++found) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) best = max(best, key[i]);
-      const uint32_t all = __reduce_max_sync(0xffffffffu, best);
-      if (all == kNoKey) break;
-      const int owner = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
-      int at = 0;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] == all) at = i;
-      if (lane == owner) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i == at) key[i] = kNoKey;
-      }
-      const int id = __shfl_sync(0xffffffffu, e0 + at, owner);
+      const uint32_t all = largest();
+      if (all <= kPlace) break;
+      const int id = take(all);
       if (lane == found) {
         my_id = id;
         my_key = all;
@@ -423,38 +482,41 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_co
       last_key = all;
     }
     float my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
-    if (!by_logit && !close) {
-      // Neighbours in the order, and the last choice against everything left.
-      const float my_c = key_value(my_key);
+    // BF16 logits fit in a key whole: ranked by them, the order is exact.
+    if (!(by_logit && (sizeof(T) == 2 || V == 1)) && !close) {
+      auto nearer = [&](uint32_t k1, uint32_t k2) {
+        const float c1 = key_value(k1 & ~kPlace), c2 = key_value(k2 & ~kPlace);
+        return by_logit ? c1 == c2 : c1 - c2 <= near + rel * (fabsf(c1) + fabsf(c2));
+      };
+      // Neighbours in the order.
       const float my_b = my_id >= 0 && p.bias != nullptr ? __ldg(p.bias + my_id) : 0.f;
-      const float next_c = __shfl_down_sync(0xffffffffu, my_c, 1);
+      const uint32_t next_key = __shfl_down_sync(0xffffffffu, my_key, 1);
       const float next_l = __shfl_down_sync(0xffffffffu, my_l, 1);
       const float next_b = __shfl_down_sync(0xffffffffu, my_b, 1);
-      close = lane + 1 < found && my_c - next_c <= near + 0x1p-21f * fabsf(my_c) &&
+      close = lane + 1 < found && nearer(my_key, next_key) &&
               !(my_l == next_l && my_b == next_b);
-      if (found == p.k) {
-        const float last_c = key_value(last_key);
-        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
-        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
-        const float limit = last_c - (near + 0x1p-21f * fabsf(last_c));
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (key[i] != kNoKey && c[i] >= limit)
-            close |= !(l[i] == last_l &&
-                       (p.bias == nullptr || __ldg(p.bias + e0 + i) == last_b));
+      // The last choice against the best ones left, past those that are equal to it.
+      while (found == p.k) {
+        const uint32_t all = largest();
+        if (all <= kPlace || !nearer(last_key, all)) break;
+        const int id = take(all);
+        if (route_load(row + id) != __shfl_sync(0xffffffffu, my_l, p.k - 1) ||
+            (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) !=
+                __shfl_sync(0xffffffffu, my_b, p.k - 1)) {
+          close = true;
+          break;
         }
       }
     }
     if (__any_sync(0xffffffffu, close)) {
       float l64[V];  // a copy, so that l itself stays in registers
 #pragma unroll
-      for (int i = 0; i < V; ++i) l64[i] = l[i];
-      my_id = route_rank64<V>(p, l64, c_sh);
+      for (int i = 0; i < V; ++i) l64[i] = off ? -INFINITY : l[i];
+      my_id = route_rank64<V>(p, l64, c_sh, by_logit);
       my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
     }
     const bool has = my_id >= 0;
-    const float prob = has && p.scoring == kRouteSoftmax && !p.renormalize
-                           ? expf(my_l - top) * inv : 0.f;
+    const float prob = has && softmax && !p.renormalize ? expf(my_l - top) * inv : 0.f;
     const float w = route_share(p.scoring, p.renormalize, has, my_l, prob);
     if (lane < p.k) {
       p.ids[t * p.k + lane] = my_id;
@@ -480,73 +542,125 @@ struct RouteGradParams {
 //   softmax:                dl_e = scale p_e (g_e - sum g p)        (g_e = 0 where not chosen)
 //   sigmoid, renormalised:  dl_j = scale r_j (g_j - sum g r) (1 - s_j)
 //   sigmoid:                dl_j = scale g_j s_j (1 - s_j)
-// One warp per token; an expert that is chosen twice gets both terms.
-template <typename T, int V>
+// L lanes per token (k <= L, experts <= L * V), so that a warp's sums and exponentials serve 32 / L
+// tokens; lane l holds the vectors l, L + l, 2 L + l, ... of the row.  An expert that is chosen
+// twice gets both terms.
+template <typename T, int L, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const RouteGradParams p) {
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRouteWarps;
-  const int e0 = lane * V;
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T)) < V ? 16 / static_cast<int>(sizeof(T)) : V;
+  constexpr int kVecs = V / kPer;  // vectors of kPer logits a lane holds
+  constexpr int kTokens = 32 / L * kRouteWarps;
+  const int sub = threadIdx.x % L;
   const bool dense = p.scoring == kRouteSoftmax && !p.renormalize;
-  for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
-       t += stride) {
-    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  auto sum_of = [](float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto max_of = [](float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  for (int64_t t0 = blockIdx.x * static_cast<int64_t>(kTokens); t0 < p.tokens;
+       t0 += static_cast<int64_t>(gridDim.x) * kTokens) {
+    const int64_t t = t0 + threadIdx.x / L;
+    const bool live = t < p.tokens;
+    const T* row = static_cast<const T*>(p.logits) + (live ? t : 0) * p.ld;
     int id = -1;
     float g = 0.f;
-    if (lane < p.k) {
-      id = p.ids[t * p.k + lane];
-      g = p.dweights[t * p.k + lane];
+    if (live && sub < p.k) {
+      id = p.ids[t * p.k + sub];
+      g = p.dweights[t * p.k + sub];
     }
-    float l[V];
-    load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
-    bool bad = false;
+    float l[kVecs][kPer];
+    float finite = 0.f;  // NaN once a logit is +-inf or NaN
 #pragma unroll
-    for (int i = 0; i < V; ++i) bad |= route_bad(l[i], p.scoring);
-    bad = __any_sync(0xffffffffu, bad);
-    float top = -INFINITY, inv = 0.f;
-    float out[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = 0.f;
-    if (dense) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-      top = warp_max(top);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        out[i] = l[i] > -INFINITY ? expf(l[i] - top) : 0.f;
-        sum += out[i];
-      }
-      sum = warp_sum(sum);
-      inv = sum > 0.f ? 1.f / sum : 0.f;
+    for (int q = 0; q < kVecs; ++q) {
+      const int e0 = (q * L + sub) * kPer;
+      load_run<T, kPer>(row, e0, live ? p.experts : 0, p.vec != 0, l[q]);
     }
     // A masked expert (logit -inf) scores 0 whatever its logit does: it takes no part.
     float lj = -INFINITY;
     if (id >= 0 && id < p.experts) lj = route_load(row + id);
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) finite = fmaf(l[q][i], 0.f, finite);
+    bool bad = false;
+    if (__any_sync(0xffffffffu, finite != finite)) {
+      float spoiled = 0.f;
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) spoiled += route_bad(l[q][i], p.scoring) ? 1.f : 0.f;
+      bad = sum_of(spoiled) > 0.f;
+    }
+    float top = -INFINITY, inv = 0.f;
+    float out[kVecs][kPer];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) out[q][i] = 0.f;
+    if (dense) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) top = fmaxf(top, l[q][i]);
+      top = max_of(top);
+      const float from = top > -INFINITY ? top : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          out[q][i] = expf(l[q][i] - from);
+          sum += out[q][i];
+        }
+      sum = sum_of(sum);
+      inv = sum > 0.f ? 1.f / sum : 0.f;
+    }
     const bool has = lj > -INFINITY && !bad;
-    const float prob = dense && has ? expf(lj - top) * inv : 0.f;
-    const float r = route_share(p.scoring, p.renormalize, has, lj, prob);
-    const float mean = warp_sum(has ? g * r : 0.f);
+    float r = 0.f;  // as route_share
+    if (!p.renormalize) {
+      if (has) r = dense ? expf(lj - top) * inv : sigmoid32(lj);
+    } else {
+      const float best = max_of(has ? lj : -INFINITY);
+      if (has)
+        r = p.scoring == kRouteSoftmax || best < -60.f ? expf(lj - best) : sigmoid32(lj);
+      const float sum = sum_of(r);
+      r = sum > 0.f ? r / sum : 0.f;
+    }
     float add = 0.f;  // the choice's own term
+    float mean = 0.f;
+    if (dense || p.renormalize) mean = sum_of(has ? g * r : 0.f);
     if (has) {
-      add = dense || !p.renormalize ? g * r : r * (g - mean);
+      add = p.renormalize ? r * (g - mean) : g * r;
       if (p.scoring == kRouteSigmoid) add *= 1.f / (1.f + expf(lj));
     }
     const int at = has ? id : -1;
     if (dense) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) out[i] *= -inv * mean;
+      for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) out[q][i] *= -inv * mean;
     }
     for (int j = 0; j < p.k; ++j) {
-      const int ej = __shfl_sync(0xffffffffu, at, j) - e0;
-      const float aj = __shfl_sync(0xffffffffu, add, j);
+      const int ej = __shfl_sync(0xffffffffu, at, j, L) - sub * kPer;
+      const float aj = __shfl_sync(0xffffffffu, add, j, L);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (ej == i) out[i] += aj;
+      for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (ej == q * L * kPer + i) out[q][i] += aj;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = bad ? nan_f32() : out[i] * p.scale;
-    store_run<T, V>(static_cast<T*>(p.dlogits) + t * p.ldd, e0, p.experts, p.vec_out != 0, out);
+    for (int q = 0; q < kVecs; ++q) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) out[q][i] = bad ? nan_f32() : out[q][i] * p.scale;
+      store_run<T, kPer>(static_cast<T*>(p.dlogits) + (live ? t : 0) * p.ldd, (q * L + sub) * kPer,
+                         live ? p.experts : 0, p.vec_out != 0, out[q]);
+    }
   }
 }
 
@@ -586,52 +700,79 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
   const uint32_t rank = blockIdx.x;
   uint32_t* total = order_smem + kOrderWarps * E;
   uint32_t* mine = order_smem + warp * E;
-  for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) order_smem[i] = 0u;
-  __syncthreads();
   // This warp's run of pairs (a multiple of 32 of them).
   const int64_t warps = static_cast<int64_t>(blocks) * kOrderWarps;
   const int64_t run = (p.pairs + warps * 32 - 1) / (warps * 32) * 32;
   const int64_t first = (static_cast<int64_t>(rank) * kOrderWarps + warp) * run;
   const int64_t last = first + run < p.pairs ? first + run : p.pairs;
   // kOrderHold pairs per lane at a time, all loaded before the first is used; a run of one such
-  // chunk keeps them for the second walk.
+  // chunk keeps them, and their ranks, for the second walk.
+  constexpr int kChunk = 32 * kOrderHold;
+  const bool hold = run <= kChunk;
   int32_t held[kOrderHold];
+  uint32_t rnk[kOrderHold];
   auto load = [&](int64_t i0) {
 #pragma unroll
     for (int u = 0; u < kOrderHold; ++u) {
       const int64_t i = i0 + u * 32 + lane;
       held[u] = i < last ? p.ids[i] : -1;
+      if (held[u] < 0 || held[u] >= E) held[u] = E;  // no expert
     }
   };
-  constexpr int kChunk = 32 * kOrderHold;
-  for (int64_t i0 = first; i0 < last; i0 += kChunk) {
-    load(i0);
+  // Ranks of the held pairs among the run's pairs of the same expert, counting on in `mine`.  The
+  // lanes with the same expert are found by one ballot per bit of it (match.any takes several
+  // times as long), and the lowest of them counts them all.
+  const int bits = 32 - __clz(E);  // of 0 .. E
+  auto count = [&](int64_t i0) {
 #pragma unroll
     for (int u = 0; u < kOrderHold; ++u) {
-      // Counts only: any order of the additions gives the same sum.
-      if (held[u] >= 0 && held[u] < E) atomicAdd(mine + held[u], 1u);
+      if (i0 + u * 32 >= last) break;
+      uint32_t peers = 0xffffffffu;
+      for (int bit = 0; bit < bits; ++bit) {
+        const bool one = (held[u] >> bit) & 1;
+        const uint32_t v = __ballot_sync(0xffffffffu, one);
+        peers &= one ? v : ~v;
+      }
+      const uint32_t before = __popc(peers & ((1u << lane) - 1u));
+      const bool real = held[u] < E;
+      rnk[u] = real ? mine[held[u]] + before : 0u;
+      __syncwarp();
+      if (real && before == 0u) mine[held[u]] = rnk[u] + __popc(peers);
+      __syncwarp();
+    }
+  };
+  if (hold) load(first);
+  for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) order_smem[i] = 0u;
+  __syncthreads();
+  if (hold) {
+    count(first);
+  } else {
+    for (int64_t i0 = first; i0 < last; i0 += kChunk) {
+      load(i0);
+      count(i0);
     }
   }
   __syncthreads();
-  // Exclusive sums over the warps; the block's counts.
+  // The block's counts of expert e, thread e.
   const int e = threadIdx.x;
   if (e < E) {
     uint32_t s = 0u;
 #pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) {
-      const uint32_t v = order_smem[w * E + e];
-      order_smem[w * E + e] = s;
-      s += v;
-    }
+    for (int w = 0; w < kOrderWarps; ++w) s += order_smem[w * E + e];
     total[e] = s;
   }
-  __syncthreads();
-  if (blocks > 1) ptx::cluster_sync();
-  uint32_t all = 0u, before = 0u;
+  if (blocks > 1) {
+    ptx::cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  uint32_t all = 0u, before = 0u;  // of the expert in the cluster, and in the blocks before
   if (e < E) {
     if (blocks > 1) {
       const uint32_t addr = ptx::smem_u32(total + e);
-      for (uint32_t b = 0; b < blocks; ++b) {
+#pragma unroll
+      for (uint32_t b = 0; b < kOrderMaxCluster; ++b) {
+        if (b >= blocks) break;
         const uint32_t v = ld_cluster_u32(ptx::mapa_shared(addr, b));
         if (b < rank) before += v;
         all += v;
@@ -649,32 +790,43 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
   }
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
-  uint32_t base = 0u;
-  for (int w = 0; w < warp; ++w) base += warp_sums[w];
+  const uint32_t base = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0u);
   const uint32_t start = base + incl - all;
   if (e < E) {
     if (rank == 0) {
       p.offsets[e] = static_cast<int32_t>(start);
       if (e == E - 1) p.offsets[E] = static_cast<int32_t>(start + all);
     }
-#pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) order_smem[w * E + e] += start + before;
+    // First slot of every warp's pairs of the expert.
+    uint32_t s = start + before;
+    for (int w0 = 0; w0 < kOrderWarps; w0 += 8) {
+      uint32_t of_warp[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) of_warp[w] = order_smem[(w0 + w) * E + e];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        order_smem[(w0 + w) * E + e] = s;
+        s += of_warp[w];
+      }
+    }
   }
   __syncthreads();
-  for (int64_t i0 = first; i0 < last; i0 += kChunk) {
-    if (run > kChunk) load(i0);
+  auto store = [&](int64_t i0, bool add) {
 #pragma unroll
     for (int u = 0; u < kOrderHold; ++u) {
       const int64_t i = i0 + u * 32 + lane;
-      const int32_t id = held[u] < E ? held[u] : -1;  // lanes past the run hold -1
-      const uint32_t peers = __match_any_sync(0xffffffffu, id);
-      const uint32_t before_me = __popc(peers & ((1u << lane) - 1u));
-      uint32_t slot = 0u;
-      if (id >= 0) slot = mine[id] + before_me;
-      __syncwarp();
-      if (id >= 0 && before_me == 0u) mine[id] += __popc(peers);
-      __syncwarp();
-      if (i < last) p.slots[i] = id >= 0 ? static_cast<int32_t>(slot) : -1;
+      if (i < last)
+        p.slots[i] = held[u] < E ? static_cast<int32_t>(rnk[u] + (add ? mine[held[u]] : 0u)) : -1;
+    }
+  };
+  if (hold) {
+    store(first, true);
+  } else {
+    // Counting on from the first slots gives the slots themselves.
+    for (int64_t i0 = first; i0 < last; i0 += kChunk) {
+      load(i0);
+      count(i0);
+      store(i0, false);
     }
   }
   if (blocks > 1) ptx::cluster_sync();  // no block leaves while another may read its totals
