@@ -14,6 +14,7 @@ using cpg_capi::fail;
 
 namespace {
 
+constexpr int64_t kRouteBlocks = 148 * 8;
 constexpr int64_t kFewThreads = 148 * 1024;  // half of the threads that fit on the SMs
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;  // rows and pairs are counted in int32
 
@@ -165,8 +166,11 @@ int32_t run_vectors(const void* p, int64_t ld, int32_t dtype) {
   return !misaligned(p, bytes) && (ld * es) % bytes == 0 ? 1 : 0;
 }
 
+// One warp per token, at most about as many as fit on the SMs at once (each then walks several
+// tokens with the biases it has loaded).
 unsigned route_grid(int64_t tokens) {
-  return static_cast<unsigned>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps);
+  return static_cast<unsigned>(
+      std::min<int64_t>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps, kRouteBlocks));
 }
 
 template <int L, int V>
@@ -296,7 +300,10 @@ int cpg_expert_order(const int32_t* ids, int64_t tokens, int32_t k, int32_t expe
   while (blocks < cpg::kOrderMaxCluster && pairs > int64_t(blocks) * cpg::kOrderWarps * 64)
     blocks *= 2;
   const int smem = static_cast<int>(sizeof(uint32_t)) * (cpg::kOrderWarps + 1) * experts;
-  const void* fn = reinterpret_cast<const void*>(&cpg::expert_order_kernel);
+  const void* fn = experts <= 16  ? reinterpret_cast<const void*>(&cpg::expert_order_kernel<4>)
+                   : experts <= 64  ? reinterpret_cast<const void*>(&cpg::expert_order_kernel<6>)
+                   : experts <= 256 ? reinterpret_cast<const void*>(&cpg::expert_order_kernel<8>)
+                                    : reinterpret_cast<const void*>(&cpg::expert_order_kernel<10>);
   // Always the limit of the largest call: a smaller later call must not lower it.
   cudaError_t e = cudaFuncSetAttribute(
       fn, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -150,8 +150,21 @@ __device__ __forceinline__ float warp_max(float v) {
   return key_value(__reduce_max_sync(0xffffffffu, order_key(v)));
 }
 
+// e^x and 1 / x by the hardware's approximations, results below 2^-126 flushed to zero: at most
+// 2 + 1.173 |x| ulp (the product with log2 e, then 2 ulp) and 1 ulp off.
+__device__ __forceinline__ float fast_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 __device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
-__device__ __forceinline__ float sigmoid32(float l) { return 1.f / (1.f + expf(-l)); }
+__device__ __forceinline__ float sigmoid32(float l) { return __fdividef(1.f, 1.f + expf(-l)); }
 
 // A logit that cannot be chosen and spoils its row's weights: NaN, and +inf under the softmax.
 __device__ __forceinline__ bool route_bad(float l, int32_t scoring) {
@@ -169,7 +182,7 @@ __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormaliz
   float v = 0.f;
   if (has) v = scoring == kRouteSoftmax || top < -60.f ? expf(l - top) : sigmoid32(l);
   const float sum = warp_sum(v);
-  return sum > 0.f ? v / sum : 0.f;
+  return sum > 0.f ? __fdividef(v, sum) : 0.f;
 }
 
 // The k best experts of a row with c (by_logit: l) in 64 bits: lane j returns choice j, or -1.  l
@@ -287,7 +300,7 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 // first), so a key names its expert in the run; what they cost in precision is part of the bound
 // below.
 //
-// Error of the 32-bit scores (ulp bounds of __expf and __fdividef, 2^-23 = one ulp of 1):
+// Error of the 32-bit scores (2^-23 = one ulp of 1):
 //   sigmoid: e^-l is off by (2 + 1.173 |l|) ulp, which s (1 - s) turns into at most 0.57 ulp of s;
 //            the sum 1 + e^-l and the quotient add 2.5: below 2^-21 altogether.
 //   softmax: p = e^(l - top) inv with inv <= 1 the common factor.  Each exponential is off by at most
@@ -301,6 +314,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps)
     route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
+  __shared__ int32_t chosen[kRouteWarps][kRouteMaxK];
   constexpr uint32_t kPlace = V - 1;  // bits of a key that hold the place in the run
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
@@ -310,21 +324,27 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
   const bool softmax = p.scoring == kRouteSoftmax;
   const int e0 = lane * V;
   const bool off = e0 >= p.experts;  // a lane without experts
+  float b[V];
+  float bias_finite = 0.f;  // NaN once a bias is not finite
+#pragma unroll
+  for (int i = 0; i < V; ++i) b[i] = 0.f;
+  if (p.bias != nullptr && !off) {
+    load_run<float, V>(p.bias, e0, p.experts, p.vec_bias != 0, b);
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias_finite = fmaf(b[i], 0.f, bias_finite);
+  }
   for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
        t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    float l[V], c[V], b[V];
+    float l[V], c[V];
     load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
-#pragma unroll
-    for (int i = 0; i < V; ++i) b[i] = 0.f;
-    if (p.bias != nullptr) load_run<float, V>(p.bias, e0, p.experts, p.vec_bias != 0, b);
     float top = -INFINITY, inv = 1.f;
-    // c of the run.  `all` assumes finite values; otherwise what cannot be chosen becomes -inf.
+    // c of the run.  `all` assumes finite logits and biases; otherwise what cannot be chosen
+    // becomes -inf.
     auto score = [&](auto all) {
       constexpr bool kAll = decltype(all)::value;
-      top = -INFINITY;
-      inv = 1.f;
       if (softmax && (!by_logit || !p.renormalize)) {
+        top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
         if (kAll && off) top = -INFINITY;
@@ -332,34 +352,37 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          c[i] = kAll || l[i] > -INFINITY ? __expf(l[i] - top) : 0.f;
+          c[i] = kAll || l[i] > -INFINITY ? fast_exp(l[i] - top) : 0.f;
           sum += c[i];
         }
         if (kAll && off) sum = 0.f;
         sum = warp_sum(sum);
-        inv = sum > 0.f ? 1.f / sum : 0.f;
+        inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
       }
+      if (by_logit) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (by_logit)
-          c[i] = l[i];
-        else
-          c[i] = (softmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-l[i]))) + b[i];
-        if (!kAll && (!(l[i] > -INFINITY) || c[i] != c[i])) c[i] = -INFINITY;
+        for (int i = 0; i < V; ++i) c[i] = l[i];
+      } else if (softmax) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = c[i] * inv + b[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = fast_rcp(1.f + fast_exp(-l[i])) + b[i];
+      }
+      if (!kAll) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = -INFINITY;
       }
     };
     if (off) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) l[i] = b[i] = 0.f;
+      for (int i = 0; i < V; ++i) l[i] = 0.f;
     }
     score(std::true_type{});
-    // 0 x l is NaN where l is not finite; a bias that is not finite makes c so.
-    float finite = 0.f;
+    float finite = bias_finite;  // 0 x l is NaN where l is not finite
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      finite = fmaf(l[i], 0.f, finite);
-      finite = fmaf(c[i], 0.f, finite);
-    }
+    for (int i = 0; i < V; ++i) finite = fmaf(l[i], 0.f, finite);
     bool bad = false;
     if (__any_sync(0xffffffffu, finite != finite)) {
 #pragma unroll
@@ -418,12 +441,18 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
         slack = 2.f * near + rel * (fabsf(a) + fabsf(a2));
         a += a2;
       }
-      int better = 0;
-      for (int g = 0; g < p.groups; ++g) {
-        const float v = __shfl_sync(0xffffffffu, a, whole ? g * lanes : g);
-        better += (v > a || (v == a && g < group)) ? 1 : 0;
+      // kept_groups times the best group left, the lowest among equals.
+      uint32_t rank_key = real && a > -INFINITY ? order_key(a) : kNoKey;
+      bool kept = false;
+      for (int i = 0; i < p.kept_groups; ++i) {
+        const uint32_t best = __reduce_max_sync(0xffffffffu, rank_key);
+        if (best == kNoKey) break;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, rank_key == best)) - 1;
+        if (group == __shfl_sync(0xffffffffu, group, owner)) {
+          kept = true;
+          rank_key = kNoKey;
+        }
       }
-      const bool kept = real && better < p.kept_groups;
       if (!by_logit) {
         const bool some = real && a > -INFINITY;
         const uint32_t worst_kept =
@@ -455,32 +484,34 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
     for (int i = 0; i < V; ++i)
       key[i] = c[i] > -INFINITY && !off ? (order_key(c[i]) & ~kPlace) | (kPlace - i) : kNoKey;
     sort_keys(key);
-    // The row's largest key without its place bits (all ones), at most kPlace if none is left.
+    // The row's largest key without its place bits (all ones), at most kPlace if none is left, and
+    // the lane that gives it: the lowest among equals.
     auto largest = [&]() { return __reduce_max_sync(0xffffffffu, key[0] | kPlace); };
-    // Takes that key away from its lane, the lowest among equals, and returns its expert.
-    auto take = [&](uint32_t all) {
-      const int owner = __ffs(__ballot_sync(0xffffffffu, (key[0] | kPlace) == all)) - 1;
-      const uint32_t taken = __shfl_sync(0xffffffffu, key[0], owner);
-      if (lane == owner) {
-#pragma unroll
-        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-        key[V - 1] = kNoKey;
-      }
-      return owner * V + static_cast<int>(kPlace - (taken & kPlace));
+    auto holds = [&](uint32_t all) {
+      const bool equal = (key[0] | kPlace) == all;
+      const uint32_t lanes = __ballot_sync(0xffffffffu, equal);
+      return equal && (lanes & ((1u << lane) - 1u)) == 0u;
     };
-    int32_t my_id = -1;
+    auto next = [&]() {  // on to the lane's next key
+#pragma unroll
+      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+      key[V - 1] = kNoKey;
+    };
     uint32_t my_key = kNoKey, last_key = kNoKey;
     int found = 0;
     for (; found < p.k; ++found) {
       const uint32_t all = largest();
       if (all <= kPlace) break;
-      const int id = take(all);
-      if (lane == found) {
-        my_id = id;
-        my_key = all;
+      if (holds(all)) {
+        chosen[warp][found] = e0 + static_cast<int>(kPlace - (key[0] & kPlace));
+        next();
       }
+      if (lane == found) my_key = all;
       last_key = all;
     }
+    __syncwarp();
+    int32_t my_id = lane < found ? chosen[warp][lane] : -1;
+    __syncwarp();
     float my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
     // BF16 logits fit in a key whole: ranked by them, the order is exact.
     if (!(by_logit && (sizeof(T) == 2 || V == 1)) && !close) {
@@ -499,10 +530,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
       while (found == p.k) {
         const uint32_t all = largest();
         if (all <= kPlace || !nearer(last_key, all)) break;
-        const int id = take(all);
-        if (route_load(row + id) != __shfl_sync(0xffffffffu, my_l, p.k - 1) ||
-            (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) !=
-                __shfl_sync(0xffffffffu, my_b, p.k - 1)) {
+        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
+        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
+        bool differs = false;
+        if (holds(all)) {
+          const int id = e0 + static_cast<int>(kPlace - (key[0] & kPlace));
+          differs = route_load(row + id) != last_l ||
+                    (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) != last_b;
+          next();
+        }
+        if (__any_sync(0xffffffffu, differs)) {
           close = true;
           break;
         }
@@ -618,7 +655,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
           sum += out[q][i];
         }
       sum = sum_of(sum);
-      inv = sum > 0.f ? 1.f / sum : 0.f;
+      inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
     }
     const bool has = lj > -INFINITY && !bad;
     float r = 0.f;  // as route_share
@@ -629,38 +666,34 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
       if (has)
         r = p.scoring == kRouteSoftmax || best < -60.f ? expf(lj - best) : sigmoid32(lj);
       const float sum = sum_of(r);
-      r = sum > 0.f ? r / sum : 0.f;
+      r = sum > 0.f ? __fdividef(r, sum) : 0.f;
     }
     float add = 0.f;  // the choice's own term
     float mean = 0.f;
     if (dense || p.renormalize) mean = sum_of(has ? g * r : 0.f);
     if (has) {
       add = p.renormalize ? r * (g - mean) : g * r;
-      if (p.scoring == kRouteSigmoid) add *= 1.f / (1.f + expf(lj));
+      if (p.scoring == kRouteSigmoid) add *= sigmoid32(-lj);
     }
+    // An expert chosen twice: every lane that holds it sums both terms, in the order of j.
     const int at = has ? id : -1;
-    if (dense) {
-#pragma unroll
-      for (int q = 0; q < kVecs; ++q)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) out[q][i] *= -inv * mean;
-    }
+    float sum_at = 0.f;
     for (int j = 0; j < p.k; ++j) {
-      const int ej = __shfl_sync(0xffffffffu, at, j, L) - sub * kPer;
+      const int ej = __shfl_sync(0xffffffffu, at, j, L);
       const float aj = __shfl_sync(0xffffffffu, add, j, L);
-#pragma unroll
-      for (int q = 0; q < kVecs; ++q)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (ej == q * L * kPer + i) out[q][i] += aj;
+      if (ej == at) sum_at += aj;
     }
+    // The row as if nothing were chosen, then the choices over it (ordered by the __syncwarp).
+    T* drow = static_cast<T*>(p.dlogits) + (live ? t : 0) * p.ldd;
+    const float all_scale = bad ? nan_f32() : dense ? -inv * mean * p.scale : 0.f;
 #pragma unroll
     for (int q = 0; q < kVecs; ++q) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) out[q][i] = bad ? nan_f32() : out[q][i] * p.scale;
-      store_run<T, kPer>(static_cast<T*>(p.dlogits) + (live ? t : 0) * p.ldd, (q * L + sub) * kPer,
-                         live ? p.experts : 0, p.vec_out != 0, out[q]);
+      for (int i = 0; i < kPer; ++i) out[q][i] *= all_scale;
+      store_run<T, kPer>(drow, (q * L + sub) * kPer, live ? p.experts : 0, p.vec_out != 0, out[q]);
     }
+    __syncwarp();
+    if (has) route_store(drow + id, (sum_at - (dense ? r * mean : 0.f)) * p.scale);
   }
 }
 
@@ -690,6 +723,8 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
 }
 
 // Shared memory: counts[kOrderWarps][experts], then total[experts].
+// kBits: bits of an expert's index.
+template <int kBits>
 __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const OrderParams p) {
   extern __shared__ uint32_t order_smem[];
   __shared__ uint32_t warp_sums[kOrderWarps];
@@ -716,25 +751,24 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
     for (int u = 0; u < kOrderHold; ++u) {
       const int64_t i = i0 + u * 32 + lane;
       held[u] = i < last ? p.ids[i] : -1;
-      if (held[u] < 0 || held[u] >= E) held[u] = E;  // no expert
+      if (held[u] >= E) held[u] = -1;  // no expert
     }
   };
   // Ranks of the held pairs among the run's pairs of the same expert, counting on in `mine`.  The
   // lanes with the same expert are found by one ballot per bit of it (match.any takes several
   // times as long), and the lowest of them counts them all.
-  const int bits = 32 - __clz(E);  // of 0 .. E
   auto count = [&](int64_t i0) {
 #pragma unroll
     for (int u = 0; u < kOrderHold; ++u) {
       if (i0 + u * 32 >= last) break;
-      uint32_t peers = 0xffffffffu;
-      for (int bit = 0; bit < bits; ++bit) {
-        const bool one = (held[u] >> bit) & 1;
-        const uint32_t v = __ballot_sync(0xffffffffu, one);
-        peers &= one ? v : ~v;
+      const bool real = held[u] >= 0;
+      uint32_t peers = __ballot_sync(0xffffffffu, real);
+#pragma unroll
+      for (int bit = 0; bit < kBits; ++bit) {
+        const uint32_t v = __ballot_sync(0xffffffffu, (held[u] >> bit) & 1);
+        peers &= v ^ (((held[u] >> bit) & 1) - 1u);  // those with the same bit
       }
       const uint32_t before = __popc(peers & ((1u << lane) - 1u));
-      const bool real = held[u] < E;
       rnk[u] = real ? mine[held[u]] + before : 0u;
       __syncwarp();
       if (real && before == 0u) mine[held[u]] = rnk[u] + __popc(peers);
@@ -816,7 +850,7 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
     for (int u = 0; u < kOrderHold; ++u) {
       const int64_t i = i0 + u * 32 + lane;
       if (i < last)
-        p.slots[i] = held[u] < E ? static_cast<int32_t>(rnk[u] + (add ? mine[held[u]] : 0u)) : -1;
+        p.slots[i] = held[u] >= 0 ? static_cast<int32_t>(rnk[u] + (add ? mine[held[u]] : 0u)) : -1;
     }
   };
   if (hold) {
