@@ -236,7 +236,7 @@ int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int6
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   by_lane_values(c->experts, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    const size_t smem = c->groups > 1 ? sizeof(double) * 32 * V * cpg::kRouteWarps : 0;
+    const size_t smem = sizeof(double) * 32 * V * cpg::kRouteWarps;
     p.vec = run_vectors<V>(logits, ld, dtype);
     p.vec_bias = run_vectors<V>(bias, 0, CPG_DTYPE_F32);
     if (dtype == CPG_DTYPE_BF16)

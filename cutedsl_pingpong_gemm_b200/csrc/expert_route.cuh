@@ -136,11 +136,11 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
-// Unsigned keys that order like the floats (no NaN; -0 as +0).  Every key of a number above -inf
-// exceeds kNoKey.
-constexpr uint32_t kNoKey = 0u;
+// Unsigned keys that order like the floats (no NaN; -0 just below +0).  Every key of a number above
+// -inf exceeds kNoKey, the key of -inf.
+constexpr uint32_t kNoKey = 0x007fffffu;
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t b = __float_as_uint(v + 0.f);
+  const uint32_t b = __float_as_uint(v);
   return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
@@ -185,16 +185,14 @@ __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormaliz
   return sum > 0.f ? __fdividef(v, sum) : 0.f;
 }
 
-// The k best experts of a row with c (by_logit: l) in 64 bits: lane j returns choice j, or -1.  l
-// holds the lane's run of logits, -inf where an expert cannot be chosen.  c_sh: 32 * V words of the
-// warp's own shared memory (groups > 1).
+// c of the lane's run (by_logit: l) in 64 bits; l is -inf where an expert cannot be chosen.
 template <int V>
-__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (&l)[V],
-                                             double* c_sh, bool by_logit) {
+__device__ __forceinline__ void route_scores64(const RouteParams& p, const float (&l)[V],
+                                               bool by_logit, double (&c)[V]) {
   const int lane = threadIdx.x & 31;
-  double c[V];
+  const bool softmax = p.scoring == kRouteSoftmax && !by_logit;
   double top = neg_inf(), sum = 0.0;
-  if (p.scoring == kRouteSoftmax && !by_logit) {
+  if (softmax) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmax(top, static_cast<double>(l[i]));
     top = warp_max(top);
@@ -205,48 +203,62 @@ __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (
     if (by_logit)
       c[i] = static_cast<double>(l[i]);
     else if (l[i] > -INFINITY)
-      c[i] = p.scoring == kRouteSoftmax ? exp(static_cast<double>(l[i]) - top)
-                                        : sigmoid64(static_cast<double>(l[i]));
+      c[i] = softmax ? exp(static_cast<double>(l[i]) - top) : sigmoid64(static_cast<double>(l[i]));
     sum += c[i];
   }
-  if (p.scoring == kRouteSoftmax && !by_logit) sum = warp_sum(sum);
+  if (softmax) sum = warp_sum(sum);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = lane * V + i;
-    if (p.scoring == kRouteSoftmax && !by_logit) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
+    if (softmax) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
     if (p.bias != nullptr && e < p.experts) c[i] += static_cast<double>(p.bias[e]);
     if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = neg_inf();
   }
-  if (p.groups > 1) {
-    // Lane g scores group g, ranks it among the others and keeps it if fewer than kept_groups are
-    // better (a higher score, or the same and a lower index).
-    __syncwarp();
+}
+
+// The kept groups of a row, one bit each, ranked in 64 bits: lane g scores group g and keeps it if
+// fewer than kept_groups are better (a higher score, or the same and a lower index).  c_sh: 32 * V
+// words of the warp's own shared memory.
+template <int V>
+__device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const float (&l)[V],
+                                                double* c_sh) {
+  const int lane = threadIdx.x & 31;
+  double c[V];
+  route_scores64<V>(p, l, false, c);
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
-    __syncwarp();
-    const int per = p.experts / p.groups;
-    double a = neg_inf(), b = neg_inf();
-    if (lane < p.groups) {
-      for (int i = 0; i < per; ++i) {
-        const double v = c_sh[lane * per + i];
-        b = fmax(b, fmin(a, v));
-        a = fmax(a, v);
-      }
-      if (p.group_score == kRouteGroupTop2 && b > neg_inf()) a += b;
+  for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
+  __syncwarp();
+  const int per = p.experts / p.groups;
+  double a = neg_inf(), b = neg_inf();
+  if (lane < p.groups) {
+    for (int i = 0; i < per; ++i) {
+      const double v = c_sh[lane * per + i];
+      b = fmax(b, fmin(a, v));
+      a = fmax(a, v);
     }
-    int better = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const double v = __shfl_sync(0xffffffffu, a, g);
-      better += (v > a || (v == a && g < lane)) ? 1 : 0;
-    }
-    const uint32_t keep = __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int g = (lane * V + i) / per;
-      if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = neg_inf();
-    }
-    __syncwarp();
+    if (p.group_score == kRouteGroupTop2 && b > neg_inf()) a += b;
   }
+  int better = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const double v = __shfl_sync(0xffffffffu, a, g);
+    better += (v > a || (v == a && g < lane)) ? 1 : 0;
+  }
+  __syncwarp();
+  return __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
+}
+
+// The k best experts of a row among those whose bit of `open` (one per place of the lane's run) is
+// set, c in 64 bits: lane j returns choice j, or -1.
+template <int V>
+__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (&l)[V],
+                                             uint32_t open, bool by_logit) {
+  const int lane = threadIdx.x & 31;
+  double c[V];
+  route_scores64<V>(p, l, by_logit, c);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (((open >> i) & 1u) == 0u) c[i] = neg_inf();
   int32_t my_id = -1;
   for (int j = 0; j < p.k; ++j) {
     double best = neg_inf();
@@ -308,10 +320,10 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 //            weighted by p, whose mean |l - top| is at most ln 1024; 37 additions; the quotient),
 //            which the largest p <= inv carries: below 2^-18 inv altogether.
 // c = s + bias adds half an ulp of c, a key's lost bits less than V ulp.  Two c nearer than twice the
-// bound are ranked in 64 bits, unless logit and bias are the same: such c are equal, and the lower
-// index goes first.  Measured with 256 experts in 8 groups: about one row in 200.
+// bound are ranked in 64 bits (the choices and what is near the last of them; groups likewise),
+// unless logit and bias are the same: such c are equal, and the lower index goes first.
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kRouteWarps)
+__global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V == 16 ? 4 : 2)))
     route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
   __shared__ int32_t chosen[kRouteWarps][kRouteMaxK];
@@ -324,6 +336,12 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
   const bool softmax = p.scoring == kRouteSoftmax;
   const int e0 = lane * V;
   const bool off = e0 >= p.experts;  // a lane without experts
+  const int per = p.experts / p.groups;  // experts of a group
+  const int lanes = per / V;             // lanes of a group, when that is a whole power of two
+  const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
+  const int group = whole ? lane / lanes : lane;     // the group this lane scores
+  const int first_group = e0 / per;                  // group of the run's first expert ...
+  const int first_left = per - (e0 - first_group * per);  // ... and how many of it follow
   float b[V];
   float bias_finite = 0.f;  // NaN once a bias is not finite
 #pragma unroll
@@ -361,7 +379,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
       }
       if (by_logit) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = l[i];
+        for (int i = 0; i < V; ++i) c[i] = l[i] + 0.f;  // -0 as +0
       } else if (softmax) {
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = c[i] * inv + b[i];
@@ -399,15 +417,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
     // Two c whose difference is at most near + rel (|c1| + |c2|) may be in another order.
     const float near = by_logit ? 0.f : 2.f * (softmax ? 0x1p-18f * inv : 0x1p-21f);
     const float rel = 0x1p-22f + V * 0x1p-23f;
-    bool close = false;
     if (p.groups > 1) {
-      const int per = p.experts / p.groups;
-      const int lanes = per / V;  // lanes of a group, when that is a whole power of two
-      const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
       float a = -INFINITY, a2 = -INFINITY;  // the group's two best
-      int group;
       if (whole) {
-        group = lane / lanes;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           a2 = fmaxf(a2, fminf(a, c[i]));
@@ -420,7 +432,6 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
           a = fmaxf(a, u);
         }
       } else {
-        group = lane;
         float* f_sh = reinterpret_cast<float*>(c_sh);
         __syncwarp();
 #pragma unroll
@@ -436,9 +447,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
         __syncwarp();
       }
       const bool real = group < p.groups;
-      float slack = near + rel * fabsf(a);
+      float slack = 0.5f * near + 0x1p-23f * fabsf(a);
       if (p.group_score == kRouteGroupTop2 && a2 > -INFINITY) {
-        slack = 2.f * near + rel * (fabsf(a) + fabsf(a2));
+        slack = near + 0x1p-22f * (fabsf(a) + fabsf(a2));
         a += a2;
       }
       // kept_groups times the best group left, the lowest among equals.
@@ -459,7 +470,12 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
             __reduce_min_sync(0xffffffffu, kept && some ? order_key(a - slack) : 0xffffffffu);
         const uint32_t best_left =
             __reduce_max_sync(0xffffffffu, !kept && some ? order_key(a + slack) : kNoKey);
-        close = best_left >= worst_kept;
+        if (best_left >= worst_kept) {
+          float l64[V];  // a copy, so that l itself stays in registers
+#pragma unroll
+          for (int i = 0; i < V; ++i) l64[i] = off ? -INFINITY : l[i];
+          kept = (route_groups64<V>(p, l64, c_sh) >> group) & 1u;
+        }
       }
       if (whole) {
         if (!kept) {
@@ -468,7 +484,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
         }
       } else {
         const uint32_t keep = __ballot_sync(0xffffffffu, kept);
-        int g = e0 / per, left = per - (e0 - g * per);  // group of the next element, its rest
+        int g = first_group, left = first_left;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = -INFINITY;
@@ -480,30 +496,35 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
       }
     }
     uint32_t key[V];
+    const uint32_t value_bits = off ? 0u : ~kPlace;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      key[i] = c[i] > -INFINITY && !off ? (order_key(c[i]) & ~kPlace) | (kPlace - i) : kNoKey;
+    for (int i = 0; i < V; ++i) key[i] = (order_key(c[i]) & value_bits) | (kPlace - i);
     sort_keys(key);
-    // The row's largest key without its place bits (all ones), at most kPlace if none is left, and
+    // The lane's first key stays in a register, the others wait in shared memory.
+    uint32_t head = key[0];
+    uint32_t* rest = reinterpret_cast<uint32_t*>(c_sh) + lane;
+#pragma unroll
+    for (int i = 1; i < V; ++i) rest[32 * (i - 1)] = key[i];
+    rest[32 * (V - 1)] = 0u;
+    // The row's largest key without its place bits (all ones), at most kNoKey if none is left, and
     // the lane that gives it: the lowest among equals.
-    auto largest = [&]() { return __reduce_max_sync(0xffffffffu, key[0] | kPlace); };
+    auto largest = [&]() { return __reduce_max_sync(0xffffffffu, head | kPlace); };
     auto holds = [&](uint32_t all) {
-      const bool equal = (key[0] | kPlace) == all;
+      const bool equal = (head | kPlace) == all;
       const uint32_t lanes = __ballot_sync(0xffffffffu, equal);
       return equal && (lanes & ((1u << lane) - 1u)) == 0u;
     };
     auto next = [&]() {  // on to the lane's next key
-#pragma unroll
-      for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-      key[V - 1] = kNoKey;
+      head = *rest;
+      rest += 32;
     };
     uint32_t my_key = kNoKey, last_key = kNoKey;
     int found = 0;
     for (; found < p.k; ++found) {
       const uint32_t all = largest();
-      if (all <= kPlace) break;
+      if (all <= kNoKey) break;
       if (holds(all)) {
-        chosen[warp][found] = e0 + static_cast<int>(kPlace - (key[0] & kPlace));
+        chosen[warp][found] = e0 + static_cast<int>(kPlace - (head & kPlace));
         next();
       }
       if (lane == found) my_key = all;
@@ -513,8 +534,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
     int32_t my_id = lane < found ? chosen[warp][lane] : -1;
     __syncwarp();
     float my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
+    bool near_pair = false;
+    int candidates = found;
     // BF16 logits fit in a key whole: ranked by them, the order is exact.
-    if (!(by_logit && (sizeof(T) == 2 || V == 1)) && !close) {
+    bool many = false;  // more candidates than lanes
+    if (!(by_logit && (sizeof(T) == 2 || V == 1))) {
       auto nearer = [&](uint32_t k1, uint32_t k2) {
         const float c1 = key_value(k1 & ~kPlace), c2 = key_value(k2 & ~kPlace);
         return by_logit ? c1 == c2 : c1 - c2 <= near + rel * (fabsf(c1) + fabsf(c2));
@@ -524,32 +548,70 @@ __global__ void __launch_bounds__(32 * kRouteWarps)
       const uint32_t next_key = __shfl_down_sync(0xffffffffu, my_key, 1);
       const float next_l = __shfl_down_sync(0xffffffffu, my_l, 1);
       const float next_b = __shfl_down_sync(0xffffffffu, my_b, 1);
-      close = lane + 1 < found && nearer(my_key, next_key) &&
-              !(my_l == next_l && my_b == next_b);
-      // The last choice against the best ones left, past those that are equal to it.
+      near_pair = lane + 1 < found && nearer(my_key, next_key) &&
+                  !(my_l == next_l && my_b == next_b);
+      // The last choice against the best ones left: those that are near become candidates too.
       while (found == p.k) {
         const uint32_t all = largest();
-        if (all <= kPlace || !nearer(last_key, all)) break;
-        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
-        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
-        bool differs = false;
-        if (holds(all)) {
-          const int id = e0 + static_cast<int>(kPlace - (key[0] & kPlace));
-          differs = route_load(row + id) != last_l ||
-                    (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) != last_b;
-          next();
-        }
-        if (__any_sync(0xffffffffu, differs)) {
-          close = true;
+        if (all <= kNoKey || !nearer(last_key, all)) break;
+        if (candidates == kRouteMaxK) {
+          many = true;
           break;
         }
+        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
+        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
+        if (holds(all)) {
+          const int id = e0 + static_cast<int>(kPlace - (head & kPlace));
+          chosen[warp][candidates] = id;
+          near_pair |= route_load(row + id) != last_l ||
+                       (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) != last_b;
+          next();
+        }
+        ++candidates;
       }
     }
-    if (__any_sync(0xffffffffu, close)) {
-      float l64[V];  // a copy, so that l itself stays in registers
+    if (__any_sync(0xffffffffu, near_pair)) {
+      __syncwarp();
+      if (many) {
+        float l64[V];
+        uint32_t open = 0u;
 #pragma unroll
-      for (int i = 0; i < V; ++i) l64[i] = off ? -INFINITY : l[i];
-      my_id = route_rank64<V>(p, l64, c_sh, by_logit);
+        for (int i = 0; i < V; ++i) {
+          l64[i] = off ? -INFINITY : l[i];
+          if (c[i] > -INFINITY) open |= 1u << i;
+        }
+        my_id = route_rank64<V>(p, l64, open, by_logit);
+      } else {
+        // Lane j ranks candidate j among the candidates in 64 bits.
+        const int32_t id = lane < candidates ? chosen[warp][lane] : -1;
+        double mine = neg_inf();
+        if (id >= 0) mine = static_cast<double>(route_load(row + id));
+        if (!by_logit) {
+          if (softmax) {
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (l[i] > -INFINITY && !off)
+                sum += exp(static_cast<double>(l[i]) - static_cast<double>(top));
+            sum = warp_sum(sum);
+            mine = exp(mine - static_cast<double>(top)) / sum;
+          } else {
+            mine = sigmoid64(mine);
+          }
+          if (id >= 0 && p.bias != nullptr) mine += static_cast<double>(p.bias[id]);
+        }
+        int rank = 0;
+        for (int i = 0; i < candidates; ++i) {
+          const double v = __shfl_sync(0xffffffffu, mine, i);
+          const int32_t other = __shfl_sync(0xffffffffu, id, i);
+          rank += (v > mine || (v == mine && other < id)) ? 1 : 0;
+        }
+        __syncwarp();
+        if (id >= 0 && rank < p.k) chosen[warp][rank] = id;
+        __syncwarp();
+        my_id = lane < found ? chosen[warp][lane] : -1;
+        __syncwarp();
+      }
       my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
     }
     const bool has = my_id >= 0;

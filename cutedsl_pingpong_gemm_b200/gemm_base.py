@@ -63,7 +63,10 @@ def _stream_handle(stream, device) -> int:
     """cudaStream_t value for None / torch stream / cuda-python CUstream / int."""
     import torch
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        index = getattr(device, "index", device)
+        if index is None:
+            index = torch.cuda.current_device()
+        return torch._C._cuda_getCurrentRawStream(index)
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     if isinstance(stream, int):
@@ -106,9 +109,19 @@ class CompiledGemm:
     def __init__(self, gemm: "GemmSM90"):
         self.gemm = gemm
         self._plans = {}
+        self._seen = {}  # plan of every combination of tensors' layouts seen so far
         self._workspaces = {}
 
     def _plan(self, a, b, c, scale_mode: int = 0, split_k: int = 1, gated: bool = False):
+        # Everything below depends on the tensors' types, sizes, strides and devices only.
+        seen = (a.dtype, a.shape, a.stride(), b.dtype, b.shape, b.stride(), c.dtype, c.shape,
+                c.stride(), a.device, b.device, c.device, scale_mode, split_k, gated)
+        plan = self._seen.get(seen)
+        if plan is None:
+            plan = self._seen[seen] = self._new_plan(a, b, c, scale_mode, split_k, gated)
+        return plan
+
+    def _new_plan(self, a, b, c, scale_mode, split_k, gated):
         import torch
         gemm = self.gemm
         ab_codes, d_codes = _dtype_tables()
@@ -299,6 +312,7 @@ class CompiledGemm:
         call plans again.  Call it only when no launch that uses them is still running and no
         captured CUDA graph will replay them (a graph keeps the pointers it was captured with)."""
         self._plans.clear()
+        self._seen.clear()
         self._workspaces.clear()
 
     def auto_split_k(self, m: int, n: int, k: int, batches: int = 1) -> int:
@@ -367,9 +381,19 @@ class _Plan:
         self.lib = _lib.load()
         self.m, self.n, self.k = m, n, k
         self.l = l
-        self.gated = bool(gated)
         self.device = device
         self.scale_mode = scale_mode
+        if scale_mode == _lib.CPG_SCALE_BLOCK:
+            nkb, nnb = -(-k // 128), -(-n // 128)
+            self.scale_shapes = {"scale_a": (nkb, m), "scale_b": (nnb, nkb)}
+        else:
+            # One value, or (INT8) one per row of A and of B, of every batch or group.
+            b_rows = 2 * n if gated else n
+            rows_a = (l, m) if l and not grouped else (m,)
+            rows_b = (l, b_rows) if l or grouped else (b_rows,)
+            self.scale_shapes = {
+                "scale_a": rows_a if scale_mode & _lib.CPG_SCALE_ROWS_A else (1,),
+                "scale_b": rows_b if scale_mode & _lib.CPG_SCALE_ROWS_B else (1,)}
         cfg = gemm._config_c()
         prob = _lib.GemmProblemC(m, n, k, lda, ldb, ldd, dtype_ab, dtype_d, scale_mode, split_k,
                                  1 if gated else 0, l, batch_stride_a, batch_stride_b,
@@ -434,22 +458,13 @@ class _Plan:
             if bias.stride(-1) != 1:
                 raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED, "bias must be contiguous")
         scales = []
-        if self.scale_mode == _lib.CPG_SCALE_BLOCK:
-            nkb, nnb = -(-self.k // 128), -(-self.n // 128)
-            want = {"scale_a": (nkb, self.m), "scale_b": (nnb, nkb)}
-        else:
-            # One value, or (INT8) one per row of A and of B, of every batch or group.
-            b_rows = 2 * self.n if self.gated else self.n
-            rows_a = (self.l, self.m) if self.l and not self.grouped else (self.m,)
-            rows_b = (self.l, b_rows) if self.l or self.grouped else (b_rows,)
-            want = {"scale_a": rows_a if self.scale_mode & _lib.CPG_SCALE_ROWS_A else (1,),
-                    "scale_b": rows_b if self.scale_mode & _lib.CPG_SCALE_ROWS_B else (1,)}
         for name, sc in (("scale_a", scale_a), ("scale_b", scale_b)):
-            if sc is not None and not (sc.is_cuda and sc.dtype == torch.float32 and sc.is_contiguous()
-                                       and sc.numel() == math.prod(want[name])):
+            if sc is not None and not (sc.is_cuda and sc.dtype == torch.float32
+                                       and sc.is_contiguous()
+                                       and sc.numel() == math.prod(self.scale_shapes[name])):
                 raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
                                     f"{name} must be a contiguous float32 CUDA tensor of shape "
-                                    f"{want[name]}")
+                                    f"{self.scale_shapes[name]}")
             scales.append(None if sc is None else sc.data_ptr())
         src_ptr, ld_src, bs_src = None, 0, 0
         if source is not None:
@@ -473,7 +488,8 @@ class _Plan:
             rc = self.lib.cpg_gemm_run(self.handle, a.data_ptr() if a.numel() else None,
                                        b.data_ptr() if b.numel() else None, c.data_ptr(),
                                        ctypes.byref(epi), st)
-        _lib.check(rc, "gemm")
+        if rc != _lib.CPG_OK:
+            _lib.check(rc, "gemm")
 
 
 class GemmSM90:

@@ -48,7 +48,9 @@ def quantize_e4m3(x, block: Optional[Tuple[int, int]] = None):
 def alloc_int8_rows(rows: int, cols: int, device):
     """int8 [rows, cols] whose rows start on 16 bytes, as the GEMM's loads need."""
     import torch
-    return torch.empty(rows, -(-cols // 16) * 16, dtype=torch.int8, device=device)[:, :cols]
+    if cols % 16 == 0:
+        return torch.empty((rows, cols), dtype=torch.int8, device=device)
+    return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
 
 
 def quantize_int8(x, out=None, scales=None):
@@ -57,29 +59,20 @@ def quantize_int8(x, out=None, scales=None):
     column stride) and ``scales`` may be given as outputs.  Rows of zeros get q = 0 and a tiny
     scale; a row that holds an infinity or NaN gets q = 0 and the scale NaN."""
     import torch
+    from . import moe
     if not x.is_cuda or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise _lib.CpgError(_lib.CPG_ERR_DTYPE, "x must be a 2-D BF16 or FP32 CUDA tensor")
-    if x.numel() and x.shape[1] > 1 and x.stride(1) != 1:
-        raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED, "x must have unit column stride")
-    rows, cols = x.shape
+    rows, cols, ldx = moe._matrix("x", x)
+    device = x.device
     if out is None:
-        out = alloc_int8_rows(rows, cols, x.device)
+        out = alloc_int8_rows(rows, cols, device)
+    ldq = moe._output("out", out, (rows, cols), torch.int8, device)
     if scales is None:
-        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    if (out.dtype != torch.int8 or out.shape != x.shape or out.device != x.device
-            or (out.numel() and ((cols > 1 and out.stride(1) != 1)
-                                 or (rows > 1 and out.stride(0) < cols)))):
-        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
-                            "out must be an int8 tensor of x's shape with unit column stride")
-    if (scales.dtype != torch.float32 or tuple(scales.shape) != (rows,)
-            or scales.device != x.device or not scales.is_contiguous()):
-        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE, "scales must be contiguous FP32 [rows]")
-    dt = _lib.CPG_DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.CPG_DTYPE_F32
-    from .moe import _call
-    _call(_lib.load().cpg_quantize_int8, "quantize_int8", x.device,
-          x.data_ptr() if x.numel() else None, dt, rows, cols, x.stride(0) if rows > 1 else cols,
-          out.data_ptr() if out.numel() else None, out.stride(0) if rows > 1 else cols,
-          scales.data_ptr() if rows else None)
+        scales = torch.empty(rows, dtype=torch.float32, device=device)
+    else:
+        moe._vector("scales", scales, (rows,), torch.float32, device)
+    moe._call(_lib.load().cpg_quantize_int8, "quantize_int8", device, moe._ptr(x),
+              moe._float_code("x", x), rows, cols, ldx, moe._ptr(out), ldq, moe._ptr(scales))
     return out, scales
 
 

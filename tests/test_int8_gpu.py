@@ -369,7 +369,7 @@ def test_quantize_refusals():
                       (lambda: quantize_int8(x[0]), _lib.CPG_ERR_DTYPE),
                       (lambda: quantize_int8(x.t()), _lib.CPG_ERR_UNSUPPORTED),
                       (lambda: quantize_int8(x, out=torch.empty(4, 8, device="cuda")),
-                       _lib.CPG_ERR_INVALID_SHAPE),
+                       _lib.CPG_ERR_DTYPE),
                       (lambda: quantize_int8(x, out=torch.empty(1, 8, dtype=torch.int8,
                                                                 device="cuda").expand(4, 8)),
                        _lib.CPG_ERR_INVALID_SHAPE),
