@@ -185,11 +185,16 @@ __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormaliz
   return sum > 0.f ? __fdividef(v, sum) : 0.f;
 }
 
-// c of the lane's run (by_logit: l) in 64 bits; l is -inf where an expert cannot be chosen.
-template <int V>
-__device__ __forceinline__ void route_scores64(const RouteParams& p, const float (&l)[V],
-                                               bool by_logit, double (&c)[V]) {
+// c of the lane's run of the row (by_logit: l) in 64 bits, -inf where an expert cannot be chosen.
+template <typename T, int V>
+__device__ __forceinline__ void route_scores64(const RouteParams& p, const T* row, bool by_logit,
+                                               double (&c)[V]) {
   const int lane = threadIdx.x & 31;
+  float l[V];
+  load_run<T, V>(row, lane * V, p.experts, p.vec != 0, l);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (route_bad(l[i], p.scoring)) l[i] = -INFINITY;
   const bool softmax = p.scoring == kRouteSoftmax && !by_logit;
   double top = neg_inf(), sum = 0.0;
   if (softmax) {
@@ -219,12 +224,12 @@ __device__ __forceinline__ void route_scores64(const RouteParams& p, const float
 // The kept groups of a row, one bit each, ranked in 64 bits: lane g scores group g and keeps it if
 // fewer than kept_groups are better (a higher score, or the same and a lower index).  c_sh: 32 * V
 // words of the warp's own shared memory.
-template <int V>
-__device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const float (&l)[V],
+template <typename T, int V>
+__device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const T* row,
                                                 double* c_sh) {
   const int lane = threadIdx.x & 31;
   double c[V];
-  route_scores64<V>(p, l, false, c);
+  route_scores64<T, V>(p, row, false, c);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
@@ -248,14 +253,49 @@ __device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const floa
   return __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
 }
 
+// Place of this lane's candidate id (-1: none) among the first `candidates` lanes', c in 64 bits.
+template <typename T, int V>
+__device__ __noinline__ int route_place64(const RouteParams& p, const T* row, int32_t id,
+                                          int candidates, bool by_logit) {
+  double mine = neg_inf();
+  if (id >= 0) mine = static_cast<double>(route_load(row + id));
+  if (!by_logit) {
+    if (p.scoring == kRouteSoftmax) {
+      float l[V];
+      load_run<T, V>(row, (threadIdx.x & 31) * V, p.experts, p.vec != 0, l);
+      double top = neg_inf(), sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (route_bad(l[i], p.scoring)) l[i] = -INFINITY;
+        top = fmax(top, static_cast<double>(l[i]));
+      }
+      top = warp_max(top);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (l[i] > -INFINITY) sum += exp(static_cast<double>(l[i]) - top);
+      mine = exp(mine - top) / warp_sum(sum);
+    } else {
+      mine = sigmoid64(mine);
+    }
+    if (id >= 0 && p.bias != nullptr) mine += static_cast<double>(p.bias[id]);
+  }
+  int place = 0;
+  for (int i = 0; i < candidates; ++i) {
+    const double v = __shfl_sync(0xffffffffu, mine, i);
+    const int32_t other = __shfl_sync(0xffffffffu, id, i);
+    place += (v > mine || (v == mine && other < id)) ? 1 : 0;
+  }
+  return place;
+}
+
 // The k best experts of a row among those whose bit of `open` (one per place of the lane's run) is
 // set, c in 64 bits: lane j returns choice j, or -1.
-template <int V>
-__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const float (&l)[V],
-                                             uint32_t open, bool by_logit) {
+template <typename T, int V>
+__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const T* row, uint32_t open,
+                                             bool by_logit) {
   const int lane = threadIdx.x & 31;
   double c[V];
-  route_scores64<V>(p, l, by_logit, c);
+  route_scores64<T, V>(p, row, by_logit, c);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (((open >> i) & 1u) == 0u) c[i] = neg_inf();
@@ -323,7 +363,7 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 // bound are ranked in 64 bits (the choices and what is near the last of them; groups likewise),
 // unless logit and bias are the same: such c are equal, and the lower index goes first.
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V == 16 ? 4 : 2)))
+__global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 2))
     route_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ double route_smem[];
   __shared__ int32_t chosen[kRouteWarps][kRouteMaxK];
@@ -342,20 +382,23 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V
   const int group = whole ? lane / lanes : lane;     // the group this lane scores
   const int first_group = e0 / per;                  // group of the run's first expert ...
   const int first_left = per - (e0 - first_group * per);  // ... and how many of it follow
-  float b[V];
-  float bias_finite = 0.f;  // NaN once a bias is not finite
-#pragma unroll
-  for (int i = 0; i < V; ++i) b[i] = 0.f;
-  if (p.bias != nullptr && !off) {
-    load_run<float, V>(p.bias, e0, p.experts, p.vec_bias != 0, b);
-#pragma unroll
-    for (int i = 0; i < V; ++i) bias_finite = fmaf(b[i], 0.f, bias_finite);
-  }
   for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
        t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
     float l[V], c[V];
     load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
+    bool bad = false;
+    // l with what cannot be chosen at -inf.
+    auto clean = [&]() {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (route_bad(l[i], p.scoring)) {
+          bad = true;
+          l[i] = -INFINITY;
+        }
+        if (off) l[i] = -INFINITY;
+      }
+    };
     float top = -INFINITY, inv = 1.f;
     // c of the run.  `all` assumes finite logits and biases; otherwise what cannot be chosen
     // becomes -inf.
@@ -380,12 +423,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V
       if (by_logit) {
 #pragma unroll
         for (int i = 0; i < V; ++i) c[i] = l[i] + 0.f;  // -0 as +0
-      } else if (softmax) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = c[i] * inv + b[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = fast_rcp(1.f + fast_exp(-l[i])) + b[i];
+        for (int i = 0; i < V; ++i)
+          c[i] = softmax ? c[i] * inv : fast_rcp(1.f + fast_exp(-l[i]));
+        if (p.bias != nullptr && !off) {
+          float b[V];
+          load_run<float, V>(p.bias, e0, p.experts, p.vec_bias != 0, b);
+#pragma unroll
+          for (int i = 0; i < V; ++i) c[i] += b[i];
+        }
       }
       if (!kAll) {
 #pragma unroll
@@ -398,25 +445,22 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V
       for (int i = 0; i < V; ++i) l[i] = 0.f;
     }
     score(std::true_type{});
-    float finite = bias_finite;  // 0 x l is NaN where l is not finite
+    float finite = 0.f;  // 0 x l is NaN where l is not finite; a bias that is not makes c so
 #pragma unroll
     for (int i = 0; i < V; ++i) finite = fmaf(l[i], 0.f, finite);
-    bool bad = false;
-    if (__any_sync(0xffffffffu, finite != finite)) {
+    if (!by_logit) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (route_bad(l[i], p.scoring)) {
-          bad = true;
-          l[i] = -INFINITY;
-        }
-        if (off) l[i] = -INFINITY;
-      }
+      for (int i = 0; i < V; ++i) finite = fmaf(c[i], 0.f, finite);
+    }
+    if (__any_sync(0xffffffffu, finite != finite)) {
+      clean();
       bad = __any_sync(0xffffffffu, bad);
       score(std::false_type{});
     }
     // Two c whose difference is at most near + rel (|c1| + |c2|) may be in another order.
     const float near = by_logit ? 0.f : 2.f * (softmax ? 0x1p-18f * inv : 0x1p-21f);
     const float rel = 0x1p-22f + V * 0x1p-23f;
+    uint32_t open = ~0u;  // one bit per place of the run: its group is kept
     if (p.groups > 1) {
       float a = -INFINITY, a2 = -INFINITY;  // the group's two best
       if (whole) {
@@ -471,28 +515,27 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V
         const uint32_t best_left =
             __reduce_max_sync(0xffffffffu, !kept && some ? order_key(a + slack) : kNoKey);
         if (best_left >= worst_kept) {
-          float l64[V];  // a copy, so that l itself stays in registers
-#pragma unroll
-          for (int i = 0; i < V; ++i) l64[i] = off ? -INFINITY : l[i];
-          kept = (route_groups64<V>(p, l64, c_sh) >> group) & 1u;
+          kept = (route_groups64<T, V>(p, row, c_sh) >> group) & 1u;
         }
       }
       if (whole) {
-        if (!kept) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) c[i] = -INFINITY;
-        }
+        if (!kept) open = 0u;
       } else {
         const uint32_t keep = __ballot_sync(0xffffffffu, kept);
         int g = first_group, left = first_left;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          if (g >= p.groups || ((keep >> g) & 1u) == 0u) c[i] = -INFINITY;
+          if (g >= p.groups || ((keep >> g) & 1u) == 0u) open &= ~(1u << i);
           if (--left == 0) {
             left = per;
             ++g;
           }
         }
+      }
+      if (open != ~0u) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (((open >> i) & 1u) == 0u) c[i] = -INFINITY;
       }
     }
     uint32_t key[V];
@@ -573,39 +616,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V < 8 ? 8 : (V == 8 ? 6 : (V
     if (__any_sync(0xffffffffu, near_pair)) {
       __syncwarp();
       if (many) {
-        float l64[V];
-        uint32_t open = 0u;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          l64[i] = off ? -INFINITY : l[i];
-          if (c[i] > -INFINITY) open |= 1u << i;
-        }
-        my_id = route_rank64<V>(p, l64, open, by_logit);
+        my_id = route_rank64<T, V>(p, row, open, by_logit);
       } else {
-        // Lane j ranks candidate j among the candidates in 64 bits.
         const int32_t id = lane < candidates ? chosen[warp][lane] : -1;
-        double mine = neg_inf();
-        if (id >= 0) mine = static_cast<double>(route_load(row + id));
-        if (!by_logit) {
-          if (softmax) {
-            double sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (l[i] > -INFINITY && !off)
-                sum += exp(static_cast<double>(l[i]) - static_cast<double>(top));
-            sum = warp_sum(sum);
-            mine = exp(mine - static_cast<double>(top)) / sum;
-          } else {
-            mine = sigmoid64(mine);
-          }
-          if (id >= 0 && p.bias != nullptr) mine += static_cast<double>(p.bias[id]);
-        }
-        int rank = 0;
-        for (int i = 0; i < candidates; ++i) {
-          const double v = __shfl_sync(0xffffffffu, mine, i);
-          const int32_t other = __shfl_sync(0xffffffffu, id, i);
-          rank += (v > mine || (v == mine && other < id)) ? 1 : 0;
-        }
+        const int rank = route_place64<T, V>(p, row, id, candidates, by_logit);
         __syncwarp();
         if (id >= 0 && rank < p.k) chosen[warp][rank] = id;
         __syncwarp();
