@@ -470,6 +470,8 @@ static int alloc_fixup_workspace(cpg_gemm* g, int64_t tiles) {
 using DecodeFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
                           const cpg::DecodeParams);
 
+constexpr int kDecodeInt8Stages = 6;
+
 static const void* decode_kernel(int dtype_ab, int dtype_d, int cta_group) {
   const bool fp8 = dtype_ab == CPG_DTYPE_E4M3, f32 = dtype_d == CPG_DTYPE_F32;
   DecodeFn fn;
@@ -547,6 +549,11 @@ static int create_decode_plan(const cpg_gemm_config* cfg, const cpg_gemm_problem
   }
   if (stages == 0) return fail(CPG_ERR_SMEM, "the small-M kernel does not fit in shared memory");
   if (kps >= 2 && stages > kps) stages = static_cast<int>(kps);
+  // INT8 halves the loads of a BF16 tile while the waits stay the same, so the next call's set-up
+  // counts for more: with at most 6 stages of 16 rows two calls' CTAs fit on an SM.  Back to back on
+  // N = K = 8192, 12 and 6 stages: M = 1 17.1 and 15.7 us, 16 18.1 and 16.6, 64 19.2 and 18.9, 128
+  // (which has room for no more) 23.2.
+  if (int8 && stages > kDecodeInt8Stages) stages = kDecodeInt8Stages;
   if (env_st != nullptr && std::atoi(env_st) >= 2 && std::atoi(env_st) < stages)
     stages = std::atoi(env_st);
   if (stages < 2) stages = 2;

@@ -14,7 +14,7 @@
 
 #include <type_traits>
 
-#include "ptx.cuh"
+#include "expert_rows.cuh"
 
 namespace cpg {
 
@@ -365,6 +365,7 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 2))
     route_kernel(const __grid_constant__ RouteParams p) {
+  kernel_begins();
   extern __shared__ double route_smem[];
   __shared__ int32_t chosen[kRouteWarps][kRouteMaxK];
   constexpr uint32_t kPlace = V - 1;  // bits of a key that hold the place in the run
@@ -660,6 +661,7 @@ struct RouteGradParams {
 // twice gets both terms.
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const RouteGradParams p) {
+  kernel_begins();
   constexpr int kPer = 16 / static_cast<int>(sizeof(T)) < V ? 16 / static_cast<int>(sizeof(T)) : V;
   constexpr int kVecs = V / kPer;  // vectors of kPer logits a lane holds
   constexpr int kTokens = 32 / L * kRouteWarps;
@@ -802,6 +804,7 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
 // kBits: bits of an expert's index.
 template <int kBits>
 __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const OrderParams p) {
+  kernel_begins();
   extern __shared__ uint32_t order_smem[];
   __shared__ uint32_t warp_sums[kOrderWarps];
   const int lane = threadIdx.x & 31;

@@ -10,6 +10,11 @@
 
 namespace cpg {
 
+// The first statement of every kernel here: the previous kernel's writes are visible after it.  (All
+// but the INT8 row kernels are launched as programmatic dependents, so they may be set up while
+// that kernel finishes; for the others it returns at once.)
+__device__ __forceinline__ void kernel_begins() { ptx::griddep_wait(); }
+
 constexpr float kInt8Max = 127.0f;
 constexpr float kInt8AmaxFloor = 1e-12f;
 
@@ -201,6 +206,7 @@ struct RowsParams {
 // q = rint(x / s) with s = max|x[t]| / 127 in scales[slot].
 template <typename T, typename OutT>
 __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
+  kernel_begins();
   constexpr bool kQuant = sizeof(OutT) == 1;
   __shared__ uint32_t red[8];
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
@@ -240,6 +246,9 @@ constexpr int kInt8Vecs = 4;
 
 template <typename T, int G, bool Resident>
 __global__ void __launch_bounds__(256, 16 / sizeof(T) / 2) rows_int8_vec_kernel(const RowsParams p) {
+  // The small-M product that reads these rows may be set up, and fetch its first weights, already.
+  ptx::griddep_launch_dependents();
+  kernel_begins();
   constexpr int NV = kInt8Vecs;
   constexpr int kVecs = 16 / RowVec<T>::kElems;
   constexpr int kE = RowVec<T>::kElems;
@@ -318,6 +327,7 @@ constexpr int kCopyVecs = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(256) rows_copy_vec_kernel(const RowsParams p, int32_t chunks) {
+  kernel_begins();
   constexpr int kE = RowVec<T>::kElems;
   const int lane = threadIdx.x & 31;
   const int32_t cols = static_cast<int32_t>(p.cols);
@@ -364,6 +374,7 @@ struct CombineParams {
 // y[t] = source[t] + sum_j w[t][j] rows[slot[t][j]], summed in fp32 in the order of j.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  kernel_begins();
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
       float acc = p.source != nullptr
@@ -387,6 +398,7 @@ constexpr int kCombineVecs = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p, int32_t chunks) {
+  kernel_begins();
   constexpr int kE = RowVec<T>::kElems;
   constexpr int kBatch = 4;
   const int lane = threadIdx.x & 31;
@@ -469,6 +481,7 @@ struct CombineGradParams {
 // drows[slot] = w dy[t] and dw[t][j] = <dy[t], rows[slot]>: one warp per (token, choice).
 template <typename T>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineGradParams p) {
+  kernel_begins();
   const int lane = threadIdx.x & 31;
   const int64_t pairs = p.tokens * p.k;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
@@ -496,6 +509,7 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineGradPara
 // As combine_grad_kernel for rows of whole vectors, four vectors of dy and of the row in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_grad_vec_kernel(const CombineGradParams p) {
+  kernel_begins();
   constexpr int kE = RowVec<T>::kElems;
   constexpr int kVecs = 4;
   const int lane = threadIdx.x & 31;

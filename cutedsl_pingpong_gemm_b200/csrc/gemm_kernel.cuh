@@ -1168,6 +1168,36 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
       // Stream-K with fixup, and split-K into peer memory: a segment with part of a tile's
       // k-blocks adds into the workspace.
       const bool partial = p.fixup != 0 && (sg.kb0 != 0 || sg.kb1 != p.k_iters);
+      const int32_t g_row = sg.row_base + pid_m * kBM + static_cast<int32_t>(row_in_tile);
+      const int32_t my_row = g_row + static_cast<int32_t>(lane);
+      // Rows of this warp that belong to the tile's problem (a grouped tile may end inside).
+      const int32_t row_end = sg.row_end < p.m ? sg.row_end : p.m;
+      // A gated 512-wide tile holds gate columns [0, 256) and up columns [256, 512) of the same
+      // 256 output columns.
+      const int out_cols = gated ? BN / 2 : BN;
+      const int n_chunks = out_cols / kStoreCols;
+      // This warp's chunks [c_begin, c_end) of the tile's columns.
+      const int c_begin = half * n_chunks / ES::kHalves;
+      const int c_end = (half + 1) * n_chunks / ES::kHalves;
+      // INT8: this row's scale (with alpha), and the columns' scales of the tile's batch or group.
+      // Rows outside the problem are not stored; they take the scale 0 without reading it.
+      float row_alpha = alpha;
+      const float* col_scale = nullptr;
+      if constexpr (OT::kInt8) {
+        if (p.row_scale != nullptr)
+          row_alpha *= my_row < row_end
+                           ? __ldg(p.row_scale + static_cast<int64_t>(sg.ab_batch) * p.m + my_row)
+                           : 0.f;
+        if (p.col_scale != nullptr) {
+          col_scale = p.col_scale + static_cast<int64_t>(sg.batch) * p.col_scale_len;
+          // Its lines of this warp's columns come into L1 while the warp waits for the accumulator.
+          const int32_t col = pid_n * out_cols + c_begin * kStoreCols + 32 * static_cast<int32_t>(lane);
+          if (static_cast<int32_t>(lane) < (c_end - c_begin) * kStoreCols / 32 && col < p.n) {
+            ptx::prefetch_l1(col_scale + col);
+            if (gated) ptx::prefetch_l1(col_scale + p.n + col);
+          }
+        }
+      }
       bool ok = ptx::mbar_wait(tfull_bar + 8u * acc, acc_phase, ctx, kSiteEpiTmemFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -1181,17 +1211,6 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
       }
       __syncwarp();
       const uint32_t t_row = tmem_base + (row_in_tile << 16) + static_cast<uint32_t>(acc * BN);
-      const int32_t g_row = sg.row_base + pid_m * kBM + static_cast<int32_t>(row_in_tile);
-      const int32_t my_row = g_row + static_cast<int32_t>(lane);
-      // Rows of this warp that belong to the tile's problem (a grouped tile may end inside).
-      const int32_t row_end = sg.row_end < p.m ? sg.row_end : p.m;
-      // A gated 512-wide tile holds gate columns [0, 256) and up columns [256, 512) of the same
-      // 256 output columns.
-      const int out_cols = gated ? BN / 2 : BN;
-      const int n_chunks = out_cols / kStoreCols;
-      // This warp's chunks [c_begin, c_end) of the tile's columns.
-      const int c_begin = half * n_chunks / ES::kHalves;
-      const int c_end = (half + 1) * n_chunks / ES::kHalves;
       // This warp's 32 workspace rows (the CTA tile's workspace tile; partial segments only).
       // Stream-K numbers the split tiles after the data-parallel ones; split-K (L = K range)
       // shares one workspace tile between the K ranges of a tile.
@@ -1242,15 +1261,7 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
       };
       // Round x (kStoreCols columns of this thread's row, from column col0) to D's type and
       // store it.
-      auto store_chunk = [&](const float (&x)[kStoreCols], int32_t col0) {
-        uint32_t packed[32];  // 128 bytes of this thread's output row
-        if constexpr (sizeof(OutT) == 2) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) packed[i] = ptx::pack_bf16x2(x[2 * i], x[2 * i + 1]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) packed[i] = __float_as_uint(x[i]);
-        }
+      auto store_packed = [&](const uint32_t (&packed)[32], int32_t col0) {
         const uint32_t sbuf = stage(packed);
         // The TMA box covers this warp's 32 rows and is clipped at D's last row; a grouped
         // tile whose group ends inside the box (before D ends) would write the next group's
@@ -1270,6 +1281,17 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
           ptx::bulk_commit_group();
         }
         __syncwarp();
+      };
+      auto store_chunk = [&](const float (&x)[kStoreCols], int32_t col0) {
+        uint32_t packed[32];  // 128 bytes of this thread's output row
+        if constexpr (sizeof(OutT) == 2) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) packed[i] = ptx::pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) packed[i] = __float_as_uint(x[i]);
+        }
+        store_packed(packed, col0);
       };
       // Peer reduce-scatter: add x (kStoreCols FP32 columns of this thread's row) into the
       // owner's buffer, 32 columns (128 bytes) per staging buffer, copied out 4 rows x 128 bytes
@@ -1303,18 +1325,6 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
         __syncwarp();
         if (lane == 0) ptx::red_release_sys_add_u32(p.rs_count[rs_owner], 1u);
       };
-      // INT8: this row's scale (with alpha), and the columns' scales of the tile's batch or group.
-      // Rows outside the problem are not stored; they take the scale 0 without reading it.
-      float row_alpha = alpha;
-      const float* col_scale = nullptr;
-      if constexpr (OT::kInt8) {
-        if (p.row_scale != nullptr)
-          row_alpha *= my_row < row_end
-                           ? __ldg(p.row_scale + static_cast<int64_t>(sg.ab_batch) * p.m + my_row)
-                           : 0.f;
-        if (p.col_scale != nullptr)
-          col_scale = p.col_scale + static_cast<int64_t>(sg.batch) * p.col_scale_len;
-      }
       // v[j] *= col_scale[col0 + j] for 32 columns of this row, of which those below `limit`
       // exist.  Every lane needs the same values: 16-byte loads broadcast to the warp where they
       // are aligned, else one coalesced load and shuffles (as the bias row below).
@@ -1363,6 +1373,58 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
         }
       };
 
+      // Gated products of 32 columns from column 32 u of this warp's tile columns: TMEM gate and up
+      // columns, scaled, act(gate) * up.
+      auto gated_cols = [&](int32_t tile_col, int32_t col0, bool last, float* x) {
+        uint32_t vg[32], vu[32];
+        const uint32_t tc = t_row + static_cast<uint32_t>(tile_col);
+        ptx::tmem_ld_32x32b_x32(tc, vg);
+        ptx::tmem_ld_32x32b_x32(tc + static_cast<uint32_t>(BN / 2), vu);
+        ptx::tmem_ld_wait();
+        if (last) release_tmem(acc);
+        float gv[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) gv[j] = acc_f32<AB>(vg[j]) * row_alpha;
+        if constexpr (OT::kInt8) {
+          if (col_scale != nullptr) scale_cols(gv, col0, p.n);
+        }
+        act_inplace(p.act, gv);
+        float uv[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) uv[j] = acc_f32<AB>(vu[j]) * row_alpha;
+        if constexpr (OT::kInt8) {
+          if (col_scale != nullptr) scale_cols(uv, p.n + col0, 2 * p.n);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = gv[j] * uv[j];
+      };
+      if constexpr (BN == 512 && sizeof(OutT) == 2 && OT::kInt8) {
+        if (gated) {
+          // A gated tile's 128 output columns of a warp fit, rounded, in 64 registers: all of them
+          // are computed before the first is stored, so the next tile's MMAs wait for the TMEM
+          // reads only, not for the staging buffers and stores.
+          constexpr int kUnits = BN / 2 / ES::kHalves / 32;
+          uint32_t packed[kUnits / 2][32];
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u) {
+            const int32_t tile_col = c_begin * kStoreCols + 32 * u;
+            float x[32];
+            gated_cols(tile_col, pid_n * out_cols + tile_col, u == kUnits - 1, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              packed[u / 2][16 * (u & 1) + i] = ptx::pack_bf16x2(x[2 * i], x[2 * i + 1]);
+          }
+#pragma unroll
+          for (int c = 0; c < kUnits / 2; ++c)
+            store_packed(packed[c], pid_n * out_cols + (c_begin + c) * kStoreCols);
+          if (++acc == kAccStages) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+          continue;
+        }
+      }
+
 #pragma unroll 1
       for (int c = c_begin; c < c_end; ++c) {
         const int32_t col0 = pid_n * out_cols + c * kStoreCols;
@@ -1393,29 +1455,9 @@ __global__ void __launch_bounds__(EpiShape<BN>::kThreads, 1)
         } else {
           // 32 gate and 32 up columns per TMEM round trip.
 #pragma unroll
-          for (int h = 0; h < kStoreCols / 32; ++h) {
-            uint32_t vg[32], vu[32];
-            const uint32_t tc = t_row + static_cast<uint32_t>(c * kStoreCols + 32 * h);
-            ptx::tmem_ld_32x32b_x32(tc, vg);
-            ptx::tmem_ld_32x32b_x32(tc + static_cast<uint32_t>(BN / 2), vu);
-            ptx::tmem_ld_wait();
-            if (c == c_end - 1 && h == kStoreCols / 32 - 1) release_tmem(acc);
-            float gv[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) gv[j] = acc_f32<AB>(vg[j]) * row_alpha;
-            if constexpr (OT::kInt8) {
-              if (col_scale != nullptr) scale_cols(gv, col0 + 32 * h, p.n);
-            }
-            act_inplace(p.act, gv);
-            float uv[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) uv[j] = acc_f32<AB>(vu[j]) * row_alpha;
-            if constexpr (OT::kInt8) {
-              if (col_scale != nullptr) scale_cols(uv, p.n + col0 + 32 * h, 2 * p.n);
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[32 * h + j] = gv[j] * uv[j];
-          }
+          for (int h = 0; h < kStoreCols / 32; ++h)
+            gated_cols(c * kStoreCols + 32 * h, col0 + 32 * h,
+                       c == c_end - 1 && h == kStoreCols / 32 - 1, &x[32 * h]);
         }
         if (partial) {
           // Add alpha * acc into the workspace, 32 FP32 columns (128 bytes) per TMA reduce.

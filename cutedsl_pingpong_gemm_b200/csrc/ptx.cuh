@@ -215,6 +215,11 @@ __device__ __forceinline__ void tma_prefetch_l2_3d(const CUtensorMap* m, int32_t
                : "memory");
 }
 
+// Bring the line at a global address into L1 (a hint).
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
+
 // Programmatic dependent launch: let the grid launched after this one on the stream be scheduled
 // once every CTA of this grid has executed this (or exited) ...
 __device__ __forceinline__ void griddep_launch_dependents() {
