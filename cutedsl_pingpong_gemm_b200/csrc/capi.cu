@@ -888,6 +888,14 @@ int cpg_gemm_create(const cpg_gemm_config* cfg, const cpg_gemm_problem* prob, in
       g->l2_policy_b = 2;
     }
   }
+  if (prob->grouped) {
+    // A group's tiles run m-fastest whatever the raster order: its rows of A are read again for
+    // every column tile, its B passes once.  8 uneven groups of 16384 rows in all, gated
+    // [2 x 14336, 4096], A / B evict-first / evict-last and the other way round: INT8 1470 and
+    // 1401 us, BF16 2790 and 2560 us.
+    g->l2_policy_a = 2;
+    g->l2_policy_b = 1;
+  }
   // D tiles are written once and never read back by the kernel.
   g->l2_policy_d = 1;
   const char* pa = std::getenv("CPG_L2_POLICY_A");

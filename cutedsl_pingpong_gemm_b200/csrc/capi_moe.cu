@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_common.h"
 #include "cpgemm.h"
@@ -84,25 +85,34 @@ bool vector_rows(const void* p, int64_t cols, int64_t ld, int elem) {
   return !misaligned(p, 16) && (ld * elem) % 16 == 0 && cols < (int64_t(1) << 30);
 }
 
-template <typename T, int G, bool Resident>
+template <typename T, int G, int NV, bool Resident>
 int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
-  constexpr int kRows = 256 / G;
-  return launch("INT8 row kernel", false, &cpg::rows_int8_vec_kernel<T, G, Resident>,
-                row_grid((p.tokens + kRows - 1) / kRows), 256, 0, st, 1, p);
+  constexpr int kThreads = cpg::int8_threads<G>();
+  constexpr int kRows = kThreads / G;
+  return launch("INT8 row kernel", false, &cpg::rows_int8_vec_kernel<T, G, NV, Resident>,
+                row_grid((p.tokens + kRows - 1) / kRows), kThreads, 0, st, 1, p);
 }
 
 template <typename T>
 int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
-  // The fewest threads that hold a row; more while the tokens leave most of the GPU idle (each
-  // then has less of a row to wait for).
-  int threads = 32;
-  while (threads < 256 && p.cols > int64_t(threads) * cpg::kInt8Vecs * 16) threads *= 2;
+  // The fewest threads that hold a row (16384 x 4096 BF16: 128 threads 49 us, 256 61 us); more while
+  // the tokens leave most of the GPU idle (each then has less of a row to wait for).
+  // Measured: FP32 16384 x 8192 102.6 us (1.00 of measured HBM), BF16 75.0 us (0.82), where the
+  // conversions bound it: three packed FMAs per two elements after 22 issue slots an element before.
+  constexpr int kVecs = cpg::kInt8Vecs;
+  constexpr int64_t kEach = kVecs * 16;
+  if (p.cols > 2 * 512 * kEach) return launch_int8_vec<T, 512, kVecs, false>(p, st);
+  if (p.cols > 512 * kEach) return launch_int8_vec<T, 512, 2 * kVecs, true>(p, st);
+  int64_t threads = 32;
+  while (p.cols > threads * kEach) threads *= 2;
   while (threads < 256 && p.tokens * threads < kFewThreads && p.cols > threads * 16) threads *= 2;
-  if (p.cols > int64_t(256) * cpg::kInt8Vecs * 16) return launch_int8_vec<T, 256, false>(p, st);
-  if (threads == 256) return launch_int8_vec<T, 256, true>(p, st);
-  if (threads == 128) return launch_int8_vec<T, 128, true>(p, st);
-  if (threads == 64) return launch_int8_vec<T, 64, true>(p, st);
-  return launch_int8_vec<T, 32, true>(p, st);
+  switch (threads) {
+    case 32: return launch_int8_vec<T, 32, kVecs, true>(p, st);
+    case 64: return launch_int8_vec<T, 64, kVecs, true>(p, st);
+    case 128: return launch_int8_vec<T, 128, kVecs, true>(p, st);
+    case 256: return launch_int8_vec<T, 256, kVecs, true>(p, st);
+    default: return launch_int8_vec<T, 512, kVecs, true>(p, st);
+  }
 }
 
 // Warps of work and blocks of 8 warps for rows cut into chunks of `vecs` vectors a lane.

@@ -127,20 +127,18 @@ __device__ __forceinline__ void st_row_vec(T* row, int32_t c, int32_t cols, cons
   }
 }
 
-// Bits of the largest |value| of a vector, given the largest so far.
+// The largest |value| seen, as bits: of FP32 one word, of BF16 one maximum per half word.
 template <typename T>
 __device__ __forceinline__ uint32_t abs_max_vec(const uint4& v, uint32_t m) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      m = max(m, (w[i] << 16) & 0x7fffffffu);
-      m = max(m, w[i] & 0x7fff0000u);
-    } else {
-      m = max(m, w[i] & 0x7fffffffu);
-    }
-  }
+  for (int i = 0; i < 4; ++i)
+    m = sizeof(T) == 2 ? __vmaxu2(m, w[i] & 0x7fff7fffu) : max(m, w[i] & 0x7fffffffu);
   return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max_bits(uint32_t m) {
+  return sizeof(T) == 2 ? max(m << 16, m & 0xffff0000u) : m;
 }
 
 // Four quotients x / s by IEEE division, rounded to integers, as the bytes of a word.
@@ -149,22 +147,34 @@ __device__ __noinline__ uint32_t int8_word_div(float x0, float x1, float x2, flo
          (int8_quotient(x3, s) << 24);
 }
 
-// The same without a division per element.  With y = RN(1 / s), q = RN(x y) is within
-// 127 * 1.5 * 2^-23 < 2.3e-5 of x / s, and the fp32 quotient within 127 * 2^-24 < 7.6e-6 of it; so
-// where q is farther than 4e-5 from a half-integer both round to the same integer, and elsewhere
-// (about 2e-4 of the elements) the word takes the division.  Adding 1.5 * 2^23 rounds to the nearest
-// even integer and leaves it in the low byte.
+// x y rounded to integers (nearest even, left in the low bytes of r0 and r1) and what the rounding
+// took away (d0, d1), two elements per packed FMA.  Adding 1.5 * 2^23 rounds to an integer.
+__device__ __forceinline__ void round2(float x0, float x1, float y, uint32_t& r0, uint32_t& r1,
+                                       float& d0, float& d1) {
+  asm("{\n\t.reg .b64 x, y, k, r, u, d;\n\t"
+      "mov.b64 x, {%4, %5};\n\t"
+      "mov.b64 y, {%6, %6};\n\t"
+      "mov.b64 k, {%7, %7};\n\t"
+      "mov.b64 u, {%8, %8};\n\t"
+      "fma.rn.f32x2 r, x, y, k;\n\t"   // k + rint(x y)
+      "fma.rn.f32x2 u, r, u, k;\n\t"   // -rint(x y), exact
+      "fma.rn.f32x2 d, x, y, u;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t"
+      "mov.b64 {%2, %3}, d;\n\t}"
+      : "=r"(r0), "=r"(r1), "=f"(d0), "=f"(d1)
+      : "f"(x0), "f"(x1), "f"(y), "f"(12582912.f), "f"(-1.f));
+}
+
+// The same without a division per element.  With y = RN(1 / s), x y is within 127 * 2^-24 < 7.6e-6
+// of x / s, and the fp32 quotient within half an ulp, 2^-18 < 3.9e-6, of it; so where x y is farther
+// than 4e-5 from a half-integer both round to the same integer, and elsewhere (about 1e-4 of the
+// elements) the word takes the division.
 __device__ __forceinline__ uint32_t int8_word(const float* x, float s, float y) {
-  constexpr float kRound = 12582912.f;
   uint32_t b[4];
-  float worst = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float q = __fmul_rn(x[i], y);
-    const float r = __fadd_rn(q, kRound);
-    worst = fmaxf(worst, fabsf(q - __fsub_rn(r, kRound)));
-    b[i] = __float_as_uint(r);
-  }
+  float d[4];
+  round2(x[0], x[1], y, b[0], b[1], d[0], d[1]);
+  round2(x[2], x[3], y, b[2], b[3], d[2], d[3]);
+  const float worst = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
   if (worst > 0.5f - 4e-5f) return int8_word_div(x[0], x[1], x[2], x[3], s);
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
@@ -239,22 +249,32 @@ __global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
   }
 }
 
-// Quantised rows of whole vectors: G threads per token hold the row packed in registers, kInt8Vecs
-// times 16 elements each, between its maximum and the quantisation, so the row is read once however
-// many copies of it are written.  Longer rows (Resident false) are read a second time, from L2.
-constexpr int kInt8Vecs = 4;
+// Quantised rows of whole vectors: G threads per token hold the row packed in registers, NV times 16
+// elements each, between its maximum and the quantisation, so the row is read once however many
+// copies of it are written.  Longer rows (Resident false) are read a second time, from L2.
+constexpr int kInt8Vecs = 2;
 
-template <typename T, int G, bool Resident>
-__global__ void __launch_bounds__(256, 16 / sizeof(T) / 2) rows_int8_vec_kernel(const RowsParams p) {
+template <int G>
+__host__ __device__ constexpr int int8_threads() {
+  return G < 256 ? 256 : G;
+}
+// Threads per SM the registers are limited for.
+template <typename T, int NV>
+__host__ __device__ constexpr int int8_sm_threads() {
+  return NV == kInt8Vecs ? (sizeof(T) == 2 ? 1536 : 1024) : (sizeof(T) == 2 ? 1024 : 512);
+}
+
+template <typename T, int G, int NV, bool Resident>
+__global__ void __launch_bounds__(int8_threads<G>(), int8_sm_threads<T, NV>() / int8_threads<G>())
+    rows_int8_vec_kernel(const RowsParams p) {
   // The small-M product that reads these rows may be set up, and fetch its first weights, already.
   ptx::griddep_launch_dependents();
   kernel_begins();
-  constexpr int NV = kInt8Vecs;
   constexpr int kVecs = 16 / RowVec<T>::kElems;
   constexpr int kE = RowVec<T>::kElems;
-  constexpr int kRowsPerBlock = 256 / G;
+  constexpr int kRowsPerBlock = int8_threads<G>() / G;
   constexpr int kPass = G * NV * 16;  // elements per pass over a row
-  __shared__ uint32_t red[2][8];
+  __shared__ uint32_t red[2][int8_threads<G>() / 32];
   const int lane = threadIdx.x & 31;
   const int li = threadIdx.x % G;
   const int32_t cols = static_cast<int32_t>(p.cols);
@@ -288,7 +308,7 @@ __global__ void __launch_bounds__(256, 16 / sizeof(T) / 2) rows_int8_vec_kernel(
     int32_t my_slot = -1;
     if (lane < p.k) my_slot = p.slots != nullptr ? p.slots[t * p.k + lane] : static_cast<int32_t>(t);
     if (my_slot >= p.num_rows) my_slot = -1;
-    m = __reduce_max_sync(0xffffffffu, m);
+    m = __reduce_max_sync(0xffffffffu, abs_max_bits<T>(m));
     if constexpr (G > 32) {
       // The parity keeps the next row's writes off the words a slow warp still reads.
       constexpr int kWarps = G / 32;

@@ -21,104 +21,21 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._tensors import call, error, float_code, matrix, output, pairs, ptr, vector
 from .quant import alloc_int8_rows
 
 Dispatched = namedtuple("Dispatched", "rows offsets slots scales")
 
 
-def _error(code, message):
-    return _lib.CpgError(code, message)
-
-
-_FLOAT_CODES = {torch.bfloat16: _lib.CPG_DTYPE_BF16, torch.float32: _lib.CPG_DTYPE_F32}
-
-
-def _float_code(name, t):
-    code = _FLOAT_CODES.get(t.dtype)
-    if code is None:
-        raise _error(_lib.CPG_ERR_DTYPE, f"{name} must be BF16 or FP32, got {t.dtype}")
-    return code
-
-
-def _matrix(name, t, shape=None, device=None):
-    """A 2-D CUDA tensor with unit column stride (of ``shape``, on ``device``): its rows, columns
-    and row stride."""
-    if not t.is_cuda:
-        raise _error(_lib.CPG_ERR_NO_DEVICE, f"{name} must be a CUDA tensor")
-    size = t.shape
-    if len(size) != 2 or (shape is not None and size != shape):
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
-                     f"{name} must be 2-D{'' if shape is None else ' of shape ' + str(tuple(shape))}"
-                     f", got {tuple(size)}")
-    rows, cols = size
-    ld, step = t.stride()
-    if step != 1 and rows > 0 and cols > 1:
-        raise _error(_lib.CPG_ERR_UNSUPPORTED, f"{name} must have unit column stride")
-    if device is not None and t.device != device:
-        raise _other_device(name, t, device)
-    return rows, cols, ld if rows > 1 else cols
-
-
-def _other_device(name, t, device):
-    return _error(_lib.CPG_ERR_NO_DEVICE, f"{name} is on {t.device}, the others on {device}")
-
-
-def _output(name, t, shape, dtype, device):
-    """Row stride of a matrix that is written: its rows must not overlap."""
-    rows, cols, ld = _matrix(name, t, shape, device)
-    if t.dtype != dtype:
-        raise _error(_lib.CPG_ERR_DTYPE, f"{name} must be {dtype}, got {t.dtype}")
-    if ld < cols:
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"{name}'s rows overlap (row stride {ld})")
-    return ld
-
-
-def _vector(name, t, shape, dtype, device):
-    if t is None:
-        raise _error(_lib.CPG_ERR_NULL, f"{name} must be given")
-    if not (t.is_cuda and t.dtype == dtype and t.shape == shape and t.is_contiguous()):
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
-                     f"{name} must be a contiguous {dtype} CUDA tensor of shape {tuple(shape)}, "
-                     f"got {t.dtype} {tuple(t.shape)}")
-    if t.device != device:
-        raise _other_device(name, t, device)
-
-
-def _pairs(name, t):
-    """T and k of the choices [T, k]."""
-    size = t.shape
-    if len(size) != 2:
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} must be [T, k], got {tuple(size)}")
-    return size
-
-
-def _ptr(t):
-    """Address of a tensor; None without one or for an empty one."""
-    return None if t is None else t.data_ptr() or None
-
-
-def _call(fn, what, device, *args):
-    """Call a C entry point on the current stream of ``device`` (made current for the call)."""
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
-    if rc != _lib.CPG_OK:
-        _lib.check(rc, what)
-
-
 @functools.lru_cache(maxsize=256)
 def _route_config(experts, k, scoring, groups, kept_groups, group_score, renormalize, scale):
     if scoring not in _lib.ROUTE_SCORINGS:
-        raise _error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown scoring {scoring!r}")
+        raise error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown scoring {scoring!r}")
     if group_score not in _lib.ROUTE_GROUP_SCORES:
-        raise _error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown group_score {group_score!r}")
+        raise error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown group_score {group_score!r}")
     for name, v in (("k", k), ("groups", groups), ("kept_groups", kept_groups)):
         if abs(v) >= 1 << 31:  # ctypes would wrap it
-            raise _error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} = {v}")
+            raise error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} = {v}")
     return ctypes.byref(_lib.RouteConfigC(
         experts, k, _lib.ROUTE_SCORINGS[scoring], groups, kept_groups,
         _lib.ROUTE_GROUP_SCORES[group_score], 1 if renormalize else 0, scale))
@@ -137,8 +54,8 @@ def route(logits, k: int, *, scoring: str = "softmax", bias=None, groups: int = 
     the default with a bias).  A logit of -inf masks an expert; where fewer than k are left the
     last ids are -1 with weight 0.  A NaN logit makes the row's weights NaN (under the softmax
     +inf too).  E <= 1024, k and groups <= 32.  ``ids`` / ``weights`` may be given as outputs."""
-    t, e, ld = _matrix("logits", logits)
-    code = _float_code("logits", logits)
+    t, e, ld = matrix("logits", logits)
+    code = float_code("logits", logits)
     dev = logits.device
     k = int(k)
     if group_score is None:
@@ -147,18 +64,18 @@ def route(logits, k: int, *, scoring: str = "softmax", bias=None, groups: int = 
                         int(groups if kept_groups is None else kept_groups), group_score,
                         bool(renormalize), float(scale))
     if bias is not None:
-        _vector("bias", bias, (e,), torch.float32, dev)
+        vector("bias", bias, (e,), torch.float32, dev)
     shape = (t, max(k, 0))
     if ids is None:
         ids = torch.empty(shape, dtype=torch.int32, device=dev)
     else:
-        _vector("ids", ids, shape, torch.int32, dev)
+        vector("ids", ids, shape, torch.int32, dev)
     if weights is None:
         weights = torch.empty(shape, dtype=torch.float32, device=dev)
     else:
-        _vector("weights", weights, shape, torch.float32, dev)
-    _call(_lib.load().cpg_route, "route", dev, cfg, _ptr(logits), code, t, ld, _ptr(bias),
-          _ptr(ids), _ptr(weights))
+        vector("weights", weights, shape, torch.float32, dev)
+    call(_lib.load().cpg_route, "route", dev, cfg, ptr(logits), code, t, ld, ptr(bias),
+          ptr(ids), ptr(weights))
     return ids, weights
 
 
@@ -167,18 +84,18 @@ def route_backward(dweights, logits, ids, *, scoring: str = "softmax", renormali
     """Gradient of ``route``'s weights: ``dlogits`` [T, E] in the logits' type from ``dweights``
     (FP32 [T, k]) for the choices ``ids`` of the forward call (same scoring, renormalize, scale).
     Entries of ``ids`` that are no expert take no part; an expert given twice counts twice."""
-    t, e, ld = _matrix("logits", logits)
-    code = _float_code("logits", logits)
+    t, e, ld = matrix("logits", logits)
+    code = float_code("logits", logits)
     dev = logits.device
-    _, k = _pairs("ids", ids)
-    _vector("ids", ids, (t, k), torch.int32, dev)
-    _vector("dweights", dweights, (t, k), torch.float32, dev)
+    _, k = pairs("ids", ids)
+    vector("ids", ids, (t, k), torch.int32, dev)
+    vector("dweights", dweights, (t, k), torch.float32, dev)
     cfg = _route_config(e, k, scoring, 1, 1, "max", bool(renormalize), float(scale))
     if out is None:
         out = torch.empty((t, e), dtype=logits.dtype, device=dev)
-    ldd = _output("out", out, (t, e), logits.dtype, dev)
-    _call(_lib.load().cpg_route_backward, "route_backward", dev, cfg, _ptr(dweights),
-          _ptr(logits), code, t, ld, _ptr(ids), _ptr(out), ldd)
+    ldd = output("out", out, (t, e), logits.dtype, dev)
+    call(_lib.load().cpg_route_backward, "route_backward", dev, cfg, ptr(dweights),
+          ptr(logits), code, t, ld, ptr(ids), ptr(out), ldd)
     return out
 
 
@@ -192,39 +109,39 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
     on are not written.  ``quantize="int8"`` makes ``rows`` the int8 rows and ``scales`` (FP32
     [T * k]) the scales of ``quant.quantize_int8``; otherwise ``scales`` is None.  ``out`` /
     ``scales`` may be given as outputs.  experts <= 1024, k <= 32."""
-    t, d, ldx = _matrix("x", x)
-    code = _float_code("x", x)
+    t, d, ldx = matrix("x", x)
+    code = float_code("x", x)
     dev = x.device
     if quantize not in (None, "int8"):
-        raise _error(_lib.CPG_ERR_UNSUPPORTED, f"quantize must be None or 'int8', got {quantize!r}")
-    _, k = _pairs("ids", ids)
-    _vector("ids", ids, (t, k), torch.int32, dev)
+        raise error(_lib.CPG_ERR_UNSUPPORTED, f"quantize must be None or 'int8', got {quantize!r}")
+    _, k = pairs("ids", ids)
+    vector("ids", ids, (t, k), torch.int32, dev)
     experts = int(experts)
     if experts < 1 or experts > _lib.CPG_ROUTE_MAX_EXPERTS:
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE,
+        raise error(_lib.CPG_ERR_INVALID_SHAPE,
                      f"1 <= experts <= {_lib.CPG_ROUTE_MAX_EXPERTS}, got {experts}")
     int8 = quantize == "int8"
     if out is None:
         out = (alloc_int8_rows(t * k, d, dev) if int8
                else torch.empty((t * k, d), dtype=x.dtype, device=dev))
-    ldr = _output("out", out, (t * k, d), torch.int8 if int8 else x.dtype, dev)
+    ldr = output("out", out, (t * k, d), torch.int8 if int8 else x.dtype, dev)
     if int8:
         if scales is None:
             scales = torch.empty(t * k, dtype=torch.float32, device=dev)
         else:
-            _vector("scales", scales, (t * k,), torch.float32, dev)
+            vector("scales", scales, (t * k,), torch.float32, dev)
     elif scales is not None:
-        raise _error(_lib.CPG_ERR_UNSUPPORTED, "scales only with quantize='int8'")
+        raise error(_lib.CPG_ERR_UNSUPPORTED, "scales only with quantize='int8'")
     # One allocation for both, the slots on 16 bytes.
     at = -(-(experts + 1) // 4) * 4
     order = torch.empty(at + t * k, dtype=torch.int32, device=dev)
     offsets, slots = order[:experts + 1], order[at:].view(t, k)
     lib = _lib.load()
     slots_ptr = order.data_ptr() + 4 * at
-    _call(lib.cpg_expert_order, "dispatch", dev, _ptr(ids), t, k, experts, order.data_ptr(),
+    call(lib.cpg_expert_order, "dispatch", dev, ptr(ids), t, k, experts, order.data_ptr(),
           slots_ptr)
-    _call(lib.cpg_dispatch_rows, "dispatch", dev, _ptr(x), code, t, d, ldx, slots_ptr, k,
-          _ptr(out), _lib.CPG_DTYPE_I8 if int8 else code, t * k, ldr, _ptr(scales))
+    call(lib.cpg_dispatch_rows, "dispatch", dev, ptr(x), code, t, d, ldx, slots_ptr, k,
+          ptr(out), _lib.CPG_DTYPE_I8 if int8 else code, t * k, ldr, ptr(scales))
     return Dispatched(out, offsets, slots, scales)
 
 
@@ -234,23 +151,23 @@ def combine(rows, slots, weights=None, *, source=None, out=None):
     ``rows`` [R, D] BF16 or FP32, ``slots`` int32 [T, k] (entries outside [0, R) are not read),
     ``weights`` FP32 [T, k] or None for ones, ``source`` an optional [T, D] of the rows' type
     (it may be ``out``), such as a shared expert's output."""
-    r, d, ldr = _matrix("rows", rows)
-    code = _float_code("rows", rows)
+    r, d, ldr = matrix("rows", rows)
+    code = float_code("rows", rows)
     dev = rows.device
-    t, k = _pairs("slots", slots)
-    _vector("slots", slots, (t, k), torch.int32, dev)
+    t, k = pairs("slots", slots)
+    vector("slots", slots, (t, k), torch.int32, dev)
     if weights is not None:
-        _vector("weights", weights, (t, k), torch.float32, dev)
+        vector("weights", weights, (t, k), torch.float32, dev)
     lds = 0
     if source is not None:
-        _, _, lds = _matrix("source", source, (t, d), dev)
+        _, _, lds = matrix("source", source, (t, d), dev)
         if source.dtype != rows.dtype:
-            raise _error(_lib.CPG_ERR_DTYPE, f"source must be {rows.dtype} like rows")
+            raise error(_lib.CPG_ERR_DTYPE, f"source must be {rows.dtype} like rows")
     if out is None:
         out = torch.empty((t, d), dtype=rows.dtype, device=dev)
-    ldy = _output("out", out, (t, d), rows.dtype, dev)
-    _call(_lib.load().cpg_combine_rows, "combine", dev, _ptr(rows), code, r, d, ldr, _ptr(slots),
-          _ptr(weights), t, k, _ptr(source), lds, _ptr(out), ldy)
+    ldy = output("out", out, (t, d), rows.dtype, dev)
+    call(_lib.load().cpg_combine_rows, "combine", dev, ptr(rows), code, r, d, ldr, ptr(slots),
+          ptr(weights), t, k, ptr(source), lds, ptr(out), ldy)
     return out
 
 
@@ -259,25 +176,25 @@ def combine_backward(dy, rows, slots, weights, *, drows=None, dweights=None):
     no slot names are left as they were) and ``dweights[t, j] = <dy[t], rows[slots[t, j]]>`` FP32
     [T, k].  No two slots may be the same row (``dispatch`` makes none).  ``drows`` / ``dweights``
     may be given as outputs."""
-    t, d, lddy = _matrix("dy", dy)
-    code = _float_code("dy", dy)
+    t, d, lddy = matrix("dy", dy)
+    code = float_code("dy", dy)
     dev = dy.device
-    r, cols, ldr = _matrix("rows", rows, None, dev)
+    r, cols, ldr = matrix("rows", rows, None, dev)
     if cols != d or rows.dtype != dy.dtype:
-        raise _error(_lib.CPG_ERR_INVALID_SHAPE if cols != d else _lib.CPG_ERR_DTYPE,
+        raise error(_lib.CPG_ERR_INVALID_SHAPE if cols != d else _lib.CPG_ERR_DTYPE,
                      f"rows must be [R, {d}] {dy.dtype} like dy, got {tuple(rows.shape)} "
                      f"{rows.dtype}")
-    _, k = _pairs("slots", slots)
-    _vector("slots", slots, (t, k), torch.int32, dev)
-    _vector("weights", weights, (t, k), torch.float32, dev)
+    _, k = pairs("slots", slots)
+    vector("slots", slots, (t, k), torch.int32, dev)
+    vector("weights", weights, (t, k), torch.float32, dev)
     if drows is None:
         drows = torch.empty((r, d), dtype=dy.dtype, device=dev)
     if dweights is None:
         dweights = torch.empty((t, k), dtype=torch.float32, device=dev)
     else:
-        _vector("dweights", dweights, (t, k), torch.float32, dev)
-    lddr = _output("drows", drows, (r, d), dy.dtype, dev)
-    _call(_lib.load().cpg_combine_rows_backward, "combine_backward", dev, _ptr(dy), code, t, d,
-          lddy, _ptr(rows), r, ldr, _ptr(slots), _ptr(weights), k, _ptr(drows), lddr,
-          _ptr(dweights))
+        vector("dweights", dweights, (t, k), torch.float32, dev)
+    lddr = output("drows", drows, (r, d), dy.dtype, dev)
+    call(_lib.load().cpg_combine_rows_backward, "combine_backward", dev, ptr(dy), code, t, d,
+          lddy, ptr(rows), r, ldr, ptr(slots), ptr(weights), k, ptr(drows), lddr,
+          ptr(dweights))
     return drows, dweights

@@ -11,16 +11,17 @@ Scale layouts are described in ``include/cpgemm.h``.
 """
 from typing import Optional, Tuple
 
+import torch
+
 from . import _lib
+from ._tensors import call, float_code, matrix, output, ptr, vector
 
 
 def _stream(t):
-    import torch
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def quantize_e4m3(x, block: Optional[Tuple[int, int]] = None):
-    import torch
     if not x.is_cuda or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise _lib.CpgError(_lib.CPG_ERR_DTYPE, "x must be a 2-D BF16 or FP32 CUDA tensor")
     if x.numel() and x.stride(1) != 1:
@@ -47,7 +48,6 @@ def quantize_e4m3(x, block: Optional[Tuple[int, int]] = None):
 
 def alloc_int8_rows(rows: int, cols: int, device):
     """int8 [rows, cols] whose rows start on 16 bytes, as the GEMM's loads need."""
-    import torch
     if cols % 16 == 0:
         return torch.empty((rows, cols), dtype=torch.int8, device=device)
     return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
@@ -58,27 +58,23 @@ def quantize_int8(x, out=None, scales=None):
     stream.  ``q`` has rows padded to 16 bytes, ready for the GEMM; ``out`` (int8, x's shape, unit
     column stride) and ``scales`` may be given as outputs.  Rows of zeros get q = 0 and a tiny
     scale; a row that holds an infinity or NaN gets q = 0 and the scale NaN."""
-    import torch
-    from . import moe
-    if not x.is_cuda or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
-        raise _lib.CpgError(_lib.CPG_ERR_DTYPE, "x must be a 2-D BF16 or FP32 CUDA tensor")
-    rows, cols, ldx = moe._matrix("x", x)
+    code = float_code("x", x)
+    rows, cols, ldx = matrix("x", x)
     device = x.device
     if out is None:
         out = alloc_int8_rows(rows, cols, device)
-    ldq = moe._output("out", out, (rows, cols), torch.int8, device)
+    ldq = output("out", out, (rows, cols), torch.int8, device)
     if scales is None:
         scales = torch.empty(rows, dtype=torch.float32, device=device)
     else:
-        moe._vector("scales", scales, (rows,), torch.float32, device)
-    moe._call(_lib.load().cpg_quantize_int8, "quantize_int8", device, moe._ptr(x),
-              moe._float_code("x", x), rows, cols, ldx, moe._ptr(out), ldq, moe._ptr(scales))
+        vector("scales", scales, (rows,), torch.float32, device)
+    call(_lib.load().cpg_quantize_int8, "quantize_int8", device, ptr(x),
+              code, rows, cols, ldx, ptr(out), ldq, ptr(scales))
     return out, scales
 
 
 def cast_f32_bf16(x, bias=None, out=None, stream=None):
     """out = bf16(x + bias) for a 2-D FP32 CUDA tensor x (on ``stream``, default current)."""
-    import torch
     if not x.is_cuda or x.dim() != 2 or x.dtype != torch.float32:
         raise _lib.CpgError(_lib.CPG_ERR_DTYPE, "x must be a 2-D FP32 CUDA tensor")
     rows, cols = x.shape

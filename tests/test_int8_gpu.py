@@ -366,7 +366,7 @@ def test_quantize_strides_and_outputs(shift, extra, dtype):
 def test_quantize_refusals():
     x = torch.randn(4, 8, device="cuda")
     for bad, code in [(lambda: quantize_int8(x.double()), _lib.CPG_ERR_DTYPE),
-                      (lambda: quantize_int8(x[0]), _lib.CPG_ERR_DTYPE),
+                      (lambda: quantize_int8(x[0]), _lib.CPG_ERR_INVALID_SHAPE),
                       (lambda: quantize_int8(x.t()), _lib.CPG_ERR_UNSUPPORTED),
                       (lambda: quantize_int8(x, out=torch.empty(4, 8, device="cuda")),
                        _lib.CPG_ERR_DTYPE),
