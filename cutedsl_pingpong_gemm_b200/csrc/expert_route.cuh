@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
 // run again handing out slots.
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
-constexpr int kOrderMaxCluster = 8;
+constexpr int kOrderMaxCluster = 16;  // 8 where 16 blocks do not fit in one cluster
 constexpr int kOrderHold = 16;  // pairs a lane loads at a time
 
 struct OrderParams {

@@ -132,16 +132,14 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
             vector("scales", scales, (t * k,), torch.float32, dev)
     elif scales is not None:
         raise error(_lib.CPG_ERR_UNSUPPORTED, "scales only with quantize='int8'")
-    # One allocation for both, the slots on 16 bytes.
-    at = -(-(experts + 1) // 4) * 4
-    order = torch.empty(at + t * k, dtype=torch.int32, device=dev)
-    offsets, slots = order[:experts + 1], order[at:].view(t, k)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty((t, k), dtype=torch.int32, device=dev)
+    slots_ptr = ptr(slots)
     lib = _lib.load()
-    slots_ptr = order.data_ptr() + 4 * at
-    call(lib.cpg_expert_order, "dispatch", dev, ptr(ids), t, k, experts, order.data_ptr(),
-          slots_ptr)
-    call(lib.cpg_dispatch_rows, "dispatch", dev, ptr(x), code, t, d, ldx, slots_ptr, k,
-          ptr(out), _lib.CPG_DTYPE_I8 if int8 else code, t * k, ldr, ptr(scales))
+    call(lib.cpg_expert_order, "dispatch", dev, ptr(ids), t, k, experts, offsets.data_ptr(),
+         slots_ptr)
+    call(lib.cpg_dispatch_rows, "dispatch", dev, ptr(x), code, t, d, ldx, slots_ptr, k, ptr(out),
+         _lib.CPG_DTYPE_I8 if int8 else code, t * k, ldr, ptr(scales))
     return Dispatched(out, offsets, slots, scales)
 
 
