@@ -1194,6 +1194,10 @@ static int run_impl(cpg_gemm* g, const void* a, const void* b, void* d, const cp
   if (a == nullptr || b == nullptr) return fail(CPG_ERR_NULL, "A and B must be non-NULL");
   if ((reinterpret_cast<uintptr_t>(a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(b) & 15u) != 0)
     return fail(CPG_ERR_ALIGNMENT, "A and B must be 16-byte aligned");
+  if (pr.dtype_ab == CPG_DTYPE_I8 && epi != nullptr &&
+      ((reinterpret_cast<uintptr_t>(epi->scale_a) | reinterpret_cast<uintptr_t>(epi->scale_b)) &
+       3u) != 0)
+    return fail(CPG_ERR_ALIGNMENT, "scales must be 4-byte aligned");
   if (g->decode) {
     if (rs != nullptr) return fail(CPG_ERR_UNSUPPORTED, "a small-M plan has no peer exchange");
     return run_decode(g, a, b, d, epi, st);

@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
         __syncwarp();
       }
       const bool real = group < p.groups;
+      const bool some = real && a > -INFINITY;
       float slack = 0.5f * near + 0x1p-23f * fabsf(a);
       if (p.group_score == kRouteGroupTop2 && a2 > -INFINITY) {
         slack = near + 0x1p-22f * (fabsf(a) + fabsf(a2));
@@ -510,12 +511,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
         }
       }
       if (!by_logit) {
-        const bool some = real && a > -INFINITY;
         const uint32_t worst_kept =
             __reduce_min_sync(0xffffffffu, kept && some ? order_key(a - slack) : 0xffffffffu);
         const uint32_t best_left =
             __reduce_max_sync(0xffffffffu, !kept && some ? order_key(a + slack) : kNoKey);
-        if (best_left >= worst_kept) {
+        // A sum that overflows (biases of the lowest value as masks) has no 32-bit rank at all.
+        const bool lost = some && !(fabsf(a) + slack < INFINITY);
+        if (best_left >= worst_kept || __any_sync(0xffffffffu, lost)) {
           kept = (route_groups64<T, V>(p, row, c_sh) >> group) & 1u;
         }
       }

@@ -156,6 +156,9 @@ class CompiledGemm:
                                     f"{name} must have unit stride in its last dimension")
             if t.numel() > 0 and not t.is_cuda:
                 raise _lib.CpgError(_lib.CPG_ERR_NO_DEVICE, f"{name} must be a CUDA tensor")
+            if t.numel() > 0 and t.device != c.device:
+                raise _lib.CpgError(_lib.CPG_ERR_NO_DEVICE,
+                                    f"{name} is on {t.device}, D on {c.device}")
         def row_stride(t, rows, cols):
             # A single-row or empty tensor's row stride is never used; give the padded row length.
             per16 = 16 // t.element_size()
@@ -250,7 +253,8 @@ class CompiledGemm:
             raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
                                 "grouped: a [T, K], b [G, N, K] and c [T, N]")
         groups = b.shape[0]
-        if not (group_offsets.is_cuda and group_offsets.dtype == torch.int32
+        if not (group_offsets.is_cuda and group_offsets.device == c.device
+                and group_offsets.dtype == torch.int32
                 and group_offsets.dim() == 1 and group_offsets.numel() == groups + 1
                 and group_offsets.is_contiguous()):
             raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
@@ -281,6 +285,9 @@ class CompiledGemm:
             if x.numel() > 0 and (x.stride(-1) != 1 or not x.is_cuda):
                 raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED,
                                     f"{name} must be a CUDA tensor with unit last stride")
+            if x.device != c.device:
+                raise _lib.CpgError(_lib.CPG_ERR_NO_DEVICE,
+                                    f"{name} is on {x.device}, D on {c.device}")
         per16 = 16 // a.element_size()
         lda = a.stride(0) if t > 1 else max(per16, -(-k // per16) * per16)
         ldb = b.stride(1) if b_rows > 1 else max(per16, -(-k // per16) * per16)
@@ -451,7 +458,8 @@ class _Plan:
             group_offsets=None) -> None:
         import torch
         if bias is not None:
-            if not (bias.dtype == torch.bfloat16 and bias.is_cuda and bias.numel() == self.n
+            if not (bias.dtype == torch.bfloat16 and bias.device == c.device
+                    and bias.numel() == self.n
                     and (bias.dim() == 1 or bias.is_contiguous())):
                 raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
                                     "bias must be a contiguous BF16 CUDA tensor of length N")
@@ -459,7 +467,7 @@ class _Plan:
                 raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED, "bias must be contiguous")
         scales = []
         for name, sc in (("scale_a", scale_a), ("scale_b", scale_b)):
-            if sc is not None and not (sc.is_cuda and sc.dtype == torch.float32
+            if sc is not None and not (sc.device == c.device and sc.dtype == torch.float32
                                        and sc.is_contiguous()
                                        and sc.numel() == math.prod(self.scale_shapes[name])):
                 raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
@@ -468,7 +476,8 @@ class _Plan:
             scales.append(None if sc is None else sc.data_ptr())
         src_ptr, ld_src, bs_src = None, 0, 0
         if source is not None:
-            if not (source.is_cuda and source.dtype == c.dtype and source.shape == c.shape
+            if not (source.device == c.device and source.dtype == c.dtype
+                    and source.shape == c.shape
                     and (source.numel() == 0 or source.stride(-1) == 1)):
                 raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
                                     "source must be a CUDA tensor of D's dtype and shape with unit "

@@ -92,8 +92,9 @@ def route_backward(dweights, logits, ids, *, scoring: str = "softmax", renormali
     vector("dweights", dweights, (t, k), torch.float32, dev)
     cfg = _route_config(e, k, scoring, 1, 1, "max", bool(renormalize), float(scale))
     if out is None:
-        out = torch.empty((t, e), dtype=logits.dtype, device=dev)
-    ldd = output("out", out, (t, e), logits.dtype, dev)
+        out, ldd = torch.empty((t, e), dtype=logits.dtype, device=dev), e
+    else:
+        ldd = output("out", out, (t, e), logits.dtype, dev)
     call(_lib.load().cpg_route_backward, "route_backward", dev, cfg, ptr(dweights),
           ptr(logits), code, t, ld, ptr(ids), ptr(out), ldd)
     return out
@@ -162,8 +163,9 @@ def combine(rows, slots, weights=None, *, source=None, out=None):
         if source.dtype != rows.dtype:
             raise error(_lib.CPG_ERR_DTYPE, f"source must be {rows.dtype} like rows")
     if out is None:
-        out = torch.empty((t, d), dtype=rows.dtype, device=dev)
-    ldy = output("out", out, (t, d), rows.dtype, dev)
+        out, ldy = torch.empty((t, d), dtype=rows.dtype, device=dev), d
+    else:
+        ldy = output("out", out, (t, d), rows.dtype, dev)
     call(_lib.load().cpg_combine_rows, "combine", dev, ptr(rows), code, r, d, ldr, ptr(slots),
           ptr(weights), t, k, ptr(source), lds, ptr(out), ldy)
     return out

@@ -63,7 +63,9 @@ def quantize_int8(x, out=None, scales=None):
     device = x.device
     if out is None:
         out = alloc_int8_rows(rows, cols, device)
-    ldq = output("out", out, (rows, cols), torch.int8, device)
+        ldq = out.stride(0) if rows > 1 else cols
+    else:
+        ldq = output("out", out, (rows, cols), torch.int8, device)
     if scales is None:
         scales = torch.empty(rows, dtype=torch.float32, device=device)
     else:

@@ -139,6 +139,43 @@ def test_route_strides_outputs_and_sizes():
         assert ((w.cpu().double() - rw).abs() <= WEIGHT_REL * rw).all()
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups,kept", [(64, 8, 3), (40, 5, 2), (256, 8, 8)])
+def test_route_biases_of_the_lowest_value(scoring, e, groups, kept):
+    """Biases of the type's lowest value as masks: ranked last but not out, also where the sum of a
+    group's two best passes the 32-bit range; infinite biases."""
+    low = torch.finfo(torch.float32).min
+    lg = logits_of(9, e, torch.float32, seed=e)
+    for pattern in range(4):
+        bias = torch.randn(e, generator=torch.Generator().manual_seed(pattern)) * 0.1
+        if pattern == 0:
+            bias[e // groups:] = low  # one group unmasked, the others wholly masked
+        elif pattern == 1:
+            bias[:] = low
+        elif pattern == 2:
+            bias[::2] = low
+            bias[1] = -low
+        else:
+            bias[3] = math.inf
+            bias[e // 2:] = -math.inf
+        check_route(lg, 6, bias=bias, scoring=scoring)
+        for score in ("max", "top2"):
+            check_route(lg, 6, bias=bias, scoring=scoring, groups=groups, kept_groups=kept,
+                        group_score=score)
+
+
+@pytest.mark.parametrize("e,k", [(64, 8), (256, 32), (1000, 20)])
+def test_route_many_equal_candidates(e, k):
+    """More candidates near the last choice than lanes: a row of few distinct values."""
+    g = torch.Generator().manual_seed(e)
+    lg = torch.randint(0, 2, (17, e), generator=g).float()
+    lg += torch.randint(0, 2, (17, e), generator=g) * 2.0 ** -23
+    bias = torch.randint(0, 2, (e,), generator=g).float() * 2.0 ** -24
+    for scoring in ("softmax", "sigmoid"):
+        check_route(lg, k, scoring=scoring)
+        check_route(lg, k, scoring=scoring, bias=bias)
+
+
 # ---------------------------------------------------------------------------------- gradient
 @pytest.mark.parametrize("e,k", [(1, 1), (8, 2), (33, 7), (100, 32), (128, 8), (256, 8), (512, 3),
                                  (1024, 32)])
