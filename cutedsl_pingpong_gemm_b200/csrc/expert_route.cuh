@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
         ++candidates;
       }
     }
-    if (__any_sync(0xffffffffu, near_pair)) {
+    if (__any_sync(0xffffffffu, near_pair || many)) {
       __syncwarp();
       if (many) {
         my_id = route_rank64<T, V>(p, row, open, by_logit);

@@ -164,6 +164,19 @@ def test_route_biases_of_the_lowest_value(scoring, e, groups, kept):
                         group_score=score)
 
 
+@pytest.mark.parametrize("e", [128, 256])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_more_equal_candidates_than_lanes(e, scoring):
+    """The last choice ties exactly with more experts than a warp has lanes, and behind those, past
+    what 32 bits tell apart, stands the better one: a bias one step higher."""
+    lg = torch.zeros(3, e)
+    bias = torch.full((e,), 0.25)
+    bias[e - 1] = 0.25 + 2.0 ** -25
+    bias[e - 2] = 0.25 + 2.0 ** -26
+    for k in (1, 8):
+        check_route(lg, k, bias=bias, scoring=scoring)
+
+
 @pytest.mark.parametrize("e,k", [(64, 8), (256, 32), (1000, 20)])
 def test_route_many_equal_candidates(e, k):
     """More candidates near the last choice than lanes: a row of few distinct values."""
