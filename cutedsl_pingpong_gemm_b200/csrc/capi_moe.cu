@@ -216,17 +216,6 @@ int check_route(const cpg_route_config* c, int64_t tokens) {
   return check_pairs(tokens, c->k);
 }
 
-// Calls f(std::integral_constant<int, V>) with the smallest V whose 32 lanes hold `experts`.
-template <typename F>
-void by_lane_values(int32_t experts, F&& f) {
-  if (experts <= 32) f(std::integral_constant<int, 1>{});
-  else if (experts <= 64) f(std::integral_constant<int, 2>{});
-  else if (experts <= 128) f(std::integral_constant<int, 4>{});
-  else if (experts <= 256) f(std::integral_constant<int, 8>{});
-  else if (experts <= 512) f(std::integral_constant<int, 16>{});
-  else f(std::integral_constant<int, 32>{});
-}
-
 // Whether every lane's run of V elements of every row starts on its vectors.
 template <int V>
 int32_t run_vectors(const void* p, int64_t ld, int32_t dtype) {
@@ -236,11 +225,18 @@ int32_t run_vectors(const void* p, int64_t ld, int32_t dtype) {
   return !misaligned(p, bytes) && (ld * es) % bytes == 0 ? 1 : 0;
 }
 
-// One warp per token, at most about as many as fit on the SMs at once (each then walks several
-// tokens with the biases it has loaded).
-unsigned route_grid(int64_t tokens) {
-  return static_cast<unsigned>(
-      std::min<int64_t>((tokens + cpg::kRouteWarps - 1) / cpg::kRouteWarps, kRouteBlocks));
+template <int L, int V>
+int launch_route(cpg::RouteParams p, int32_t dtype, cudaStream_t st) {
+  p.vec = run_vectors<V>(p.logits, p.ld, dtype);
+  p.vec_bias = run_vectors<V>(p.bias, 0, CPG_DTYPE_F32);
+  const size_t smem = sizeof(double) * 32 * V * cpg::kRouteWarps;
+  // At most about as many blocks as fit on the SMs at once; each then walks several tokens.
+  const int64_t per = 32 / L * cpg::kRouteWarps;
+  const unsigned grid =
+      static_cast<unsigned>(std::min<int64_t>((p.tokens + per - 1) / per, kRouteBlocks));
+  auto fn = dtype == CPG_DTYPE_BF16 ? &cpg::route_kernel<__nv_bfloat16, L, V>
+                                    : &cpg::route_kernel<float, L, V>;
+  return launch("route kernel", true, fn, grid, 32 * cpg::kRouteWarps, smem, st, 1, p);
 }
 
 template <int L, int V>
@@ -306,16 +302,23 @@ int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int6
                      weights,        c->experts,     c->k,       c->scoring, c->groups,
                      c->kept_groups, c->group_score, c->renormalize != 0 ? 1 : 0, 0, 0, c->scale};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  by_lane_values(c->experts, [&](auto v) {
-    constexpr int V = decltype(v)::value;
-    const size_t smem = sizeof(double) * 32 * V * cpg::kRouteWarps;
-    p.vec = run_vectors<V>(logits, ld, dtype);
-    p.vec_bias = run_vectors<V>(bias, 0, CPG_DTYPE_F32);
-    auto fn = dtype == CPG_DTYPE_BF16 ? &cpg::route_kernel<__nv_bfloat16, V>
-                                      : &cpg::route_kernel<float, V>;
-    rc = launch("route kernel", true, fn, route_grid(tokens), 32 * cpg::kRouteWarps, smem, st, 1, p);
-  });
-  return rc;
+  // Fewer lanes per token (and more experts a lane) while they hold the choices and the groups, and
+  // where scores are ranked one candidate more.  16384 tokens, top 8, ranked by logit / by sigmoid
+  // and bias in 8 groups: 64 experts 32 lanes 10.5 / 14.8 us, 8 and 16 lanes 5.3 / 11.0;
+  // 128 experts 32 lanes 11.2 / 15.7 us, 16 lanes 9.4 / 14.8; 256 experts 32 lanes 14.4 / 21.8 us,
+  // 16 lanes (whose 16 experts a lane leave room for too few warps) 14.8 / 27.5.
+  const bool by_logit = bias == nullptr && (c->groups == 1 || c->group_score == CPG_GROUP_MAX);
+  const int32_t e = c->experts, need = std::max(by_logit ? c->k : c->k + 1, c->groups);
+  if (need <= 8 && e <= 32) return launch_route<8, 4>(p, dtype, st);
+  if (need <= 8 && e <= 64) return launch_route<8, 8>(p, dtype, st);
+  if (need <= 16 && e <= 64) return launch_route<16, 4>(p, dtype, st);
+  if (need <= 16 && e <= 128) return launch_route<16, 8>(p, dtype, st);
+  if (e <= 32) return launch_route<32, 1>(p, dtype, st);
+  if (e <= 64) return launch_route<32, 2>(p, dtype, st);
+  if (e <= 128) return launch_route<32, 4>(p, dtype, st);
+  if (e <= 256) return launch_route<32, 8>(p, dtype, st);
+  if (e <= 512) return launch_route<32, 16>(p, dtype, st);
+  return launch_route<32, 32>(p, dtype, st);
 }
 
 int cpg_route_backward(const cpg_route_config* c, const float* dweights, const void* logits,

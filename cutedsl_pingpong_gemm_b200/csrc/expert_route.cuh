@@ -124,16 +124,43 @@ __device__ __forceinline__ void store_run(T* row, int e0, int experts, bool vec,
 __device__ __forceinline__ double neg_inf() { return __longlong_as_double(0xfff0000000000000ll); }
 __device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fc00000u); }
 
-template <typename F>
-__device__ __forceinline__ F warp_sum(F v) {
+// Reductions and ballots over the L consecutive lanes that share a token (all 32 lanes of the warp
+// must call them).
+template <int L, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ double warp_max(double v) {
+template <int L>
+__device__ __forceinline__ double lanes_max(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = L / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (L == 32) {
+    return __reduce_max_sync(0xffffffffu, v);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+}
+template <int L>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+  return ~lanes_max<L>(~v);
+}
+// One bit per lane of the token.
+template <int L>
+__device__ __forceinline__ uint32_t lanes_ballot(bool b) {
+  const uint32_t all = __ballot_sync(0xffffffffu, b);
+  if constexpr (L == 32) {
+    return all;
+  } else {
+    return (all >> (threadIdx.x & 31u & ~(L - 1u))) & ((1u << L) - 1u);
+  }
 }
 
 // Unsigned keys that order like the floats (no NaN; -0 just below +0).  Every key of a number above
@@ -146,8 +173,15 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
-__device__ __forceinline__ float warp_max(float v) {
-  return key_value(__reduce_max_sync(0xffffffffu, order_key(v)));
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (L == 32) {
+    return key_value(__reduce_max_sync(0xffffffffu, order_key(v)));
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
 }
 
 // e^x and 1 / x by the hardware's approximations, results below 2^-126 flushed to zero: at most
@@ -175,23 +209,24 @@ __device__ __forceinline__ bool route_bad(float l, int32_t scoring) {
 // probability.  Renormalised softmax shares are the softmax of the chosen logits alone;
 // renormalised sigmoid shares of logits all below -60, where sigmoid(l) = e^l, likewise (the sum
 // of the scores would underflow).  Lanes without a choice get 0.
+template <int L>
 __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormalize, bool has, float l,
                                              float prob) {
   if (!renormalize) return has ? (scoring == kRouteSoftmax ? prob : sigmoid32(l)) : 0.f;
-  const float top = warp_max(has ? l : -INFINITY);
+  const float top = lanes_max<L>(has ? l : -INFINITY);
   float v = 0.f;
   if (has) v = scoring == kRouteSoftmax || top < -60.f ? expf(l - top) : sigmoid32(l);
-  const float sum = warp_sum(v);
+  const float sum = lanes_sum<L>(v);
   return sum > 0.f ? __fdividef(v, sum) : 0.f;
 }
 
 // c of the lane's run of the row (by_logit: l) in 64 bits, -inf where an expert cannot be chosen.
-template <typename T, int V>
+template <typename T, int L, int V>
 __device__ __forceinline__ void route_scores64(const RouteParams& p, const T* row, bool by_logit,
                                                double (&c)[V]) {
-  const int lane = threadIdx.x & 31;
+  const int sub = threadIdx.x % L;
   float l[V];
-  load_run<T, V>(row, lane * V, p.experts, p.vec != 0, l);
+  load_run<T, V>(row, sub * V, p.experts, p.vec != 0, l);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (route_bad(l[i], p.scoring)) l[i] = -INFINITY;
@@ -200,7 +235,7 @@ __device__ __forceinline__ void route_scores64(const RouteParams& p, const T* ro
   if (softmax) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmax(top, static_cast<double>(l[i]));
-    top = warp_max(top);
+    top = lanes_max<L>(top);
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -211,10 +246,10 @@ __device__ __forceinline__ void route_scores64(const RouteParams& p, const T* ro
       c[i] = softmax ? exp(static_cast<double>(l[i]) - top) : sigmoid64(static_cast<double>(l[i]));
     sum += c[i];
   }
-  if (softmax) sum = warp_sum(sum);
+  if (softmax) sum = lanes_sum<L>(sum);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
+    const int e = sub * V + i;
     if (softmax) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
     if (p.bias != nullptr && e < p.experts) c[i] += static_cast<double>(p.bias[e]);
     if (!(l[i] > -INFINITY) || c[i] != c[i]) c[i] = neg_inf();
@@ -222,23 +257,23 @@ __device__ __forceinline__ void route_scores64(const RouteParams& p, const T* ro
 }
 
 // The kept groups of a row, one bit each, ranked in 64 bits: lane g scores group g and keeps it if
-// fewer than kept_groups are better (a higher score, or the same and a lower index).  c_sh: 32 * V
-// words of the warp's own shared memory.
-template <typename T, int V>
-__device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const T* row,
+// fewer than kept_groups are better (a higher score, or the same and a lower index).  c_sh: L * V
+// words of the token's own shared memory.
+template <typename T, int L, int V>
+__device__ __forceinline__ uint32_t route_groups64(const RouteParams& p, const T* row,
                                                 double* c_sh) {
-  const int lane = threadIdx.x & 31;
+  const int sub = threadIdx.x % L;
   double c[V];
-  route_scores64<T, V>(p, row, false, c);
+  route_scores64<T, L, V>(p, row, false, c);
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < V; ++i) c_sh[lane * V + i] = c[i];
+  for (int i = 0; i < V; ++i) c_sh[sub * V + i] = c[i];
   __syncwarp();
   const int per = p.experts / p.groups;
   double a = neg_inf(), b = neg_inf();
-  if (lane < p.groups) {
+  if (sub < p.groups) {
     for (int i = 0; i < per; ++i) {
-      const double v = c_sh[lane * per + i];
+      const double v = c_sh[sub * per + i];
       b = fmax(b, fmin(a, v));
       a = fmax(a, v);
     }
@@ -246,56 +281,56 @@ __device__ __noinline__ uint32_t route_groups64(const RouteParams& p, const T* r
   }
   int better = 0;
   for (int g = 0; g < p.groups; ++g) {
-    const double v = __shfl_sync(0xffffffffu, a, g);
-    better += (v > a || (v == a && g < lane)) ? 1 : 0;
+    const double v = __shfl_sync(0xffffffffu, a, g, L);
+    better += (v > a || (v == a && g < sub)) ? 1 : 0;
   }
   __syncwarp();
-  return __ballot_sync(0xffffffffu, lane < p.groups && better < p.kept_groups);
+  return lanes_ballot<L>(sub < p.groups && better < p.kept_groups);
 }
 
-// Place of this lane's candidate id (-1: none) among the first `candidates` lanes', c in 64 bits.
-template <typename T, int V>
-__device__ __noinline__ int route_place64(const RouteParams& p, const T* row, int32_t id,
-                                          int candidates, bool by_logit) {
+// Place of this lane's candidate id (-1: none) among those of the token's lanes, c in 64 bits.
+template <typename T, int L, int V>
+__device__ __forceinline__ int route_place64(const RouteParams& p, const T* row, int32_t id,
+                                          bool by_logit) {
   double mine = neg_inf();
   if (id >= 0) mine = static_cast<double>(route_load(row + id));
   if (!by_logit) {
     if (p.scoring == kRouteSoftmax) {
       float l[V];
-      load_run<T, V>(row, (threadIdx.x & 31) * V, p.experts, p.vec != 0, l);
+      load_run<T, V>(row, (threadIdx.x % L) * V, p.experts, p.vec != 0, l);
       double top = neg_inf(), sum = 0.0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (route_bad(l[i], p.scoring)) l[i] = -INFINITY;
         top = fmax(top, static_cast<double>(l[i]));
       }
-      top = warp_max(top);
+      top = lanes_max<L>(top);
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (l[i] > -INFINITY) sum += exp(static_cast<double>(l[i]) - top);
-      mine = exp(mine - top) / warp_sum(sum);
+      mine = exp(mine - top) / lanes_sum<L>(sum);
     } else {
       mine = sigmoid64(mine);
     }
     if (id >= 0 && p.bias != nullptr) mine += static_cast<double>(p.bias[id]);
   }
   int place = 0;
-  for (int i = 0; i < candidates; ++i) {
-    const double v = __shfl_sync(0xffffffffu, mine, i);
-    const int32_t other = __shfl_sync(0xffffffffu, id, i);
-    place += (v > mine || (v == mine && other < id)) ? 1 : 0;
+  for (int i = 0; i < L; ++i) {
+    const double v = __shfl_sync(0xffffffffu, mine, i, L);
+    const int32_t other = __shfl_sync(0xffffffffu, id, i, L);
+    if (other >= 0) place += (v > mine || (v == mine && other < id)) ? 1 : 0;
   }
   return place;
 }
 
 // The k best experts of a row among those whose bit of `open` (one per place of the lane's run) is
 // set, c in 64 bits: lane j returns choice j, or -1.
-template <typename T, int V>
-__device__ __noinline__ int32_t route_rank64(const RouteParams& p, const T* row, uint32_t open,
+template <typename T, int L, int V>
+__device__ __forceinline__ int32_t route_rank64(const RouteParams& p, const T* row, uint32_t open,
                                              bool by_logit) {
-  const int lane = threadIdx.x & 31;
+  const int sub = threadIdx.x % L;
   double c[V];
-  route_scores64<T, V>(p, row, by_logit, c);
+  route_scores64<T, L, V>(p, row, by_logit, c);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (((open >> i) & 1u) == 0u) c[i] = neg_inf();
@@ -310,12 +345,12 @@ __device__ __noinline__ int32_t route_rank64(const RouteParams& p, const T* row,
         at = i;
       }
     }
-    const double all = warp_max(best);
-    if (!(all > neg_inf())) break;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, best == all)) - 1;
-    const int id = __shfl_sync(0xffffffffu, lane * V + at, owner);
-    if (lane == j) my_id = id;
-    if (lane == owner) {
+    const double all = lanes_max<L>(best);
+    const bool some = all > neg_inf();
+    const int owner = __ffs(lanes_ballot<L>(best == all)) - 1;
+    const int id = __shfl_sync(0xffffffffu, sub * V + at, owner, L);
+    if (some && sub == j) my_id = id;
+    if (some && sub == owner) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (i == at) c[i] = neg_inf();
@@ -346,9 +381,10 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
   }
 }
 
-// One warp per token; lane l holds experts l * V .. l * V + V - 1.  Each lane sorts the keys of its
-// run; the choices are then k warp-wide maxima of the lanes' first keys, the lane that holds the
-// maximum moving up by one.  The low log2 V bits of a key hold the place in the run (lower places
+// L lanes per token (k and groups <= L, experts <= L * V), so that what a warp does per token serves
+// 32 / L of them; lane l of them holds experts l * V .. l * V + V - 1.  Each lane sorts the keys of
+// its run; the choices are then k maxima over the lanes' first keys, the lane that holds the maximum
+// moving up by one.  The low log2 V bits of a key hold the place in the run (lower places
 // first), so a key names its expert in the run; what they cost in precision is part of the bound
 // below.
 //
@@ -357,35 +393,42 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 //            the sum 1 + e^-l and the quotient add 2.5: below 2^-21 altogether.
 //   softmax: p = e^(l - top) inv with inv <= 1 the common factor.  Each exponential is off by at most
 //            (2.9 ulp) inv absolutely; inv by (10.2 + 18.5 + 1) ulp relatively (the terms' errors
-//            weighted by p, whose mean |l - top| is at most ln 1024; 37 additions; the quotient),
+//            weighted by p, whose mean |l - top| is at most ln 1024; V + log2 L <= 37 additions;
+//            the quotient),
 //            which the largest p <= inv carries: below 2^-18 inv altogether.
 // c = s + bias adds half an ulp of c, a key's lost bits less than V ulp.  Two c nearer than twice the
 // bound are ranked in 64 bits (the choices and what is near the last of them; groups likewise),
 // unless logit and bias are the same: such c are equal, and the lower index goes first.
-template <typename T, int V>
+template <typename T, int L, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 2))
     route_kernel(const __grid_constant__ RouteParams p) {
   kernel_begins();
   extern __shared__ double route_smem[];
   __shared__ int32_t chosen[kRouteWarps][kRouteMaxK];
   constexpr uint32_t kPlace = V - 1;  // bits of a key that hold the place in the run
+  constexpr int kTokens = 32 / L;  // of a warp
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
+  const int sub = lane % L;     // lane of the token
+  const int first = lane - sub; // the warp's lane that is the token's first
   double* c_sh = route_smem + warp * (32 * V);
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRouteWarps;
+  int32_t* picks = &chosen[warp][first];
   const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_score == kRouteGroupMax);
   const bool softmax = p.scoring == kRouteSoftmax;
-  const int e0 = lane * V;
+  const int e0 = sub * V;
   const bool off = e0 >= p.experts;  // a lane without experts
   const int per = p.experts / p.groups;  // experts of a group
   const int lanes = per / V;             // lanes of a group, when that is a whole power of two
   const bool whole = lanes * V == per && (lanes & (lanes - 1)) == 0;
-  const int group = whole ? lane / lanes : lane;     // the group this lane scores
+  const int group = whole ? sub / lanes : sub;       // the group this lane scores
   const int first_group = e0 / per;                  // group of the run's first expert ...
   const int first_left = per - (e0 - first_group * per);  // ... and how many of it follow
-  for (int64_t t = blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp; t < p.tokens;
-       t += stride) {
-    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRouteWarps * kTokens;
+  for (int64_t t0 = (blockIdx.x * static_cast<int64_t>(kRouteWarps) + warp) * kTokens;
+       t0 < p.tokens; t0 += step) {
+    const int64_t t = t0 + lane / L;
+    const bool live = t < p.tokens;  // past the last token a lane works on row 0 and stores nothing
+    const T* row = static_cast<const T*>(p.logits) + (live ? t : 0) * p.ld;
     float l[V], c[V];
     load_run<T, V>(row, e0, p.experts, p.vec != 0, l);
     bool bad = false;
@@ -410,7 +453,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
 #pragma unroll
         for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
         if (kAll && off) top = -INFINITY;
-        top = warp_max(top);
+        top = lanes_max<L>(top);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -418,7 +461,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
           sum += c[i];
         }
         if (kAll && off) sum = 0.f;
-        sum = warp_sum(sum);
+        sum = lanes_sum<L>(sum);
         inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
       }
       if (by_logit) {
@@ -455,7 +498,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
     }
     if (__any_sync(0xffffffffu, finite != finite)) {
       clean();
-      bad = __any_sync(0xffffffffu, bad);
+      bad = lanes_ballot<L>(bad) != 0u;
       score(std::false_type{});
     }
     // Two c whose difference is at most near + rel (|c1| + |c2|) may be in another order.
@@ -477,14 +520,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
           a = fmaxf(a, u);
         }
       } else {
-        float* f_sh = reinterpret_cast<float*>(c_sh);
+        float* f_sh = reinterpret_cast<float*>(c_sh + first * V);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < V; ++i) f_sh[e0 + i] = c[i];
         __syncwarp();
-        if (lane < p.groups) {
+        if (sub < p.groups) {
           for (int i = 0; i < per; ++i) {
-            const float v = f_sh[lane * per + i];
+            const float v = f_sh[sub * per + i];
             a2 = fmaxf(a2, fminf(a, v));
             a = fmaxf(a, v);
           }
@@ -502,29 +545,30 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
       uint32_t rank_key = real && a > -INFINITY ? order_key(a) : kNoKey;
       bool kept = false;
       for (int i = 0; i < p.kept_groups; ++i) {
-        const uint32_t best = __reduce_max_sync(0xffffffffu, rank_key);
-        if (best == kNoKey) break;
-        const int owner = __ffs(__ballot_sync(0xffffffffu, rank_key == best)) - 1;
-        if (group == __shfl_sync(0xffffffffu, group, owner)) {
+        const uint32_t best = lanes_max<L>(rank_key);
+        const int owner = __ffs(lanes_ballot<L>(rank_key == best)) - 1;
+        if (group == __shfl_sync(0xffffffffu, group, owner, L) && best != kNoKey) {
           kept = true;
           rank_key = kNoKey;
         }
       }
       if (!by_logit) {
         const uint32_t worst_kept =
-            __reduce_min_sync(0xffffffffu, kept && some ? order_key(a - slack) : 0xffffffffu);
+            lanes_min<L>(kept && some ? order_key(a - slack) : 0xffffffffu);
         const uint32_t best_left =
-            __reduce_max_sync(0xffffffffu, !kept && some ? order_key(a + slack) : kNoKey);
+            lanes_max<L>(!kept && some ? order_key(a + slack) : kNoKey);
         // A sum that overflows (biases of the lowest value as masks) has no 32-bit rank at all.
         const bool lost = some && !(fabsf(a) + slack < INFINITY);
-        if (best_left >= worst_kept || __any_sync(0xffffffffu, lost)) {
-          kept = (route_groups64<T, V>(p, row, c_sh) >> group) & 1u;
-        }
+        // Every lane votes, and one token's doubt has all tokens of the warp ranked again: lanes that
+        // skipped a vote or a shuffle because of their token would leave the others waiting in it.
+        const bool close = best_left >= worst_kept;
+        if (__any_sync(0xffffffffu, close | lost))
+          kept = (route_groups64<T, L, V>(p, row, c_sh + first * V) >> group) & 1u;
       }
       if (whole) {
         if (!kept) open = 0u;
       } else {
-        const uint32_t keep = __ballot_sync(0xffffffffu, kept);
+        const uint32_t keep = lanes_ballot<L>(kept);
         int g = first_group, left = first_left;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -554,11 +598,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
     rest[32 * (V - 1)] = 0u;
     // The row's largest key without its place bits (all ones), at most kNoKey if none is left, and
     // the lane that gives it: the lowest among equals.
-    auto largest = [&]() { return __reduce_max_sync(0xffffffffu, head | kPlace); };
+    auto largest = [&]() { return lanes_max<L>(head | kPlace); };
     auto holds = [&](uint32_t all) {
       const bool equal = (head | kPlace) == all;
-      const uint32_t lanes = __ballot_sync(0xffffffffu, equal);
-      return equal && (lanes & ((1u << lane) - 1u)) == 0u;
+      const uint32_t those = lanes_ballot<L>(equal);
+      return equal && (those & ((1u << sub) - 1u)) == 0u;
     };
     auto next = [&]() {  // on to the lane's next key
       head = *rest;
@@ -566,18 +610,21 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
     };
     uint32_t my_key = kNoKey, last_key = kNoKey;
     int found = 0;
-    for (; found < p.k; ++found) {
+    for (int j = 0; j < p.k; ++j) {
       const uint32_t all = largest();
-      if (all <= kNoKey) break;
-      if (holds(all)) {
-        chosen[warp][found] = e0 + static_cast<int>(kPlace - (head & kPlace));
+      const bool some = all > kNoKey;
+      if (holds(all) && some) {
+        picks[j] = e0 + static_cast<int>(kPlace - (head & kPlace));
         next();
       }
-      if (lane == found) my_key = all;
-      last_key = all;
+      if (some) {
+        if (sub == j) my_key = all;
+        last_key = all;
+        ++found;
+      }
     }
     __syncwarp();
-    int32_t my_id = lane < found ? chosen[warp][lane] : -1;
+    int32_t my_id = sub < found ? picks[sub] : -1;
     __syncwarp();
     float my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
     bool near_pair = false;
@@ -591,52 +638,55 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
       };
       // Neighbours in the order.
       const float my_b = my_id >= 0 && p.bias != nullptr ? __ldg(p.bias + my_id) : 0.f;
-      const uint32_t next_key = __shfl_down_sync(0xffffffffu, my_key, 1);
-      const float next_l = __shfl_down_sync(0xffffffffu, my_l, 1);
-      const float next_b = __shfl_down_sync(0xffffffffu, my_b, 1);
-      near_pair = lane + 1 < found && nearer(my_key, next_key) &&
+      const uint32_t next_key = __shfl_down_sync(0xffffffffu, my_key, 1, L);
+      const float next_l = __shfl_down_sync(0xffffffffu, my_l, 1, L);
+      const float next_b = __shfl_down_sync(0xffffffffu, my_b, 1, L);
+      near_pair = sub + 1 < found && nearer(my_key, next_key) &&
                   !(my_l == next_l && my_b == next_b);
       // The last choice against the best ones left: those that are near become candidates too.
-      while (found == p.k) {
+      const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1, L);
+      const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1, L);
+      bool more = found == p.k;
+      while (true) {
         const uint32_t all = largest();
-        if (all <= kNoKey || !nearer(last_key, all)) break;
-        if (candidates == kRouteMaxK) {
+        more = more && all > kNoKey && nearer(last_key, all);
+        if (more && candidates == L) {
           many = true;
-          break;
+          more = false;
         }
-        const float last_l = __shfl_sync(0xffffffffu, my_l, p.k - 1);
-        const float last_b = __shfl_sync(0xffffffffu, my_b, p.k - 1);
-        if (holds(all)) {
+        if (!__any_sync(0xffffffffu, more)) break;
+        if (holds(all) && more) {
           const int id = e0 + static_cast<int>(kPlace - (head & kPlace));
-          chosen[warp][candidates] = id;
+          picks[candidates] = id;
           near_pair |= route_load(row + id) != last_l ||
                        (p.bias != nullptr ? __ldg(p.bias + id) : 0.f) != last_b;
           next();
         }
-        ++candidates;
+        if (more) ++candidates;
       }
     }
     if (__any_sync(0xffffffffu, near_pair || many)) {
       __syncwarp();
-      if (many) {
-        my_id = route_rank64<T, V>(p, row, open, by_logit);
+      // For all tokens of the warp alike, again: the 64-bit order is right for every one of them.
+      if (__any_sync(0xffffffffu, many)) {
+        my_id = route_rank64<T, L, V>(p, row, open, by_logit);
       } else {
-        const int32_t id = lane < candidates ? chosen[warp][lane] : -1;
-        const int rank = route_place64<T, V>(p, row, id, candidates, by_logit);
+        const int32_t id = sub < candidates ? picks[sub] : -1;
+        const int place = route_place64<T, L, V>(p, row, id, by_logit);
         __syncwarp();
-        if (id >= 0 && rank < p.k) chosen[warp][rank] = id;
+        if (id >= 0 && place < p.k) picks[place] = id;
         __syncwarp();
-        my_id = lane < found ? chosen[warp][lane] : -1;
+        my_id = sub < found ? picks[sub] : -1;
         __syncwarp();
       }
       my_l = my_id >= 0 ? route_load(row + my_id) : 0.f;
     }
     const bool has = my_id >= 0;
     const float prob = has && softmax && !p.renormalize ? expf(my_l - top) * inv : 0.f;
-    const float w = route_share(p.scoring, p.renormalize, has, my_l, prob);
-    if (lane < p.k) {
-      p.ids[t * p.k + lane] = my_id;
-      p.weights[t * p.k + lane] = bad ? nan_f32() : w * p.scale;
+    const float w = route_share<L>(p.scoring, p.renormalize, has, my_l, prob);
+    if (live && sub < p.k) {
+      p.ids[t * p.k + sub] = my_id;
+      p.weights[t * p.k + sub] = bad ? nan_f32() : w * p.scale;
     }
   }
 }
