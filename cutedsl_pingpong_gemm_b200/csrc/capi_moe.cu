@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <type_traits>
 
@@ -19,6 +20,7 @@ namespace {
 constexpr int64_t kRouteBlocks = 148 * 8;
 constexpr int64_t kFewThreads = 148 * 1024;  // half of the threads that fit on the SMs
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;  // rows and pairs are counted in int32
+constexpr int64_t kMaxCols = int64_t(1) << 30;         // the kernels' column arithmetic is 32-bit
 
 bool float_dtype(int32_t dtype) { return dtype == CPG_DTYPE_BF16 || dtype == CPG_DTYPE_F32; }
 int bytes_of(int32_t dtype) { return dtype == CPG_DTYPE_F32 ? 4 : (dtype == CPG_DTYPE_I8 ? 1 : 2); }
@@ -31,8 +33,8 @@ unsigned row_grid(int64_t rows) { return static_cast<unsigned>(std::min<int64_t>
 
 // rows x cols of a row-major matrix with row stride ld: sizes and stride make sense.
 int check_matrix(const char* name, int64_t rows, int64_t cols, int64_t ld) {
-  if (rows < 0 || rows > kMaxRows || cols < 0 || cols > kMaxRows)
-    return fail(CPG_ERR_INVALID_SHAPE, "%s: %lld x %lld is not within [0, 2^31)", name,
+  if (rows < 0 || rows > kMaxRows || cols < 0 || cols >= kMaxCols)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: %lld x %lld is not within [0, 2^31) x [0, 2^30)", name,
                 static_cast<long long>(rows), static_cast<long long>(cols));
   if (ld < cols)
     return fail(CPG_ERR_INVALID_SHAPE, "%s: row stride %lld below the row length %lld", name,
@@ -81,9 +83,39 @@ int launch(const char* what, bool early, void (*kernel)(P...), unsigned grid, un
   return e == cudaSuccess ? CPG_OK : cuda_fail(e, what);
 }
 
-// Rows that start on 16 bytes (the vector kernels, whose column arithmetic is 32-bit).
-bool vector_rows(const void* p, int64_t cols, int64_t ld, int elem) {
-  return !misaligned(p, 16) && (ld * elem) % 16 == 0 && cols < (int64_t(1) << 30);
+// Rows that start on 16 bytes.
+bool vector_rows(const void* p, int64_t ld, int elem) {
+  return !misaligned(p, 16) && (ld * elem) % 16 == 0;
+}
+
+// The widest access (16, 8, 4 or 2 bytes) that every row of these matrices starts on.
+// 8192 tokens x 4 choices, BF16, in us with accesses of 16 / 8 / 4 / 2 bytes (2048, 2052, 2050 and
+// 2049 columns) and, in brackets, of the kernels of one element an access that these replaced:
+// copy 36 / 39 / 41 / 41 [79], combine 30 / 41 / 50 / 67 [82], its gradient 50 / 57 / 61 / 81 [116].
+struct Rows {
+  const void* p;
+  int64_t ld;
+};
+int row_width(std::initializer_list<Rows> all, int elem) {
+  uint64_t bits = 16;
+  for (const Rows& r : all)
+    bits |= reinterpret_cast<uintptr_t>(r.p) | static_cast<uint64_t>(r.ld * elem);
+  return static_cast<int>(bits & (~bits + 1));
+}
+
+// f(type of the elements, width of the accesses) for the pair at hand.
+template <typename F>
+int by_width(int32_t dtype, int width, F&& f) {
+  using std::integral_constant;
+  if (dtype == CPG_DTYPE_BF16) {
+    if (width == 16) return f(__nv_bfloat16{}, integral_constant<int, 16>{});
+    if (width == 8) return f(__nv_bfloat16{}, integral_constant<int, 8>{});
+    if (width == 4) return f(__nv_bfloat16{}, integral_constant<int, 4>{});
+    return f(__nv_bfloat16{}, integral_constant<int, 2>{});
+  }
+  if (width == 16) return f(float{}, integral_constant<int, 16>{});
+  if (width == 8) return f(float{}, integral_constant<int, 8>{});
+  return f(float{}, integral_constant<int, 4>{});
 }
 
 template <typename T, int G, int NV, bool Resident>
@@ -116,41 +148,21 @@ int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
   }
 }
 
-// Warps of work and blocks of 8 warps for rows cut into chunks of `vecs` vectors a lane.
-template <typename T>
-int32_t row_chunks(int64_t cols, int vecs) {
-  const int64_t per = int64_t(32) * vecs * cpg::RowVec<T>::kElems;
+// Chunks of a row for warps whose lanes make n accesses of W bytes, and blocks of 8 warps.
+template <typename T, int W>
+int32_t row_chunks(int64_t cols, int n) {
+  const int64_t per = int64_t(32) * n * cpg::RowAccess<T, W>::kElems;
   return static_cast<int32_t>((cols + per - 1) / per);
 }
 unsigned warp_grid(int64_t warps) { return row_grid((warps + 7) / 8); }
 
-template <typename T>
-int launch_copy_vec(const cpg::RowsParams& p, cudaStream_t st) {
-  const int32_t chunks = row_chunks<T>(p.cols, cpg::kCopyVecs);
-  return launch("row copy kernel", true, &cpg::rows_copy_vec_kernel<T>, warp_grid(p.tokens * chunks), 256,
-                0, st, 1, p, chunks);
-}
-
-template <typename T>
-int launch_combine_vec(const cpg::CombineParams& p, cudaStream_t st) {
-  const int32_t chunks = row_chunks<T>(p.cols, cpg::kCombineVecs);
-  return launch("combine kernel", true, &cpg::combine_vec_kernel<T>, warp_grid(p.tokens * chunks), 256, 0,
-                st, 1, p, chunks);
-}
-
-int launch_rows(const cpg::RowsParams& p, int32_t dtype_x, bool int8, cudaStream_t st) {
-  const unsigned grid = row_grid(p.tokens);
-  if (vector_rows(p.x, p.cols, p.ldx, bytes_of(dtype_x)) &&
-      vector_rows(p.rows, p.cols, p.ldr, int8 ? 1 : bytes_of(dtype_x))) {
-    if (dtype_x == CPG_DTYPE_BF16)
-      return int8 ? launch_int8_vec<__nv_bfloat16>(p, st) : launch_copy_vec<__nv_bfloat16>(p, st);
-    return int8 ? launch_int8_vec<float>(p, st) : launch_copy_vec<float>(p, st);
-  }
-  auto fn = dtype_x == CPG_DTYPE_BF16
-                ? (int8 ? &cpg::rows_kernel<__nv_bfloat16, int8_t>
-                        : &cpg::rows_kernel<__nv_bfloat16, __nv_bfloat16>)
-                : (int8 ? &cpg::rows_kernel<float, int8_t> : &cpg::rows_kernel<float, float>);
-  return launch("row kernel", true, fn, grid, 256, 0, st, 1, p);
+int launch_int8(const cpg::RowsParams& p, int32_t dtype_x, cudaStream_t st) {
+  if (vector_rows(p.x, p.ldx, bytes_of(dtype_x)) && vector_rows(p.rows, p.ldr, 1))
+    return dtype_x == CPG_DTYPE_BF16 ? launch_int8_vec<__nv_bfloat16>(p, st)
+                                     : launch_int8_vec<float>(p, st);
+  auto fn = dtype_x == CPG_DTYPE_BF16 ? &cpg::rows_int8_kernel<__nv_bfloat16>
+                                      : &cpg::rows_int8_kernel<float>;
+  return launch("INT8 row kernel", false, fn, row_grid(p.tokens), 256, 0, st, 1, p);
 }
 
 // Blocks the cluster of an expert order kernel (`which`: its place among the variants) may have on
@@ -282,7 +294,7 @@ int cpg_quantize_int8(const void* x, int32_t dtype_x, int64_t rows, int64_t cols
   if (misaligned(x, bytes_of(dtype_x)) || misaligned(scales, 4))
     return fail(CPG_ERR_ALIGNMENT, "x and scales must be aligned to their elements");
   const cpg::RowsParams p{x, rows, cols, ldx, nullptr, 1, q, rows, ldq, scales};
-  return launch_rows(p, dtype_x, true, static_cast<cudaStream_t>(stream));
+  return launch_int8(p, dtype_x, static_cast<cudaStream_t>(stream));
 }
 
 int cpg_route(const cpg_route_config* c, const void* logits, int32_t dtype, int64_t tokens,
@@ -406,7 +418,16 @@ int cpg_dispatch_rows(const void* x, int32_t dtype_x, int64_t tokens, int64_t co
       misaligned(slots, 4) || misaligned(scales, 4))
     return fail(CPG_ERR_ALIGNMENT, "x, rows, slots and scales must be aligned to their elements");
   const cpg::RowsParams p{x, tokens, cols, ldx, slots, k, rows, num_rows, ldr, scales};
-  return launch_rows(p, dtype_x, int8, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int8) return launch_int8(p, dtype_x, st);
+  return by_width(dtype_x, row_width({{x, ldx}, {rows, ldr}}, bytes_of(dtype_x)),
+                  [&](auto type, auto width) {
+    using T = decltype(type);
+    constexpr int W = decltype(width)::value;
+    const int32_t chunks = row_chunks<T, W>(cols, cpg::row_accesses<W>(cpg::kCopyVecs));
+    return launch("row copy kernel", true, &cpg::rows_copy_kernel<T, W>,
+                  warp_grid(tokens * chunks), 256, 0, st, 1, p, chunks);
+  });
 }
 
 int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
@@ -429,14 +450,14 @@ int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t 
   const cpg::CombineParams p{rows,   num_rows, cols,   ldr,       slots, weights,
                              tokens, k,        source, ld_source, y,     ldy};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (vector_rows(rows, cols, ldr, es) && vector_rows(y, cols, ldy, es) &&
-      (source == nullptr || vector_rows(source, cols, ld_source, es))) {
-    return dtype == CPG_DTYPE_BF16 ? launch_combine_vec<__nv_bfloat16>(p, st)
-                                   : launch_combine_vec<float>(p, st);
-  }
-  auto fn = dtype == CPG_DTYPE_BF16 ? &cpg::combine_kernel<__nv_bfloat16>
-                                    : &cpg::combine_kernel<float>;
-  return launch("combine kernel", true, fn, row_grid(tokens), 256, 0, st, 1, p);
+  const Rows src = source != nullptr ? Rows{source, ld_source} : Rows{y, ldy};
+  return by_width(dtype, row_width({{rows, ldr}, {y, ldy}, src}, es), [&](auto type, auto width) {
+    using T = decltype(type);
+    constexpr int W = decltype(width)::value;
+    const int32_t chunks = row_chunks<T, W>(cols, cpg::combine_accesses<T, W>());
+    return launch("combine kernel", true, &cpg::combine_kernel<T, W>, warp_grid(tokens * chunks),
+                  256, 0, st, 1, p, chunks);
+  });
 }
 
 int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int64_t cols,
@@ -462,14 +483,12 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
   const cpg::CombineGradParams p{dy,    tokens,  cols, lddy,  rows, num_rows, ldr,
                                  slots, weights, k,    drows, lddr, dweights};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = warp_grid(tokens * k);
-  const bool vec = vector_rows(dy, cols, lddy, es) && vector_rows(rows, cols, ldr, es) &&
-                   vector_rows(drows, cols, lddr, es);
-  auto fn = dtype == CPG_DTYPE_BF16
-                ? (vec ? &cpg::combine_grad_vec_kernel<__nv_bfloat16>
-                       : &cpg::combine_grad_kernel<__nv_bfloat16>)
-                : (vec ? &cpg::combine_grad_vec_kernel<float> : &cpg::combine_grad_kernel<float>);
-  return launch("combine gradient kernel", true, fn, grid, 256, 0, st, 1, p);
+  return by_width(dtype, row_width({{dy, lddy}, {rows, ldr}, {drows, lddr}}, es),
+                  [&](auto type, auto width) {
+    return launch("combine gradient kernel", true,
+                  &cpg::combine_grad_kernel<decltype(type), decltype(width)::value>,
+                  warp_grid(tokens * k), 256, 0, st, 1, p);
+  });
 }
 
 }  // extern "C"

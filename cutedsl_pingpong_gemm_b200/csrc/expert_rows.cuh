@@ -32,15 +32,8 @@ struct RowVec<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  __device__ __forceinline__ static uint4 pack(const float* f) {
-    return make_uint4(ptx::pack_bf16x2(f[0], f[1]), ptx::pack_bf16x2(f[2], f[3]),
-                      ptx::pack_bf16x2(f[4], f[5]), ptx::pack_bf16x2(f[6], f[7]));
-  }
   __device__ __forceinline__ static float load(const __nv_bfloat16* p) {
     return __bfloat162float(*p);
-  }
-  __device__ __forceinline__ static void store(__nv_bfloat16* p, float v) {
-    *p = __float2bfloat16_rn(v);
   }
 };
 template <>
@@ -52,12 +45,7 @@ struct RowVec<float> {
     f[2] = __uint_as_float(v.z);
     f[3] = __uint_as_float(v.w);
   }
-  __device__ __forceinline__ static uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                      __float_as_uint(f[3]));
-  }
   __device__ __forceinline__ static float load(const float* p) { return *p; }
-  __device__ __forceinline__ static void store(float* p, float v) { *p = v; }
 };
 
 // The bit pattern of |v|: non-negative floats order like their bits, infinities and NaN last.
@@ -76,8 +64,8 @@ __device__ __forceinline__ uint32_t int8_quotient(float x, float s) {
 }
 
 // ---------------------------------------------------------------- rows of whole vectors
-// The vector kernels need rows that start on 16 bytes (input and output) and fewer than 2^30
-// columns; the last vector of a row may be partial.  Loads bypass L1 (every row is read once).
+// Rows that start on 16 bytes and have fewer than 2^30 columns; the last vector of a row may be
+// partial.  Loads bypass L1 (every row is read once).
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 r;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -107,24 +95,6 @@ template <typename T>
 __device__ __forceinline__ uint4 ld_row_vec(const T* row, int32_t c, int32_t cols) {
   if (c + RowVec<T>::kElems <= cols) return ld_stream_v4(row + c);
   return ld_tail_v4(row + c, cols - c);
-}
-
-template <typename T>
-__device__ __forceinline__ void st_row_vec(T* row, int32_t c, int32_t cols, const uint4& v) {
-  if (c + RowVec<T>::kElems <= cols) {
-    ptx::st_global_v4(row + c, v.x, v.y, v.z, v.w);
-    return;
-  }
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < RowVec<T>::kElems; ++j) {
-    if (c + j < cols) {
-      if constexpr (sizeof(T) == 2)
-        row[c + j] = __ushort_as_bfloat16(static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))));
-      else
-        row[c + j] = __uint_as_float(w[j]);
-    }
-  }
 }
 
 // The largest |value| seen, as bits: of FP32 one word, of BF16 one maximum per half word.
@@ -202,6 +172,119 @@ __device__ __forceinline__ void st_int8_vec(int8_t* row, int32_t c, int32_t cols
     if (c + j < cols) row[c + j] = static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3)));
 }
 
+// ------------------------------------------------------ accesses as wide as the rows' alignment
+// W bytes of a row of T at a time (16, 8, 4, or 2 for BF16): all the rows' addresses are multiples of
+// W.  The last access of a row may be partial.
+template <typename T, int W>
+struct RowAccess {
+  static constexpr int kElems = W / static_cast<int>(sizeof(T));
+  static constexpr int kWords = W < 4 ? 1 : W / 4;
+  struct Data {
+    uint32_t w[kWords];
+  };
+  __device__ __forceinline__ static Data zero() {
+    Data d;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) d.w[i] = 0u;
+    return d;
+  }
+  __device__ __forceinline__ static uint32_t bits(const T* p) {
+    if constexpr (sizeof(T) == 2)
+      return *reinterpret_cast<const uint16_t*>(p);
+    else
+      return *reinterpret_cast<const uint32_t*>(p);
+  }
+  // kElems elements at p.  `Once`: read by this kernel only and once (16 bytes: past L1; narrower
+  // accesses share their sectors with the neighbours' through L1).
+  template <bool Once>
+  __device__ __forceinline__ static Data load_all(const T* p) {
+    Data d;
+    if constexpr (W == 16) {
+      const uint4 v = Once ? ld_stream_v4(p) : *reinterpret_cast<const uint4*>(p);
+      d.w[0] = v.x;
+      d.w[1] = v.y;
+      d.w[2] = v.z;
+      d.w[3] = v.w;
+    } else if constexpr (W == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      d.w[0] = v.x;
+      d.w[1] = v.y;
+    } else if constexpr (W == 4) {
+      d.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      d.w[0] = bits(p);
+    }
+    return d;
+  }
+  // Elements [c, c + kElems), zeros past the row's end.
+  template <bool Once>
+  __device__ __forceinline__ static Data load(const T* row, int32_t c, int32_t cols) {
+    if (c + kElems <= cols) return load_all<Once>(row + c);
+    Data d = zero();
+#pragma unroll
+    for (int j = 0; j < kElems; ++j) {
+      if (c + j < cols) {
+        if constexpr (sizeof(T) == 2)
+          d.w[j >> 1] |= bits(row + c + j) << (16 * (j & 1));
+        else
+          d.w[j] = bits(row + c + j);
+      }
+    }
+    return d;
+  }
+  __device__ __forceinline__ static void store(T* row, int32_t c, int32_t cols, const Data& d) {
+    if (c + kElems <= cols) {
+      T* p = row + c;
+      if constexpr (W == 16)
+        ptx::st_global_v4(p, d.w[0], d.w[1], d.w[2], d.w[3]);
+      else if constexpr (W == 8)
+        *reinterpret_cast<uint2*>(p) = make_uint2(d.w[0], d.w[1]);
+      else if constexpr (W == 4)
+        *reinterpret_cast<uint32_t*>(p) = d.w[0];
+      else
+        *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(d.w[0]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kElems; ++j) {
+      if (c + j < cols) {
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint16_t*>(row + c + j) =
+              static_cast<uint16_t>(d.w[j >> 1] >> (16 * (j & 1)));
+        else
+          *reinterpret_cast<uint32_t*>(row + c + j) = d.w[j];
+      }
+    }
+  }
+  __device__ __forceinline__ static void unpack(const Data& d, float* f) {
+#pragma unroll
+    for (int j = 0; j < kElems; ++j) {
+      if constexpr (sizeof(T) == 2)
+        f[j] = __uint_as_float((j & 1) ? d.w[j >> 1] & 0xffff0000u : d.w[j >> 1] << 16);
+      else
+        f[j] = __uint_as_float(d.w[j]);
+    }
+  }
+  __device__ __forceinline__ static Data pack(const float* f) {
+    Data d;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        d.w[i] = ptx::pack_bf16x2(f[2 * i], kElems > 1 ? f[2 * i + (kElems > 1 ? 1 : 0)] : 0.f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) d.w[i] = __float_as_uint(f[i]);
+    }
+    return d;
+  }
+};
+
+// Accesses a lane has in flight where 16-byte ones have n: as many bytes, at most 8 of them.
+template <int W>
+__host__ __device__ constexpr int row_accesses(int n) {
+  return n * (16 / W) < 8 ? n * (16 / W) : (n > 8 ? n : 8);
+}
+
 struct RowsParams {
   const void* x;
   int64_t tokens, cols, ldx;
@@ -212,40 +295,41 @@ struct RowsParams {
   float* scales;  // INT8: [num_rows]
 };
 
-// rows[slot] = x[t] for the k slots of every token, one block per token.  OutT is T, or int8_t for
-// q = rint(x / s) with s = max|x[t]| / 127 in scales[slot].
-template <typename T, typename OutT>
-__global__ void __launch_bounds__(256) rows_kernel(const RowsParams p) {
+// Quantised rows of any alignment: rows[slot] = q and scales[slot] = s of x[t] for the k slots of
+// every token, q = rint(x / s), s = max|x[t]| / 127; one block per token, the row read twice.
+template <typename T>
+__global__ void __launch_bounds__(256) rows_int8_kernel(const RowsParams p) {
+  ptx::griddep_launch_dependents();
   kernel_begins();
-  constexpr bool kQuant = sizeof(OutT) == 1;
   __shared__ uint32_t red[8];
+  const int lane = threadIdx.x & 31;
+  const int32_t cols = static_cast<int32_t>(p.cols);
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-    float s = 1.f;
-    if constexpr (kQuant) {
-      uint32_t m = 0u;
-      for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x)
-        m = max(m, abs_bits(RowVec<T>::load(x + c)));
-      m = __reduce_max_sync(0xffffffffu, m);
-      if ((threadIdx.x & 31u) == 0u) red[threadIdx.x >> 5] = m;
-      __syncthreads();
-      for (int w = 0; w < 8; ++w) m = max(m, red[w]);
-      __syncthreads();
-      s = int8_scale(m);
-    }
-    for (int32_t j = 0; j < p.k; ++j) {
-      const int64_t slot = p.slots != nullptr ? p.slots[t * p.k + j] : t;
-      if (slot < 0 || slot >= p.num_rows) continue;
-      OutT* out = static_cast<OutT*>(p.rows) + slot * p.ldr;
-      for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
-        if constexpr (kQuant) {
-          out[c] = static_cast<OutT>(int8_quotient(RowVec<T>::load(x + c), s));
-        } else {
-          out[c] = x[c];
-        }
+    uint32_t m = 0u;
+#pragma unroll 4
+    for (int32_t c = threadIdx.x; c < cols; c += 256) m = max(m, abs_bits(RowVec<T>::load(x + c)));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) m = max(m, red[w]);
+    __syncthreads();
+    const float s = int8_scale(m);
+    int32_t my_slot = -1;
+    if (lane < p.k) my_slot = p.slots != nullptr ? p.slots[t * p.k + lane] : static_cast<int32_t>(t);
+    if (my_slot >= p.num_rows) my_slot = -1;
+    const int32_t turns = (cols + 255) / 256;  // the same for every lane: the slots are shuffled
+#pragma unroll 2
+    for (int32_t i = 0; i < turns; ++i) {
+      const int32_t c = i * 256 + static_cast<int32_t>(threadIdx.x);
+      int8_t q = 0;
+      if (c < cols) q = static_cast<int8_t>(int8_quotient(RowVec<T>::load(x + c), s));
+      for (int32_t j = 0; j < p.k; ++j) {
+        const int32_t slot = __shfl_sync(0xffffffffu, my_slot, j);
+        if (slot >= 0 && c < cols) static_cast<int8_t*>(p.rows)[slot * p.ldr + c] = q;
       }
-      if (kQuant && threadIdx.x == 0) p.scales[slot] = s;
     }
+    if (threadIdx.x < static_cast<unsigned>(p.k) && my_slot >= 0) p.scales[my_slot] = s;
   }
 }
 
@@ -341,38 +425,38 @@ __global__ void __launch_bounds__(int8_threads<G>(), int8_sm_threads<T, NV>() / 
   }
 }
 
-// Copied rows of whole vectors: a warp takes 32 * kCopyVecs vectors of one token and writes them
-// k times.
+// Copied rows: a warp takes 32 x row_accesses(kCopyVecs) accesses of one token and writes them k times.
 constexpr int kCopyVecs = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(256) rows_copy_vec_kernel(const RowsParams p, int32_t chunks) {
+template <typename T, int W>
+__global__ void __launch_bounds__(256) rows_copy_kernel(const RowsParams p, int32_t chunks) {
   kernel_begins();
-  constexpr int kE = RowVec<T>::kElems;
+  using A = RowAccess<T, W>;
+  constexpr int kN = row_accesses<W>(kCopyVecs);
   const int lane = threadIdx.x & 31;
   const int32_t cols = static_cast<int32_t>(p.cols);
   const int64_t units = p.tokens * chunks;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
   for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < units; u += step) {
     const int64_t t = u / chunks;
-    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kCopyVecs + lane) * kE;
+    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kN + lane) * A::kElems;
     int64_t my_slot = -1;
     if (lane < p.k) my_slot = p.slots[t * p.k + lane];
     const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-    uint4 raw[kCopyVecs];
+    typename A::Data raw[kN];
 #pragma unroll
-    for (int i = 0; i < kCopyVecs; ++i) {
-      const int32_t c = c0 + i * 32 * kE;
-      if (c < cols) raw[i] = ld_row_vec(x, c, cols);
+    for (int i = 0; i < kN; ++i) {
+      const int32_t c = c0 + i * 32 * A::kElems;
+      if (c < cols) raw[i] = A::template load<true>(x, c, cols);
     }
     for (int32_t j = 0; j < p.k; ++j) {
       const int64_t slot = __shfl_sync(0xffffffffu, my_slot, j);
       if (slot < 0 || slot >= p.num_rows) continue;
       T* out = static_cast<T*>(p.rows) + slot * p.ldr;
 #pragma unroll
-      for (int i = 0; i < kCopyVecs; ++i) {
-        const int32_t c = c0 + i * 32 * kE;
-        if (c < cols) st_row_vec(out, c, cols, raw[i]);
+      for (int i = 0; i < kN; ++i) {
+        const int32_t c = c0 + i * 32 * A::kElems;
+        if (c < cols) A::store(out, c, cols, raw[i]);
       }
     }
   }
@@ -391,35 +475,23 @@ struct CombineParams {
   int64_t ldy;
 };
 
-// y[t] = source[t] + sum_j w[t][j] rows[slot[t][j]], summed in fp32 in the order of j.
-template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
-  kernel_begins();
-  for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
-      float acc = p.source != nullptr
-                      ? RowVec<T>::load(static_cast<const T*>(p.source) + t * p.lds + c)
-                      : 0.f;
-      for (int32_t j = 0; j < p.k; ++j) {
-        const int64_t slot = p.slots[t * p.k + j];
-        if (slot < 0 || slot >= p.num_rows) continue;
-        const float w = p.weights != nullptr ? p.weights[t * p.k + j] : 1.f;
-        acc = fmaf(w, RowVec<T>::load(static_cast<const T*>(p.rows) + slot * p.ldr + c), acc);
-      }
-      RowVec<T>::store(static_cast<T*>(p.y) + t * p.ldy + c, acc);
-    }
-  }
+// y[t] = source[t] + sum_j w[t][j] rows[slot[t][j]], summed in fp32 in the order of j.  A warp takes
+// 32 x combine_accesses() accesses of one token and keeps the loads of four choices in flight.
+// Three blocks a SM: without that bound BF16 takes 113 registers, and 16-byte rows of 2048 columns
+// (8192 tokens, 4 choices) 36.4 us for 29.8.  Accesses of one element come four at a time: 69 us with
+// 2049 BF16 columns, 77 with eight; with two elements (2050 columns) eight are the faster, 50 for 58.
+constexpr int kCombineVecs = 2;
+template <typename T, int W>
+__host__ __device__ constexpr int combine_accesses() {
+  return W == static_cast<int>(sizeof(T)) ? 4 : row_accesses<W>(kCombineVecs);
 }
 
-// As combine_kernel for rows of whole vectors: a warp takes 32 * kCombineVecs vectors of one token
-// and keeps the loads of four choices in flight.  Every output element sums its choices in the
-// same order as combine_kernel.
-constexpr int kCombineVecs = 2;
-
-template <typename T>
-__global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p, int32_t chunks) {
+template <typename T, int W>
+__global__ void __launch_bounds__(256, 3) combine_kernel(const CombineParams p, int32_t chunks) {
   kernel_begins();
-  constexpr int kE = RowVec<T>::kElems;
+  using A = RowAccess<T, W>;
+  constexpr int kE = A::kElems;
+  constexpr int kN = combine_accesses<T, W>();
   constexpr int kBatch = 4;
   const int lane = threadIdx.x & 31;
   const int32_t cols = static_cast<int32_t>(p.cols);
@@ -427,7 +499,7 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
   const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
   for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < units; u += step) {
     const int64_t t = u / chunks;
-    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kCombineVecs + lane) * kE;
+    const int32_t c0 = static_cast<int32_t>((u - t * chunks) * 32 * kN + lane) * kE;
     int64_t my_slot = -1;
     float my_w = 1.f;
     if (lane < p.k) {
@@ -435,21 +507,18 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
       if (p.weights != nullptr) my_w = p.weights[t * p.k + lane];
     }
     if (my_slot >= p.num_rows) my_slot = -1;
-    float acc[kCombineVecs][kE];
+    float acc[kN][kE];
 #pragma unroll
-    for (int i = 0; i < kCombineVecs; ++i) {
+    for (int i = 0; i < kN; ++i) {
       const int32_t c = c0 + i * 32 * kE;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (p.source != nullptr && c < cols) {
-        // The source may be y itself, so it is not a read-only load.
-        const T* src = static_cast<const T*>(p.source) + t * p.lds + c;
-        v = c + kE <= cols ? *reinterpret_cast<const uint4*>(src)
-                             : ld_tail_v4(src, cols - c);
-      }
-      RowVec<T>::unpack(v, acc[i]);
+      typename A::Data v = A::zero();
+      // The source may be y itself, so it is not a read-only load.
+      if (p.source != nullptr && c < cols)
+        v = A::template load<false>(static_cast<const T*>(p.source) + t * p.lds, c, cols);
+      A::unpack(v, acc[i]);
     }
     for (int32_t j0 = 0; j0 < p.k; j0 += kBatch) {
-      uint4 raw[kBatch][kCombineVecs];
+      typename A::Data raw[kBatch][kN];
       int64_t slot[kBatch];
       float w[kBatch];
 #pragma unroll
@@ -459,28 +528,34 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
         w[b] = __shfl_sync(0xffffffffu, my_w, (j0 + b) & 31);
         const T* row = static_cast<const T*>(p.rows) + slot[b] * p.ldr;
 #pragma unroll
-        for (int i = 0; i < kCombineVecs; ++i) {
+        for (int i = 0; i < kN; ++i) {
           const int32_t c = c0 + i * 32 * kE;
-          if (slot[b] >= 0 && c < cols) raw[b][i] = ld_row_vec(row, c, cols);
+          if (slot[b] < 0) continue;
+          if constexpr (kE == 1)
+            // Without a branch, a lane past the end loads the last element: the loads go out
+            // together (with it they took 106 us where these take 69).
+            raw[b][i] = A::template load_all<true>(row + min(c, cols - 1));
+          else if (c < cols)
+            raw[b][i] = A::template load<true>(row, c, cols);
         }
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (slot[b] < 0) continue;
 #pragma unroll
-        for (int i = 0; i < kCombineVecs; ++i) {
+        for (int i = 0; i < kN; ++i) {
           float f[kE];
-          RowVec<T>::unpack(raw[b][i], f);
+          A::unpack(raw[b][i], f);
 #pragma unroll
           for (int e = 0; e < kE; ++e) acc[i][e] = fmaf(w[b], f[e], acc[i][e]);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < kCombineVecs; ++i) {
+    for (int i = 0; i < kN; ++i) {
       const int32_t c = c0 + i * 32 * kE;
       if (c < cols)
-        st_row_vec(static_cast<T*>(p.y) + t * p.ldy, c, cols, RowVec<T>::pack(acc[i]));
+        A::store(static_cast<T*>(p.y) + t * p.ldy, c, cols, A::pack(acc[i]));
     }
   }
 }
@@ -498,40 +573,16 @@ struct CombineGradParams {
   float* dweights;
 };
 
-// drows[slot] = w dy[t] and dw[t][j] = <dy[t], rows[slot]>: one warp per (token, choice).
-template <typename T>
+// drows[slot] = w dy[t] and dw[t][j] = <dy[t], rows[slot]>: one warp per (token, choice), with
+// row_accesses(kGradVecs) accesses of dy and of the row in flight per lane.
+constexpr int kGradVecs = 4;
+
+template <typename T, int W>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineGradParams p) {
   kernel_begins();
-  const int lane = threadIdx.x & 31;
-  const int64_t pairs = p.tokens * p.k;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5);
-       i < pairs; i += stride) {
-    const int64_t slot = p.slots[i];
-    float dot = 0.f;
-    if (slot >= 0 && slot < p.num_rows) {
-      const float w = p.weights[i];
-      const T* dy = static_cast<const T*>(p.dy) + (i / p.k) * p.lddy;
-      const T* row = static_cast<const T*>(p.rows) + slot * p.ldr;
-      T* out = static_cast<T*>(p.drows) + slot * p.lddr;
-      for (int64_t c = lane; c < p.cols; c += 32) {
-        const float g = RowVec<T>::load(dy + c);
-        dot = fmaf(g, RowVec<T>::load(row + c), dot);
-        RowVec<T>::store(out + c, w * g);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
-    if (lane == 0) p.dweights[i] = dot;
-  }
-}
-
-// As combine_grad_kernel for rows of whole vectors, four vectors of dy and of the row in flight.
-template <typename T>
-__global__ void __launch_bounds__(256) combine_grad_vec_kernel(const CombineGradParams p) {
-  kernel_begins();
-  constexpr int kE = RowVec<T>::kElems;
-  constexpr int kVecs = 4;
+  using A = RowAccess<T, W>;
+  constexpr int kE = A::kElems;
+  constexpr int kVecs = row_accesses<W>(kGradVecs);
   const int lane = threadIdx.x & 31;
   const int32_t cols = static_cast<int32_t>(p.cols);
   const int64_t pairs = p.tokens * p.k;
@@ -545,28 +596,28 @@ __global__ void __launch_bounds__(256) combine_grad_vec_kernel(const CombineGrad
       const T* row = static_cast<const T*>(p.rows) + slot * p.ldr;
       T* out = static_cast<T*>(p.drows) + slot * p.lddr;
       for (int32_t c0 = lane * kE; c0 < cols; c0 += 32 * kE * kVecs) {
-        uint4 g[kVecs], r[kVecs];
+        typename A::Data g[kVecs], r[kVecs];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
           const int32_t c = c0 + i * 32 * kE;
-          g[i] = r[i] = make_uint4(0u, 0u, 0u, 0u);
+          g[i] = r[i] = A::zero();
           if (c < cols) {
-            g[i] = ld_row_vec(dy, c, cols);
-            r[i] = ld_row_vec(row, c, cols);
+            g[i] = A::template load<true>(dy, c, cols);
+            r[i] = A::template load<true>(row, c, cols);
           }
         }
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
           const int32_t c = c0 + i * 32 * kE;
           float gf[kE], rf[kE];
-          RowVec<T>::unpack(g[i], gf);
-          RowVec<T>::unpack(r[i], rf);
+          A::unpack(g[i], gf);
+          A::unpack(r[i], rf);
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
             dot = fmaf(gf[e], rf[e], dot);
             gf[e] *= w;
           }
-          if (c < cols) st_row_vec(out, c, cols, RowVec<T>::pack(gf));
+          if (c < cols) A::store(out, c, cols, A::pack(gf));
         }
       }
 #pragma unroll
