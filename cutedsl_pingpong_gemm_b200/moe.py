@@ -9,9 +9,11 @@ ABI: cpg_route, cpg_expert_order, cpg_dispatch_rows, cpg_combine_rows and their 
 
 Nothing synchronises with the host: offsets and slots stay on the device.  Every function runs on
 the current stream of its tensors' device and keeps nothing between calls, so calls on several
-streams and captured graphs are independent.  Gradients: ``route_backward``, ``combine_backward``;
-the gradient of ``dispatch`` is ``combine`` of the rows' gradients without weights (a quantised
-dispatch: of the rows it stands for, rounding ignored).  The reference has no such operators.
+streams and captured graphs are independent.  Outputs must not overlap inputs, but for ``combine``'s
+``source``, which may be ``out``.  Rows may have any alignment and stride (and fewer than 2**30
+columns).  Gradients: ``route_backward``, ``combine_backward``; the gradient of ``dispatch`` is
+``combine`` of the rows' gradients without weights (a quantised dispatch: of the rows it stands for,
+rounding ignored).  The reference has no such operators.
 """
 import ctypes
 import functools

@@ -67,7 +67,8 @@ extern "C" {
  * B, i.e. per column of the product ([batches or groups][N], or [..][2N] when gated; the scale of
  * an output channel); an operand without its flag has one value, and a NULL pointer means 1.  Each
  * batch's or group's scales follow the previous one's without a gap.  The sum over k is exact in
- * 32-bit integers (K <= 131071) and is rounded once to fp32 before the scales. */
+ * 32-bit integers (K <= 131071) and is rounded once to fp32 before the scales, which are applied
+ * one after the other in fp32 (each product should stay finite). */
 #define CPG_SCALE_ROWS_A 2
 #define CPG_SCALE_ROWS_B 4
 
@@ -310,8 +311,9 @@ int cpg_quantize_int8(const void* x, int32_t dtype_x, int64_t rows, int64_t cols
  * of cpg_gemm_run_grouped and the row of every (token, choice); cpg_dispatch_rows copies (or
  * quantises) token rows into that order; cpg_combine_rows adds the experts' output rows back.
  * All are stream-ordered, run on the current device, keep no state and never synchronise; ids,
- * weights, slots and their gradients are contiguous [tokens][k].  The reference has no such
- * operators. */
+ * weights, slots and their gradients are contiguous [tokens][k].  Rows may have any alignment (of
+ * their elements) and fewer than 2^30 columns; outputs must not overlap inputs, but for the source
+ * of cpg_combine_rows, which may be y.  The reference has no such operators. */
 #define CPG_ROUTE_MAX_EXPERTS 1024
 #define CPG_ROUTE_MAX_K 32
 #define CPG_ROUTE_MAX_GROUPS 32

@@ -374,6 +374,59 @@ def test_combine(t, k, cols, dtype):
     assert moe_ref.within(y, ref, slack) <= 0
 
 
+@pytest.mark.parametrize("cols", [1, 2, 31, 63, 130, 258, 515, 1029, 2051])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_every_alignment(cols, dtype):
+    """Copies, weighted sums and row gradients are the same bits whatever the rows' alignment (the
+    sums of each element go in the order of the choices); what lies beyond a row stays."""
+    t, k, e = 37, 5, 6
+    g = torch.Generator().manual_seed(cols)
+    ids = ids_of(t, k, e, seed=cols)
+    w = torch.randn(t, k, generator=g).cuda()
+    x0 = torch.randn(t, cols, generator=g).to(dtype)
+    src0 = torch.randn(t, cols, generator=g).to(dtype)
+    results = []
+    for step in (16, 8, 4, 2):  # bytes the rows' addresses are multiples of
+        unit = max(step // x0.element_size(), 1)
+        ld = -(-(cols + 1) // unit) * unit
+        if (ld // unit) % 2 == 0 and unit * x0.element_size() < 16:
+            ld += unit  # and of no more
+
+        def view(rows, fill=7.0):
+            buf = torch.full((rows * ld + unit,), fill, dtype=dtype, device="cuda")
+            v = buf[unit if unit * x0.element_size() < 16 else 0:][:rows * ld].view(rows, ld)
+            return v, v[:, :cols]
+        _, x = view(t)
+        _, src = view(t)
+        x.copy_(x0)
+        src.copy_(src0)
+        rows_all, rows = view(t * k)
+        y_all, y = view(t)
+        dr_all, dr = view(t * k)
+        d = moe.dispatch(x, ids.cuda(), e, out=rows)
+        moe.combine(rows, d.slots, w, source=src, out=y)
+        _, dw = moe.combine_backward(x, rows, d.slots, w, drows=dr)
+        torch.cuda.synchronize()
+        for whole in (rows_all, y_all, dr_all):
+            assert (whole[:, cols:] == 7).all()
+        used = int(d.offsets[-1])
+        assert (rows[used:] == 7).all() and (dr[used:] == 7).all()
+        results.append((rows.clone(), y.clone(), dr.clone(), dw))
+    for got in results[1:]:
+        for a, b in zip(got[:3], results[0][:3]):
+            assert torch.equal(a, b)
+    ref, slack = moe_ref.combine(results[0][0].cpu(), d.slots.cpu(), w.cpu(), source=src0)
+    assert moe_ref.within(results[0][1], ref, slack) <= 0
+    # Each product of a dot product is rounded to at most half a step and so are its cols - 1 sums.
+    rows64 = results[0][0].double().cpu()
+    slot = d.slots.cpu().long()
+    real = (slot >= 0)[..., None]
+    prod = x0.double()[:, None, :] * rows64[slot.clamp(min=0)] * real
+    bound = (cols + 1) * moe_ref.F32_HALF * prod.abs().sum(-1) * 1.01 + 1e-37
+    for got in results:
+        assert ((got[3].cpu().double() - prod.sum(-1)).abs() <= bound).all()
+
+
 def test_combine_infinite_rows():
     """An infinity or NaN in a chosen row reaches its token and no other."""
     t, k, cols = 6, 2, 64

@@ -93,6 +93,15 @@ def test_order_and_row_refusals(lib):
     assert back(tokens=0) == _lib.CPG_OK
 
 
+def test_rows_of_too_many_columns(lib):
+    """Columns are counted in 32 bits: 2^30 and more are refused by every row operator."""
+    S, w = _lib.CPG_ERR_INVALID_SHAPE, 2 ** 30
+    assert lib.cpg_dispatch_rows(P, BF16, 4, w, w, P, 2, P, BF16, 8, w, None, None) == S
+    assert lib.cpg_combine_rows(P, F32, 8, w, w, P, P, 4, 2, None, 0, P, w, None) == S
+    assert lib.cpg_combine_rows_backward(P, F32, 4, w, w, P, 8, w, P, P, 2, P, w, P, None) == S
+    assert lib.cpg_quantize_int8(P, F32, 4, w, w, P, w, P, None) == S
+
+
 def test_quantize_refusals(lib):
     def quant(x=P, dt=F32, rows=4, cols=8, ldx=8, q=P, ldq=8, s=P):
         return lib.cpg_quantize_int8(x, dt, rows, cols, ldx, q, ldq, s, None)
