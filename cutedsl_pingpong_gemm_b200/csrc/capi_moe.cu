@@ -118,15 +118,15 @@ int by_width(int32_t dtype, int width, F&& f) {
   return f(float{}, integral_constant<int, 4>{});
 }
 
-template <typename T, int G, int NV, bool Resident>
+template <typename T, int W, int G, int NV, bool Resident>
 int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
   constexpr int kThreads = cpg::int8_threads<G>();
   constexpr int kRows = kThreads / G;
-  return launch("INT8 row kernel", false, &cpg::rows_int8_vec_kernel<T, G, NV, Resident>,
+  return launch("INT8 row kernel", false, &cpg::rows_int8_vec_kernel<T, W, G, NV, Resident>,
                 row_grid((p.tokens + kRows - 1) / kRows), kThreads, 0, st, 1, p);
 }
 
-template <typename T>
+template <typename T, int W>
 int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
   // The fewest threads that hold a row (16384 x 4096 BF16: 128 threads 49 us, 256 61 us); more while
   // the tokens leave most of the GPU idle (each then has less of a row to wait for).
@@ -134,17 +134,17 @@ int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
   // conversions bound it: three packed FMAs per two elements after 22 issue slots an element before.
   constexpr int kVecs = cpg::kInt8Vecs;
   constexpr int64_t kEach = kVecs * 16;
-  if (p.cols > 2 * 512 * kEach) return launch_int8_vec<T, 512, kVecs, false>(p, st);
-  if (p.cols > 512 * kEach) return launch_int8_vec<T, 512, 2 * kVecs, true>(p, st);
+  if (p.cols > 2 * 512 * kEach) return launch_int8_vec<T, W, 512, kVecs, false>(p, st);
+  if (p.cols > 512 * kEach) return launch_int8_vec<T, W, 512, 2 * kVecs, true>(p, st);
   int64_t threads = 32;
   while (p.cols > threads * kEach) threads *= 2;
   while (threads < 256 && p.tokens * threads < kFewThreads && p.cols > threads * 16) threads *= 2;
   switch (threads) {
-    case 32: return launch_int8_vec<T, 32, kVecs, true>(p, st);
-    case 64: return launch_int8_vec<T, 64, kVecs, true>(p, st);
-    case 128: return launch_int8_vec<T, 128, kVecs, true>(p, st);
-    case 256: return launch_int8_vec<T, 256, kVecs, true>(p, st);
-    default: return launch_int8_vec<T, 512, kVecs, true>(p, st);
+    case 32: return launch_int8_vec<T, W, 32, kVecs, true>(p, st);
+    case 64: return launch_int8_vec<T, W, 64, kVecs, true>(p, st);
+    case 128: return launch_int8_vec<T, W, 128, kVecs, true>(p, st);
+    case 256: return launch_int8_vec<T, W, 256, kVecs, true>(p, st);
+    default: return launch_int8_vec<T, W, 512, kVecs, true>(p, st);
   }
 }
 
@@ -156,10 +156,17 @@ int32_t row_chunks(int64_t cols, int n) {
 }
 unsigned warp_grid(int64_t warps) { return row_grid((warps + 7) / 8); }
 
+// Rows of INT8 that start on 16 bytes (as the GEMM wants them) whatever the alignment of x; others
+// one element at a time.  16384 rows in us, by accesses of 16 / 8 / 4 / 2 bytes (4096, 4100, 4098 and
+// 4097 columns) and [by elements]: BF16 52 / 64 / 67 / 89 [150]; FP32 57 / 89 / 144 by 16, 8 (4098)
+// and 4 (4097) bytes [150].
 int launch_int8(const cpg::RowsParams& p, int32_t dtype_x, cudaStream_t st) {
-  if (vector_rows(p.x, p.ldx, bytes_of(dtype_x)) && vector_rows(p.rows, p.ldr, 1))
-    return dtype_x == CPG_DTYPE_BF16 ? launch_int8_vec<__nv_bfloat16>(p, st)
-                                     : launch_int8_vec<float>(p, st);
+  if (vector_rows(p.rows, p.ldr, 1)) {
+    const int width = row_width({{p.x, p.ldx}}, bytes_of(dtype_x));
+    return by_width(dtype_x, width, [&](auto type, auto w) {
+      return launch_int8_vec<decltype(type), decltype(w)::value>(p, st);
+    });
+  }
   auto fn = dtype_x == CPG_DTYPE_BF16 ? &cpg::rows_int8_kernel<__nv_bfloat16>
                                       : &cpg::rows_int8_kernel<float>;
   return launch("INT8 row kernel", false, fn, row_grid(p.tokens), 256, 0, st, 1, p);

@@ -295,7 +295,7 @@ struct RowsParams {
   float* scales;  // INT8: [num_rows]
 };
 
-// Quantised rows of any alignment: rows[slot] = q and scales[slot] = s of x[t] for the k slots of
+// Quantised rows whose INT8 rows do not start on 16 bytes: rows[slot] = q and scales[slot] = s of x[t] for the k slots of
 // every token, q = rint(x / s), s = max|x[t]| / 127; one block per token, the row read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) rows_int8_kernel(const RowsParams p) {
@@ -333,7 +333,51 @@ __global__ void __launch_bounds__(256) rows_int8_kernel(const RowsParams p) {
   }
 }
 
-// Quantised rows of whole vectors: G threads per token hold the row packed in registers, NV times 16
+// 16 elements of a row from c on as vectors, zeros past its end, read by accesses of W bytes.
+// Narrow ones go out without a branch between them; lanes share their sectors through L1.
+template <typename T, int W>
+__device__ __forceinline__ void ld_16(const T* x, int32_t c, int32_t cols,
+                                      uint4 (&raw)[16 / RowVec<T>::kElems]) {
+  constexpr int kE = RowVec<T>::kElems;
+  constexpr int kVecs = 16 / kE;
+  if constexpr (W == 16) {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      raw[v] = make_uint4(0u, 0u, 0u, 0u);
+      if (c + v * kE < cols) raw[v] = ld_row_vec(x, c + v * kE, cols);
+    }
+  } else {
+    using A = RowAccess<T, W>;
+    constexpr int kN = 16 / A::kElems;
+    uint32_t w[4 * kVecs];
+#pragma unroll
+    for (int i = 0; i < 4 * kVecs; ++i) w[i] = 0u;
+    auto place = [&](int a, const typename A::Data& d) {
+      if constexpr (W == 2) {
+        w[a >> 1] |= d.w[0] << (16 * (a & 1));
+      } else {
+#pragma unroll
+        for (int i = 0; i < A::kWords; ++i) w[a * A::kWords + i] = d.w[i];
+      }
+    };
+    if (c + 16 <= cols) {
+      typename A::Data d[kN];
+#pragma unroll
+      for (int a = 0; a < kN; ++a) d[a] = A::template load_all<true>(x + c + a * A::kElems);
+#pragma unroll
+      for (int a = 0; a < kN; ++a) place(a, d[a]);
+    } else if (c < cols) {
+#pragma unroll
+      for (int a = 0; a < kN; ++a)
+        if (c + a * A::kElems < cols) place(a, A::template load<true>(x, c + a * A::kElems, cols));
+    }
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      raw[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+  }
+}
+
+// Quantised rows stored by whole vectors: G threads per token hold the row packed in registers, NV times 16
 // elements each, between its maximum and the quantisation, so the row is read once however many
 // copies of it are written.  Longer rows (Resident false) are read a second time, from L2.
 constexpr int kInt8Vecs = 2;
@@ -348,14 +392,13 @@ __host__ __device__ constexpr int int8_sm_threads() {
   return NV == kInt8Vecs ? (sizeof(T) == 2 ? 1536 : 1024) : (sizeof(T) == 2 ? 1024 : 512);
 }
 
-template <typename T, int G, int NV, bool Resident>
+template <typename T, int W, int G, int NV, bool Resident>
 __global__ void __launch_bounds__(int8_threads<G>(), int8_sm_threads<T, NV>() / int8_threads<G>())
     rows_int8_vec_kernel(const RowsParams p) {
   // The small-M product that reads these rows may be set up, and fetch its first weights, already.
   ptx::griddep_launch_dependents();
   kernel_begins();
   constexpr int kVecs = 16 / RowVec<T>::kElems;
-  constexpr int kE = RowVec<T>::kElems;
   constexpr int kRowsPerBlock = int8_threads<G>() / G;
   constexpr int kPass = G * NV * 16;  // elements per pass over a row
   __shared__ uint32_t red[2][int8_threads<G>() / 32];
@@ -371,12 +414,7 @@ __global__ void __launch_bounds__(int8_threads<G>(), int8_sm_threads<T, NV>() / 
     auto load = [&](int32_t c0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int32_t c = c0 + (i * G + li) * 16;
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-          raw[i][v] = make_uint4(0u, 0u, 0u, 0u);
-          if (c + v * kE < cols) raw[i][v] = ld_row_vec(x, c + v * kE, cols);
-        }
+        ld_16<T, W>(x, c0 + (i * G + li) * 16, cols, raw[i]);
       }
     };
     uint32_t m = 0u;
