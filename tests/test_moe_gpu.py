@@ -427,6 +427,38 @@ def test_rows_of_every_alignment(cols, dtype):
         assert ((got[3].cpu().double() - prod.sum(-1)).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("cols", [4096, 4097])
+def test_rows_past_32_bit_offsets(cols):
+    """Rows whose element offsets pass 2^31: token t goes to expert 7 - t % 8 with every choice, so
+    the last rows are those of expert 7."""
+    t, k, e = 66000, 8, 8
+    assert t * k * cols > 2 ** 31
+    tok = torch.arange(t, device="cuda")
+    ids = ((7 - tok % 8)[:, None] + torch.zeros(k, dtype=torch.int64, device="cuda")).int()
+    x = (tok % 251 - 125).to(torch.bfloat16)[:, None].expand(t, cols).contiguous()
+    w = torch.full((t, k), 0.5, device="cuda")
+    d = moe.dispatch(x, ids, e)
+    q = moe.dispatch(x, ids, e, quantize="int8")
+    torch.cuda.synchronize()
+    assert torch.equal(q.slots, d.slots)
+    of_row = torch.empty(t * k, dtype=torch.int64, device="cuda")
+    of_row[d.slots.long().flatten()] = tok.repeat_interleave(k)
+    for lo in range(0, t * k, 66000):
+        want = x[of_row[lo:lo + 66000], :1]
+        assert (d.rows[lo:lo + 66000] == want).all()
+        assert (q.rows[lo:lo + 66000] == (127 * want.sign()).to(torch.int8)).all()
+    del q
+    # 8 halves of a whole number below 2^7: exact.
+    assert torch.equal(moe.combine(d.rows, d.slots, w), 4 * x)
+    drows, dw = moe.combine_backward(x, d.rows, d.slots, w, drows=d.rows.clone())
+    torch.cuda.synchronize()
+    for lo in range(0, t * k, 66000):
+        assert (drows[lo:lo + 66000] == 0.5 * x[of_row[lo:lo + 66000], :1]).all()
+    # cols squares below 2^14: their sums are whole numbers below 2^27, rounded where above 2^24.
+    want = cols * x[:, 0].double() ** 2
+    assert ((dw.double() - want[:, None]).abs() <= cols * moe_ref.F32_HALF * want[:, None]).all()
+
+
 def test_combine_infinite_rows():
     """An infinity or NaN in a chosen row reaches its token and no other."""
     t, k, cols = 6, 2, 64
