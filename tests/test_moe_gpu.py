@@ -281,6 +281,47 @@ def test_dispatch_order(t, k, e):
     assert torch.equal(d.rows.cpu()[slots[here].long()], x.cpu()[token])
 
 
+def expected_order(ids, e):
+    """Offsets and slots by a stable sort of the pairs by expert."""
+    flat = ids.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < e), flat, torch.full_like(flat, e))
+    order = key.argsort(stable=True)
+    off = torch.zeros(e + 1, dtype=torch.int64)
+    off[1:] = torch.bincount(key, minlength=e + 1)[:e].cumsum(0)
+    slots = torch.full_like(flat, -1)
+    used = int(off[-1])
+    slots[order[:used]] = torch.arange(used)
+    return off.int(), slots.reshape(ids.shape).int()
+
+
+# A cluster of 16 blocks (8 where 16 do not fit) holds 512 pairs of each of its warps; with more
+# every warp walks its run twice.
+@pytest.mark.parametrize("pairs", [131071, 131073, 262143, 262144, 262145, 300000, 1000003])
+@pytest.mark.parametrize("e", [3, 16, 17, 64, 65, 256, 257, 1024])
+def test_dispatch_order_of_many_pairs(pairs, e):
+    ids = ids_of(pairs, 1, e, seed=pairs + e)
+    ids[100] = e  # no expert
+    ids[5000:5040] = ids[5000]
+    ids[pairs // 2:pairs // 2 + 3000] = -1
+    x = torch.zeros(pairs, 1, device="cuda")
+    d = moe.dispatch(x, ids.cuda(), e)
+    torch.cuda.synchronize()
+    off, slots = expected_order(ids, e)
+    assert torch.equal(d.offsets.cpu(), off) and torch.equal(d.slots.cpu(), slots)
+
+
+def test_dispatch_order_of_equal_choices():
+    """528000 pairs: token t goes to expert 7 - t % 8 with each of its 8 choices."""
+    t, k, e = 66000, 8, 8
+    tok = torch.arange(t)
+    d = moe.dispatch(torch.zeros(t, 1, device="cuda"),
+                     (7 - tok % 8)[:, None].expand(t, k).int().contiguous().cuda(), e)
+    torch.cuda.synchronize()
+    assert torch.equal(d.offsets.cpu(), torch.arange(e + 1, dtype=torch.int32) * (t * k // e))
+    first = (7 - tok % 8) * (t * k // e) + tok // 8 * k
+    assert torch.equal(d.slots.cpu(), (first[:, None] + torch.arange(k)).int())
+
+
 @pytest.mark.parametrize("cols", [1, 7, 64, 100, 1032, 4096, 5000, 16392, 40000])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("int8", [False, True])
