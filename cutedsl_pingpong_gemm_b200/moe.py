@@ -174,10 +174,10 @@ def combine(rows, slots, weights=None, *, source=None, out=None):
 
 
 def combine_backward(dy, rows, slots, weights, *, drows=None, dweights=None):
-    """Gradients of ``combine``: ``drows[slots[t, j]] = weights[t, j] * dy[t]`` [R, D] (rows that
-    no slot names are left as they were) and ``dweights[t, j] = <dy[t], rows[slots[t, j]]>`` FP32
-    [T, k].  No two slots may be the same row (``dispatch`` makes none).  ``drows`` / ``dweights``
-    may be given as outputs."""
+    """Gradients of ``combine``: ``drows[slots[t, j]] = weights[t, j] * dy[t]`` [R, D], 0 in the rows
+    that no slot names, and ``dweights[t, j] = <dy[t], rows[slots[t, j]]>`` FP32 [T, k].  No two
+    slots may be the same row (``dispatch`` makes none).  ``drows`` / ``dweights`` may be given as
+    outputs; rows of a given ``drows`` that no slot names are left as they were."""
     t, d, lddy = matrix("dy", dy)
     code = float_code("dy", dy)
     dev = dy.device
@@ -190,7 +190,8 @@ def combine_backward(dy, rows, slots, weights, *, drows=None, dweights=None):
     vector("slots", slots, (t, k), torch.int32, dev)
     vector("weights", weights, (t, k), torch.float32, dev)
     if drows is None:
-        drows = torch.empty((r, d), dtype=dy.dtype, device=dev)
+        # Cleared whole: which rows the slots name is known on the device only.
+        drows = torch.zeros((r, d), dtype=dy.dtype, device=dev)
     if dweights is None:
         dweights = torch.empty((t, k), dtype=torch.float32, device=dev)
     else:

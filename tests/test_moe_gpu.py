@@ -534,6 +534,33 @@ def test_combine_backward(t, k, cols, dtype):
     assert ((dw.cpu().double() - rw).abs() <= slack + 1e-37).all()
 
 
+@pytest.mark.parametrize("cols", [1, 64, 1031])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine_backward_of_unused_rows(cols, dtype):
+    """A row that enters no sum has the gradient 0 where the function makes the tensor, whatever its
+    memory held before."""
+    t, k, e = 40, 4, 6
+    ids = ids_of(t, k, e, seed=cols, skip=0.4)
+    ids[-3:] = -1
+    _, slots = moe_ref.expert_order(ids, e)
+    slots[0, 0] = t * k  # no row
+    g = torch.Generator().manual_seed(cols)
+    rows = torch.randn(t * k, cols, generator=g).to(dtype)
+    dy = torch.randn(t, cols, generator=g).to(dtype)
+    w = torch.rand(t, k, generator=g)
+    args = dy.cuda(), rows.cuda(), slots.cuda(), w.cuda()
+    stale = torch.full((t * k, cols), math.nan, dtype=dtype, device="cuda")
+    del stale  # the allocator hands out its memory again
+    drows, _ = moe.combine_backward(*args)
+    torch.cuda.synchronize()
+    ref, _, _ = moe_ref.combine_backward(dy, rows, slots, w)
+    unused = torch.isnan(ref).all(1)
+    assert unused.sum() > 10
+    assert (drows.cpu()[unused] == 0).all()
+    ref = ref.masked_fill(unused[:, None], 0.0)
+    assert moe_ref.within(drows, ref, moe_ref.F32_HALF * ref.abs()) <= 0
+
+
 def test_gradients_against_differences():
     """combine's gradients and dispatch's (a combine without weights) against central differences;
     both are linear, so with h = 1 the difference is exact up to fp32 rounding."""
