@@ -69,6 +69,9 @@ def pairs(name, t):
     size = t.shape
     if len(size) != 2:
         raise error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} must be [T, k], got {tuple(size)}")
+    if size[1] > _lib.CPG_ROUTE_MAX_K:  # here: ctypes would wrap a k past 32 bits
+        raise error(_lib.CPG_ERR_INVALID_SHAPE,
+                    f"{name}: at most {_lib.CPG_ROUTE_MAX_K} choices, got {size[1]}")
     return size
 
 

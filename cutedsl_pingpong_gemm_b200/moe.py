@@ -35,7 +35,8 @@ def _route_config(experts, k, scoring, groups, kept_groups, group_score, renorma
         raise error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown scoring {scoring!r}")
     if group_score not in _lib.ROUTE_GROUP_SCORES:
         raise error(_lib.CPG_ERR_INVALID_CONFIG, f"unknown group_score {group_score!r}")
-    for name, v in (("k", k), ("groups", groups), ("kept_groups", kept_groups)):
+    for name, v in (("experts", experts), ("k", k), ("groups", groups),
+                    ("kept_groups", kept_groups)):
         if abs(v) >= 1 << 31:  # ctypes would wrap it
             raise error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} = {v}")
     return ctypes.byref(_lib.RouteConfigC(

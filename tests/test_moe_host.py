@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from cutedsl_pingpong_gemm_b200 import _lib
+from cutedsl_pingpong_gemm_b200 import _lib, _tensors, moe
 from oracle import moe_ref
 
 F32, BF16, I8, E4M3 = (_lib.CPG_DTYPE_F32, _lib.CPG_DTYPE_BF16, _lib.CPG_DTYPE_I8,
@@ -100,6 +100,20 @@ def test_rows_of_too_many_columns(lib):
     assert lib.cpg_combine_rows(P, F32, 8, w, w, P, P, 4, 2, None, 0, P, w, None) == S
     assert lib.cpg_combine_rows_backward(P, F32, 4, w, w, P, 8, w, P, P, 2, P, w, P, None) == S
     assert lib.cpg_quantize_int8(P, F32, 4, w, w, P, w, P, None) == S
+
+
+def test_counts_that_32_bits_would_wrap():
+    """More experts or choices than the C entry points' 32-bit counts hold are refused before they
+    could be cut to another, valid number."""
+    for experts in (2 ** 32 + 8, 2 ** 31, 2 ** 33 + 4):
+        with pytest.raises(_lib.CpgError) as e:
+            moe._route_config(experts, 2, "softmax", 1, 1, "max", True, 1.0)
+        assert e.value.code == _lib.CPG_ERR_INVALID_SHAPE
+    for k in (2 ** 32 + 2, 2 ** 31, 33):
+        with pytest.raises(_lib.CpgError) as e:
+            _tensors.pairs("ids", torch.empty(0, k, dtype=torch.int32))
+        assert e.value.code == _lib.CPG_ERR_INVALID_SHAPE
+    assert tuple(_tensors.pairs("ids", torch.empty(3, 32, dtype=torch.int32))) == (3, 32)
 
 
 def test_quantize_refusals(lib):
