@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from ._tensors import call, error, float_code, matrix, output, pairs, ptr, vector
-from .quant import alloc_int8_rows
+from .quant import alloc_operand_rows
 
 Dispatched = namedtuple("Dispatched", "rows offsets slots scales")
 
@@ -110,9 +110,10 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
     Returns ``Dispatched(rows, offsets, slots, scales)``: ``rows`` [T * k, D] holds the rows of
     expert e at ``offsets[e] <= r < offsets[e + 1]`` (int32 [experts + 1]) in token order, ``slots``
     int32 [T, k] the row of every (token, choice), -1 if skipped.  Rows from ``offsets[experts]``
-    on are not written.  ``quantize="int8"`` makes ``rows`` the int8 rows and ``scales`` (FP32
-    [T * k]) the scales of ``quant.quantize_int8``; otherwise ``scales`` is None.  ``out`` /
-    ``scales`` may be given as outputs.  experts <= 1024, k <= 32."""
+    on are not written (undefined without a given ``out``).  BF16 and INT8 rows that it allocates
+    are padded to 16 bytes, as the product needs.  ``quantize="int8"`` makes ``rows`` the int8 rows
+    and ``scales`` (FP32 [T * k]) the scales of ``quant.quantize_int8``; otherwise ``scales`` is
+    None.  ``out`` / ``scales`` may be given as outputs.  experts <= 1024, k <= 32."""
     t, d, ldx = matrix("x", x)
     code = float_code("x", x)
     dev = x.device
@@ -125,10 +126,12 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
         raise error(_lib.CPG_ERR_INVALID_SHAPE,
                      f"1 <= experts <= {_lib.CPG_ROUTE_MAX_EXPERTS}, got {experts}")
     int8 = quantize == "int8"
+    dtype = torch.int8 if int8 else x.dtype
     if out is None:
-        out = (alloc_int8_rows(t * k, d, dev) if int8
-               else torch.empty((t * k, d), dtype=x.dtype, device=dev))
-    ldr = output("out", out, (t * k, d), torch.int8 if int8 else x.dtype, dev)
+        # FP32 rows are no operand of a product: without padding.
+        out = (torch.empty((t * k, d), dtype=dtype, device=dev) if dtype == torch.float32
+               else alloc_operand_rows(t * k, d, dtype, dev))
+    ldr = output("out", out, (t * k, d), dtype, dev)
     if int8:
         if scales is None:
             scales = torch.empty(t * k, dtype=torch.float32, device=dev)

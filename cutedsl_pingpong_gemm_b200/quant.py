@@ -46,11 +46,12 @@ def quantize_e4m3(x, block: Optional[Tuple[int, int]] = None):
     return q, scales
 
 
-def alloc_int8_rows(rows: int, cols: int, device):
-    """int8 [rows, cols] whose rows start on 16 bytes, as the GEMM's loads need."""
-    if cols % 16 == 0:
-        return torch.empty((rows, cols), dtype=torch.int8, device=device)
-    return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
+def alloc_operand_rows(rows: int, cols: int, dtype, device):
+    """[rows, cols] whose rows start on 16 bytes, as the GEMM's loads need."""
+    per16 = 16 // dtype.itemsize
+    if cols % per16 == 0:
+        return torch.empty((rows, cols), dtype=dtype, device=device)
+    return torch.empty((rows, -(-cols // per16) * per16), dtype=dtype, device=device)[:, :cols]
 
 
 def quantize_int8(x, out=None, scales=None):
@@ -62,7 +63,7 @@ def quantize_int8(x, out=None, scales=None):
     rows, cols, ldx = matrix("x", x)
     device = x.device
     if out is None:
-        out = alloc_int8_rows(rows, cols, device)
+        out = alloc_operand_rows(rows, cols, torch.int8, device)
         ldq = out.stride(0) if rows > 1 else cols
     else:
         ldq = output("out", out, (rows, cols), torch.int8, device)

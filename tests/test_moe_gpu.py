@@ -381,6 +381,41 @@ def test_dispatch_combine_strided_views(shift, extra, int8, dtype):
     assert (ybuf[:, 0] == 5).all() and (ybuf[:, 1 + cols:] == 5).all()
 
 
+@pytest.mark.parametrize("d", [8, 100, 129])
+@pytest.mark.parametrize("t", [1, 50])
+def test_dispatched_rows_are_operands(d, t):
+    """The rows that dispatch allocates go into the grouped product at every width, BF16 and INT8."""
+    e, k, n = 4, 2, 72
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(t, d, generator=g).bfloat16()
+    ids = ids_of(t, k, e, seed=d, skip=0.0)
+    per = -(-d // 8) * 8
+    b = torch.zeros(e, n, per, dtype=torch.bfloat16)
+    b[..., :d] = (torch.randn(e, n, d, generator=g) * d ** -0.5).bfloat16()
+    gemm = GemmSM90(tile_shape_mn=(128, 128), epi_tile_mn=(128, 32), cluster_shape_mnk=(1, 1, 1),
+                    atom_layout_mn=(1, 1), ab_stage=3, reuse_ab=False, is_persistent=True)
+    p = moe.dispatch(x.cuda(), ids.cuda(), e)
+    y = torch.zeros(t * k, n, dtype=torch.bfloat16, device="cuda")
+    gemm.grouped(p.rows, b.cuda()[..., :d], y, p.offsets)
+    torch.cuda.synchronize()
+    off, slots = moe_ref.expert_order(ids, e)
+    for i in range(t):
+        for j in range(k):
+            ref = x[i].double() @ b[ids[i, j], :, :d].double().t()
+            mag = x[i].double().abs() @ b[ids[i, j], :, :d].double().abs().t()
+            # d products exact in fp32, at most d sums of it, one rounding to BF16.
+            slack = d * moe_ref.F32_HALF * 2 * mag
+            assert moe_ref.within(y[slots[i, j]], ref, slack) <= 0
+    q = moe.dispatch(x.cuda(), ids.cuda(), e, quantize="int8")
+    bq = torch.randint(-127, 128, (e, n, -(-d // 16) * 16), generator=g, dtype=torch.int8)
+    gemm.grouped(q.rows, bq.cuda()[..., :d], y, q.offsets, scale_a=q.scales)
+    torch.cuda.synchronize()
+    for i in range(e):
+        r = slice(int(off[i]), int(off[i + 1]))
+        ref, slack = moe_ref.int8_product(q.rows[r].cpu(), bq[i, :, :d], q.scales[r].cpu())
+        assert moe_ref.within(y[r], ref, slack) <= 0
+
+
 # ----------------------------------------------------------------------------------- combine
 COMBINE = [(1, 1, 1), (1, 8, 4096), (16, 2, 4096), (37, 5, 100), (64, 32, 24), (300, 8, 1032),
            (9, 3, 16385), (0, 2, 64)]
