@@ -103,7 +103,8 @@ def route_backward(dweights, logits, ids, *, scoring: str = "softmax", renormali
     return out
 
 
-def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, scales=None):
+def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, scales=None,
+             offsets=None, slots=None):
     """Rows of ``x`` [T, D] (BF16 or FP32) in expert order, for ``GemmSM90.grouped``.
 
     ``ids`` int32 [T, k] gives each token's experts (entries outside [0, experts) are skipped).
@@ -113,7 +114,8 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
     on are not written (undefined without a given ``out``).  BF16 and INT8 rows that it allocates
     are padded to 16 bytes, as the product needs.  ``quantize="int8"`` makes ``rows`` the int8 rows
     and ``scales`` (FP32 [T * k]) the scales of ``quant.quantize_int8``; otherwise ``scales`` is
-    None.  ``out`` / ``scales`` may be given as outputs.  experts <= 1024, k <= 32."""
+    None.  ``out`` / ``scales`` / ``offsets`` / ``slots`` may be given as outputs.  experts <= 1024,
+    k <= 32."""
     t, d, ldx = matrix("x", x)
     code = float_code("x", x)
     dev = x.device
@@ -139,8 +141,14 @@ def dispatch(x, ids, experts: int, *, quantize: Optional[str] = None, out=None, 
             vector("scales", scales, (t * k,), torch.float32, dev)
     elif scales is not None:
         raise error(_lib.CPG_ERR_UNSUPPORTED, "scales only with quantize='int8'")
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
-    slots = torch.empty((t, k), dtype=torch.int32, device=dev)
+    if offsets is None:
+        offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    else:
+        vector("offsets", offsets, (experts + 1,), torch.int32, dev)
+    if slots is None:
+        slots = torch.empty((t, k), dtype=torch.int32, device=dev)
+    else:
+        vector("slots", slots, (t, k), torch.int32, dev)
     slots_ptr = ptr(slots)
     lib = _lib.load()
     call(lib.cpg_expert_order, "dispatch", dev, ptr(ids), t, k, experts, offsets.data_ptr(),

@@ -416,6 +416,37 @@ def test_dispatched_rows_are_operands(d, t):
         assert moe_ref.within(y[r], ref, slack) <= 0
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_dispatch_into_given_outputs(int8):
+    """With every output given, dispatch allocates nothing and returns them."""
+    t, k, e, d = 30, 3, 8, 64
+    ids = ids_of(t, k, e, seed=2)
+    x = torch.randn(t, d, device="cuda").bfloat16()
+    out = torch.zeros(t * k, d, dtype=torch.int8 if int8 else x.dtype, device="cuda")
+    scales = torch.zeros(t * k, device="cuda") if int8 else None
+    offsets = torch.full((e + 1,), -7, dtype=torch.int32, device="cuda")
+    slots = torch.full((t, k), -7, dtype=torch.int32, device="cuda")
+    on = ids.cuda()
+    kw = dict(quantize="int8" if int8 else None, out=out, scales=scales, offsets=offsets,
+              slots=slots)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    p = moe.dispatch(x, on, e, **kw)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+    torch.cuda.synchronize()
+    assert p.rows is out and p.offsets is offsets and p.slots is slots and p.scales is scales
+    off, want = moe_ref.expert_order(ids, e)
+    assert torch.equal(offsets.cpu(), off) and torch.equal(slots.cpu(), want)
+    again = moe.dispatch(x, on, e, quantize=kw["quantize"])
+    used = int(off[-1])
+    assert torch.equal(again.rows[:used], out[:used])
+    for bad in (dict(offsets=offsets[:-1]), dict(offsets=offsets.long()), dict(slots=slots[:-1]),
+                dict(slots=slots.t()), dict(slots=slots.cpu()), dict(offsets=offsets.cpu())):
+        with pytest.raises(CpgError) as err:
+            moe.dispatch(x, on, e, **bad)
+        assert err.value.code == _lib.CPG_ERR_INVALID_SHAPE
+
+
 # ----------------------------------------------------------------------------------- combine
 COMBINE = [(1, 1, 1), (1, 8, 4096), (16, 2, 4096), (37, 5, 100), (64, 32, 24), (300, 8, 1032),
            (9, 3, 16385), (0, 2, 64)]
