@@ -83,23 +83,29 @@ int launch(const char* what, bool early, void (*kernel)(P...), unsigned grid, un
   return e == cudaSuccess ? CPG_OK : cuda_fail(e, what);
 }
 
-// Rows that start on 16 bytes.
-bool vector_rows(const void* p, int64_t ld, int elem) {
-  return !misaligned(p, 16) && (ld * elem) % 16 == 0;
+// A matrix whose rows' alignment selects a kernel.  The stride of a single row is not used.
+struct Rows {
+  const void* p;
+  int64_t ld, rows;
+};
+// Address bits that some row has set (of the lowest ones).
+uint64_t address_bits(const Rows& r, int elem) {
+  return reinterpret_cast<uintptr_t>(r.p) |
+         (r.rows > 1 ? static_cast<uint64_t>(r.ld * elem) : uint64_t(0));
+}
+
+// Rows that start on `bytes` (a power of two).
+bool rows_start_on(const Rows& r, int elem, int bytes) {
+  return (address_bits(r, elem) & static_cast<uint64_t>(bytes - 1)) == 0;
 }
 
 // The widest access (16, 8, 4 or 2 bytes) that every row of these matrices starts on.
 // 8192 tokens x 4 choices, BF16, in us with accesses of 16 / 8 / 4 / 2 bytes (2048, 2052, 2050 and
 // 2049 columns) and, in brackets, of the kernels of one element an access that these replaced:
 // copy 36 / 39 / 41 / 41 [79], combine 30 / 41 / 50 / 67 [82], its gradient 50 / 57 / 61 / 81 [116].
-struct Rows {
-  const void* p;
-  int64_t ld;
-};
 int row_width(std::initializer_list<Rows> all, int elem) {
   uint64_t bits = 16;
-  for (const Rows& r : all)
-    bits |= reinterpret_cast<uintptr_t>(r.p) | static_cast<uint64_t>(r.ld * elem);
+  for (const Rows& r : all) bits |= address_bits(r, elem);
   return static_cast<int>(bits & (~bits + 1));
 }
 
@@ -161,8 +167,8 @@ unsigned warp_grid(int64_t warps) { return row_grid((warps + 7) / 8); }
 // 4097 columns) and [by elements]: BF16 52 / 64 / 67 / 89 [150]; FP32 57 / 89 / 144 by 16, 8 (4098)
 // and 4 (4097) bytes [150].
 int launch_int8(const cpg::RowsParams& p, int32_t dtype_x, cudaStream_t st) {
-  if (vector_rows(p.rows, p.ldr, 1)) {
-    const int width = row_width({{p.x, p.ldx}}, bytes_of(dtype_x));
+  if (rows_start_on({p.rows, p.ldr, p.num_rows}, 1, 16)) {
+    const int width = row_width({{p.x, p.ldx, p.tokens}}, bytes_of(dtype_x));
     return by_width(dtype_x, width, [&](auto type, auto w) {
       return launch_int8_vec<decltype(type), decltype(w)::value>(p, st);
     });
@@ -237,17 +243,16 @@ int check_route(const cpg_route_config* c, int64_t tokens) {
 
 // Whether every lane's run of V elements of every row starts on its vectors.
 template <int V>
-int32_t run_vectors(const void* p, int64_t ld, int32_t dtype) {
-  const int es = bytes_of(dtype);
+int32_t run_vectors(const Rows& r, int32_t dtype) {
   const int bytes = dtype == CPG_DTYPE_BF16 ? cpg::run_vector_bytes<__nv_bfloat16, V>()
                                             : cpg::run_vector_bytes<float, V>();
-  return !misaligned(p, bytes) && (ld * es) % bytes == 0 ? 1 : 0;
+  return rows_start_on(r, bytes_of(dtype), bytes) ? 1 : 0;
 }
 
 template <int L, int V>
 int launch_route(cpg::RouteParams p, int32_t dtype, cudaStream_t st) {
-  p.vec = run_vectors<V>(p.logits, p.ld, dtype);
-  p.vec_bias = run_vectors<V>(p.bias, 0, CPG_DTYPE_F32);
+  p.vec = run_vectors<V>({p.logits, p.ld, p.tokens}, dtype);
+  p.vec_bias = run_vectors<V>({p.bias, 0, 1}, CPG_DTYPE_F32);
   const size_t smem = sizeof(double) * 32 * V * cpg::kRouteWarps;
   // At most about as many blocks as fit on the SMs at once; each then walks several tokens.
   const int64_t per = 32 / L * cpg::kRouteWarps;
@@ -265,13 +270,13 @@ int launch_route_grad(cpg::RouteGradParams p, int32_t dtype, cudaStream_t st) {
   // Vectors of as many logits as 16 bytes or V hold.
   if (dtype == CPG_DTYPE_BF16) {
     constexpr int kPer = V < 8 ? V : 8;
-    p.vec = run_vectors<kPer>(p.logits, p.ld, dtype);
-    p.vec_out = run_vectors<kPer>(p.dlogits, p.ldd, dtype);
+    p.vec = run_vectors<kPer>({p.logits, p.ld, p.tokens}, dtype);
+    p.vec_out = run_vectors<kPer>({p.dlogits, p.ldd, p.tokens}, dtype);
     return launch("route gradient kernel", true, &cpg::route_grad_kernel<__nv_bfloat16, L, V>, grid,
                   32 * cpg::kRouteWarps, 0, st, 1, p);
   } else {
-    p.vec = run_vectors<4>(p.logits, p.ld, dtype);
-    p.vec_out = run_vectors<4>(p.dlogits, p.ldd, dtype);
+    p.vec = run_vectors<4>({p.logits, p.ld, p.tokens}, dtype);
+    p.vec_out = run_vectors<4>({p.dlogits, p.ldd, p.tokens}, dtype);
     return launch("route gradient kernel", true, &cpg::route_grad_kernel<float, L, V>, grid,
                   32 * cpg::kRouteWarps, 0, st, 1, p);
   }
@@ -427,7 +432,7 @@ int cpg_dispatch_rows(const void* x, int32_t dtype_x, int64_t tokens, int64_t co
   const cpg::RowsParams p{x, tokens, cols, ldx, slots, k, rows, num_rows, ldr, scales};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int8) return launch_int8(p, dtype_x, st);
-  return by_width(dtype_x, row_width({{x, ldx}, {rows, ldr}}, bytes_of(dtype_x)),
+  return by_width(dtype_x, row_width({{x, ldx, tokens}, {rows, ldr, num_rows}}, bytes_of(dtype_x)),
                   [&](auto type, auto width) {
     using T = decltype(type);
     constexpr int W = decltype(width)::value;
@@ -457,8 +462,9 @@ int cpg_combine_rows(const void* rows, int32_t dtype, int64_t num_rows, int64_t 
   const cpg::CombineParams p{rows,   num_rows, cols,   ldr,       slots, weights,
                              tokens, k,        source, ld_source, y,     ldy};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Rows src = source != nullptr ? Rows{source, ld_source} : Rows{y, ldy};
-  return by_width(dtype, row_width({{rows, ldr}, {y, ldy}, src}, es), [&](auto type, auto width) {
+  const Rows src = source != nullptr ? Rows{source, ld_source, tokens} : Rows{y, ldy, tokens};
+  const int w = row_width({{rows, ldr, num_rows}, {y, ldy, tokens}, src}, es);
+  return by_width(dtype, w, [&](auto type, auto width) {
     using T = decltype(type);
     constexpr int W = decltype(width)::value;
     const int32_t chunks = row_chunks<T, W>(cols, cpg::combine_accesses<T, W>());
@@ -490,8 +496,9 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
   const cpg::CombineGradParams p{dy,    tokens,  cols, lddy,  rows, num_rows, ldr,
                                  slots, weights, k,    drows, lddr, dweights};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_width(dtype, row_width({{dy, lddy}, {rows, ldr}, {drows, lddr}}, es),
-                  [&](auto type, auto width) {
+  const int w =
+      row_width({{dy, lddy, tokens}, {rows, ldr, num_rows}, {drows, lddr, num_rows}}, es);
+  return by_width(dtype, w, [&](auto type, auto width) {
     return launch("combine gradient kernel", true,
                   &cpg::combine_grad_kernel<decltype(type), decltype(width)::value>,
                   warp_grid(tokens * k), 256, 0, st, 1, p);

@@ -534,6 +534,68 @@ def test_rows_of_every_alignment(cols, dtype):
         assert ((got[3].cpu().double() - prod.sum(-1)).abs() <= bound).all()
 
 
+def launched_kernels(f):
+    """Names of the kernels that f launches, from the graph of a captured call."""
+    from cuda.bindings import driver
+
+    def ok(result):
+        assert result[0] == driver.CUresult.CUDA_SUCCESS, result
+        return result[1]
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        f()
+    names = []
+    count = driver.cuGraphGetNodes(graph.raw_cuda_graph(), 0)[2]
+    for node in ok(driver.cuGraphGetNodes(graph.raw_cuda_graph(), count)):
+        if ok(driver.cuGraphNodeGetType(node)) == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            params = ok(driver.cuGraphKernelNodeGetParams(node))
+            names.append(ok(driver.cuFuncGetName(params.func) if int(params.func)
+                            else driver.cuKernelGetName(params.kern)).decode())
+    return " ".join(names)
+
+
+@pytest.mark.parametrize("cols", [4097, 260, 17])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_is_read_as_its_memory_is_aligned(cols, dtype):
+    """The row stride of one row is not used: a 16-byte aligned row takes the kernels of 16-byte
+    accesses whatever its length, with the same bits."""
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(1, cols, generator=g).to(dtype).cuda()
+    name = "13__nv_bfloat16" if dtype == torch.bfloat16 else "f"
+    got = {}
+
+    def quantise():
+        got["q"] = quantize_int8(x)
+    text = launched_kernels(quantise)
+    assert f"rows_int8_vec_kernelI{name}Li16E" in text
+    rq, rs = moe_ref.quantize_int8(x.cpu())
+    quantise()
+    assert torch.equal(got["q"][0].cpu(), rq) and torch.equal(got["q"][1].cpu(), rs)
+
+    ids = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    w = torch.full((1, 1), 0.5, device="cuda")
+
+    def chain():
+        p = moe.dispatch(x, ids, 1)
+        y = moe.combine(p.rows, p.slots, w, source=x)
+        got["c"] = (p.rows, y, *moe.combine_backward(x, p.rows, p.slots, w))
+    text = launched_kernels(chain)
+    for kernel in ("rows_copy_kernel", "combine_kernel", "combine_grad_kernel"):
+        assert f"{kernel}I{name}Li16E" in text, kernel
+    chain()
+    rows, y, drows, _ = got["c"]
+    assert torch.equal(rows, x) and torch.equal(drows, (x.float() * 0.5).to(dtype))
+    assert torch.equal(y, (x.float() * 1.5).to(dtype))
+
+    q = torch.zeros(1, cols, dtype=torch.int8, device="cuda")
+    text = launched_kernels(lambda: moe.dispatch(x, ids, 1, quantize="int8", out=q))
+    assert f"rows_int8_vec_kernelI{name}Li16E" in text
+    torch.cuda.synchronize()
+    assert torch.equal(q.cpu(), rq)
+
+
 @pytest.mark.parametrize("cols", [4096, 4097])
 def test_rows_past_32_bit_offsets(cols):
     """Rows whose element offsets pass 2^31: token t goes to expert 7 - t % 8 with every choice, so
