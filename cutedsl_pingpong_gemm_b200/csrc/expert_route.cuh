@@ -388,17 +388,20 @@ __device__ __forceinline__ void sort_keys(uint32_t (&a)[N]) {
 // first), so a key names its expert in the run; what they cost in precision is part of the bound
 // below.
 //
-// Error of the 32-bit scores (2^-23 = one ulp of 1):
-//   sigmoid: e^-l is off by (2 + 1.173 |l|) ulp, which s (1 - s) turns into at most 0.57 ulp of s;
-//            the sum 1 + e^-l and the quotient add 2.5: below 2^-21 altogether.
-//   softmax: p = e^(l - top) inv with inv <= 1 the common factor.  Each exponential is off by at most
-//            (2.9 ulp) inv absolutely; inv by (10.2 + 18.5 + 1) ulp relatively (the terms' errors
-//            weighted by p, whose mean |l - top| is at most ln 1024; V + log2 L <= 37 additions;
-//            the quotient),
-//            which the largest p <= inv carries: below 2^-18 inv altogether.
-// c = s + bias adds half an ulp of c, a key's lost bits less than V ulp.  Two c nearer than twice the
-// bound are ranked in 64 bits (the choices and what is near the last of them; groups likewise),
-// unless logit and bias are the same: such c are equal, and the lower index goes first.
+// Error of the 32-bit scores (u = 2^-23, one ulp of 1):
+//   sigmoid: e^-l is off by (2 + 1.173 |l|) u, which s (1 - s) turns into at most 0.63 u of s;
+//            the sum 1 + e^-l and the quotient add 2.5: below 4 u = 2^-21 altogether.
+//   softmax: p = e^(l - top) inv with inv <= 1 the common factor.  inv is off by at most
+//            d = (10.2 + 18.5 + 2) u of itself: the terms' errors weighted by p, whose mean
+//            |l - top| is at most ln 1024; V + log2 L <= 37 additions; the quotient.  Two p share
+//            it, and since p <= inv it moves their difference by at most d inv.  Beside it each p has
+//            its exponential's error, at most 2 u inv, and the product's rounding, at most u / 2
+//            inv.  So a difference of two p is off by at most (30.7 + 2 (2 + 0.5)) u inv = 35.7 u inv
+//            and one of two sums of two p by twice that; `near` below is 64 u inv = 2^-17 inv.
+// c = s + bias adds half an ulp of c, a key's lost bits less than V ulp (`rel`).  Two c nearer than
+// the bound are ranked in 64 bits (the choices and what is near the last of them; groups likewise,
+// whose scores are not cut to keys), unless logit and bias are the same: such c are equal, and the
+// lower index goes first.
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 2))
     route_kernel(const __grid_constant__ RouteParams p) {
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, V <= 8 ? 8 : (V == 16 ? 4 : 
       score(std::false_type{});
     }
     // Two c whose difference is at most near + rel (|c1| + |c2|) may be in another order.
-    const float near = by_logit ? 0.f : 2.f * (softmax ? 0x1p-18f * inv : 0x1p-21f);
+    const float near = by_logit ? 0.f : (softmax ? 0x1p-17f * inv : 2.f * 0x1p-21f);
     const float rel = 0x1p-22f + V * 0x1p-23f;
     uint32_t open = ~0u;  // one bit per place of the run: its group is kept
     if (p.groups > 1) {

@@ -84,6 +84,22 @@ def test_route_near_ties():
                         group_score="top2")
 
 
+@pytest.mark.parametrize("e", [8, 32, 64, 128, 256, 512, 1024])
+@pytest.mark.parametrize("level", [-23, -20, -18, -17, -16, -14])
+def test_route_softmax_biases_that_cancel_the_scores(e, level):
+    """Biases near the scores' negatives leave ranked values of 2^level of the largest score, about
+    the 32-bit scores' error: still ranked as in 64 bits, alone and in groups."""
+    g = torch.Generator().manual_seed(e - level)
+    k = min(8, e)
+    for spread in (0.1, 2.0):
+        lg = torch.randn(1, e, generator=g) * spread
+        p = lg.double().softmax(1)
+        bias = (p.max() * 2.0 ** level * torch.randn(e, generator=g) - p[0]).float()
+        check_route(lg.expand(5, e).contiguous(), k, bias=bias)
+        for score in ("max", "top2"):
+            check_route(lg, min(k, 4), bias=bias, groups=4, kept_groups=2, group_score=score)
+
+
 def test_route_equal_scores_go_to_the_lowest_index():
     lg = torch.zeros(5, 96)
     ids, _ = check_route(lg, 7, scoring="sigmoid", bias=torch.zeros(96))
