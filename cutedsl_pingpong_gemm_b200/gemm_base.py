@@ -15,10 +15,15 @@ the last dimension (the reference's harness layout, gemm_base.py:587-590).  Beyo
 ``a``/``b`` may be FP8 E4M3 (``torch.float8_e4m3fn``, with per-tensor ``scale_a``/``scale_b``
 device scalars) or INT8 (``torch.int8``, with scales per tensor, or per row of ``a`` and per row of
 ``b``: FP32 [M] and [N], of a batched call [L, M] and [L, N]) and ``c`` may be FP32 (split-K
-partials); ``bias`` adds a BF16 per-column vector.  INT8 sums are exact 32-bit integers (K <=
-131071), rounded once before the scales.  Underneath, every call goes through the C ABI of
-``libcpgemm.so`` into hand-written sm_100a kernels (tcgen05 MMA into TMEM, TMA loads/stores,
-persistent grouped tile scheduler); there is no other execution path.
+partials); ``bias`` adds a BF16 per-column vector.  INT8 sums over the whole K (``split_k=1``, the
+small-M kernel, grouped calls) are exact 32-bit integers (K <= 131071), rounded once before the
+scales.  Where K is split (``split_k`` > 1, -1, -2, or 0 where it picks one of these: M > 128 with
+few tiles) the sum of each range is exact, but the ranges' scaled FP32 results are added, each
+addition rounded, in an order that may differ between runs.
+
+Underneath, every call goes through the C ABI of ``libcpgemm.so`` into hand-written sm_100a kernels
+(tcgen05 MMA into TMEM, TMA loads/stores, persistent grouped tile scheduler); there is no other
+execution path.
 
 Argument meaning on sm_100a:
 

@@ -68,7 +68,9 @@ extern "C" {
  * an output channel); an operand without its flag has one value, and a NULL pointer means 1.  Each
  * batch's or group's scales follow the previous one's without a gap.  The sum over k is exact in
  * 32-bit integers (K <= 131071) and is rounded once to fp32 before the scales, which are applied
- * one after the other in fp32 (each product should stay finite). */
+ * one after the other in fp32 (each product should stay finite).  That holds for the whole K in
+ * one pass (split_k 0, 1 and CPG_SPLIT_K_DECODE).  K ranges, Stream-K and the hybrid do it per
+ * range and add the scaled fp32 results, each addition rounded, in an order that may vary. */
 #define CPG_SCALE_ROWS_A 2
 #define CPG_SCALE_ROWS_B 4
 
