@@ -25,6 +25,9 @@ Underneath, every call goes through the C ABI of ``libcpgemm.so`` into hand-writ
 (tcgen05 MMA into TMEM, TMA loads/stores, persistent grouped tile scheduler); there is no other
 execution path.
 
+All tensors of a call are on D's device (A, B, bias, scales, source, group offsets): one on another
+device is refused, since the kernel would fault unless that device's memory happened to be mapped.
+
 Argument meaning on sm_100a:
 
 * ``tile_shape_mn``: the CTA tile, (128, N) with N in {64, 128, 256, 512} (512: CTA pairs only,

@@ -3,6 +3,7 @@ and the C ABI's copy of the same checks (cpg_config_validate)."""
 import inspect
 
 import pytest
+import torch
 
 from cutedsl_pingpong_gemm_b200 import GemmSM90, GemmSM100, RasterOrder, _lib
 
@@ -158,3 +159,35 @@ def test_release_drops_cached_plans_and_workspaces():
     compiled._workspaces["workspace"] = object()
     gemm.release()
     assert compiled._plans == {} and compiled._workspaces == {}
+
+
+class Layout:
+    """What a plan looks at of a tensor."""
+
+    def __init__(self, rows, cols, dtype, device):
+        self.shape, self.dtype, self.device = torch.Size((rows, cols)), dtype, torch.device(device)
+        self.is_cuda = self.device.type == "cuda"
+
+    def dim(self):
+        return 2
+
+    def numel(self):
+        return self.shape.numel()
+
+    def stride(self, i=None):
+        return (self.shape[1], 1) if i is None else (self.shape[1], 1)[i]
+
+    def element_size(self):
+        return self.dtype.itemsize
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn, torch.int8])
+def test_operands_of_another_device_are_refused(dtype):
+    from cutedsl_pingpong_gemm_b200.gemm_base import CompiledGemm
+    gemm = GemmSM90(tile_shape_mn=(128, 256), epi_tile_mn=(128, 32), cluster_shape_mnk=(1, 1, 1),
+                    atom_layout_mn=(1, 1), reuse_ab=False, is_persistent=True)
+    for da, db in (("cuda:1", "cuda:0"), ("cuda:0", "cuda:1"), ("cpu", "cuda:0")):
+        with pytest.raises(_lib.CpgError) as e:
+            CompiledGemm(gemm).plan_for(Layout(64, 128, dtype, da), Layout(32, 128, dtype, db),
+                                        Layout(64, 32, torch.bfloat16, "cuda:0"))
+        assert e.value.code == _lib.CPG_ERR_NO_DEVICE
