@@ -470,6 +470,8 @@ static int alloc_fixup_workspace(cpg_gemm* g, int64_t tiles) {
 using DecodeFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
                           const cpg::DecodeParams);
 
+// Bytes of A per group below which a grouped plan keeps A in L2 (cpg_gemm_create).
+constexpr int64_t kGroupKeepsA = int64_t(64) << 20;
 constexpr int kDecodeInt8Stages = 6;
 
 static const void* decode_kernel(int dtype_ab, int dtype_d, int cta_group) {
@@ -888,11 +890,23 @@ int cpg_gemm_create(const cpg_gemm_config* cfg, const cpg_gemm_problem* prob, in
       g->l2_policy_b = 2;
     }
   }
-  if (prob->grouped) {
+  if (prob->grouped &&
+      prob->m * prob->k / prob->l < kGroupKeepsA / elem_bytes(prob->dtype_ab)) {
     // A group's tiles run m-fastest whatever the raster order: its rows of A are read again for
-    // every column tile, its B passes once.  8 uneven groups of 16384 rows in all, gated
-    // [2 x 14336, 4096], A / B evict-first / evict-last and the other way round: INT8 1470 and
-    // 1401 us, BF16 2790 and 2560 us.
+    // every column tile, its B passes once, so A is kept while the L2 holds an average group's
+    // rows (the offsets are on the device).  A kept / by raster order (B kept), us, after 0.25 s of
+    // rest [and in a loop, under the power cap]; groups, rows of A x K x N, 512-wide tiles:
+    //   8 uneven, 16384 x 4096 x 2*14336 gated: INT8 1421 / 1513 [1681 / 1643], BF16 2622 / 2827
+    //     [3215 / 3175], E4M3 1421 / 1513 [1687 / 1661]; even: 1364 / 1408 [1598 / 1553], 2497 /
+    //     2631 [2950 / 2944], 1358 / 1414 [1602 / 1576]
+    //   2 even, 8192 x 8192 x 8192 (32 MiB a group): INT8 351 / 361 [398 / 397]
+    //   8 uneven, 4096 x 4096 x 4096, 256-wide, loop: INT8 88 / 92, BF16 154 / 160, E4M3 89 / 91
+    //   weights read once, loop: 8 uneven, 32 x 4096 x 2*14336 gated: INT8 164 / 176, BF16 313 /
+    //     316, E4M3 176 / 178; 64 uneven, 512 x 2048 x 2048, 256-wide: 80 / 84, 133 / 136, 80 / 83
+    // and from 64 MiB a group on, where A no longer stays:
+    //   2 uneven, 16384 x 8192 x 8192: INT8 823 / 809 [974 / 913], BF16 1593 / 1592 [1895 / 1833],
+    //     E4M3 835 / 831 [980 / 952]; even, 32768 rows, loop: 1853 / 1763, 3623 / 3473, 1915 / 1875
+    //   (the other way round only 2 even, 32768 x 4096 x 8192: INT8 782 / 849 [935 / 952]).
     g->l2_policy_a = 2;
     g->l2_policy_b = 1;
   }
