@@ -551,10 +551,14 @@ static int create_decode_plan(const cpg_gemm_config* cfg, const cpg_gemm_problem
   }
   if (stages == 0) return fail(CPG_ERR_SMEM, "the small-M kernel does not fit in shared memory");
   if (kps >= 2 && stages > kps) stages = static_cast<int>(kps);
-  // INT8 halves the loads of a BF16 tile while the waits stay the same, so the next call's set-up
-  // counts for more: with at most 6 stages of 16 rows two calls' CTAs fit on an SM.  Back to back on
-  // N = K = 8192, 12 and 6 stages: M = 1 17.1 and 15.7 us, 16 18.1 and 16.6, 64 19.2 and 18.9, 128
-  // (which has room for no more) 23.2.
+  // INT8 halves a BF16 tile's loads while the waits per k-block stay the same, and fewer stages
+  // measured better.  Calls back to back in a graph, us, with 12 (or as many as fit) / 8 / 6 / 4
+  // stages, N x K: 8192 x 8192 M = 1 17.3 / 16.0 / 15.8 / 16.7, M = 16 18.3 / 17.0 / 16.8 / 17.7,
+  // M = 64 19.3 / 19.3 / 19.0 / 19.8, M = 128 23.4 / 23.4 / 23.4 / 24.2; 4096 x 14336 M = 16
+  // 17.5 / 16.3 / 16.0 / 16.7; 4096 x 4096 M = 16 10.6 / 10.6 / 10.0 / 9.6; 28672 x 4096 M = 16
+  // 30.0 / 29.1 / 29.6 / 31.6; 14336 x 8192 M = 16 24.5 / 24.1 / 24.7 / 27.2 (M = 128 30.0 / 30.1 /
+  // 30.4 / 33.1).  Not because two calls' CTAs share an SM: 164 registers x 320 threads leave room
+  // for one.
   if (int8 && stages > kDecodeInt8Stages) stages = kDecodeInt8Stages;
   if (env_st != nullptr && std::atoi(env_st) >= 2 && std::atoi(env_st) < stages)
     stages = std::atoi(env_st);
