@@ -298,6 +298,95 @@ def test_empty_rows():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 8, 64), (257, 264, 300), (130, 1003, 128)])
+@pytest.mark.parametrize("rows_b", [True, False])
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_gated_fp32(m, n, k, rows_b, dynamic):
+    a, b, sa, sb = operands(m, 2 * n, k, seed=33)
+    sa = sa * 0.1
+    if not rows_b:
+        sb = sb[:1]
+    d = output(m, n, torch.float32)
+    make_gemm(512, dynamic=dynamic)(padded(a.cuda(), 16), padded(b.cuda(), 16), d,
+                                    scale_a=sa.cuda(), scale_b=sb.cuda(), activation="silu",
+                                    gated=True, split_k=0)
+    torch.cuda.synchronize()
+    ref, slack = moe_ref.int8_product(a, b, sa, sb, activation="silu", gated=True)
+    assert moe_ref.within(d, ref, slack) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [130, 264])
+def test_batched_gated(n, dtype):
+    l, m, k = 3, 150, 160
+    a, b, sa, sb = operands(m, 2 * n, k, 43, (l,), (l,))
+    sa = sa * 0.1
+    d = output(m, n, dtype, lead=(l,))
+    make_gemm(512)(a.cuda(), b.cuda(), d, scale_a=sa.cuda(), scale_b=sb.cuda(), activation="silu",
+                   gated=True)
+    torch.cuda.synchronize()
+    for i in range(l):
+        ref, slack = moe_ref.int8_product(a[i], b[i], sa[i], sb[i], activation="silu", gated=True)
+        assert moe_ref.within(d[i], ref, slack) <= 0, i
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("split", [0, 3])
+def test_batched_split_k(dtype, split):
+    """Every K range of every batch takes its batch's scales (tolerance as in test_split_k)."""
+    l, m, n, k = 3, 200, 264, 5008
+    a, b, sa, sb = operands(m, n, k, 44, (l,), (l,))
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(6)).bfloat16()
+    d = output(m, n, dtype, lead=(l,))
+    make_gemm(256, (1, 1, 1))(a.cuda(), b.cuda(), d, bias=bias.cuda(), scale_a=sa.cuda(),
+                              scale_b=sb.cuda(), split_k=split)
+    torch.cuda.synchronize()
+    ranges = -(-k // 128)
+    for i in range(l):
+        ref, slack = moe_ref.int8_product(a[i], b[i], sa[i], sb[i], bias=bias)
+        parts = (a[i].double().abs() @ b[i].double().abs().t()) * sa[i].double()[:, None]
+        parts = parts * sb[i].double()
+        slack = slack + 2 * ranges * moe_ref.F32_HALF * (parts + ref.abs())
+        assert moe_ref.within(d[i], ref, slack) <= 0, i
+
+
+@pytest.mark.parametrize("m", [1, 16, 100, 128])
+@pytest.mark.parametrize("captured", [False, True])
+def test_quantise_and_small_m_back_to_back(m, captured):
+    """Each product is a dependent launch that may be set up while the quantiser before it still runs:
+    every step reads the rows and scales of its own quantiser, though all steps share their buffers;
+    eager and in a graph replayed on new inputs."""
+    n, k, steps = 1024, 1040, 6
+    _, b, _, sb = operands(m, n, k, seed=81)
+    g = torch.Generator().manual_seed(m)
+    xs = torch.zeros(steps, m, k, dtype=torch.bfloat16, device="cuda")
+    db, dsb, gemm = b.cuda(), sb.cuda(), make_gemm()
+    q = torch.zeros(m, k, dtype=torch.int8, device="cuda")
+    s = torch.zeros(m, device="cuda")
+    outs = [output(m, n) for _ in range(steps)]
+
+    def run():
+        for i in range(steps):
+            quantize_int8(xs[i], out=q, scales=s)
+            gemm(q, db, outs[i], scale_a=s, scale_b=dsb, split_k=0)
+    run()
+    torch.cuda.synchronize()
+    graph = None
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(3):
+        x = (torch.randn(steps, m, k, generator=g) * torch.rand(steps, m, 1, generator=g)).bfloat16()
+        xs.copy_(x)
+        run() if graph is None else graph.replay()
+        torch.cuda.synchronize()
+        for i in range(steps):
+            rq, rs = moe_ref.quantize_int8(x[i])
+            ref, slack = moe_ref.int8_product(rq, b, rs, sb)
+            assert moe_ref.within(outs[i], ref, slack) <= 0, i
+
+
 # --------------------------------------------------------------------------------- quantiser
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 16), (33, 100), (4, 1024), (17, 1032),
                                        (2, 4096), (9, 8192), (2, 16384), (3, 16400), (2, 70001)])
