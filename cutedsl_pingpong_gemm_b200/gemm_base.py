@@ -318,7 +318,10 @@ class CompiledGemm:
         key = (tuple(c.shape), c.device, _stream_handle(stream, c.device))
         ws = self._workspaces.get(key)
         if ws is None:
-            ws = torch.empty(c.shape, dtype=torch.float32, device=c.device)
+            # The kernel adds into it by TMA: rows padded to 16 bytes, whatever N is.
+            n = c.shape[-1]
+            ws = torch.empty(*c.shape[:-1], -(-n // 4) * 4, dtype=torch.float32,
+                             device=c.device)[..., :n]
             self._workspaces[key] = ws
         return ws
 

@@ -146,6 +146,37 @@ def test_split_k(split, dtype):
     assert moe_ref.within(d, ref, slack + 2 * ranges * moe_ref.F32_HALF * (parts + ref.abs())) <= 0
 
 
+@pytest.mark.parametrize("n", [1, 107, 130, 263])
+@pytest.mark.parametrize("split", [0, 2, -1])
+@pytest.mark.parametrize("lead", [(), (3,)])
+@pytest.mark.parametrize("operand", [torch.int8, torch.bfloat16])
+def test_split_k_into_bf16_of_any_width(n, split, lead, operand):
+    """The FP32 workspace of a split has rows of its own padding: any N, as in one pass."""
+    m, k = 310, 2240
+    if operand == torch.int8:
+        a, b, sa, sb = operands(m, n, k, 13, lead, lead)
+    else:
+        g = torch.Generator().manual_seed(13)
+        a = torch.randn(*lead, m, k, generator=g).bfloat16()
+        b = torch.randn(*lead, n, k, generator=g).bfloat16()
+        sa = sb = None
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(6)).bfloat16()
+    d = torch.full((*lead, m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    make_gemm(256, (1, 1, 1))(a.cuda(), b.cuda(), d, bias=bias.cuda(), split_k=split,
+                              scale_a=None if sa is None else sa.cuda(),
+                              scale_b=None if sb is None else sb.cuda())
+    torch.cuda.synchronize()
+    for i in range(lead[0]) if lead else (slice(None),):
+        ref, slack = moe_ref.int8_product(a[i], b[i], None if sa is None else sa[i],
+                                          None if sb is None else sb[i], bias=bias)
+        mag = a[i].double().abs() @ b[i].double().abs().t()
+        if sa is not None:
+            mag = mag * sa[i].double()[:, None] * sb[i].double()
+        # INT8: one rounding per range and addition; BF16: k fp32 additions of exact products.
+        terms = 2 * -(-k // 128) if sa is not None else 2 * k
+        assert moe_ref.within(d[i], ref, slack + terms * moe_ref.F32_HALF * (mag + ref.abs())) <= 0
+
+
 @pytest.mark.parametrize("activation", ["relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_epilogue(activation, dtype):
