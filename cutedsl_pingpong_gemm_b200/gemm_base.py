@@ -299,7 +299,8 @@ class CompiledGemm:
         per16 = 16 // a.element_size()
         lda = a.stride(0) if t > 1 else max(per16, -(-k // per16) * per16)
         ldb = b.stride(1) if b_rows > 1 else max(per16, -(-k // per16) * per16)
-        ldd = c.stride(0) if t > 1 else max(16 // c.element_size(), n)
+        per_d = 16 // c.element_size()
+        ldd = c.stride(0) if t > 1 else max(per_d, -(-n // per_d) * per_d)
         dev = c.device.index
         dt_ab, dt_d = ab_codes[a.dtype], d_codes[c.dtype]
         key = ("grouped", t, n, k, groups, lda, ldb, ldd, b.stride(0), dev, dt_ab, dt_d,

@@ -176,3 +176,14 @@ def test_grouped_rejections():
                           is_persistent=False)
     with pytest.raises(_lib.CpgError):  # needs a persistent kernel
         nonpersist.grouped(a.cuda(), b.cuda(), d, offs)
+
+
+@pytest.mark.parametrize("n", [1, 107, 392])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_grouped_single_row(n, dtype):
+    """One row of any width: its stride is not used."""
+    a, b, off = grouped_inputs([0, 1, 0], n, 128, seed=70)
+    d = torch.full((1, n), float("nan"), dtype=dtype, device="cuda")
+    make_gemm().grouped(a.cuda(), b.cuda(), d, torch.tensor(off, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    check_groups(d, a, b, off)
