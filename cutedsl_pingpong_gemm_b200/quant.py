@@ -83,8 +83,16 @@ def cast_f32_bf16(x, bias=None, out=None, stream=None):
     rows, cols = x.shape
     if out is None:
         out = torch.empty(rows, cols, dtype=torch.bfloat16, device=x.device)
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != cols):
-        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE, "bias must be BF16 of length cols")
+    elif out.dtype != torch.bfloat16 or out.shape != x.shape or out.device != x.device:
+        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
+                            f"out must be BF16 of shape {tuple(x.shape)} on {x.device}")
+    for name, t in (("x", x), ("out", out)):
+        if t.numel() and cols > 1 and t.stride(1) != 1:
+            raise _lib.CpgError(_lib.CPG_ERR_UNSUPPORTED, f"{name} must have unit column stride")
+    if bias is not None and not (bias.dtype == torch.bfloat16 and bias.numel() == cols
+                                 and bias.device == x.device and bias.is_contiguous()):
+        raise _lib.CpgError(_lib.CPG_ERR_INVALID_SHAPE,
+                            f"bias must be a contiguous BF16 tensor of length {cols} on {x.device}")
     ldx = x.stride(0) if rows > 1 else cols
     ldy = out.stride(0) if rows > 1 else cols
     lib = _lib.load()

@@ -3,6 +3,7 @@ the fp32 scales must be identical, since both follow s = amax/448, q = RN-even e
 import pytest
 import torch
 
+from cutedsl_pingpong_gemm_b200 import GemmSM90, _lib
 from cutedsl_pingpong_gemm_b200.quant import cast_f32_bf16, quantize_e4m3
 from oracle import gemm_ref
 
@@ -130,3 +131,32 @@ def test_cast_odd_and_strided_shapes(shape):
     x = full[:, 1:cols + 1]
     y = cast_f32_bf16(x.cuda())
     assert torch.equal(y.cpu(), x.to(torch.bfloat16))
+
+
+def test_cast_refusals():
+    """Tensors that the kernel could not read or write as they lie are refused before a launch, also
+    where a split GEMM casts its FP32 sums."""
+    x = torch.randn(6, 8, device="cuda")
+    bias = torch.randn(16).bfloat16()
+    out = torch.zeros(6, 16, dtype=torch.bfloat16, device="cuda")
+    S, U = _lib.CPG_ERR_INVALID_SHAPE, _lib.CPG_ERR_UNSUPPORTED
+    for kw, code in [(dict(bias=bias[:8]), S), (dict(bias=bias.cuda()[::2]), S),
+                     (dict(bias=bias.cuda()), S), (dict(out=out[:, ::2]), U),
+                     (dict(out=out[:5, :8]), S), (dict(out=out[:, :8].cpu()), S),
+                     (dict(out=out[:, :8].float()), S)]:
+        with pytest.raises(_lib.CpgError) as e:
+            cast_f32_bf16(x, **kw)
+        assert e.value.code == code, kw
+    with pytest.raises(_lib.CpgError) as e:
+        cast_f32_bf16(torch.randn(6, 16, device="cuda")[:, ::2])
+    assert e.value.code == U
+    gemm = GemmSM90(tile_shape_mn=(128, 128), epi_tile_mn=(128, 32), cluster_shape_mnk=(1, 1, 1),
+                    atom_layout_mn=(1, 1), reuse_ab=False, is_persistent=True)
+    a = torch.randn(130, 256, device="cuda").bfloat16()
+    b = torch.randn(8, 256, device="cuda").bfloat16()
+    d = torch.zeros(130, 16, dtype=torch.bfloat16, device="cuda")
+    for c, kw, code in [(d[:, :8], dict(bias=bias[:8]), S), (d[:, ::2], {}, U)]:
+        with pytest.raises(_lib.CpgError) as e:
+            gemm(a, b, c, split_k=2, **kw)
+        assert e.value.code == code
+    assert (d == 0).all()
