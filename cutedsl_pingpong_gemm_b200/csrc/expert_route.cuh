@@ -198,7 +198,12 @@ __device__ __forceinline__ float fast_rcp(float x) {
 }
 
 __device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
-__device__ __forceinline__ float sigmoid32(float l) { return __fdividef(1.f, 1.f + expf(-l)); }
+// Within 4.5 ulp: e^-|l| has 2, the sum half of one and the quotient 2.  Nothing overflows, so small
+// values keep their size down to the subnormals.
+__device__ __forceinline__ float sigmoid32(float l) {
+  const float t = expf(-fabsf(l));
+  return __fdividef(l >= 0.f ? 1.f : t, 1.f + t);
+}
 
 // A logit that cannot be chosen and spoils its row's weights: NaN, and +inf under the softmax.
 __device__ __forceinline__ bool route_bad(float l, int32_t scoring) {
@@ -207,15 +212,16 @@ __device__ __forceinline__ bool route_bad(float l, int32_t scoring) {
 
 // Shares of the chosen experts: lane j holds choice j's logit and (softmax over all experts) its
 // probability.  Renormalised softmax shares are the softmax of the chosen logits alone;
-// renormalised sigmoid shares of logits all below -60, where sigmoid(l) = e^l, likewise (the sum
-// of the scores would underflow).  Lanes without a choice get 0.
+// renormalised sigmoid shares of logits all below kSmallLogit likewise: there sigmoid(l) = e^l within
+// e^-17 < 2^-24 of it, and scores that underflow still have shares.  Lanes without a choice get 0.
+constexpr float kSmallLogit = -17.f;
 template <int L>
 __device__ __forceinline__ float route_share(int32_t scoring, int32_t renormalize, bool has, float l,
                                              float prob) {
   if (!renormalize) return has ? (scoring == kRouteSoftmax ? prob : sigmoid32(l)) : 0.f;
   const float top = lanes_max<L>(has ? l : -INFINITY);
   float v = 0.f;
-  if (has) v = scoring == kRouteSoftmax || top < -60.f ? expf(l - top) : sigmoid32(l);
+  if (has) v = scoring == kRouteSoftmax || top < kSmallLogit ? expf(l - top) : sigmoid32(l);
   const float sum = lanes_sum<L>(v);
   return sum > 0.f ? __fdividef(v, sum) : 0.f;
 }
@@ -797,7 +803,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const Rout
     } else {
       const float best = max_of(has ? lj : -INFINITY);
       if (has)
-        r = p.scoring == kRouteSoftmax || best < -60.f ? expf(lj - best) : sigmoid32(lj);
+        r = p.scoring == kRouteSoftmax || best < kSmallLogit ? expf(lj - best) : sigmoid32(lj);
       const float sum = sum_of(r);
       r = sum > 0.f ? __fdividef(r, sum) : 0.f;
     }

@@ -108,6 +108,28 @@ def test_route_equal_scores_go_to_the_lowest_index():
     assert (ids.cpu() == torch.arange(7)).all()
 
 
+def test_route_small_sigmoid_scores():
+    """Scores near and below the smallest normal number: shares keep their ratios, and so does their
+    gradient."""
+    lg = torch.tensor([[-59.0, -88.0, -95.0], [-16.0, -60.0, -60.5], [-17.5, -30.0, -62.0],
+                       [-86.0, -89.0, -110.0], [-3.0, -40.0, -62.0], [-61.0, -87.5, -88.5],
+                       [-200.0, -201.0, -230.0], [-45.0, -87.4, -88.6]])
+    for dtype in DTYPES:
+        x = lg.to(dtype)
+        for renorm in (True, False):
+            kw = dict(scoring="sigmoid", renormalize=renorm)
+            ids, _ = check_route(x, 3, **kw)
+            _, share = moe_ref.route(x, 3, **kw)
+            for j in range(3):
+                dw = torch.zeros(x.shape[0], 3)
+                dw[:, j] = 1.0
+                out = moe.route_backward(dw.cuda(), x.float().cuda(), ids, **kw).cpu().double()
+                ref = moe_ref.route_backward(dw, x.float(), ids.cpu(), **kw)
+                # Two shares multiply; the choice's own 1 - share is good to its share's error.
+                size = ref.abs().scatter(1, ids.cpu().long()[:, j:j + 1], share[:, j:j + 1])
+                assert ((out - ref).abs() <= 2 * WEIGHT_REL * size + 1e-37).all()
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [True, False])
 @pytest.mark.parametrize("with_bias", [True, False])
