@@ -180,6 +180,7 @@ SIGNATURES = {
                                         _i64, _vp, _i64, _vp]),
     "cpg_combine_rows_backward": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64,
                                                  _vp, _vp, _i32, _vp, _i64, _vp, _vp]),
+    "cpg_clear_unnamed_rows": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp]),
     "cpg_cast_f32_bf16": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "cpg_gemm_splitk_static": (ctypes.c_int, [_P(GemmConfigC), _P(GemmProblemC), _vp, _vp, _vp,
                                               _P(EpilogueC), _vp]),

@@ -505,4 +505,31 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
   });
 }
 
+int cpg_clear_unnamed_rows(void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
+                           const int32_t* slots, int64_t tokens, int32_t k, void* stream) {
+  int rc = check_pairs(tokens, k);
+  if (rc != CPG_OK) return rc;
+  if (!float_dtype(dtype)) return fail(CPG_ERR_DTYPE, "rows must be BF16 or FP32");
+  rc = check_matrix("rows", num_rows, cols, ldr);
+  if (rc != CPG_OK) return rc;
+  if (num_rows == 0 || cols == 0) return CPG_OK;
+  if (rows == nullptr || (tokens > 0 && slots == nullptr))
+    return fail(CPG_ERR_NULL, "rows and slots must be non-NULL");
+  if (misaligned(rows, bytes_of(dtype)) || misaligned(slots, 4))
+    return fail(CPG_ERR_ALIGNMENT, "rows and slots must be aligned to their elements");
+  // A block per SM while there are 32 rows for each, and no more rows than its marks hold.
+  int64_t per = ((num_rows + 147) / 148 + 31) / 32 * 32;
+  per = std::min<int64_t>(per, cpg::kClearMaxRows);
+  const cpg::ClearRowsParams p{rows, num_rows, cols, ldr, slots, tokens * k,
+                               static_cast<int32_t>(per)};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_width(dtype, row_width({{rows, ldr, num_rows}}, bytes_of(dtype)),
+                  [&](auto type, auto width) {
+    return launch("row clearing kernel", true,
+                  &cpg::rows_clear_kernel<decltype(type), decltype(width)::value>,
+                  static_cast<unsigned>((num_rows + per - 1) / per), cpg::kClearThreads,
+                  static_cast<size_t>(per / 8), st, 1, p);
+  });
+}
+
 }  // extern "C"

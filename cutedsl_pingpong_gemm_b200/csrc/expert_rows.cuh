@@ -665,4 +665,53 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineGradPara
   }
 }
 
+struct ClearRowsParams {
+  void* rows;
+  int64_t num_rows, cols, ldr;
+  const int32_t* slots;
+  int64_t pairs;
+  int32_t per_block;  // rows of a block, a multiple of 32
+};
+
+// Zeros in the rows that no slot names.  Every block walks all slots and marks those of its own rows
+// in shared memory, so there is no workspace and no order to wait for; the slots stay in L2.
+// Clearing all of drows costs 35 us where this costs 5 (16382 x 4096 BF16 beside a gradient of 54 us).
+constexpr int kClearThreads = 1024;
+constexpr int32_t kClearMaxRows = 1 << 18;  // of a block: 32 KB of marks
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kClearThreads) rows_clear_kernel(const ClearRowsParams p) {
+  kernel_begins();
+  using A = RowAccess<T, W>;
+  extern __shared__ uint32_t named[];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.per_block;
+  const int64_t left = p.num_rows - first;
+  const int32_t count = left < p.per_block ? static_cast<int32_t>(left) : p.per_block;
+  for (int32_t i = threadIdx.x; i < p.per_block / 32; i += kClearThreads) named[i] = 0u;
+  __syncthreads();
+  constexpr int kBatch = 8;  // slots a thread loads before it marks the first
+  for (int64_t i0 = threadIdx.x; i0 < p.pairs; i0 += kBatch * kClearThreads) {
+    int32_t slot[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t i = i0 + u * kClearThreads;
+      slot[u] = i < p.pairs ? p.slots[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t r = slot[u] - first;
+      if (r >= 0 && r < count) atomicOr(named + (r >> 5), 1u << (r & 31));
+    }
+  }
+  __syncthreads();
+  const int32_t cols = static_cast<int32_t>(p.cols);
+  const int lane = threadIdx.x & 31;
+  for (int32_t r = threadIdx.x >> 5; r < count; r += kClearThreads / 32) {
+    if ((named[r >> 5] >> (r & 31)) & 1u) continue;
+    T* row = static_cast<T*>(p.rows) + (first + r) * p.ldr;
+    for (int32_t c = lane * A::kElems; c < cols; c += 32 * A::kElems)
+      A::store(row, c, cols, A::zero());
+  }
+}
+
 }  // namespace cpg

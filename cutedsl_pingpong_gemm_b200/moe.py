@@ -201,15 +201,20 @@ def combine_backward(dy, rows, slots, weights, *, drows=None, dweights=None):
     _, k = pairs("slots", slots)
     vector("slots", slots, (t, k), torch.int32, dev)
     vector("weights", weights, (t, k), torch.float32, dev)
-    if drows is None:
-        # Cleared whole: which rows the slots name is known on the device only.
-        drows = torch.zeros((r, d), dtype=dy.dtype, device=dev)
+    fresh = drows is None
+    if fresh:
+        drows, lddr = torch.empty((r, d), dtype=dy.dtype, device=dev), d
+    else:
+        lddr = output("drows", drows, (r, d), dy.dtype, dev)
     if dweights is None:
         dweights = torch.empty((t, k), dtype=torch.float32, device=dev)
     else:
         vector("dweights", dweights, (t, k), torch.float32, dev)
-    lddr = output("drows", drows, (r, d), dy.dtype, dev)
-    call(_lib.load().cpg_combine_rows_backward, "combine_backward", dev, ptr(dy), code, t, d,
+    lib = _lib.load()
+    if fresh:
+        call(lib.cpg_clear_unnamed_rows, "combine_backward", dev, ptr(drows), code, r, d, lddr,
+             ptr(slots), t, k)
+    call(lib.cpg_combine_rows_backward, "combine_backward", dev, ptr(dy), code, t, d,
           lddy, ptr(rows), r, ldr, ptr(slots), ptr(weights), k, ptr(drows), lddr,
           ptr(dweights))
     return drows, dweights

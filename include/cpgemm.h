@@ -380,6 +380,11 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
                               const int32_t* slots, const float* weights, int32_t k, void* drows,
                               int64_t lddr, float* dweights, void* stream);
 
+/* Zeros in the rows that none of the slots [tokens][k] names: with cpg_combine_rows_backward into
+ * the same drows, the gradient of every row. */
+int cpg_clear_unnamed_rows(void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
+                           const int32_t* slots, int64_t tokens, int32_t k, void* stream);
+
 /* y = bf16(x + bias) for x FP32 [rows, cols]: the last step of split-K after the reduction.
  * bias is optional (BF16, length cols). */
 int cpg_cast_f32_bf16(const float* x, int64_t rows, int64_t cols, int64_t ldx, void* y,

@@ -729,6 +729,31 @@ def test_combine_backward_of_unused_rows(cols, dtype):
     assert moe_ref.within(drows, ref, moe_ref.F32_HALF * ref.abs()) <= 0
 
 
+@pytest.mark.parametrize("t,k,r,cols", [(0, 2, 5, 9), (1, 1, 1, 3), (3, 2, 20000, 130), (3, 32, 31, 8),
+                                        (5, 1, 300001, 2), (20000, 8, 160000, 6),
+                                        (9, 4, 4737, 1030)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_combine_backward_clears_what_no_slot_names(t, k, r, cols, dtype):
+    """Any number of rows, more or fewer than pairs, and slots anywhere among them."""
+    g = torch.Generator().manual_seed(r)
+    slots = torch.randperm(max(r, t * k), generator=g)[:t * k].reshape(t, k).int()
+    slots[torch.rand(t, k, generator=g) < 0.3] = -1
+    if t:
+        slots[0, 0] = 2 ** 31 - 1
+    dy = torch.randn(t, cols, generator=g).to(dtype).cuda()
+    w = torch.rand(t, k, generator=g).cuda()
+    rows = torch.zeros(r, cols, dtype=dtype, device="cuda")
+    stale = torch.full((r, cols), math.nan, dtype=dtype, device="cuda")
+    del stale
+    drows, _ = moe.combine_backward(dy, rows, slots.cuda(), w)
+    torch.cuda.synchronize()
+    want = torch.zeros(r, cols, dtype=dtype, device="cuda")
+    on = slots.cuda().long()
+    token, choice = ((on >= 0) & (on < r)).nonzero(as_tuple=True)
+    want[on[token, choice]] = (w[token, choice, None] * dy[token].float()).to(dtype)
+    assert torch.equal(drows, want)
+
+
 def test_gradients_against_differences():
     """combine's gradients and dispatch's (a combine without weights) against central differences;
     both are linear, so with h = 1 the difference is exact up to fp32 rounding."""

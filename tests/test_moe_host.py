@@ -102,6 +102,18 @@ def test_rows_of_too_many_columns(lib):
     assert lib.cpg_quantize_int8(P, F32, 4, w, w, P, w, P, None) == S
 
 
+def test_clear_refusals(lib):
+    def clear(x=P, dt=F32, n=8, cols=8, ldr=8, slots=P, tokens=4, k=2):
+        return lib.cpg_clear_unnamed_rows(x, dt, n, cols, ldr, slots, tokens, k, None)
+    S, N, A = _lib.CPG_ERR_INVALID_SHAPE, _lib.CPG_ERR_NULL, _lib.CPG_ERR_ALIGNMENT
+    assert clear(dt=I8) == _lib.CPG_ERR_DTYPE and clear(ldr=7) == S and clear(n=BIG) == S
+    assert clear(k=0) == S and clear(k=33) == S and clear(tokens=-1) == S
+    assert clear(cols=2 ** 30, ldr=2 ** 30) == S
+    assert clear(x=None) == N and clear(slots=None) == N
+    assert clear(x=ODD) == A and clear(slots=ODD) == A
+    assert clear(n=0, x=None) == _lib.CPG_OK and clear(cols=0, x=None) == _lib.CPG_OK
+
+
 def test_counts_that_32_bits_would_wrap():
     """More experts or choices than the C entry points' 32-bit counts hold are refused before they
     could be cut to another, valid number."""
