@@ -1,4 +1,4 @@
-// Error reporting and device selection shared by the translation units of the C ABI.
+// Error reporting shared by the translation units of the C ABI.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -102,7 +102,8 @@ bool rows_start_on(const Rows& r, int elem, int bytes) {
 // The widest access (16, 8, 4 or 2 bytes) that every row of these matrices starts on.
 // 8192 tokens x 4 choices, BF16, in us with accesses of 16 / 8 / 4 / 2 bytes (2048, 2052, 2050 and
 // 2049 columns) and, in brackets, of the kernels of one element an access that these replaced:
-// copy 36 / 39 / 41 / 41 [79], combine 30 / 41 / 50 / 67 [82], its gradient 50 / 57 / 61 / 81 [116].
+// copy 28 / 31 / 34 / 33 (dispatch, with the order kernel's 7: 36 / 39 / 41 / 41 [79]), combine
+// 30 / 41 / 50 / 67 [82], its gradient 50 / 57 / 61 / 81 [116].
 int row_width(std::initializer_list<Rows> all, int elem) {
   uint64_t bits = 16;
   for (const Rows& r : all) bits |= address_bits(r, elem);
@@ -138,6 +139,8 @@ int launch_int8_vec(const cpg::RowsParams& p, cudaStream_t st) {
   // the tokens leave most of the GPU idle (each then has less of a row to wait for).
   // Measured: FP32 16384 x 8192 102.6 us (1.00 of measured HBM), BF16 75.0 us (0.82), where the
   // conversions bound it: three packed FMAs per two elements after 22 issue slots an element before.
+  // BF16 16384 x 4096 takes 49-52 us (0.6): a group waits for its row, the maximum and the
+  // conversions in turn and has nothing of its next row in flight.
   constexpr int kVecs = cpg::kInt8Vecs;
   constexpr int64_t kEach = kVecs * 16;
   if (p.cols > 2 * 512 * kEach) return launch_int8_vec<T, W, 512, kVecs, false>(p, st);
