@@ -1,10 +1,10 @@
 """Build recipe for the sm_100a shared library (``libcpgemm.so``), built in-tree.
 
-The library holds the C ABI of ``include/cpgemm.h`` in two translation units, compiled side by
-side: ``csrc/capi.cu`` (the tcgen05 GEMM kernels, the FP8 quantiser and the scheduler/FastDivmod
-device helpers) and ``csrc/capi_moe.cu`` (the INT8 quantiser and the operators around the experts'
-products).  It links the CUDA runtime
-statically and reaches ``cuTensorMapEncodeTiled`` through the runtime's driver entry-point
+The library holds the C ABI of ``include/cpgemm.h`` in three translation units, compiled side
+by side: ``csrc/capi.cu`` (the tcgen05 GEMM kernels, the FP8 quantiser and the scheduler/FastDivmod
+device helpers), ``csrc/capi_moe.cu`` (the INT8 quantiser and the operators around the experts'
+products) and ``csrc/capi_attention.cu`` (norm and rotation of heads, linear attention).  It links
+the CUDA runtime statically and reaches ``cuTensorMapEncodeTiled`` through the runtime's driver entry-point
 query, so it needs no link against ``libcuda``.
 """
 import os
@@ -19,7 +19,7 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libcpgemm.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
-SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "capi_moe.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "capi_moe.cu", "capi_attention.cu")]
 # Every source and header of csrc/ and the public header: a change to any of them rebuilds.
 DEPENDS = SOURCES + sorted(
     os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))

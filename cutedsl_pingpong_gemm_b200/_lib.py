@@ -51,7 +51,7 @@ CPG_ACT_GELU_TANH = 4
 ACTIVATIONS = {None: CPG_ACT_NONE, "none": CPG_ACT_NONE, "relu": CPG_ACT_RELU,
                "silu": CPG_ACT_SILU, "gelu": CPG_ACT_GELU, "gelu_tanh": CPG_ACT_GELU_TANH}
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 
 class CpgError(RuntimeError):
@@ -125,6 +125,26 @@ class RouteConfigC(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+CPG_HEAD_MAX_CHANNELS = 256
+CPG_LINEAR_MAX_CHANNELS = 128
+
+
+class HeadsC(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+class LinearProblemC(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("sequences", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("dk", ctypes.c_int32), ("dv", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class StatesC(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("places", ctypes.c_int64)]
+
+
 CPG_MAX_PEERS = 8
 
 
@@ -143,6 +163,8 @@ _P = ctypes.POINTER
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
+_H = _P(HeadsC)
+_S = _P(StatesC)
 
 # name -> (restype, argtypes).  Must list every function declared in include/cpgemm.h.
 SIGNATURES = {
@@ -181,6 +203,20 @@ SIGNATURES = {
     "cpg_combine_rows_backward": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64,
                                                  _vp, _vp, _i32, _vp, _i64, _vp, _vp]),
     "cpg_clear_unnamed_rows": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "cpg_norm_rope": (ctypes.c_int, [_H, _H, _i64, _i32, _vp, _vp, _i32, ctypes.c_float, _vp, _i64,
+                                     _i64, _i32, _vp, _i32, _H, _H, _vp]),
+    "cpg_norm_rope_backward": (ctypes.c_int, [_H, _H, _H, _H, _i64, _i32, _vp, _vp, _i32,
+                                              ctypes.c_float, _vp, _i64, _i64, _i32, _vp, _i32, _H,
+                                              _H, _vp, _vp, _vp, _i64, _vp]),
+    "cpg_norm_rope_workspace": (ctypes.c_int, [_i64, _i32, _i32, _i32, _P(_i64)]),
+    "cpg_linear_attention": (ctypes.c_int, [_P(LinearProblemC), _H, _H, _H, _vp, _vp, _S, _S, _H,
+                                            _vp, _i64, _vp]),
+    "cpg_linear_attention_backward": (ctypes.c_int, [_P(LinearProblemC), _H, _H, _H, _H, _vp, _vp,
+                                                     _S, _S, _H, _H, _H, _S, _i32, _vp, _i64, _vp]),
+    "cpg_linear_attention_workspace": (ctypes.c_int, [_P(LinearProblemC), _i32, _i32, _i32, _i32,
+                                                      _P(_i64)]),
+    "cpg_linear_attention_step": (ctypes.c_int, [_P(LinearProblemC), _H, _H, _H, _vp, _S, _H,
+                                                 _vp]),
     "cpg_cast_f32_bf16": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "cpg_gemm_splitk_static": (ctypes.c_int, [_P(GemmConfigC), _P(GemmProblemC), _vp, _vp, _vp,
                                               _P(EpilogueC), _vp]),

@@ -1,5 +1,7 @@
 """Checks of tensor arguments and the call into the C ABI on the current stream, shared by the
-operators that allocate their outputs (``quant``, ``moe``)."""
+operators that allocate their outputs (``quant``, ``moe``, ``attention``)."""
+import ctypes
+
 import torch
 
 from . import _lib
@@ -73,6 +75,42 @@ def pairs(name, t):
         raise error(_lib.CPG_ERR_INVALID_SHAPE,
                     f"{name}: at most {_lib.CPG_ROUTE_MAX_K} choices, got {size[1]}")
     return size
+
+
+def heads(name, t, device=None, tokens=None, channels=None):
+    """Heads [T, H, d] with unit channel stride: T, H, d and the C description."""
+    if t is None:
+        raise error(_lib.CPG_ERR_NULL, f"{name} must be given")
+    if not t.is_cuda:
+        raise error(_lib.CPG_ERR_NO_DEVICE, f"{name} must be a CUDA tensor")
+    size = t.shape
+    if (len(size) != 3 or (tokens is not None and size[0] != tokens)
+            or (channels is not None and size[2] != channels)):
+        raise error(_lib.CPG_ERR_INVALID_SHAPE,
+                    f"{name} must be [{'T' if tokens is None else tokens}, heads, "
+                    f"{'channels' if channels is None else channels}], got {tuple(size)}")
+    if size[1] >= 1 << 31 or size[2] >= 1 << 31:  # ctypes would wrap it
+        raise error(_lib.CPG_ERR_INVALID_SHAPE, f"{name} is {tuple(size)}")
+    step = t.stride()
+    if step[2] != 1 and size[2] > 1 and size[0] > 0:
+        raise error(_lib.CPG_ERR_UNSUPPORTED, f"{name} must have unit channel stride")
+    if device is not None and t.device != device:
+        raise other_device(name, t, device)
+    code = FLOAT_CODES.get(t.dtype, -1)
+    return size[0], size[1], size[2], ctypes.byref(
+        _lib.HeadsC(t.data_ptr() or None, step[0], step[1], size[1], code))
+
+
+def same_heads(name, t, shape, dtype, device):
+    """C description of heads of this shape and type."""
+    if t is None:
+        raise error(_lib.CPG_ERR_NULL, f"{name} must be given")
+    if t.dtype != dtype:
+        raise error(_lib.CPG_ERR_DTYPE, f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise error(_lib.CPG_ERR_INVALID_SHAPE,
+                    f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    return heads(name, t, device)[3]
 
 
 def ptr(t):

@@ -381,7 +381,7 @@ struct cpg_gemm {
 
 extern "C" {
 
-int cpg_abi_version(void) { return 16; }
+int cpg_abi_version(void) { return 17; }
 
 const char* cpg_strerror(int code) {
   switch (code) {

@@ -1,0 +1,601 @@
+// C ABI of the operators between a layer's projections: norm and rotation of query and key heads,
+// linear attention with a decay per head, and their gradients (include/cpgemm.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+#include <type_traits>
+
+#include "capi_common.h"
+#include "capi_launch.h"
+#include "cpgemm.h"
+#include "head_norm.cuh"
+#include "linear_attention.cuh"
+
+using cpg_capi::bytes_of;
+using cpg_capi::fail;
+using cpg_capi::float_dtype;
+using cpg_capi::launch;
+using cpg_capi::misaligned;
+
+namespace {
+
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxStride = int64_t(1) << 40;
+
+// Heads [tokens, heads, channels] with elements aligned to `bytes`; `written`: no two overlap.
+int check_heads(const char* name, const cpg_heads* x, int64_t tokens, int64_t channels, int bytes,
+                bool written) {
+  if (x == nullptr) return fail(CPG_ERR_NULL, "%s is NULL", name);
+  if (!float_dtype(x->dtype)) return fail(CPG_ERR_DTYPE, "%s must be BF16 or FP32", name);
+  if (x->heads < 1) return fail(CPG_ERR_INVALID_SHAPE, "%s has %d heads", name, x->heads);
+  if (tokens == 0) return CPG_OK;
+  if (x->ptr == nullptr) return fail(CPG_ERR_NULL, "%s is NULL", name);
+  const int64_t ts = tokens > 1 ? x->token_stride : 0, hs = x->heads > 1 ? x->head_stride : 0;
+  if (ts < 0 || hs < 0 || ts > kMaxStride || hs > kMaxStride)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: token stride %lld, head stride %lld", name,
+                static_cast<long long>(ts), static_cast<long long>(hs));
+  const int eb = bytes_of(x->dtype);
+  if (misaligned(x->ptr, bytes) || (ts * eb) % bytes != 0 || (hs * eb) % bytes != 0)
+    return fail(CPG_ERR_ALIGNMENT, "%s: address and strides must be multiples of %d bytes", name,
+                bytes);
+  if (!written) return CPG_OK;
+  const bool heads_inside = (x->heads < 2 || hs >= channels) &&
+                            (tokens < 2 || ts >= (x->heads - 1) * hs + channels);
+  const bool tokens_inside = (tokens < 2 || ts >= channels) &&
+                             (x->heads < 2 || hs >= (tokens - 1) * ts + channels);
+  if (!heads_inside && !tokens_inside)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: heads overlap (token stride %lld, head stride %lld)",
+                name, static_cast<long long>(ts), static_cast<long long>(hs));
+  return CPG_OK;
+}
+
+// ------------------------------------------------------------------------- norm and rotation
+constexpr int kGradBlocks = 148 * 4;  // of both parts together
+
+// Address bits that some head of x has set (of the lowest ones).
+uint64_t address_bits(const cpg_heads* x, int64_t tokens) {
+  const int eb = bytes_of(x->dtype);
+  return reinterpret_cast<uintptr_t>(x->ptr) |
+         (tokens > 1 ? static_cast<uint64_t>(x->token_stride * eb) : 0u) |
+         (x->heads > 1 ? static_cast<uint64_t>(x->head_stride * eb) : 0u);
+}
+
+struct NormRope {
+  const cpg_heads *q, *k, *q_out, *k_out, *dq, *dk;  // dq, dk: gradient only
+  int64_t tokens;
+  int32_t channels;
+  const void *wq, *wk;
+  int32_t dtype_w;
+  float eps;
+  const float* table;
+  int64_t table_rows, table_ld;
+  int32_t rotary;
+  const int32_t* positions;
+  int32_t interleaved;
+};
+
+int check_norm_sizes(int64_t tokens, int64_t heads, int32_t channels) {
+  if (tokens < 0 || heads < 1 || heads > kMaxRows || tokens > kMaxRows ||
+      tokens * heads > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE, "%lld tokens x %lld heads: at most 2^31 - 1 rows",
+                static_cast<long long>(tokens), static_cast<long long>(heads));
+  if (channels < 2 || channels > CPG_HEAD_MAX_CHANNELS)
+    return fail(CPG_ERR_INVALID_SHAPE, "2 <= channels <= %d, got %d", CPG_HEAD_MAX_CHANNELS,
+                channels);
+  return CPG_OK;
+}
+
+int check_norm_rope(const NormRope& n, bool back) {
+  if (n.q == nullptr || n.q_out == nullptr || (back && n.dq == nullptr))
+    return fail(CPG_ERR_NULL, "q and its outputs must be non-NULL");
+  if ((n.k == nullptr) != (n.k_out == nullptr) || (back && (n.k == nullptr) != (n.dk == nullptr)))
+    return fail(CPG_ERR_NULL, "k, its outputs and its gradient go together");
+  const int64_t heads = int64_t(n.q->heads) + (n.k != nullptr ? n.k->heads : 0);
+  int rc = check_norm_sizes(n.tokens, heads, n.channels);
+  if (rc != CPG_OK) return rc;
+  if (n.rotary < 0 || n.rotary > n.channels || n.rotary % 2 != 0)
+    return fail(CPG_ERR_INVALID_SHAPE, "rotary %d of %d channels: even, at most all", n.rotary,
+                n.channels);
+  if (!float_dtype(n.dtype_w)) return fail(CPG_ERR_DTYPE, "weights must be BF16 or FP32");
+  if (!(n.eps >= 0.f) || std::isinf(n.eps))
+    return fail(CPG_ERR_INVALID_CONFIG, "eps must be finite and not negative");
+  for (int i = 0; i < 2; ++i) {
+    const cpg_heads* x = i == 0 ? n.q : n.k;
+    const cpg_heads* y = i == 0 ? n.q_out : n.k_out;
+    const cpg_heads* dy = i == 0 ? n.dq : n.dk;
+    if (x == nullptr) continue;
+    if (!float_dtype(x->dtype)) return fail(CPG_ERR_DTYPE, "q and k must be BF16 or FP32");
+    const int eb = bytes_of(x->dtype);
+    rc = check_heads(i == 0 ? "q" : "k", x, n.tokens, n.channels, eb, false);
+    if (rc == CPG_OK)
+      rc = check_heads(i == 0 ? "q's output" : "k's output", y, n.tokens, n.channels, eb, true);
+    if (rc == CPG_OK && back)
+      rc = check_heads(i == 0 ? "dq" : "dk", dy, n.tokens, n.channels, eb, false);
+    if (rc != CPG_OK) return rc;
+    if (x->dtype != n.q->dtype || y->dtype != n.q->dtype || (back && dy->dtype != n.q->dtype))
+      return fail(CPG_ERR_DTYPE, "q, k, their outputs and gradients have one type");
+    if (y->heads != x->heads || (back && dy->heads != x->heads))
+      return fail(CPG_ERR_INVALID_SHAPE, "%s's output or gradient has another number of heads",
+                  i == 0 ? "q" : "k");
+  }
+  if (n.tokens == 0) return CPG_OK;
+  if (n.positions == nullptr || (n.rotary > 0 && n.table == nullptr))
+    return fail(CPG_ERR_NULL, "table and positions must be non-NULL");
+  if (n.table_rows < 0 || n.table_rows > kMaxRows || n.table_ld < n.rotary ||
+      n.table_ld > kMaxStride)
+    return fail(CPG_ERR_INVALID_SHAPE, "table: %lld rows of stride %lld",
+                static_cast<long long>(n.table_rows), static_cast<long long>(n.table_ld));
+  if (misaligned(n.positions, 4) || misaligned(n.table, 4) ||
+      misaligned(n.wq, bytes_of(n.dtype_w)) || misaligned(n.wk, bytes_of(n.dtype_w)))
+    return fail(CPG_ERR_ALIGNMENT,
+                "table, positions and weights must be aligned to their elements");
+  return CPG_OK;
+}
+
+cpg::HeadParams head_params(const NormRope& n) {
+  cpg::HeadParams p = {};
+  for (int i = 0; i < 2; ++i) {
+    const cpg_heads* x = i == 0 ? n.q : n.k;
+    const cpg_heads* y = i == 0 ? n.q_out : n.k_out;
+    const cpg_heads* dy = i == 0 ? n.dq : n.dk;
+    if (x == nullptr) continue;
+    cpg::HeadPart& h = p.part[i];
+    h.x = x->ptr;
+    h.x_token = x->token_stride;
+    h.x_head = x->head_stride;
+    h.y = y->ptr;
+    h.y_token = y->token_stride;
+    h.y_head = y->head_stride;
+    if (dy != nullptr) {
+      h.dy = dy->ptr;
+      h.dy_token = dy->token_stride;
+      h.dy_head = dy->head_stride;
+    }
+    h.w = i == 0 ? n.wq : n.wk;
+    h.w_f32 = n.dtype_w == CPG_DTYPE_F32 ? 1 : 0;
+    h.heads = x->heads;
+  }
+  p.table = n.table;
+  p.table_rows = n.table_rows;
+  p.table_ld = n.table_ld;
+  p.positions = n.positions;
+  p.tokens = n.tokens;
+  p.d = n.channels;
+  p.half = n.rotary / 2;
+  p.interleaved = n.interleaved != 0 ? 1 : 0;
+  p.table_vec = !misaligned(n.table, 16) && n.table_ld % 4 == 0 && p.half % 4 == 0 ? 1 : 0;
+  p.eps = n.eps;
+  return p;
+}
+
+// Elements of the widest vector that every head starts on and that the turned channels, each half
+// of them and the others divide into.
+int head_vector(const NormRope& n) {
+  uint64_t bits = 16;
+  for (const cpg_heads* x : {n.q, n.k, n.q_out, n.k_out, n.dq, n.dk})
+    if (x != nullptr) bits |= address_bits(x, n.tokens);
+  const int eb = bytes_of(n.q->dtype);
+  const int turned = n.interleaved ? n.rotary : n.rotary / 2;
+  const uint64_t sizes =
+      static_cast<uint64_t>(n.channels * eb) | static_cast<uint64_t>(turned * eb);
+  bits |= sizes;
+  return static_cast<int>(bits & (~bits + 1)) / eb;
+}
+
+// f(type, vector, lanes, pairs a lane) for the sizes at hand: the fewest lanes that hold a head.
+template <typename T, int V, typename F>
+int by_lanes(const NormRope& n, F&& f) {
+  using std::integral_constant;
+  const int vectors = n.channels / V;
+  int pairs = (vectors + 1) / 2;
+  if (!(n.interleaved && V > 1)) {
+    const int turned = n.rotary / 2 / V;
+    pairs = turned + (vectors - 2 * turned + 1) / 2;
+  }
+  const integral_constant<int, V> v;
+  const integral_constant<int, 1> one;
+  if (pairs <= 4) return f(T{}, v, integral_constant<int, 4>{}, one);
+  if (pairs <= 8) return f(T{}, v, integral_constant<int, 8>{}, one);
+  if (pairs <= 16) return f(T{}, v, integral_constant<int, 16>{}, one);
+  const integral_constant<int, 32> warp;
+  // At most kHeadMaxChannels / V / 2 pairs: V = 8 has 16, V = 4 32, V = 2 64, V = 1 128.
+  if constexpr (V <= 4) {
+    if (pairs <= 32) return f(T{}, v, warp, one);
+  }
+  if constexpr (V <= 2) {
+    if (pairs <= 64) return f(T{}, v, warp, integral_constant<int, 2>{});
+  }
+  if constexpr (V == 1) {
+    if (pairs <= 128) return f(T{}, v, warp, integral_constant<int, 4>{});
+  }
+  return fail(CPG_ERR_UNSUPPORTED, "%d channels", n.channels);
+}
+
+template <typename F>
+int by_head(const NormRope& n, F&& f) {
+  const int v = head_vector(n);
+  if (n.q->dtype == CPG_DTYPE_BF16) {
+    using B = __nv_bfloat16;
+    if (v == 8) return by_lanes<B, 8>(n, f);
+    if (v == 4) return by_lanes<B, 4>(n, f);
+    if (v == 2) return by_lanes<B, 2>(n, f);
+    return by_lanes<B, 1>(n, f);
+  }
+  if (v == 4) return by_lanes<float, 4>(n, f);
+  if (v == 2) return by_lanes<float, 2>(n, f);
+  return by_lanes<float, 1>(n, f);
+}
+
+// Blocks of each part in the gradient, in proportion to their heads and at most one per row.
+void grad_blocks(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t* blocks) {
+  const int64_t heads = int64_t(q_heads) + k_heads;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t h = i == 0 ? q_heads : k_heads;
+    blocks[i] = h == 0 ? 0
+                       : static_cast<int32_t>(std::max<int64_t>(
+                             1, std::min<int64_t>(tokens * h, kGradBlocks * h / heads)));
+  }
+}
+
+// ---------------------------------------------------------------------------- linear attention
+int check_linear(const cpg_linear_problem* p) {
+  if (p == nullptr) return fail(CPG_ERR_NULL, "the problem is NULL");
+  if (p->tokens < 0 || p->tokens > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE, "%lld tokens", static_cast<long long>(p->tokens));
+  if (p->sequences < 0 || p->heads < 1 || int64_t(p->sequences) * p->heads > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE, "%d sequences x %d heads", p->sequences, p->heads);
+  if (p->dk < 8 || p->dk > CPG_LINEAR_MAX_CHANNELS || p->dk % 8 != 0 || p->dv < 8 ||
+      p->dv > CPG_LINEAR_MAX_CHANNELS || p->dv % 8 != 0)
+    return fail(CPG_ERR_INVALID_SHAPE,
+                "dk = %d, dv = %d must be multiples of 8 from 8 to %d", p->dk, p->dv,
+                CPG_LINEAR_MAX_CHANNELS);
+  if (!std::isfinite(p->scale) || p->scale == 0.f)
+    return fail(CPG_ERR_INVALID_CONFIG, "scale must be finite and not 0");
+  return CPG_OK;
+}
+
+int check_operand(const char* name, const cpg_linear_problem* p, const cpg_heads* x, int32_t d,
+                  bool written, bool f32_too = false) {
+  if (x == nullptr) return fail(CPG_ERR_NULL, "%s is NULL", name);
+  if (x->dtype != CPG_DTYPE_BF16 && !(f32_too && x->dtype == CPG_DTYPE_F32))
+    return fail(CPG_ERR_DTYPE, "%s must be BF16%s", name, f32_too ? " or FP32" : "");
+  const int rc = check_heads(name, x, p->tokens, d, 16, written);
+  if (rc != CPG_OK) return rc;
+  if (p->heads % x->heads != 0)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: %d heads do not divide %d", name, x->heads, p->heads);
+  return CPG_OK;
+}
+
+int check_states(const char* name, const cpg_linear_problem* p, const cpg_states* s) {
+  if (s == nullptr) return CPG_OK;
+  if (s->places < 0 || s->places > kMaxRows)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: %lld places", name, static_cast<long long>(s->places));
+  if (s->slots == nullptr && s->places < p->sequences)
+    return fail(CPG_ERR_INVALID_SHAPE, "%s: %lld places for %d sequences", name,
+                static_cast<long long>(s->places), p->sequences);
+  if (s->ptr == nullptr && s->places > 0) return fail(CPG_ERR_NULL, "%s is NULL", name);
+  if (misaligned(s->ptr, 16) || misaligned(s->slots, 4))
+    return fail(CPG_ERR_ALIGNMENT, "%s must start on 16 bytes, its slots on 4", name);
+  return CPG_OK;
+}
+
+int check_sequences(const cpg_linear_problem* p, const float* log_decay, const int32_t* offsets) {
+  if (log_decay == nullptr) return fail(CPG_ERR_NULL, "log_decay is NULL");
+  if (offsets == nullptr && p->sequences != 1)
+    return fail(CPG_ERR_NULL, "%d sequences need offsets", p->sequences);
+  if (misaligned(log_decay, 4) || misaligned(offsets, 4))
+    return fail(CPG_ERR_ALIGNMENT, "log_decay and offsets must be aligned to their elements");
+  return CPG_OK;
+}
+
+cpg::LinearRows linear_rows(const cpg_linear_problem* p, const cpg_heads* x) {
+  return {static_cast<const __nv_bfloat16*>(x->ptr), x->token_stride, x->head_stride,
+          p->heads / x->heads};
+}
+
+cpg::LinearParams linear_params(const cpg_linear_problem* p, const cpg_heads* a,
+                                const cpg_heads* b, const cpg_heads* c, int32_t da, int32_t dc,
+                                const cpg_heads* o, const float* log_decay,
+                                const int32_t* offsets) {
+  cpg::LinearParams r = {};
+  r.a = linear_rows(p, a);
+  r.b = linear_rows(p, b);
+  r.c = linear_rows(p, c);
+  r.o = o->ptr;
+  r.o_token = o->token_stride;
+  r.o_head = o->head_stride;
+  r.o_f32 = o->dtype == CPG_DTYPE_F32 ? 1 : 0;
+  r.log_decay = log_decay;
+  r.offsets = offsets;
+  r.tokens = p->tokens;
+  r.sequences = p->sequences;
+  r.heads = p->heads;
+  r.da = da;
+  r.dc = dc;
+  r.scale = p->scale;
+  r.state_factor = r.final_factor = 1.f;
+  return r;
+}
+
+void set_state(cpg::LinearParams* r, const cpg_states* s, bool transposed, float factor) {
+  if (s == nullptr) return;
+  r->state = s->ptr;
+  r->state_slots = s->slots;
+  r->state_places = s->places;
+  r->state_transposed = transposed ? 1 : 0;
+  r->state_factor = factor;
+}
+
+void set_final(cpg::LinearParams* r, const cpg_states* s, float factor) {
+  if (s == nullptr) return;
+  r->final = s->ptr;
+  r->final_slots = s->slots;
+  r->final_places = s->places;
+  r->final_factor = factor;
+}
+
+int run_pass(const cpg::LinearParams& r, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(r.sequences) * static_cast<unsigned>(r.heads);
+  if (grid == 0) return CPG_OK;
+  auto fn = r.da > 64 ? &cpg::linear_tokens_kernel<128> : &cpg::linear_tokens_kernel<64>;
+  return launch("linear attention kernel", true, fn, grid, cpg::kLinearMaxChannels, 0, st, 1, r);
+}
+
+// FP32 sums of a head each, of the widest shared gradient.
+int64_t share_bytes(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
+                    int32_t v_heads) {
+  int64_t d = 0;
+  if (q_heads < p->heads || k_heads < p->heads) d = p->dk;
+  if (v_heads < p->heads) d = std::max<int64_t>(d, p->dv);
+  return p->tokens * p->heads * d * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cpg_norm_rope(const cpg_heads* q, const cpg_heads* k, int64_t tokens, int32_t channels,
+                  const void* q_weight, const void* k_weight, int32_t dtype_w, float eps,
+                  const float* table, int64_t table_rows, int64_t table_ld, int32_t rotary,
+                  const int32_t* positions, int32_t interleaved, const cpg_heads* q_out,
+                  const cpg_heads* k_out, void* stream) {
+  const NormRope n{q,        k,        q_out, k_out, nullptr,    nullptr,  tokens, channels,
+                   q_weight, k_weight, dtype_w, eps, table,      table_rows, table_ld, rotary,
+                   positions, interleaved};
+  const int rc = check_norm_rope(n, false);
+  if (rc != CPG_OK || tokens == 0) return rc;
+  const cpg::HeadParams p = head_params(n);
+  const int64_t rows = tokens * (int64_t(p.part[0].heads) + p.part[1].heads);
+  return by_head(n, [&](auto type, auto v, auto lanes, auto pairs) {
+    constexpr int kRows = cpg::kHeadThreads / decltype(lanes)::value;
+    return launch("head norm kernel", true,
+                  &cpg::head_norm_kernel<decltype(type), decltype(v)::value,
+                                         decltype(lanes)::value, decltype(pairs)::value>,
+                  static_cast<unsigned>((rows + kRows - 1) / kRows), cpg::kHeadThreads, 0,
+                  static_cast<cudaStream_t>(stream), 1, p);
+  });
+}
+
+int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t channels,
+                            int64_t* bytes) {
+  if (bytes == nullptr) return fail(CPG_ERR_NULL, "bytes is NULL");
+  if (q_heads < 1 || k_heads < 0)
+    return fail(CPG_ERR_INVALID_SHAPE, "%d query and %d key heads", q_heads, k_heads);
+  const int rc = check_norm_sizes(tokens, int64_t(q_heads) + k_heads, channels);
+  if (rc != CPG_OK) return rc;
+  int32_t blocks[2];
+  grad_blocks(tokens, q_heads, k_heads, blocks);
+  *bytes = (int64_t(blocks[0]) + blocks[1]) * channels * 4;
+  return CPG_OK;
+}
+
+int cpg_norm_rope_backward(const cpg_heads* dq, const cpg_heads* dk, const cpg_heads* q,
+                           const cpg_heads* k, int64_t tokens, int32_t channels,
+                           const void* q_weight, const void* k_weight, int32_t dtype_w, float eps,
+                           const float* table, int64_t table_rows, int64_t table_ld,
+                           int32_t rotary, const int32_t* positions, int32_t interleaved,
+                           const cpg_heads* dq_in, const cpg_heads* dk_in, float* dq_weight,
+                           float* dk_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+  const NormRope n{q,        k,        dq_in,   dk_in, dq,    dk,         tokens,   channels,
+                   q_weight, k_weight, dtype_w, eps,   table, table_rows, table_ld, rotary,
+                   positions, interleaved};
+  int rc = check_norm_rope(n, true);
+  if (rc != CPG_OK) return rc;
+  if (misaligned(dq_weight, 4) || misaligned(dk_weight, 4) || misaligned(workspace, 16))
+    return fail(CPG_ERR_ALIGNMENT, "weight gradients must be aligned to 4 bytes, workspace to 16");
+  if (dk_weight != nullptr && k == nullptr)
+    return fail(CPG_ERR_NULL, "the gradient of k's weight needs k");
+  cpg::HeadParams p = head_params(n);
+  grad_blocks(tokens, p.part[0].heads, p.part[1].heads, p.blocks);
+  int64_t bytes = 0;
+  rc = cpg_norm_rope_workspace(tokens, p.part[0].heads, p.part[1].heads, channels, &bytes);
+  if (rc != CPG_OK) return rc;
+  if (tokens > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(CPG_ERR_NULL, "the workspace must have %lld bytes", static_cast<long long>(bytes));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  p.partial = static_cast<float*>(workspace);
+  if (tokens > 0) {
+    rc = by_head(n, [&](auto type, auto v, auto lanes, auto pairs) {
+      return launch("head norm gradient kernel", true,
+                    &cpg::head_norm_grad_kernel<decltype(type), decltype(v)::value,
+                                                decltype(lanes)::value, decltype(pairs)::value>,
+                    static_cast<unsigned>(p.blocks[0] + p.blocks[1]), cpg::kHeadThreads, 0, st, 1,
+                    p);
+    });
+    if (rc != CPG_OK) return rc;
+  }
+  if (dq_weight == nullptr && dk_weight == nullptr) return CPG_OK;
+  const unsigned grid = static_cast<unsigned>((2 * channels + 7) / 8);
+  return launch("head norm sum kernel", true, &cpg::head_norm_sum_kernel, grid,
+                cpg::kHeadThreads, 0, st, 1, static_cast<const float*>(p.partial),
+                tokens > 0 ? p.blocks[0] : 0, tokens > 0 ? p.blocks[1] : 0, channels, dq_weight,
+                dk_weight);
+}
+
+int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
+                                   int32_t v_heads, int32_t backward, int64_t* bytes) {
+  if (bytes == nullptr) return fail(CPG_ERR_NULL, "bytes is NULL");
+  const int rc = check_linear(p);
+  if (rc != CPG_OK) return rc;
+  if (q_heads < 1 || k_heads < 1 || v_heads < 1)
+    return fail(CPG_ERR_INVALID_SHAPE, "%d, %d and %d heads", q_heads, k_heads, v_heads);
+  *bytes = backward ? share_bytes(p, q_heads, k_heads, v_heads) : 0;
+  return CPG_OK;
+}
+
+int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,
+                         const cpg_heads* v, const float* log_decay, const int32_t* offsets,
+                         const cpg_states* state, const cpg_states* final, const cpg_heads* out,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_linear(p);
+  if (rc == CPG_OK) rc = check_operand("q", p, q, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("k", p, k, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("v", p, v, p->dv, false);
+  if (rc == CPG_OK) rc = check_operand("out", p, out, p->dv, true, true);
+  if (rc == CPG_OK) rc = check_sequences(p, log_decay, offsets);
+  if (rc == CPG_OK) rc = check_states("state", p, state);
+  if (rc == CPG_OK) rc = check_states("final", p, final);
+  if (rc != CPG_OK) return rc;
+  if (out->heads != p->heads)
+    return fail(CPG_ERR_INVALID_SHAPE, "out has %d heads, not %d", out->heads, p->heads);
+  int64_t bytes = 0;
+  rc = cpg_linear_attention_workspace(p, q->heads, k->heads, v->heads, 0, &bytes);
+  if (rc != CPG_OK) return rc;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(CPG_ERR_NULL, "the workspace must have %lld bytes", static_cast<long long>(bytes));
+  if (misaligned(workspace, 16))
+    return fail(CPG_ERR_ALIGNMENT, "the workspace must start on 16 bytes");
+  cpg::LinearParams r = linear_params(p, q, k, v, p->dk, p->dv, out, log_decay, offsets);
+  set_state(&r, state, false, 1.f);
+  set_final(&r, final, 1.f);
+  return run_pass(r, static_cast<cudaStream_t>(stream));
+}
+
+int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* dy,
+                                  const cpg_heads* q, const cpg_heads* k, const cpg_heads* v,
+                                  const float* log_decay, const int32_t* offsets,
+                                  const cpg_states* state, const cpg_states* dfinal,
+                                  const cpg_heads* dq, const cpg_heads* dk, const cpg_heads* dv,
+                                  const cpg_states* dstate, int32_t clear, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  int rc = check_linear(p);
+  if (rc == CPG_OK) rc = check_operand("dy", p, dy, p->dv, false);
+  if (rc == CPG_OK) rc = check_operand("q", p, q, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("k", p, k, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("v", p, v, p->dv, false);
+  if (rc == CPG_OK) rc = check_operand("dq", p, dq, p->dk, true);
+  if (rc == CPG_OK) rc = check_operand("dk", p, dk, p->dk, true);
+  if (rc == CPG_OK) rc = check_operand("dv", p, dv, p->dv, true);
+  if (rc == CPG_OK) rc = check_sequences(p, log_decay, offsets);
+  if (rc == CPG_OK) rc = check_states("state", p, state);
+  if (rc == CPG_OK) rc = check_states("dfinal", p, dfinal);
+  if (rc == CPG_OK) rc = check_states("dstate", p, dstate);
+  if (rc != CPG_OK) return rc;
+  if (dy->heads != p->heads || dq->heads != q->heads || dk->heads != k->heads ||
+      dv->heads != v->heads)
+    return fail(CPG_ERR_INVALID_SHAPE, "dy has %d heads, gradients those of q, k and v", p->heads);
+  int64_t bytes = 0;
+  rc = cpg_linear_attention_workspace(p, q->heads, k->heads, v->heads, 1, &bytes);
+  if (rc != CPG_OK) return rc;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(CPG_ERR_NULL, "the workspace must have %lld bytes", static_cast<long long>(bytes));
+  if (misaligned(workspace, 16))
+    return fail(CPG_ERR_ALIGNMENT, "the workspace must start on 16 bytes");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // The gradient of a head that several read: each one's in FP32, then their sum.
+  auto pass = [&](const cpg_heads* a, const cpg_heads* b, const cpg_heads* c, int32_t da,
+                  int32_t dc, const cpg_heads* o, bool reverse, const cpg_states* from,
+                  bool transposed, float factor, const cpg_states* to) {
+    const cpg_heads sums{workspace, int64_t(p->heads) * dc, dc, p->heads, CPG_DTYPE_F32};
+    const bool shared = o->heads < p->heads;
+    cpg::LinearParams r =
+        linear_params(p, a, b, c, da, dc, shared ? &sums : o, log_decay, offsets);
+    r.reverse = reverse ? 1 : 0;
+    set_state(&r, from, transposed, factor);
+    set_final(&r, to, p->scale);
+    int e = run_pass(r, st);
+    if (e != CPG_OK || !shared || p->tokens == 0) return e;
+    const cpg::LinearShareParams s{static_cast<const float*>(workspace),
+                                   static_cast<__nv_bfloat16*>(o->ptr),
+                                   o->token_stride,
+                                   o->head_stride,
+                                   p->tokens,
+                                   o->heads,
+                                   p->heads / o->heads,
+                                   dc,
+                                   offsets,
+                                   p->sequences};
+    const int64_t n = p->tokens * o->heads * dc;
+    return launch("shared gradient kernel", true, &cpg::linear_share_kernel,
+                  static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 148 * 8)), 256, 0, st,
+                  1, s);
+  };
+  rc = pass(dy, v, k, p->dv, p->dk, dq, false, state, true, 1.f, nullptr);
+  if (rc == CPG_OK)
+    rc = pass(v, dy, q, p->dv, p->dk, dk, true, dfinal, true, 1.f / p->scale, nullptr);
+  if (rc == CPG_OK)
+    rc = pass(k, q, dy, p->dk, p->dv, dv, true, dfinal, false, 1.f / p->scale, dstate);
+  if (rc != CPG_OK || clear == 0 || offsets == nullptr || p->tokens == 0) return rc;
+  cpg::LinearClearParams c = {};
+  const cpg_heads* grads[3] = {dq, dk, dv};
+  for (int i = 0; i < 3; ++i) {
+    c.p[i] = static_cast<__nv_bfloat16*>(grads[i]->ptr);
+    c.token[i] = grads[i]->token_stride;
+    c.head[i] = grads[i]->head_stride;
+    c.heads[i] = grads[i]->heads;
+    c.d[i] = i < 2 ? p->dk : p->dv;
+  }
+  c.offsets = offsets;
+  c.tokens = p->tokens;
+  c.sequences = p->sequences;
+  return launch("clear kernel", true, &cpg::linear_clear_kernel,
+                static_cast<unsigned>(std::min<int64_t>(p->tokens, 148)), 256, 0, st, 1, c);
+}
+
+int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,
+                              const cpg_heads* v, const float* log_decay, const cpg_states* state,
+                              const cpg_heads* out, void* stream) {
+  int rc = check_linear(p);
+  if (rc == CPG_OK && p->tokens * p->heads > kMaxRows)
+    rc = fail(CPG_ERR_INVALID_SHAPE, "%lld tokens x %d heads", static_cast<long long>(p->tokens),
+              p->heads);
+  if (rc == CPG_OK) rc = check_operand("q", p, q, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("k", p, k, p->dk, false);
+  if (rc == CPG_OK) rc = check_operand("v", p, v, p->dv, false);
+  if (rc == CPG_OK) rc = check_operand("out", p, out, p->dv, true, true);
+  if (rc != CPG_OK) return rc;
+  if (log_decay == nullptr || state == nullptr)
+    return fail(CPG_ERR_NULL, "log_decay and state must be non-NULL");
+  if (misaligned(log_decay, 4)) return fail(CPG_ERR_ALIGNMENT, "log_decay must be aligned");
+  cpg_linear_problem one = *p;
+  one.sequences = static_cast<int32_t>(p->tokens);
+  rc = check_states("state", &one, state);
+  if (rc != CPG_OK) return rc;
+  if (out->heads != p->heads)
+    return fail(CPG_ERR_INVALID_SHAPE, "out has %d heads, not %d", out->heads, p->heads);
+  if (p->tokens == 0) return CPG_OK;
+  const cpg::LinearStepParams r{linear_rows(p, q),
+                                linear_rows(p, k),
+                                linear_rows(p, v),
+                                out->ptr,
+                                out->token_stride,
+                                out->head_stride,
+                                out->dtype == CPG_DTYPE_F32 ? 1 : 0,
+                                log_decay,
+                                state->ptr,
+                                state->slots,
+                                state->places,
+                                static_cast<int32_t>(p->tokens),
+                                p->heads,
+                                p->dk,
+                                p->dv,
+                                p->scale};
+  return launch("linear attention step kernel", true, &cpg::linear_step_kernel,
+                static_cast<unsigned>(p->tokens * p->heads), cpg::kStepThreads, 0,
+                static_cast<cudaStream_t>(stream), 1, r);
+}
+
+}  // extern "C"

@@ -8,12 +8,17 @@
 #include <type_traits>
 
 #include "capi_common.h"
+#include "capi_launch.h"
 #include "cpgemm.h"
 #include "expert_route.cuh"
 #include "expert_rows.cuh"
 
+using cpg_capi::bytes_of;
 using cpg_capi::cuda_fail;
 using cpg_capi::fail;
+using cpg_capi::float_dtype;
+using cpg_capi::launch;
+using cpg_capi::misaligned;
 
 namespace {
 
@@ -21,13 +26,6 @@ constexpr int64_t kRouteBlocks = 148 * 8;
 constexpr int64_t kFewThreads = 148 * 1024;  // half of the threads that fit on the SMs
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;  // rows and pairs are counted in int32
 constexpr int64_t kMaxCols = int64_t(1) << 30;         // the kernels' column arithmetic is 32-bit
-
-bool float_dtype(int32_t dtype) { return dtype == CPG_DTYPE_BF16 || dtype == CPG_DTYPE_F32; }
-int bytes_of(int32_t dtype) { return dtype == CPG_DTYPE_F32 ? 4 : (dtype == CPG_DTYPE_I8 ? 1 : 2); }
-
-bool misaligned(const void* p, int bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) != 0;
-}
 
 unsigned row_grid(int64_t rows) { return static_cast<unsigned>(std::min<int64_t>(rows, kMaxRows)); }
 
@@ -48,39 +46,6 @@ int check_pairs(int64_t tokens, int32_t k) {
                 "%lld tokens x %d choices: 1 <= k <= %d and at most 2^31 - 1 pairs",
                 static_cast<long long>(tokens), k, CPG_ROUTE_MAX_K);
   return CPG_OK;
-}
-
-// Launches a kernel, `early` as a programmatic dependent of the stream's previous kernel: it may be
-// set up while that one finishes and waits for it before its first access (kernel_begins).
-// Measured in a captured chain of route, dispatch and combine of 16 tokens: 12.0 us plain, 10.6 us
-// early; letting the next kernel in from the start of each as well: 11.2 us, since its blocks wait
-// on the SMs the first still needs.  The INT8 row kernels are not launched early but do let the next
-// kernel in: quantise + small-M product of 64 x 8192 x 8192 takes 24.8 us with neither, 25.1 us with
-// both and 23.2 us so (16 rows: 22.1, 20.1 and 20.4 us).
-template <typename... P>
-int launch(const char* what, bool early, void (*kernel)(P...), unsigned grid, unsigned threads,
-           size_t smem, cudaStream_t st, int cluster, P... args) {
-  cudaLaunchConfig_t lc = {};
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (early) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[n].val.clusterDim.y = 1;
-    attr[n++].val.clusterDim.z = 1;
-  }
-  lc.gridDim = dim3(grid, 1, 1);
-  lc.blockDim = dim3(threads, 1, 1);
-  lc.dynamicSmemBytes = smem;
-  lc.stream = st;
-  lc.attrs = attr;
-  lc.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&lc, kernel, args...);
-  return e == cudaSuccess ? CPG_OK : cuda_fail(e, what);
 }
 
 // A matrix whose rows' alignment selects a kernel.  The stride of a single row is not used.

@@ -1,0 +1,248 @@
+// Linear attention with one decay per head over packed sequences.
+//
+// One kernel computes, for every sequence and head, in the order of its tokens or against it,
+//   S_t = e^g S_{t-1} + b_t c_t^T,    o_t = scale * S_t^T a_t
+// and with it both directions of training: the forward pass is (a, b, c) = (q, k, v), and with do
+// the gradient of o,
+//   dq = pass(do, v, k),   dk = reversed pass(v, do, q),   dv = reversed pass(k, q, do).
+// In a reversed pass the state that arrives from behind is the gradient of the state after a token:
+// it is used by that token without another decay (forward: the state before it, decayed once).
+#pragma once
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "row_access.cuh"
+
+namespace cpg {
+
+constexpr int kLinearMaxChannels = 128;
+
+struct LinearRows {
+  const __nv_bfloat16* p;
+  int64_t token, head;  // strides in elements
+  int32_t share;        // heads of the decay that read one head of this
+};
+
+struct LinearParams {
+  LinearRows a, b, c;
+  void* o;
+  int64_t o_token, o_head;
+  int32_t o_f32;
+  const float* log_decay;
+  const int32_t* offsets;  // null: one sequence of all tokens
+  int64_t tokens;
+  int32_t sequences, heads;
+  int32_t da, dc;          // channels of a and b, of c and o
+  float scale;
+  int32_t reverse;
+  const float* state;      // [places, heads, da, dc] (transposed: [.., dc, da]); null: zeros
+  const int32_t* state_slots;
+  int64_t state_places;
+  int32_t state_transposed;
+  float state_factor;
+  float* final;            // [places, heads, da, dc]; may be state
+  const int32_t* final_slots;
+  int64_t final_places;
+  float final_factor;
+};
+
+struct LinearSpan {
+  int64_t first;
+  int64_t count;
+};
+
+// Tokens of sequence s; whatever the offsets hold, they lie within the tensors.
+__device__ __forceinline__ LinearSpan linear_span(const int32_t* offsets, int32_t s,
+                                                  int64_t tokens) {
+  if (offsets == nullptr) return {0, tokens};
+  const int64_t a = min(max(static_cast<int64_t>(offsets[s]), int64_t(0)), tokens);
+  const int64_t b = min(max(static_cast<int64_t>(offsets[s + 1]), a), tokens);
+  return {a, b - a};
+}
+
+// Place of sequence s in a pool of states, -1 if it has none.
+__device__ __forceinline__ int64_t linear_place(const int32_t* slots, int32_t s, int64_t places) {
+  const int64_t at = slots == nullptr ? s : slots[s];
+  return at >= 0 && at < places ? at : -1;
+}
+
+// One block per sequence and head, one thread per channel of c, token by token.
+template <int DA>
+__global__ void __launch_bounds__(kLinearMaxChannels) linear_tokens_kernel(const LinearParams p) {
+  kernel_begins();
+  __shared__ float sa[DA], sb[DA];
+  const int32_t s = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int32_t x = threadIdx.x;
+  const LinearSpan span = linear_span(p.offsets, s, p.tokens);
+  const float lambda = expf(p.log_decay[h]);
+  float state[DA];
+  const int64_t from = p.state == nullptr ? -1 : linear_place(p.state_slots, s, p.state_places);
+  const int64_t size = static_cast<int64_t>(p.da) * p.dc;
+#pragma unroll
+  for (int i = 0; i < DA; ++i) {
+    state[i] = 0.f;
+    if (from >= 0 && i < p.da && x < p.dc)
+      state[i] = p.state_factor * p.state[(from * p.heads + h) * size +
+                                          (p.state_transposed ? x * p.da + i : i * p.dc + x)];
+  }
+  for (int64_t n = 0; n < span.count; ++n) {
+    const int64_t t = span.first + (p.reverse ? span.count - 1 - n : n);
+    __syncthreads();
+    if (x < DA) {
+      sa[x] = x < p.da ? __bfloat162float(p.a.p[t * p.a.token + h / p.a.share * p.a.head + x]) : 0.f;
+      sb[x] = x < p.da ? __bfloat162float(p.b.p[t * p.b.token + h / p.b.share * p.b.head + x]) : 0.f;
+    }
+    const float c =
+        x < p.dc ? __bfloat162float(p.c.p[t * p.c.token + h / p.c.share * p.c.head + x]) : 0.f;
+    __syncthreads();
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < DA; ++i) {
+      if (!p.reverse) state[i] *= lambda;
+      state[i] = fmaf(sb[i], c, state[i]);
+      o = fmaf(sa[i], state[i], o);
+      if (p.reverse) state[i] *= lambda;
+    }
+    if (x < p.dc) {
+      const int64_t at = t * p.o_token + h * p.o_head + x;
+      if (p.o_f32)
+        static_cast<float*>(p.o)[at] = p.scale * o;
+      else
+        static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(p.scale * o);
+    }
+  }
+  const int64_t to = p.final == nullptr ? -1 : linear_place(p.final_slots, s, p.final_places);
+  if (to >= 0 && x < p.dc)
+#pragma unroll
+    for (int i = 0; i < DA; ++i)
+      if (i < p.da) p.final[(to * p.heads + h) * size + i * p.dc + x] = p.final_factor * state[i];
+}
+
+// Rows of a [tokens, heads, d] outside the sequences, set to zero.
+struct LinearClearParams {
+  __nv_bfloat16* p[3];
+  int64_t token[3], head[3];
+  int32_t heads[3], d[3];
+  const int32_t* offsets;
+  int64_t tokens;
+  int32_t sequences;
+};
+
+__global__ void __launch_bounds__(256) linear_clear_kernel(const LinearClearParams p) {
+  kernel_begins();
+  const int64_t first = min(max(static_cast<int64_t>(p.offsets[0]), int64_t(0)), p.tokens);
+  const int64_t last =
+      min(max(static_cast<int64_t>(p.offsets[p.sequences]), first), p.tokens);
+  const int64_t rows = first + p.tokens - last;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int64_t t = r < first ? r : last + r - first;
+#pragma unroll
+    for (int n = 0; n < 3; ++n)
+      for (int32_t i = threadIdx.x; i < p.heads[n] * p.d[n]; i += blockDim.x)
+        p.p[n][t * p.token[n] + i / p.d[n] * p.head[n] + i % p.d[n]] = __float2bfloat16_rn(0.f);
+  }
+}
+
+// The gradient of shared heads: the sums over the heads that read one, rounded once.
+struct LinearShareParams {
+  const float* partial;  // [tokens, heads * share, d]
+  __nv_bfloat16* out;
+  int64_t token, head;
+  int64_t tokens;
+  int32_t heads, share, d;
+  const int32_t* offsets;
+  int32_t sequences;
+};
+
+__global__ void __launch_bounds__(256) linear_share_kernel(const LinearShareParams p) {
+  kernel_begins();
+  int64_t first = 0, last = p.tokens;
+  if (p.offsets != nullptr) {
+    first = min(max(static_cast<int64_t>(p.offsets[0]), int64_t(0)), p.tokens);
+    last = min(max(static_cast<int64_t>(p.offsets[p.sequences]), first), p.tokens);
+  }
+  const int32_t row = p.heads * p.d;
+  const int64_t n = (last - first) * row;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += gridDim.x * int64_t(256)) {
+    const int64_t t = first + i / row;
+    const int32_t h = static_cast<int32_t>(i % row) / p.d, x = static_cast<int32_t>(i % row) % p.d;
+    const float* from = p.partial + (t * p.heads + h) * int64_t(p.share) * p.d + x;
+    float s = 0.f;
+    for (int32_t j = 0; j < p.share; ++j) s += from[static_cast<int64_t>(j) * p.d];
+    p.out[t * p.token + h * p.head + x] = __float2bfloat16_rn(s);
+  }
+}
+
+// One token of each of many sequences: S <- e^g S + k v^T in place, o = scale * S^T q.
+// Bound by HBM: every state is read and written once.  A block takes `cols` columns of a state;
+// a lane four neighbouring ones of every (32 * warps / lanes)-th row, whose loads are independent.
+struct LinearStepParams {
+  LinearRows q, k, v;
+  void* o;
+  int64_t o_token, o_head;
+  int32_t o_f32;
+  const float* log_decay;
+  float* state;  // [places, heads, dk, dv]
+  const int32_t* slots;
+  int64_t places;
+  int32_t batch, heads, dk, dv;
+  float scale;
+};
+
+constexpr int kStepThreads = 256;
+
+__global__ void __launch_bounds__(kStepThreads) linear_step_kernel(const LinearStepParams p) {
+  kernel_begins();
+  __shared__ float4 sums[kStepThreads];
+  const int32_t i = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int32_t groups = p.dv / 4;             // lanes across a row
+  const int32_t rows = kStepThreads / groups;  // rows at a time
+  const int32_t x = threadIdx.x % groups, y = threadIdx.x / groups;
+  const int64_t at = linear_place(p.slots, i, p.places);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (at >= 0 && y < rows) {
+    const float lambda = expf(p.log_decay[h]);
+    float4* s = reinterpret_cast<float4*>(p.state + (at * p.heads + h) * int64_t(p.dk) * p.dv) + x;
+    const __nv_bfloat16* q = p.q.p + i * p.q.token + h / p.q.share * p.q.head;
+    const __nv_bfloat16* k = p.k.p + i * p.k.token + h / p.k.share * p.k.head;
+    const __nv_bfloat16* vp = p.v.p + i * p.v.token + h / p.v.share * p.v.head + 4 * x;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __bfloat162float(vp[j]);
+    for (int32_t r = y; r < p.dk; r += rows) {
+      float4 f = s[r * groups];
+      const float kr = __bfloat162float(k[r]), qr = __bfloat162float(q[r]);
+      f.x = fmaf(kr, v[0], lambda * f.x);
+      f.y = fmaf(kr, v[1], lambda * f.y);
+      f.z = fmaf(kr, v[2], lambda * f.z);
+      f.w = fmaf(kr, v[3], lambda * f.w);
+      s[r * groups] = f;
+      o.x = fmaf(qr, f.x, o.x);
+      o.y = fmaf(qr, f.y, o.y);
+      o.z = fmaf(qr, f.z, o.z);
+      o.w = fmaf(qr, f.w, o.w);
+    }
+  }
+  sums[threadIdx.x] = o;
+  __syncthreads();
+  if (threadIdx.x >= groups) return;
+  o = sums[threadIdx.x];
+  for (int32_t r = 1; r < rows; ++r) {
+    const float4 f = sums[r * groups + threadIdx.x];
+    o.x += f.x;
+    o.y += f.y;
+    o.z += f.z;
+    o.w += f.w;
+  }
+  const int64_t to = i * p.o_token + h * p.o_head + 4 * x;
+  const float f[4] = {p.scale * o.x, p.scale * o.y, p.scale * o.z, p.scale * o.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.o_f32)
+      static_cast<float*>(p.o)[to + j] = f[j];
+    else
+      static_cast<__nv_bfloat16*>(p.o)[to + j] = __float2bfloat16_rn(f[j]);
+  }
+}
+
+}  // namespace cpg

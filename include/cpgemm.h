@@ -385,6 +385,99 @@ int cpg_combine_rows_backward(const void* dy, int32_t dtype, int64_t tokens, int
 int cpg_clear_unnamed_rows(void* rows, int32_t dtype, int64_t num_rows, int64_t cols, int64_t ldr,
                            const int32_t* slots, int64_t tokens, int32_t k, void* stream);
 
+/* ---- Between a layer's projections: norm and rotation of heads, linear attention ------------
+ * No counterpart in the reference.  Heads [tokens, heads, channels]: unit channel stride, any
+ * token and head stride (a fused projection's rows, for instance).  Nothing is kept between calls;
+ * all run on `stream`. */
+typedef struct cpg_heads {
+  void* ptr;
+  int64_t token_stride, head_stride; /* in elements */
+  int32_t heads;
+  int32_t dtype;                     /* CPG_DTYPE_BF16 or, where allowed, CPG_DTYPE_F32 */
+} cpg_heads;
+
+#define CPG_HEAD_MAX_CHANNELS 256
+#define CPG_LINEAR_MAX_CHANNELS 128
+
+/* y = R(x / sqrt(mean(x^2) + eps) * w) for every head of q and k (k may be NULL, and then k_out).
+ * R turns the channels i and i + rotary / 2 (interleaved: 2i and 2i + 1) of the first `rotary` by
+ * the angle i of the token's position: table FP32 [table_rows, rotary] with row stride table_ld
+ * holds the cosines of a position's angles, then their sines.  A position outside the table makes
+ * the turned channels NaN.  q_weight / k_weight: BF16 or FP32 (dtype_w) [channels], NULL for ones.
+ * q and k BF16 or FP32, 2 <= channels <= CPG_HEAD_MAX_CHANNELS, rotary even, 0 allowed.  The
+ * outputs may be the inputs. */
+int cpg_norm_rope(const cpg_heads* q, const cpg_heads* k, int64_t tokens, int32_t channels,
+                  const void* q_weight, const void* k_weight, int32_t dtype_w, float eps,
+                  const float* table, int64_t table_rows, int64_t table_ld, int32_t rotary,
+                  const int32_t* positions, int32_t interleaved, const cpg_heads* q_out,
+                  const cpg_heads* k_out, void* stream);
+
+/* Its gradient: dq_in / dk_in from dq / dk (all of q's type; dq_in may be dq), and the weights'
+ * FP32 [channels] where dq_weight / dk_weight are not NULL.  workspace: device memory of
+ * cpg_norm_rope_workspace bytes for these sizes. */
+int cpg_norm_rope_backward(const cpg_heads* dq, const cpg_heads* dk, const cpg_heads* q,
+                           const cpg_heads* k, int64_t tokens, int32_t channels,
+                           const void* q_weight, const void* k_weight, int32_t dtype_w, float eps,
+                           const float* table, int64_t table_rows, int64_t table_ld,
+                           int32_t rotary, const int32_t* positions, int32_t interleaved,
+                           const cpg_heads* dq_in, const cpg_heads* dk_in, float* dq_weight,
+                           float* dk_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t channels,
+                            int64_t* bytes);
+
+/* Linear attention with a decay per head, over sequences packed along the tokens:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t    (S [dk, dv], FP32)
+ * offsets: int32 [sequences + 1], token rows of every sequence (not decreasing; cut to the tokens
+ * there are), NULL for one sequence of all tokens.  Rows outside are neither read nor written.
+ * q, k, v BF16, their heads divide `heads` (head h reads head h / (heads / x.heads)); dk and dv
+ * multiples of 8 up to CPG_LINEAR_MAX_CHANNELS; rows and strides multiples of 16 bytes.
+ * log_decay FP32 [heads], at most 0.  scale finite and not 0. */
+typedef struct cpg_linear_problem {
+  int64_t tokens;
+  int32_t sequences;
+  int32_t heads;
+  int32_t dk, dv;
+  float scale;
+} cpg_linear_problem;
+
+/* States FP32 [places, heads, dk, dv], contiguous; sequence s is at place slots[s] (NULL: s, and
+ * places = sequences).  A slot outside [0, places) has no state: it starts from zeros and its final
+ * state is not written.  No two sequences may share a place that is written. */
+typedef struct cpg_states {
+  float* ptr;
+  const int32_t* slots;
+  int64_t places;
+} cpg_states;
+
+/* state: where every sequence starts (NULL: zeros); final: gets the state after its last token
+ * (NULL: not wanted; may be the same places as state).  out BF16 or FP32 [tokens, heads, dv].
+ * workspace: cpg_linear_attention_workspace bytes, 16-byte aligned; may be NULL if that is 0. */
+int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,
+                         const cpg_heads* v, const float* log_decay, const int32_t* offsets,
+                         const cpg_states* state, const cpg_states* final, const cpg_heads* out,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of q, k and v (BF16, summed in FP32 over the heads that share one) from dy, the
+ * gradient of out (BF16 [tokens, heads, dv]), and dfinal, that of the final states (NULL: zeros);
+ * dstate (NULL: not wanted) gets that of the starting states.  clear != 0: rows outside the
+ * sequences are set to zero, else left as they were. */
+int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* dy,
+                                  const cpg_heads* q, const cpg_heads* k, const cpg_heads* v,
+                                  const float* log_decay, const int32_t* offsets,
+                                  const cpg_states* state, const cpg_states* dfinal,
+                                  const cpg_heads* dq, const cpg_heads* dk, const cpg_heads* dv,
+                                  const cpg_states* dstate, int32_t clear, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
+                                   int32_t v_heads, int32_t backward, int64_t* bytes);
+
+/* One token of each of p->tokens sequences: q, k, v and out [tokens, heads, channels], the states
+ * updated in place.  Tokens whose slot is outside [0, places) are padding: their out is 0. */
+int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,
+                              const cpg_heads* v, const float* log_decay, const cpg_states* state,
+                              const cpg_heads* out, void* stream);
+
 /* y = bf16(x + bias) for x FP32 [rows, cols]: the last step of split-K after the reduction.
  * bias is optional (BF16, length cols). */
 int cpg_cast_f32_bf16(const float* x, int64_t rows, int64_t cols, int64_t ldx, void* y,
