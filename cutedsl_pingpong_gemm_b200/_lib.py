@@ -215,6 +215,7 @@ SIGNATURES = {
                                                      _S, _S, _H, _H, _H, _S, _i32, _vp, _i64, _vp]),
     "cpg_linear_attention_workspace": (ctypes.c_int, [_P(LinearProblemC), _i32, _i32, _i32, _i32,
                                                       _P(_i64)]),
+    "cpg_attention_status": (ctypes.c_int, [_P(_i32)]),
     "cpg_linear_attention_step": (ctypes.c_int, [_P(LinearProblemC), _H, _H, _H, _vp, _S, _H,
                                                  _vp]),
     "cpg_cast_f32_bf16": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),

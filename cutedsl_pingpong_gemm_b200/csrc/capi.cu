@@ -2,7 +2,6 @@
 // constructor asserts), problem checks, kernel selection, tensor-map encoding and launch.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cstdlib>
@@ -10,6 +9,7 @@
 #include <mutex>
 
 #include "capi_common.h"
+#include "capi_launch.h"
 #include "cpgemm.h"
 #include "gemm_decode.cuh"
 #include "gemm_fp8_block.cuh"
@@ -18,6 +18,7 @@
 #include "quant_kernels.cuh"
 
 using cpg_capi::cuda_fail;
+using cpg_capi::encode_fn;
 using cpg_capi::fail;
 using cpg_capi::g_last_error;
 
@@ -37,21 +38,6 @@ struct DeviceGuard {
     if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
   }
 };
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
-                                         &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
-  });
-  return fn;
-}
 
 // 3-D tiled tensor map (columns, rows, batches) with a box of box_rows x box_cols x 1, 128-byte
 // swizzled unless told otherwise.  An unbatched operand has one batch; its batch stride is then

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <mutex>
 #include <type_traits>
 
 #include "capi_common.h"
@@ -12,8 +13,11 @@
 #include "cpgemm.h"
 #include "head_norm.cuh"
 #include "linear_attention.cuh"
+#include "linear_chunks.cuh"
 
 using cpg_capi::bytes_of;
+using cpg_capi::cuda_fail;
+using cpg_capi::encode_fn;
 using cpg_capi::fail;
 using cpg_capi::float_dtype;
 using cpg_capi::launch;
@@ -22,7 +26,7 @@ using cpg_capi::misaligned;
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
-constexpr int64_t kMaxStride = int64_t(1) << 40;
+constexpr int64_t kMaxStride = int64_t(1) << 38;  // elements; tensor maps take 2^40 bytes
 
 // Heads [tokens, heads, channels] with elements aligned to `bytes`; `written`: no two overlap.
 int check_heads(const char* name, const cpg_heads* x, int64_t tokens, int64_t channels, int bytes,
@@ -265,6 +269,8 @@ int check_operand(const char* name, const cpg_linear_problem* p, const cpg_heads
   if (rc != CPG_OK) return rc;
   if (p->heads % x->heads != 0)
     return fail(CPG_ERR_INVALID_SHAPE, "%s: %d heads do not divide %d", name, x->heads, p->heads);
+  if ((p->tokens > 1 && x->token_stride == 0) || (x->heads > 1 && x->head_stride == 0))
+    return fail(CPG_ERR_UNSUPPORTED, "%s: a stride of 0 (give a shared head once)", name);
   return CPG_OK;
 }
 
@@ -336,11 +342,96 @@ void set_final(cpg::LinearParams* r, const cpg_states* s, float factor) {
   r->final_factor = factor;
 }
 
-int run_pass(const cpg::LinearParams& r, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(r.sequences) * static_cast<unsigned>(r.heads);
-  if (grid == 0) return CPG_OK;
-  auto fn = r.da > 64 ? &cpg::linear_tokens_kernel<128> : &cpg::linear_tokens_kernel<64>;
-  return launch("linear attention kernel", true, fn, grid, cpg::kLinearMaxChannels, 0, st, 1, r);
+// Tiles of 128 tokens x 64 channels of one head; channels and tokens past the end read as zeros.
+int encode_heads(CUtensorMap* m, const cpg::LinearRows& x, int64_t tokens, int32_t heads,
+                 int32_t d) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(CPG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int64_t any = d;  // the stride of a single head or token is not used
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(2 * (heads > 1 ? x.head : any)),
+                           static_cast<cuuint64_t>(2 * (tokens > 1 ? x.token : any))};
+  cuuint32_t box[3] = {64, 1, cpg::kChunk};
+  cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r =
+      fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(x.p), dims, strides,
+         box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(CPG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): %lld tokens x %d heads x %d",
+                static_cast<int>(r), static_cast<long long>(tokens), heads, d);
+  return CPG_OK;
+}
+
+constexpr uint64_t kTimeoutNs = 10000000000ull;
+
+// SMs of the current device; also raises the shared-memory limit of the chunk kernels there, once.
+int device_ready(int* sms) {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static int known[kDevices];
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (dev < 0 || dev >= kDevices) return fail(CPG_ERR_NO_DEVICE, "device %d", dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (known[dev] == 0) {
+    int n = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
+    auto raise = [&](auto kernel, uint32_t bytes) {
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(bytes));
+    };
+    auto both = [&](auto da, auto dc) {
+      constexpr int kDA = decltype(da)::value, kDC = decltype(dc)::value;
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, false>, cpg::ChunkLayout<kDA, kDC>::kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, true>, cpg::ChunkLayout<kDA, kDC>::kBytes);
+    };
+    const std::integral_constant<int, 64> d64;
+    const std::integral_constant<int, 128> d128;
+    both(d64, d64);
+    both(d64, d128);
+    both(d128, d64);
+    both(d128, d128);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(linear attention)");
+    known[dev] = n;
+  }
+  *sms = known[dev];
+  return CPG_OK;
+}
+
+template <int DA, int DC>
+int run_chunks(const cpg::LinearParams& r, bool reverse, int sms, cudaStream_t st) {
+  CUtensorMap maps[3] = {};
+  const cpg::LinearRows* x[3] = {&r.a, &r.b, &r.c};
+  for (int i = 0; i < 3 && r.tokens > 0; ++i) {
+    const int rc =
+        encode_heads(&maps[i], *x[i], r.tokens, r.heads / x[i]->share, i < 2 ? r.da : r.dc);
+    if (rc != CPG_OK) return rc;
+  }
+  const int64_t units = int64_t(r.sequences) * r.heads;
+  auto fn = reverse ? &cpg::linear_chunks_kernel<DA, DC, true>
+                    : &cpg::linear_chunks_kernel<DA, DC, false>;
+  return launch("linear attention kernel", true, fn,
+                static_cast<unsigned>(std::min<int64_t>(units, sms)), cpg::kChunkThreads,
+                cpg::ChunkLayout<DA, DC>::kBytes, st, 1, maps[0], maps[1], maps[2], r);
+}
+
+int run_pass(cpg::LinearParams r, bool reverse, cudaStream_t st) {
+  if (r.sequences == 0) return CPG_OK;
+  int sms = 0;
+  const int rc = device_ready(&sms);
+  if (rc != CPG_OK) return rc;
+  r.exact = r.final != nullptr ? 1 : 0;
+  r.timeout_ns = kTimeoutNs;
+  if (r.da > 64)
+    return r.dc > 64 ? run_chunks<128, 128>(r, reverse, sms, st)
+                     : run_chunks<128, 64>(r, reverse, sms, st);
+  return r.dc > 64 ? run_chunks<64, 128>(r, reverse, sms, st)
+                   : run_chunks<64, 64>(r, reverse, sms, st);
 }
 
 // FP32 sums of a head each, of the widest shared gradient.
@@ -471,7 +562,7 @@ int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const 
   cpg::LinearParams r = linear_params(p, q, k, v, p->dk, p->dv, out, log_decay, offsets);
   set_state(&r, state, false, 1.f);
   set_final(&r, final, 1.f);
-  return run_pass(r, static_cast<cudaStream_t>(stream));
+  return run_pass(r, false, static_cast<cudaStream_t>(stream));
 }
 
 int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* dy,
@@ -513,10 +604,9 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
     const bool shared = o->heads < p->heads;
     cpg::LinearParams r =
         linear_params(p, a, b, c, da, dc, shared ? &sums : o, log_decay, offsets);
-    r.reverse = reverse ? 1 : 0;
     set_state(&r, from, transposed, factor);
     set_final(&r, to, p->scale);
-    int e = run_pass(r, st);
+    int e = run_pass(r, reverse, st);
     if (e != CPG_OK || !shared || p->tokens == 0) return e;
     const cpg::LinearShareParams s{static_cast<const float*>(workspace),
                                    static_cast<__nv_bfloat16*>(o->ptr),
@@ -553,6 +643,12 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
   c.sequences = p->sequences;
   return launch("clear kernel", true, &cpg::linear_clear_kernel,
                 static_cast<unsigned>(std::min<int64_t>(p->tokens, 148)), 256, 0, st, 1, c);
+}
+
+int cpg_attention_status(int32_t* status) {
+  if (status == nullptr) return fail(CPG_ERR_NULL, "status is NULL");
+  const cudaError_t e = cudaMemcpyFromSymbol(status, cpg::linear_status_word, sizeof(*status));
+  return e == cudaSuccess ? CPG_OK : cuda_fail(e, "cudaMemcpyFromSymbol");
 }
 
 int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,

@@ -1,7 +1,11 @@
-// Launches and small checks shared by the translation units whose operators keep no plan.
+// Launches, small checks and the tensor-map encoder, shared by the translation units.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <mutex>
 
 #include "capi_common.h"
 
@@ -12,6 +16,21 @@ inline int bytes_of(int32_t dtype) { return dtype == CPG_DTYPE_F32 ? 4 : (dtype 
 
 inline bool misaligned(const void* p, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) != 0;
+}
+
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+  });
+  return fn;
 }
 
 // Launches a kernel, `early` as a programmatic dependent of the stream's previous kernel: it may be

@@ -34,7 +34,6 @@ struct LinearParams {
   int32_t sequences, heads;
   int32_t da, dc;          // channels of a and b, of c and o
   float scale;
-  int32_t reverse;
   const float* state;      // [places, heads, da, dc] (transposed: [.., dc, da]); null: zeros
   const int32_t* state_slots;
   int64_t state_places;
@@ -44,6 +43,8 @@ struct LinearParams {
   const int32_t* final_slots;
   int64_t final_places;
   float final_factor;
+  int32_t exact;           // states to FP32 accuracy (they are outputs)
+  uint64_t timeout_ns;     // limit of a wait within the kernel
 };
 
 struct LinearSpan {
@@ -64,58 +65,6 @@ __device__ __forceinline__ LinearSpan linear_span(const int32_t* offsets, int32_
 __device__ __forceinline__ int64_t linear_place(const int32_t* slots, int32_t s, int64_t places) {
   const int64_t at = slots == nullptr ? s : slots[s];
   return at >= 0 && at < places ? at : -1;
-}
-
-// One block per sequence and head, one thread per channel of c, token by token.
-template <int DA>
-__global__ void __launch_bounds__(kLinearMaxChannels) linear_tokens_kernel(const LinearParams p) {
-  kernel_begins();
-  __shared__ float sa[DA], sb[DA];
-  const int32_t s = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
-  const int32_t x = threadIdx.x;
-  const LinearSpan span = linear_span(p.offsets, s, p.tokens);
-  const float lambda = expf(p.log_decay[h]);
-  float state[DA];
-  const int64_t from = p.state == nullptr ? -1 : linear_place(p.state_slots, s, p.state_places);
-  const int64_t size = static_cast<int64_t>(p.da) * p.dc;
-#pragma unroll
-  for (int i = 0; i < DA; ++i) {
-    state[i] = 0.f;
-    if (from >= 0 && i < p.da && x < p.dc)
-      state[i] = p.state_factor * p.state[(from * p.heads + h) * size +
-                                          (p.state_transposed ? x * p.da + i : i * p.dc + x)];
-  }
-  for (int64_t n = 0; n < span.count; ++n) {
-    const int64_t t = span.first + (p.reverse ? span.count - 1 - n : n);
-    __syncthreads();
-    if (x < DA) {
-      sa[x] = x < p.da ? __bfloat162float(p.a.p[t * p.a.token + h / p.a.share * p.a.head + x]) : 0.f;
-      sb[x] = x < p.da ? __bfloat162float(p.b.p[t * p.b.token + h / p.b.share * p.b.head + x]) : 0.f;
-    }
-    const float c =
-        x < p.dc ? __bfloat162float(p.c.p[t * p.c.token + h / p.c.share * p.c.head + x]) : 0.f;
-    __syncthreads();
-    float o = 0.f;
-#pragma unroll
-    for (int i = 0; i < DA; ++i) {
-      if (!p.reverse) state[i] *= lambda;
-      state[i] = fmaf(sb[i], c, state[i]);
-      o = fmaf(sa[i], state[i], o);
-      if (p.reverse) state[i] *= lambda;
-    }
-    if (x < p.dc) {
-      const int64_t at = t * p.o_token + h * p.o_head + x;
-      if (p.o_f32)
-        static_cast<float*>(p.o)[at] = p.scale * o;
-      else
-        static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(p.scale * o);
-    }
-  }
-  const int64_t to = p.final == nullptr ? -1 : linear_place(p.final_slots, s, p.final_places);
-  if (to >= 0 && x < p.dc)
-#pragma unroll
-    for (int i = 0; i < DA; ++i)
-      if (i < p.da) p.final[(to * p.heads + h) * size + i * p.dc + x] = p.final_factor * state[i];
 }
 
 // Rows of a [tokens, heads, d] outside the sequences, set to zero.

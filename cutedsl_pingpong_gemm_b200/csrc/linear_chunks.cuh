@@ -1,0 +1,895 @@
+// Linear attention by chunks of 128 tokens on the tensor cores (see linear_attention.cuh for what a
+// pass computes).  Within a chunk, with i and j its tokens, w the decays between them and S the state
+// before it,
+//   scores = A B^T,   P = scores . w (0 where j is later than i),
+//   O = scale * (P C + e^(g (i + 1)) (A S)),   S <- e^(g 128) S + (left . B)^T C
+// (left: the decay from a token to the chunk's end).  Four products of 128 x 128 x 128 per chunk of
+// four 32 KiB tiles read or written: 128 flop per byte, so HBM is the bound as long as the products of a
+// chunk, which depend on one another, take less time than its tiles: 3.0 us when 148 blocks share the
+// measured bandwidth.
+//
+// One block per SM walks (sequence, head) pairs with 768 threads:
+//   warp 0       TMA producer: tiles of A, B and C, 128 tokens x 64 channels a box, 128-byte swizzle.
+//   warp 1       MMA issuer.  TMEM, 128 columns each: scores and P, A S, P C, and the state in FP32.
+//   warps 2-3    infinities and NaN in C (below).
+//   warps 4-7    scores -> P (BF16, back into TMEM as the A operand of P C).
+//   warps 8-15   the output.
+//   warps 16-19  the state: its BF16 copy in shared memory for A S, and its decay in TMEM.
+//   warps 20-23  left . B.
+// Roundings: P and the copy of S are BF16, as operands have to be; the state itself stays FP32.  left . B
+// is split into BF16 parts whose sum it is to 2^-17 (two products), or, where the state is an output
+// (`exact`), to 2^-25 (three), so that a state keeps FP32 accuracy.
+// An infinity or NaN in C would spoil its channel in all of the chunk's outputs, the earlier ones too
+// (0 times it is NaN).  It is replaced by 0, and its channel is NaN from its token on in what is
+// written.
+#pragma once
+#include "linear_attention.cuh"
+#include "ptx.cuh"
+
+namespace cpg {
+
+constexpr int kChunk = 128;
+constexpr int kChunkThreads = 768;
+
+// Wait sites (low byte of the status word).
+enum : int32_t {
+  kSiteLinearProducer = 0x60,
+  kSiteLinearMma = 0x61,
+  kSiteLinearScores = 0x62,
+  kSiteLinearState = 0x63,
+  kSiteLinearOutput = 0x64,
+  kSiteLinearLeft = 0x65,
+  kSiteLinearScan = 0x66,
+  kSiteLinearDrain = 0x67,
+};
+
+constexpr uint64_t kLinearDrainNs = 100000000;
+
+// First error of any launch on this device (0: none).
+__device__ int32_t linear_status_word;
+
+template <int DA, int DC>
+struct ChunkLayout {
+  static constexpr uint32_t kTileA = kChunk * DA * 2;  // also of B and its parts
+  static constexpr uint32_t kTileC = kChunk * DC * 2;
+  static constexpr uint32_t kTileS = DA * DC * 2;
+  static constexpr uint32_t kA = 0;
+  static constexpr uint32_t kB = kA + kTileA;          // 2 slots
+  static constexpr uint32_t kMid = kB + 2 * kTileA;    // second part of left . B
+  static constexpr uint32_t kC = kMid + kTileA;        // 2 slots
+  // Third part: a tile of its own, or where there is no room for one C's second slot, so that C has
+  // one then.  (The state's product takes 128 rows of a part even where B has 64 channels: its second
+  // 64, rows of the result that nothing reads, are whatever lies one box further on, in the next
+  // tile.)
+  static constexpr bool kShared = DA == 128 && DC == 128;
+  static constexpr uint32_t kLo = kShared ? kC + kTileC : kC + 2 * kTileC;
+  static constexpr uint32_t kS = kLo + kTileA;
+  static constexpr uint32_t kBars = kS + (kTileS > 16384u ? kTileS : 16384u);
+  static constexpr uint32_t kNumBars = 20;
+  static constexpr uint32_t kSlot = kBars + kNumBars * 8;
+  static constexpr uint32_t kPowers = kSlot + 16;      // 64 for each warp of the scores
+  static_assert(kPowers % 16 == 0, "read four at a time");
+  static constexpr uint32_t kBad = kPowers + 4 * 256;  // of every channel of C, the last of all, progress
+  static constexpr uint32_t kBytes = kBad + kChunk * 4 + 64 + 1024;
+  static_assert(kBytes <= 232448, "shared memory of a block");
+};
+
+// TMEM columns.
+constexpr uint32_t kColScores = 0, kColInter = 128, kColIntra = 256, kColState = 384;
+
+// Instruction descriptor of kind::f16 with BF16 operands, FP32 accumulators; a set bit: the operand's
+// rows run along the reduction (its M or N channels are contiguous).
+__host__ __device__ constexpr uint32_t linear_idesc(int n, bool a_mn, bool b_mn) {
+  return ptx::make_idesc_bf16_f32(128, n) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// Low halves of shared-memory descriptors (the high half is the GEMM kernels': rows of 128 bytes,
+// 128-byte swizzle, 8-row groups 1024 bytes apart).  For an operand whose rows run along the
+// reduction the leading offset is that from one box of 64 channels to the next.
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t addr, uint32_t box_bytes) {
+  return ((addr >> 4) & 0x3FFFu) | (box_bytes >> 4) << 16;
+}
+
+// Step k of 16 channels in an operand along its channels (in units of 16 bytes).
+__device__ __forceinline__ uint32_t k_step(uint32_t k) { return (k >> 2) * 1024 + (k & 3) * 2; }
+
+// D[tmem] (+)= A * B[smem], A in TMEM or shared memory, issued by the lane whose `issue` is set.  All
+// lanes of the warp come here together: descriptors that are the same in each can then be made in
+// uniform registers, where the instruction wants them (made by one lane of a divergent warp, they
+// took twice the time of the products).
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+                                            uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(ptx::sw128_desc_hi()), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                            uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(ptx::sw128_desc_hi()), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t bar, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// 16 lanes x 32 columns: thread t receives lanes t / 4 and t / 4 + 8, and of each 8 columns the two
+// from 2 (t % 4) on: words 4 j, 4 j + 1 of the first lane, 4 j + 2, 4 j + 3 of the second.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// Twice four words of each of four lanes: lane q gets word q of lanes 0 to 3.
+__device__ __forceinline__ void quad_transpose(uint32_t (&v)[2][4], uint32_t lane) {
+  const bool odd = lane & 1u, upper = lane & 2u;
+  uint32_t got[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      got[i][j] = __shfl_xor_sync(0xffffffffu, odd ? v[i][2 * j] : v[i][2 * j + 1], 1);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (odd) v[i][2 * j] = got[i][j];
+      else v[i][2 * j + 1] = got[i][j];
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      got[i][j] = __shfl_xor_sync(0xffffffffu, upper ? v[i][j] : v[i][j + 2], 2);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (upper) v[i][j] = got[i][j];
+      else v[i][j + 2] = got[i][j];
+    }
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(addr)
+               : "memory");
+  return r;
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// x y + z in BF16, two values a word, rounded once.
+__device__ __forceinline__ uint32_t bf16x2_fma(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
+  return r;
+}
+__device__ __forceinline__ uint32_t bf16_twice(float f) { return ptx::pack_bf16x2(f, f); }
+
+// (x0, x1) *= (y0, y1), two FP32 products an instruction.
+__device__ __forceinline__ void mul2(uint32_t& x0, uint32_t& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+r"(x0), "+r"(x1)
+      : "f"(y0), "f"(y1));
+}
+
+// (x0, x1) += f (y0, y1).
+__device__ __forceinline__ void add2(uint32_t& x0, uint32_t& x1, float f, uint32_t y0, uint32_t y1) {
+  asm("{\n\t.reg .b64 x, y, f;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "mov.b64 f, {%4, %4};\n\t"
+      "fma.rn.f32x2 x, y, f, x;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+r"(x0), "+r"(x1)
+      : "r"(y0), "r"(y1), "f"(f));
+}
+
+// Sign bits set where a half word, as BF16, is no finite number.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// e^(g n) from g / ln 2, 1 for n = 0 whatever g.
+__device__ __forceinline__ float decay_power(float g2, int32_t n) {
+  return n == 0 ? 1.f : exp2f(g2 * static_cast<float>(n));
+}
+
+// Byte offset of 16-byte piece `piece` (of 8 channels) of row r in a tile of boxes of `rows` rows.
+__device__ __forceinline__ uint32_t tile_offset(uint32_t r, uint32_t piece, uint32_t rows) {
+  return (piece >> 3) * rows * 128u + r * 128u + (((piece & 7u) ^ (r & 7u)) << 4);
+}
+
+// What a block does: (sequence, head) pairs u = blockIdx.x, + gridDim.x, ... and their chunks.
+struct LinearUnit {
+  int32_t sequence, head;
+  int64_t first, count;
+  int32_t chunks;
+  int64_t from, to;  // places of its starting and final state, -1: none
+};
+
+__device__ __forceinline__ LinearUnit linear_unit(const LinearParams& p, int32_t u) {
+  LinearUnit r;
+  r.sequence = u / p.heads;
+  r.head = u - r.sequence * p.heads;
+  const LinearSpan span = linear_span(p.offsets, r.sequence, p.tokens);
+  r.first = span.first;
+  r.count = span.count;
+  r.chunks = static_cast<int32_t>((span.count + kChunk - 1) / kChunk);
+  r.from = p.state == nullptr ? -1 : linear_place(p.state_slots, r.sequence, p.state_places);
+  r.to = p.final == nullptr ? -1 : linear_place(p.final_slots, r.sequence, p.final_places);
+  return r;
+}
+
+// The x-th chunk to be done: its first token and how many it has.
+template <bool Reverse>
+__device__ __forceinline__ int32_t chunk_at(const LinearUnit& u, int32_t x, int32_t* count) {
+  const int64_t at = static_cast<int64_t>(Reverse ? u.chunks - 1 - x : x) * kChunk;
+  const int64_t left = u.count - at;
+  *count = left < kChunk ? static_cast<int32_t>(left) : kChunk;
+  return static_cast<int32_t>(u.first + at);
+}
+
+template <int DA, int DC, bool Reverse>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    linear_chunks_kernel(const __grid_constant__ CUtensorMap tm_a,
+                         const __grid_constant__ CUtensorMap tm_b,
+                         const __grid_constant__ CUtensorMap tm_c,
+                         const __grid_constant__ LinearParams p) {
+#if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
+  using L = ChunkLayout<DA, DC>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw);
+  const uint32_t bars = base + L::kBars;
+  // One phase per chunk each; those with two entries, per chunk of the slot.
+  const uint32_t a_full = bars, a_empty = bars + 8, b_full = bars + 16, c_full = bars + 32,
+                 b_empty = bars + 48, c_empty = bars + 64, s_full = bars + 80, p_ready = bars + 88,
+                 o_full = bars + 96, o_free = bars + 104, h_ready = bars + 112,
+                 b_ready = bars + 120, h_full = bars + 128, c_ready = bars + 136,
+                 drain = bars + 152;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + L::kSlot);
+  volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(base_ptr + L::kSlot + 4);
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = ptx::lane_id();
+
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < L::kNumBars; ++i) {
+      const uint32_t bar = bars + 8 * i;
+      ptx::mbar_init(bar, bar == o_free ? 8
+                          : bar == p_ready || bar == h_ready || bar == b_ready ? 4
+                          : bar == c_ready || bar == c_ready + 8 ? 2
+                                                                 : 1);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbarrier_init_cluster();
+    ptx::fence_proxy_async_shared();
+  }
+  if (warp == 0 && lane == 0 && p.tokens > 0) {
+    ptx::prefetch_tensormap(&tm_a);
+    ptx::prefetch_tensormap(&tm_b);
+    ptx::prefetch_tensormap(&tm_c);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    ptx::tmem_relinquish<1>();
+  }
+  uint32_t* bad = reinterpret_cast<uint32_t*>(base_ptr + L::kBad);
+  volatile uint32_t* last_bad = bad + kChunk;
+  // Chunks that each warp of the output has done, and that each of the state has begun.
+  volatile uint32_t* done = bad + kChunk + 4;
+  if (threadIdx.x < kChunk + 16) bad[threadIdx.x] = 0u;
+  kernel_begins();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const ptx::WaitCtx ctx{abort_flag, &linear_status_word, p.timeout_ns};
+  const int32_t units = p.sequences * p.heads;
+  const int32_t step = static_cast<int32_t>(gridDim.x);
+  // Thread of a warpgroup: the token of the chunk, or the row of the state, that it has, and the TMEM
+  // lanes of its warp.
+  const int32_t i = static_cast<int32_t>(threadIdx.x & 127u);
+  const uint32_t lanes = tmem + ((warp & 3u) << 21);
+  uint32_t n = 0;  // chunks done
+  bool ok = true;
+  // C's slot of chunk m and the parity of its phases.
+  const bool one_c = L::kShared && p.exact;
+  auto c_slot = [&](uint32_t m) { return one_c ? 0u : m & 1u; };
+  auto c_phase = [&](uint32_t m) { return one_c ? m & 1u : (m >> 1) & 1u; };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------------------- producer
+    if (lane == 0) {
+      const uint64_t policy = ptx::policy_evict_first();
+      for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+        const LinearUnit unit = linear_unit(p, u);
+        const int32_t ha = unit.head / p.a.share, hb = unit.head / p.b.share,
+                      hc = unit.head / p.c.share;
+#pragma unroll 1
+        for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+          int32_t count;
+          const int32_t t = chunk_at<Reverse>(unit, x, &count);
+          const uint32_t slot = n & 1u;
+          const uint32_t b = base + L::kB + slot * L::kTileA;
+          const uint32_t c = base + L::kC + c_slot(n) * L::kTileC;
+          const uint32_t cf = c_full + 8 * c_slot(n);
+          if (!(ok = ptx::mbar_wait_brief(b_empty + 8 * slot, ((n >> 1) & 1u) ^ 1u, ctx,
+                                          kSiteLinearProducer)))
+            break;
+          ptx::mbar_arrive_expect_tx(b_full + 8 * slot, L::kTileA);
+          for (int j = 0; j < DA / 64; ++j)
+            ptx::tma_load_3d(&tm_b, b + j * 16384, b_full + 8 * slot, 64 * j, hb, t, policy);
+          // What waits for room below comes into L2 meanwhile.
+          for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_a, 64 * j, ha, t);
+          if (one_c)
+            for (int j = 0; j < DC / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_c, 64 * j, hc, t);
+          // C first unless its only slot is the last to become free.
+          for (int turn = 0; turn < 2 && ok; ++turn) {
+            if ((turn == 0) == one_c) {
+              if (!(ok = ptx::mbar_wait_brief(a_empty, (n & 1u) ^ 1u, ctx, kSiteLinearProducer)))
+                break;
+              ptx::mbar_arrive_expect_tx(a_full, L::kTileA);
+              for (int j = 0; j < DA / 64; ++j)
+                ptx::tma_load_3d(&tm_a, base + L::kA + j * 16384, a_full, 64 * j, ha, t, policy);
+            } else {
+              if (!(ok = ptx::mbar_wait_brief(c_empty + 8 * c_slot(n), c_phase(n) ^ 1u, ctx,
+                                              kSiteLinearProducer)))
+                break;
+              ptx::mbar_arrive_expect_tx(cf, L::kTileC);
+              for (int j = 0; j < DC / 64; ++j)
+                ptx::tma_load_3d(&tm_c, c + j * 16384, cf, 64 * j, hc, t, policy);
+            }
+          }
+          if (!ok) {
+            ++n;
+            break;
+          }
+        }
+      }
+      if (!ok) {
+        // Copies in flight land before the block ends.  (Where the waits above all succeeded, the
+        // consumers have waited for every one.)
+        volatile int32_t none = 0;
+        const ptx::WaitCtx brief{&none, nullptr, kLinearDrainNs};
+#pragma unroll 1
+        for (uint32_t j = n > 2 ? n - 2 : 0; j < n; ++j) {
+          none = 0;
+          ptx::mbar_wait_tries(b_full + 8 * (j & 1u), (j >> 1) & 1u, brief, kSiteLinearDrain);
+          none = 0;
+          ptx::mbar_wait_tries(c_full + 8 * c_slot(j), c_phase(j), brief, kSiteLinearDrain);
+          none = 0;
+          ptx::mbar_wait_tries(a_full, j & 1u, brief, kSiteLinearDrain);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------------------- MMA issuer
+    {
+      const uint32_t issue = elect_one();
+      constexpr uint32_t kScores = linear_idesc(kChunk, false, false);
+      constexpr uint32_t kInter = linear_idesc(DC, false, true);
+      constexpr uint32_t kState = linear_idesc(DC, true, true);
+      const uint32_t a_k = ptx::sw128_desc_lo(base + L::kA);  // A along its channels
+      const uint32_t s_mn = desc_lo_mn(base + L::kS, DA * 128);
+      for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+        const LinearUnit unit = linear_unit(p, u);
+        bool state = unit.from >= 0;
+#pragma unroll 1
+        for (int32_t x = 0; x < unit.chunks && ok; ++x, ++n) {
+          int32_t count;
+          chunk_at<Reverse>(unit, x, &count);
+          const uint32_t slot = n & 1u, twice = (n >> 1) & 1u, once = n & 1u;
+          const uint32_t b = base + L::kB + slot * L::kTileA;
+          const uint32_t c_mn = desc_lo_mn(base + L::kC + c_slot(n) * L::kTileC, 16384);
+          // A B^T.  Its columns hold P of the chunk before until that one's product is done.
+          if (n > 0) ok = ptx::mbar_wait_brief(o_full, once ^ 1u, ctx, kSiteLinearMma);
+          ok = ok && ptx::mbar_wait_brief(a_full, once, ctx, kSiteLinearMma) &&
+               ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearMma);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          const uint32_t b_k = ptx::sw128_desc_lo(b);
+#pragma unroll
+          for (int k = 0; k < DA / 16; ++k)
+            umma_f16_ss(tmem + kColScores, a_k + k_step(k), b_k + k_step(k), kScores, k > 0, issue);
+          umma_commit_if(s_full, issue);
+          // A S into its own columns, once the output before has been read.
+          ok = ptx::mbar_wait_brief(h_ready, once, ctx, kSiteLinearMma);
+          if (n > 0) ok = ok && ptx::mbar_wait_brief(o_free, once ^ 1u, ctx, kSiteLinearMma);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          if (state) {
+#pragma unroll
+            for (int k = 0; k < DA / 16; ++k)
+              umma_f16_ss(tmem + kColInter, a_k + k_step(k), s_mn + k * 128, kInter, k > 0, issue);
+          }
+          umma_commit_if(a_empty, issue);
+          // P C.  A partial chunk's rows of C past its end are cleared before b_ready.
+          ok = ptx::mbar_wait_brief(p_ready, once, ctx, kSiteLinearMma) &&
+               ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearMma) &&
+               ptx::mbar_wait_brief(c_ready + 8 * slot, twice, ctx, kSiteLinearMma) &&
+               (count == kChunk || ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma));
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k)
+            umma_f16_ts(tmem + kColIntra, tmem + kColScores + k * 8, c_mn + k * 128, kInter, k > 0,
+                        issue);
+          umma_commit_if(o_full, issue);
+          // The state's addend, by the parts of left . B.
+          if (!(ok = ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma))) break;
+          ptx::tc_fence_after();
+          uint32_t accumulate = state ? 1u : 0u;
+#pragma unroll 1
+          for (int j = 0; j < (p.exact ? 3 : 2); ++j) {
+            const uint32_t part =
+                desc_lo_mn(j == 0 ? b : base + (j == 1 ? L::kMid : L::kLo), 16384);
+#pragma unroll
+            for (int k = 0; k < kChunk / 16; ++k) {
+              umma_f16_ss(tmem + kColState, part + k * 128, c_mn + k * 128, kState, accumulate,
+                          issue);
+              accumulate = 1u;
+            }
+          }
+          umma_commit_if(b_empty + 8 * slot, issue);
+          umma_commit_if(c_empty + 8 * c_slot(n), issue);
+          umma_commit_if(h_full, issue);
+          state = true;
+        }
+      }
+      if (!ok) {  // products in flight end before TMEM is freed
+        volatile int32_t none = 0;
+        umma_commit_if(drain, issue);
+        ptx::mbar_wait_tries(drain, 0, {&none, nullptr, kLinearDrainNs}, kSiteLinearDrain);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ----------------------------------------------------------- infinities and NaN in a box of C
+    const uint32_t box = warp - 2;
+    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      const LinearUnit unit = linear_unit(p, u);
+      const uint32_t unit_first = n * kChunk;  // place of the unit's first token in the block's work
+#pragma unroll 1
+      for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+        int32_t count;
+        chunk_at<Reverse>(unit, x, &count);
+        const uint32_t c = base + L::kC + c_slot(n) * L::kTileC + box * 16384;
+        if (!(ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearScan)))
+          break;
+        uint32_t found = 0;
+        if (box < DC / 64) {
+#pragma unroll 1
+          for (int32_t row = static_cast<int32_t>(lane); row < count; row += 32)
+#pragma unroll
+            for (uint32_t piece = 0; piece < 8; ++piece) {
+              const uint4 v = ld_shared_v4(c + tile_offset(row, piece, kChunk));
+              found |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+            }
+        }
+        if (__any_sync(0xffffffffu, found != 0u)) {
+          // The table is the earlier chunks' outputs' and the unit before's state's until then.
+          const uint64_t t0 = ptx::globaltimer();
+          while (ok && !__all_sync(0xffffffffu, lane >= 12 || done[lane] >= n + (lane < 8 ? 0u : 1u)))
+            if (*abort_flag || ptx::globaltimer() - t0 > ctx.timeout_ns) {
+              ptx::record_timeout(ctx, kSiteLinearScan);
+              ok = false;
+            }
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          uint32_t* mine = bad + 64 * box + 2 * lane;  // of the two channels a lane has
+#pragma unroll 1
+          for (int32_t place = Reverse ? kChunk - count : 0; place < (Reverse ? kChunk : count);
+               ++place) {
+            const int32_t row = Reverse ? kChunk - 1 - place : place;
+            const uint32_t at = c + tile_offset(row, lane / 4, kChunk) + 4 * (lane & 3u);
+            const uint32_t v = ptx::ld_shared_u32(at), f = not_finite(v);
+            if (f == 0) continue;
+            st_shared_u32(at, v & ((f & 0x8000u ? 0u : 0xffffu) | (f >> 16 ? 0u : 0xffff0000u)));
+            const uint32_t here = n * kChunk + place + 1;
+            if ((f & 0x8000u) && mine[0] <= unit_first) mine[0] = here;
+            if ((f >> 16) && mine[1] <= unit_first) mine[1] = here;
+          }
+          __syncwarp();
+          if (lane == 0) *last_bad = n * kChunk + kChunk;
+          ptx::fence_proxy_async_shared();
+          __syncwarp();
+        }
+        if (lane == 0) ptx::mbar_arrive(c_ready + 8 * (n & 1u));
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // ------------------------------------------------------------------------- scores -> P
+    const uint32_t w = warp - 4;
+    // scale e^(g |m - 32|): with 32 + (this token) - (another of its 32) for m the decay between them, and
+    // with the other's place for m the decay to 32 others but for a factor of the block (each
+    // factor an exponent of one sign, so that none is above 1).
+    float* powers = reinterpret_cast<float*>(base_ptr + L::kPowers) + 64 * w;
+    const float* own = powers + 32 + lane;
+    const float* others = powers + (Reverse ? 32 : 0);
+    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      const LinearUnit unit = linear_unit(p, u);
+      const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
+      __syncwarp();
+      powers[lane] = p.scale * decay_power(g2, 32 - static_cast<int32_t>(lane));
+      powers[lane + 32] = p.scale * decay_power(g2, static_cast<int32_t>(lane));
+      __syncwarp();
+#pragma unroll 1
+      for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+        int32_t count;
+        chunk_at<Reverse>(unit, x, &count);
+        if (!(ok = ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearScores))) break;
+        ptx::tc_fence_after();
+#pragma unroll 1
+        for (uint32_t blk = 0; blk < 4; ++blk) {
+          uint32_t s[32];
+          if (Reverse ? blk < w : blk > w) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) s[k] = 0u;
+          } else {
+            ptx::tmem_ld_32x32b_x32(lanes + kColScores + 32 * blk, s);
+            ptx::tmem_ld_wait();
+            if (blk == w) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float f = __uint_as_float(s[k]) * own[-k];
+                const bool seen = Reverse ? static_cast<int32_t>(lane) <= k
+                                          : static_cast<int32_t>(lane) >= k;
+                s[k] = seen ? __float_as_uint(f) : 0u;
+              }
+            } else {
+              const int32_t first = static_cast<int32_t>(32 * blk);
+              const float r = decay_power(g2, Reverse ? first - i : i - first - 32);
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const float4 d = *reinterpret_cast<const float4*>(others + k);
+                mul2(s[k], s[k + 1], r, r);
+                mul2(s[k + 2], s[k + 3], r, r);
+                mul2(s[k], s[k + 1], d.x, d.y);
+                mul2(s[k + 2], s[k + 3], d.z, d.w);
+              }
+            }
+            // (In order, tokens past the end are later than any whose output is kept.)
+            if (Reverse && count < kChunk) {
+              const int32_t left = count - static_cast<int32_t>(32 * blk);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[k] = k < left ? s[k] : 0u;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              s[k] = ptx::pack_bf16x2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+          }
+          // Over scores that this lane has read: those of blocks up to this one.
+          const uint32_t packed[16] = {s[0], s[1], s[2],  s[3],  s[4],  s[5],  s[6],  s[7],
+                                       s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15]};
+          tmem_st_32x32b_x16(lanes + kColScores + 16 * blk, packed);
+        }
+        tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready);
+      }
+    }
+  } else if (warp >= 8 && warp < 16) {
+    // ------------------------------------------------------------------------------ output
+    constexpr int kCols = DC / 2;  // of each of the two warps that share TMEM lanes
+    const int32_t col0 = static_cast<int32_t>((warp - 8) / 4) * kCols;
+    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      const LinearUnit unit = linear_unit(p, u);
+      const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
+      const uint32_t unit_first = n * kChunk;
+      bool state = unit.from >= 0;
+#pragma unroll 1
+      for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+        int32_t count;
+        const int64_t t = chunk_at<Reverse>(unit, x, &count);
+        if (!(ok = ptx::mbar_wait_brief(o_full, n & 1u, ctx, kSiteLinearOutput))) break;
+        ptx::tc_fence_after();
+        const bool spoilt = *last_bad > unit_first;
+        // 16 tokens x 32 channels at a time: a lane has neighbouring pairs of channels of two tokens,
+        // four lanes a token's eight channels.  (A token's channels in one lane would make each
+        // store touch 32 rows: 2270 cycles of the SM's data path a chunk, which the products need.)
+#pragma unroll 1
+        for (int32_t half = 0; half < 2; ++half) {
+          const int32_t token = static_cast<int32_t>((warp & 3u) * 32 + 16 * half + lane / 4);
+          float since[2];
+          int64_t row[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int32_t at = token + 8 * r;
+            since[r] = p.scale * decay_power(g2, Reverse ? max(count - 1 - at, 0) : at + 1);
+            row[r] = (t + at) * p.o_token + unit.head * p.o_head;
+          }
+#pragma unroll 1
+          for (int32_t col = col0; col < col0 + kCols; col += 32) {
+            const uint32_t at = lanes + (static_cast<uint32_t>(16 * half) << 16) + col;
+            uint32_t o[16], s[16];
+            __syncwarp();
+            tmem_ld_16x256b_x4(at + kColIntra, o);
+            if (state) tmem_ld_16x256b_x4(at + kColInter, s);
+            ptx::tmem_ld_wait();
+            if (state) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 2)
+                add2(o[j], o[j + 1], since[(j >> 1) & 1], s[j], s[j + 1]);
+            }
+            if (spoilt) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int32_t at = token + 8 * ((j >> 1) & 1);
+                const uint32_t first =
+                    bad[col + 8 * (j / 4) + 2 * static_cast<int32_t>(lane & 3u) + (j & 1)];
+                const uint32_t here = n * kChunk + (Reverse ? kChunk - 1 - at : at) + 1;
+                if (first > unit_first && here >= first) o[j] = 0x7fc00000u;
+              }
+            }
+            if (p.o_f32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int32_t channel = col + 8 * (j / 2) + 2 * static_cast<int32_t>(lane & 3u);
+                if (token + 8 * (j & 1) < count && channel < p.dc)
+                  *reinterpret_cast<uint2*>(static_cast<float*>(p.o) + row[j & 1] + channel) =
+                      make_uint2(o[2 * j], o[2 * j + 1]);
+              }
+              continue;
+            }
+            uint32_t v[2][4];  // of both tokens
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j & 1][j / 2] =
+                  ptx::pack_bf16x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+            quad_transpose(v, lane);
+            const int32_t channel = col + 8 * static_cast<int32_t>(lane & 3u);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (token + 8 * j < count && channel < p.dc)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row[j] + channel) =
+                    make_uint4(v[j][0], v[j][1], v[j][2], v[j][3]);
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(o_free);
+          done[warp - 8] = n + 1;
+        }
+        state = true;
+      }
+    }
+  } else if (warp >= 16 && warp < 20) {
+    // --------------------------------------------------------------------------- the state
+    const uint32_t mine = lanes + kColState;
+    const int64_t size = static_cast<int64_t>(p.da) * p.dc;
+    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      const LinearUnit unit = linear_unit(p, u);
+      const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
+      const float* from =
+          unit.from < 0 ? nullptr : p.state + (unit.from * p.heads + unit.head) * size;
+      const uint32_t unit_first = n * kChunk;
+      float* to = unit.to < 0 ? nullptr : p.final + (unit.to * p.heads + unit.head) * size;
+      auto starting = [&](int32_t c) {  // column c of row i of the starting state
+        return from != nullptr && i < p.da && c < p.dc
+                   ? p.state_factor * from[p.state_transposed ? c * p.da + i : i * p.dc + c]
+                   : 0.f;
+      };
+      if (unit.chunks == 0) {
+        if (to != nullptr && i < p.da) {
+#pragma unroll 1
+          for (int32_t c = 0; c < p.dc; ++c) to[i * p.dc + c] = p.final_factor * starting(c);
+        }
+        continue;
+      }
+      if (from != nullptr) {
+#pragma unroll 1
+        for (int32_t col = 0; col < DC; col += 16) {
+          uint32_t s[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) s[k] = __float_as_uint(starting(col + k));
+          __syncwarp();
+          tmem_st_32x32b_x16(mine + col, s);
+        }
+        tmem_st_wait();
+      }
+#pragma unroll 1
+      for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+        int32_t count;
+        chunk_at<Reverse>(unit, x, &count);
+        const float decay = decay_power(g2, count);
+        // The chunk before is done with the state and its copy (at a unit's first chunk: waited for
+        // at the end of the last one).
+        if (x > 0) {
+          if (!(ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
+          ptx::tc_fence_after();
+        }
+        if ((warp & 3u) * 32 < DA && (x > 0 || from != nullptr)) {
+#pragma unroll 1
+          for (int32_t col = 0; col < DC; col += 16) {
+            uint32_t s[16];
+            ptx::tmem_ld_32x32b_x16(mine + col, s);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              ptx::st_shared_v4(
+                  base + L::kS + tile_offset(i, col / 8 + k, DA),
+                  ptx::pack_bf16x2(__uint_as_float(s[8 * k]), __uint_as_float(s[8 * k + 1])),
+                  ptx::pack_bf16x2(__uint_as_float(s[8 * k + 2]), __uint_as_float(s[8 * k + 3])),
+                  ptx::pack_bf16x2(__uint_as_float(s[8 * k + 4]), __uint_as_float(s[8 * k + 5])),
+                  ptx::pack_bf16x2(__uint_as_float(s[8 * k + 6]), __uint_as_float(s[8 * k + 7])));
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) mul2(s[k], s[k + 1], decay, decay);
+            tmem_st_32x32b_x16(mine + col, s);
+          }
+          tmem_st_wait();
+        }
+        ptx::fence_proxy_async_shared();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(h_ready);
+          done[warp - 8] = n + 1;
+        }
+      }
+      if (!ok || !(ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
+      ptx::tc_fence_after();
+      if (to != nullptr) {
+#pragma unroll 1
+        for (int32_t col = 0; col < DC; col += 16) {
+          uint32_t s[16];
+          __syncwarp();
+          ptx::tmem_ld_32x32b_x16(mine + col, s);
+          ptx::tmem_ld_wait();
+          if (*last_bad > unit_first) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (bad[col + k] > unit_first) s[k] = 0x7fc00000u;
+          }
+          if (i < p.da) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              if (col + k < p.dc)
+                *reinterpret_cast<float4*>(to + i * p.dc + col + k) =
+                    make_float4(p.final_factor * __uint_as_float(s[k]),
+                                p.final_factor * __uint_as_float(s[k + 1]),
+                                p.final_factor * __uint_as_float(s[k + 2]),
+                                p.final_factor * __uint_as_float(s[k + 3]));
+          }
+        }
+      }
+      ptx::tc_fence_before();
+    }
+  } else if (warp >= 20) {
+    // ----------------------------------------------------------------------------- left . B
+    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      const LinearUnit unit = linear_unit(p, u);
+      const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
+#pragma unroll 1
+      for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
+        int32_t count;
+        chunk_at<Reverse>(unit, x, &count);
+        const uint32_t slot = n & 1u, twice = (n >> 1) & 1u;
+        const uint32_t b = base + L::kB + slot * L::kTileA;
+        const bool inside = i < count;
+        const float left = inside ? decay_power(g2, Reverse ? i + 1 : count - 1 - i) : 0.f;
+        // In place of B, which the scores no longer need; the second part's tile is the chunk
+        // before's until its product is done.
+        ok = ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearLeft) &&
+             ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearLeft);
+        if (ok && n > 0) ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearLeft);
+        if (ok && count < kChunk)
+          ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearLeft);
+        if (!ok) break;
+        if (p.exact) {
+#pragma unroll 1
+          for (uint32_t piece = 0; piece < DA / 8; ++piece) {
+            const uint32_t at = tile_offset(i, piece, kChunk);
+            const uint4 v = ld_shared_v4(b + at);
+            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float f0 = inside ? bf16_lo(word[k]) * left : 0.f;
+              const float f1 = inside ? bf16_hi(word[k]) * left : 0.f;
+              hi[k] = ptx::pack_bf16x2(f0, f1);
+              const float m0 = f0 - bf16_lo(hi[k]), m1 = f1 - bf16_hi(hi[k]);
+              mid[k] = ptx::pack_bf16x2(m0, m1);
+              lo[k] = ptx::pack_bf16x2(m0 - bf16_lo(mid[k]), m1 - bf16_hi(mid[k]));
+            }
+            ptx::st_shared_v4(b + at, hi[0], hi[1], hi[2], hi[3]);
+            ptx::st_shared_v4(base + L::kMid + at, mid[0], mid[1], mid[2], mid[3]);
+            ptx::st_shared_v4(base + L::kLo + at, lo[0], lo[1], lo[2], lo[3]);
+          }
+        } else {
+          // With left = l1 + l2 to 2^-17 (BF16 parts) and y an element of B: the first part is
+          // h = RN(y l1), and y l1 - h, which BF16 holds, + y l2 rounded is the second.
+          const uint32_t l1 = bf16_twice(left);
+          const uint32_t l2 = bf16_twice(left - bf16_lo(l1));
+#pragma unroll 2
+          for (uint32_t piece = 0; piece < DA / 8; ++piece) {
+            const uint32_t at = tile_offset(i, piece, kChunk);
+            const uint4 v = ld_shared_v4(b + at);
+            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4], mid[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t y = inside ? word[k] : 0u;
+              hi[k] = bf16x2_fma(y, l1, 0x80008000u);
+              mid[k] = bf16x2_fma(y, l2, bf16x2_fma(y, l1, hi[k] ^ 0x80008000u));
+            }
+            ptx::st_shared_v4(b + at, hi[0], hi[1], hi[2], hi[3]);
+            ptx::st_shared_v4(base + L::kMid + at, mid[0], mid[1], mid[2], mid[3]);
+          }
+        }
+        if (!inside) {  // other sequences' rows, or none
+          const uint32_t c = base + L::kC + c_slot(n) * L::kTileC;
+#pragma unroll 1
+          for (uint32_t piece = 0; piece < DC / 8; ++piece)
+            ptx::st_shared_v4(c + tile_offset(i, piece, kChunk), 0u, 0u, 0u, 0u);
+        }
+        ptx::fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(b_ready);
+      }
+    }
+  }
+  // Every product has completed: the state's of the last chunk is waited for above.
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc<1>(tmem, 512);
+#endif
+}
+
+}  // namespace cpg

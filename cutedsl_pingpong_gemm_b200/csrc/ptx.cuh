@@ -197,6 +197,28 @@ __device__ __forceinline__ bool mbar_wait_spin(uint32_t bar, uint32_t parity, co
   }
 }
 
+// As mbar_wait, but without a suspend hint, which is carried out as naps that outlast short phases:
+// for hand-overs between the warps of a block.  Bounded the same way (deadline and abort flag, checked
+// every 64 tries); the tries after the first are out of line, to keep a kernel of many waits small.
+inline __device__ __noinline__ bool mbar_wait_tries(uint32_t bar, uint32_t parity,
+                                                    const WaitCtx& ctx, int32_t site) {
+  const uint64_t t0 = globaltimer();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*ctx.abort_flag) return false;
+    if (globaltimer() - t0 > ctx.timeout_ns) {
+      record_timeout(ctx, site);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait_brief(uint32_t bar, uint32_t parity, const WaitCtx& ctx,
+                                                int32_t site) {
+  return mbar_try_wait(bar, parity) || mbar_wait_tries(bar, parity, ctx, site);
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

@@ -472,6 +472,10 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
 int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
                                    int32_t v_heads, int32_t backward, int64_t* bytes);
 
+/* Synchronises and reads the current device's word of the linear attention kernels: 0, or the code of
+ * the first wait that ever ran out there (10 s; the outputs of that launch are not valid). */
+int cpg_attention_status(int32_t* status);
+
 /* One token of each of p->tokens sequences: q, k, v and out [tokens, heads, channels], the states
  * updated in place.  Tokens whose slot is outside [0, places) are padding: their out is 0. */
 int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,

@@ -344,8 +344,16 @@ def test_linear_attention_backward_outputs():
     got = attention.linear_attention_backward(dy, q, k, v, decay, offsets=offsets, dstate=dstate,
                                               out=tuple(x[:, 1:3] for x in out))
     assert got[3] is dstate
-    for x, w in zip(out, want):
-        assert torch.equal(x[2:272, 1:3], w[2:272])
+    # dstate makes the states of dv's pass FP32-exact, so that their BF16 copies may be rounded the
+    # other way than without (see the tolerances above); asked for twice it gives the same bits.
+    twice = attention.linear_attention_backward(dy, q, k, v, decay, offsets=offsets,
+                                                dstate=torch.empty_like(dstate))
+    assert torch.equal(twice[3], dstate)
+    grads, _ = ref.linear_attention_backward(dy, q, k, v, decay, 1.0, offsets)
+    for x, w, y, (g, near, far) in zip(out, want, twice, grads):
+        assert torch.equal(x[2:272, 1:3], y[2:272])
+        for z in (y, w):
+            within(z, g, 2 ** -8 * near + half(BF) * g.abs() + 2 ** -15 * far)
         assert (x[:2] == 3).all() and (x[272:] == 3).all()
         assert (x[:, 0] == 3).all() and (x[:, 3:] == 3).all()
     _, (ds, size) = ref.linear_attention_backward(dy, q, k, v, decay, 1.0, offsets)
