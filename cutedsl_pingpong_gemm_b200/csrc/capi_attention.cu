@@ -387,8 +387,11 @@ int device_ready(int* sms) {
     };
     auto both = [&](auto da, auto dc) {
       constexpr int kDA = decltype(da)::value, kDC = decltype(dc)::value;
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, false>, cpg::ChunkLayout<kDA, kDC>::kBytes);
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, true>, cpg::ChunkLayout<kDA, kDC>::kBytes);
+      constexpr uint32_t kBytes = cpg::ChunkLayout<kDA, kDC>::kBytes;
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, false, false>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, false, true>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, true, false>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, true, true>, kBytes);
     };
     const std::integral_constant<int, 64> d64;
     const std::integral_constant<int, 128> d128;
@@ -403,8 +406,57 @@ int device_ready(int* sms) {
   return CPG_OK;
 }
 
-template <int DA, int DC>
-int run_chunks(const cpg::LinearParams& r, bool reverse, int sms, cudaStream_t st) {
+// How a pass is cut: the tokens of a segment (0: sequences stay whole) and the most segments there can
+// be.  A unit (a sequence or segment of one head) is a chain of chunks of one SM, 2.8 us each alone
+// and 3.5 us where all SMs share the bandwidth.  Cutting sequences costs a pass over B and C for the
+// segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
+// channels 1480 -> XX us.  The lengths are known to the device alone: the mean stands for them.
+struct LinearCut {
+  int64_t length, items;
+};
+
+LinearCut linear_cut(const cpg_linear_problem* p) {
+  constexpr int64_t kSms = 148, kMostCut = 1024;
+  if (p->sequences == 0 || p->tokens == 0) return {0, 0};
+  const int64_t mean = (p->tokens + p->sequences - 1) / p->sequences;
+  const int64_t chunks = (mean + cpg::kChunk - 1) / cpg::kChunk;
+  const int64_t units = int64_t(p->sequences) * p->heads;
+  const int64_t waves = (units + kSms - 1) / kSms;
+  const double whole = chunks * (units < kSms ? 2.8 : 3.5 * waves);
+  double best = whole;
+  int64_t cut = 0;
+  if (units > kMostCut) return {0, 0};
+  for (int64_t length = 2; length < std::min<int64_t>(chunks, 128); ++length) {
+    const int64_t segments = (chunks + length - 1) / length;
+    const int64_t turns = (segments * units + kSms - 1) / kSms;
+    // The last segment's state is not needed; 30 us: the launches in between.
+    const double cost = turns * (length + 1.0) * 3.5 + 30.0 +
+                        (((segments - 1) * units + kSms - 1) / kSms) * (length + 1.0) * 2.0;
+    if (cost < best) {
+      best = cost;
+      cut = length;
+    }
+  }
+  if (cut == 0) return {0, 0};
+  return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences};
+}
+
+// Workspace of a cut pass: the segments' states, the table of segments.
+struct LinearSpace {
+  int64_t items, first, count, bytes;  // offsets in bytes (the states are at 0)
+};
+LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut) {
+  if (cut.length == 0) return {0, 0, 0, 0};
+  LinearSpace r;
+  r.items = cut.items * p->heads * p->dk * p->dv * 4;
+  r.first = r.items + cut.items * static_cast<int64_t>(sizeof(cpg::LinearItem));
+  r.count = r.first + (int64_t(p->sequences) + 1) * 4;
+  r.bytes = (r.count + 4 + 15) / 16 * 16;
+  return r;
+}
+
+template <int DA, int DC, bool Out>
+int run_chunks(const cpg::LinearParams& r, bool reverse, int64_t units, int sms, cudaStream_t st) {
   CUtensorMap maps[3] = {};
   const cpg::LinearRows* x[3] = {&r.a, &r.b, &r.c};
   for (int i = 0; i < 3 && r.tokens > 0; ++i) {
@@ -412,26 +464,53 @@ int run_chunks(const cpg::LinearParams& r, bool reverse, int sms, cudaStream_t s
         encode_heads(&maps[i], *x[i], r.tokens, r.heads / x[i]->share, i < 2 ? r.da : r.dc);
     if (rc != CPG_OK) return rc;
   }
-  const int64_t units = int64_t(r.sequences) * r.heads;
-  auto fn = reverse ? &cpg::linear_chunks_kernel<DA, DC, true>
-                    : &cpg::linear_chunks_kernel<DA, DC, false>;
+  auto fn = reverse ? &cpg::linear_chunks_kernel<DA, DC, true, Out>
+                    : &cpg::linear_chunks_kernel<DA, DC, false, Out>;
   return launch("linear attention kernel", true, fn,
                 static_cast<unsigned>(std::min<int64_t>(units, sms)), cpg::kChunkThreads,
                 cpg::ChunkLayout<DA, DC>::kBytes, st, 1, maps[0], maps[1], maps[2], r);
 }
 
-int run_pass(cpg::LinearParams r, bool reverse, cudaStream_t st) {
+template <bool Out>
+int run_chunks(const cpg::LinearParams& r, bool reverse, int64_t units, int sms, cudaStream_t st) {
+  if (r.da > 64)
+    return r.dc > 64 ? run_chunks<128, 128, Out>(r, reverse, units, sms, st)
+                     : run_chunks<128, 64, Out>(r, reverse, units, sms, st);
+  return r.dc > 64 ? run_chunks<64, 128, Out>(r, reverse, units, sms, st)
+                   : run_chunks<64, 64, Out>(r, reverse, units, sms, st);
+}
+
+int run_pass(const cpg_linear_problem* p, cpg::LinearParams r, bool reverse, void* space,
+             cudaStream_t st) {
   if (r.sequences == 0) return CPG_OK;
   int sms = 0;
-  const int rc = device_ready(&sms);
+  int rc = device_ready(&sms);
   if (rc != CPG_OK) return rc;
   r.exact = r.final != nullptr ? 1 : 0;
   r.timeout_ns = kTimeoutNs;
-  if (r.da > 64)
-    return r.dc > 64 ? run_chunks<128, 128>(r, reverse, sms, st)
-                     : run_chunks<128, 64>(r, reverse, sms, st);
-  return r.dc > 64 ? run_chunks<64, 128>(r, reverse, sms, st)
-                   : run_chunks<64, 64>(r, reverse, sms, st);
+  const LinearCut cut = linear_cut(p);
+  if (cut.length == 0)
+    return run_chunks<true>(r, reverse, int64_t(r.sequences) * r.heads, sms, st);
+  const LinearSpace at = linear_space(p, cut);
+  char* const bytes = static_cast<char*>(space);
+  auto* items = reinterpret_cast<cpg::LinearItem*>(bytes + at.items);
+  auto* first = reinterpret_cast<int32_t*>(bytes + at.first);
+  auto* count = reinterpret_cast<int32_t*>(bytes + at.count);
+  rc = launch("segment table kernel", true, &cpg::linear_items_kernel, 1, cpg::kItemThreads, 0, st,
+              1, r.offsets, r.tokens, r.sequences, static_cast<int32_t>(cut.length),
+              reverse ? 1 : 0, items, count, first);
+  if (rc != CPG_OK) return rc;
+  r.items = items;
+  r.first_item = first;
+  r.item_count = count;
+  r.segments = reinterpret_cast<float*>(bytes);
+  rc = run_chunks<false>(r, reverse, cut.items * r.heads, sms, st);
+  if (rc != CPG_OK) return rc;
+  const unsigned parts = static_cast<unsigned>((r.da * r.dc + 1023) / 1024);
+  rc = launch("segment state kernel", true, &cpg::linear_segments_kernel,
+              static_cast<unsigned>(r.sequences) * r.heads * parts, 256, 0, st, 1, r);
+  if (rc != CPG_OK) return rc;
+  return run_chunks<true>(r, reverse, cut.items * r.heads, sms, st);
 }
 
 // FP32 sums of a head each, of the widest shared gradient.
@@ -533,7 +612,8 @@ int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads,
   if (rc != CPG_OK) return rc;
   if (q_heads < 1 || k_heads < 1 || v_heads < 1)
     return fail(CPG_ERR_INVALID_SHAPE, "%d, %d and %d heads", q_heads, k_heads, v_heads);
-  *bytes = backward ? share_bytes(p, q_heads, k_heads, v_heads) : 0;
+  *bytes = linear_space(p, linear_cut(p)).bytes +
+           (backward ? share_bytes(p, q_heads, k_heads, v_heads) : 0);
   return CPG_OK;
 }
 
@@ -562,7 +642,7 @@ int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const 
   cpg::LinearParams r = linear_params(p, q, k, v, p->dk, p->dv, out, log_decay, offsets);
   set_state(&r, state, false, 1.f);
   set_final(&r, final, 1.f);
-  return run_pass(r, false, static_cast<cudaStream_t>(stream));
+  return run_pass(p, r, false, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* dy,
@@ -597,18 +677,19 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
     return fail(CPG_ERR_ALIGNMENT, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // The gradient of a head that several read: each one's in FP32, then their sum.
+  void* const share_space = static_cast<char*>(workspace) + linear_space(p, linear_cut(p)).bytes;
   auto pass = [&](const cpg_heads* a, const cpg_heads* b, const cpg_heads* c, int32_t da,
                   int32_t dc, const cpg_heads* o, bool reverse, const cpg_states* from,
                   bool transposed, float factor, const cpg_states* to) {
-    const cpg_heads sums{workspace, int64_t(p->heads) * dc, dc, p->heads, CPG_DTYPE_F32};
+    const cpg_heads sums{share_space, int64_t(p->heads) * dc, dc, p->heads, CPG_DTYPE_F32};
     const bool shared = o->heads < p->heads;
     cpg::LinearParams r =
         linear_params(p, a, b, c, da, dc, shared ? &sums : o, log_decay, offsets);
     set_state(&r, from, transposed, factor);
     set_final(&r, to, p->scale);
-    int e = run_pass(r, reverse, st);
+    int e = run_pass(p, r, reverse, workspace, st);
     if (e != CPG_OK || !shared || p->tokens == 0) return e;
-    const cpg::LinearShareParams s{static_cast<const float*>(workspace),
+    const cpg::LinearShareParams s{static_cast<const float*>(share_space),
                                    static_cast<__nv_bfloat16*>(o->ptr),
                                    o->token_stride,
                                    o->head_stride,

@@ -23,6 +23,14 @@ struct LinearRows {
   int32_t share;        // heads of the decay that read one head of this
 };
 
+// A segment of a sequence, in the order of work: whole chunks but for the sequence's end.
+struct LinearItem {
+  int32_t sequence;
+  int32_t first, count;  // tokens
+  int32_t index;         // segments of the sequence that come before it
+  int32_t last;
+};
+
 struct LinearParams {
   LinearRows a, b, c;
   void* o;
@@ -43,6 +51,11 @@ struct LinearParams {
   const int32_t* final_slots;
   int64_t final_places;
   float final_factor;
+  const LinearItem* items;       // null: a unit is a whole sequence
+  const int32_t* item_count;
+  const int32_t* first_item;     // [sequences + 1]
+  float* segments;         // [items, heads, da, dc]: what the segment before adds to the state, then the
+                           // state before each
   int32_t exact;           // states to FP32 accuracy (they are outputs)
   uint64_t timeout_ns;     // limit of a wait within the kernel
 };
@@ -65,6 +78,99 @@ __device__ __forceinline__ LinearSpan linear_span(const int32_t* offsets, int32_
 __device__ __forceinline__ int64_t linear_place(const int32_t* slots, int32_t s, int64_t places) {
   const int64_t at = slots == nullptr ? s : slots[s];
   return at >= 0 && at < places ? at : -1;
+}
+
+// The segments of `length` tokens (whole chunks) of every sequence, one after the other in the order of
+// work; an empty sequence has one without tokens.  One block.
+constexpr int kItemThreads = 1024;
+
+__global__ void __launch_bounds__(kItemThreads)
+    linear_items_kernel(const int32_t* offsets, int64_t tokens, int32_t sequences, int32_t length,
+                        int32_t reverse, LinearItem* items, int32_t* item_count,
+                        int32_t* first_item) {
+  kernel_begins();
+  __shared__ int32_t sums[kItemThreads / 32];
+  const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int32_t base = 0;
+  for (int32_t from = 0; from < sequences; from += kItemThreads) {
+    const int32_t s = from + static_cast<int32_t>(threadIdx.x);
+    LinearSpan span = {0, 0};
+    if (s < sequences) span = linear_span(offsets, s, tokens);
+    int32_t n = s < sequences ? static_cast<int32_t>((span.count + length - 1) / length) : 0;
+    if (s < sequences && n == 0) n = 1;
+    int32_t before = n;  // inclusive sum within the warp
+    for (int o = 1; o < 32; o *= 2) {
+      const int32_t v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    int32_t all = 0;
+    for (int w = 0; w < kItemThreads / 32; ++w) {
+      if (w == warp) before += all;
+      all += sums[w];
+    }
+    if (s < sequences) {
+      const int32_t at = base + before - n;
+      first_item[s] = at;
+      for (int32_t k = 0; k < n; ++k) {
+        const int64_t first = static_cast<int64_t>(reverse ? n - 1 - k : k) * length;
+        const int64_t left = span.count - first;
+        items[at + k] = {s, static_cast<int32_t>(span.first + first),
+                         static_cast<int32_t>(left < length ? left : length), k, k == n - 1};
+      }
+    }
+    base += all;
+  }
+  if (threadIdx.x == 0) {
+    *item_count = base;
+    first_item[sequences] = base;
+  }
+}
+
+// The state before every segment of a sequence that has several: the state before the previous one,
+// decayed by that one's tokens, plus what it adds.  Four neighbouring elements a thread; blockIdx.x:
+// sequence and head, then the elements.
+__global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams p) {
+  kernel_begins();
+  const int32_t size = p.da * p.dc;
+  const int32_t parts = (size + 1023) / 1024;
+  const int32_t pair = blockIdx.x / parts;
+  const int32_t s = pair / p.heads, h = pair % p.heads;
+  const int32_t e = (blockIdx.x % parts) * 1024 + static_cast<int32_t>(threadIdx.x) * 4;
+  const int32_t first = p.first_item[s], last = p.first_item[s + 1] - 1;
+  if (e >= size || first >= last) return;
+  const float g2 = p.log_decay[h] * 1.4426950408889634f;
+  const int64_t step = static_cast<int64_t>(p.heads) * size;
+  float* x = p.segments + first * step + static_cast<int64_t>(h) * size + e;
+  float4 state = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.state != nullptr) {
+    const int64_t place = linear_place(p.state_slots, s, p.state_places);
+    if (place >= 0) {
+      const float* from = p.state + (place * p.heads + h) * static_cast<int64_t>(size);
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        f[k] = p.state_factor * (p.state_transposed
+                                     ? from[(e + k) % p.dc * p.da + (e + k) / p.dc]
+                                     : from[e + k]);
+      state = make_float4(f[0], f[1], f[2], f[3]);
+    }
+    *reinterpret_cast<float4*>(x) = state;
+  }
+#pragma unroll 4
+  for (int32_t at = first; at < last; ++at) {
+    x += step;
+    const int32_t n = p.items[at].count;
+    const float decay = exp2f(g2 * static_cast<float>(n));
+    const float4 v = *reinterpret_cast<const float4*>(x);
+    state.x = fmaf(state.x, decay, v.x);
+    state.y = fmaf(state.y, decay, v.y);
+    state.z = fmaf(state.z, decay, v.z);
+    state.w = fmaf(state.w, decay, v.w);
+    *reinterpret_cast<float4*>(x) = state;
+  }
 }
 
 // Rows of a [tokens, heads, d] outside the sequences, set to zero.

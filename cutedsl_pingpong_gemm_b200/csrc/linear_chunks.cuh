@@ -139,6 +139,19 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -207,6 +220,19 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t x, uint32_t y, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
   return r;
 }
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+// x y - z.
+__device__ __forceinline__ uint32_t bf16x2_residual(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tneg.bf16x2 t, %3;\n\tfma.rn.bf16x2 %0, %1, %2, t;\n\t}"
+      : "=r"(r)
+      : "r"(x), "r"(y), "r"(z));
+  return r;
+}
 __device__ __forceinline__ uint32_t bf16_twice(float f) { return ptx::pack_bf16x2(f, f); }
 
 // (x0, x1) *= (y0, y1), two FP32 products an instruction.
@@ -250,24 +276,57 @@ __device__ __forceinline__ uint32_t tile_offset(uint32_t r, uint32_t piece, uint
   return (piece >> 3) * rows * 128u + r * 128u + (((piece & 7u) ^ (r & 7u)) << 4);
 }
 
-// What a block does: (sequence, head) pairs u = blockIdx.x, + gridDim.x, ... and their chunks.
+// What a block does: units u = blockIdx.x, + gridDim.x, ... (a sequence's or a segment's tokens of one
+// head) and their chunks.
 struct LinearUnit {
-  int32_t sequence, head;
+  int32_t head;
   int64_t first, count;
   int32_t chunks;
-  int64_t from, to;  // places of its starting and final state, -1: none
+  const float* from;  // starting state, null: zeros
+  float* to;          // final state, null: not wanted
+  float from_factor, to_factor;
+  bool transposed;    // from
 };
 
-__device__ __forceinline__ LinearUnit linear_unit(const LinearParams& p, int32_t u) {
-  LinearUnit r;
-  r.sequence = u / p.heads;
-  r.head = u - r.sequence * p.heads;
-  const LinearSpan span = linear_span(p.offsets, r.sequence, p.tokens);
-  r.first = span.first;
-  r.count = span.count;
-  r.chunks = static_cast<int32_t>((span.count + kChunk - 1) / kChunk);
-  r.from = p.state == nullptr ? -1 : linear_place(p.state_slots, r.sequence, p.state_places);
-  r.to = p.final == nullptr ? -1 : linear_place(p.final_slots, r.sequence, p.final_places);
+// (Out of line: once per unit in each of eight roles.)
+template <bool Out>
+__device__ __noinline__ LinearUnit linear_unit(const LinearParams& p, int32_t u) {
+  LinearUnit r = {};
+  const int32_t at = u / p.heads;
+  const int64_t size = static_cast<int64_t>(p.da) * p.dc;
+  r.head = u - at * p.heads;
+  LinearItem item = {at, 0, 0, 0, 1};
+  if (p.items != nullptr) {
+    item = p.items[at];
+  } else {
+    const LinearSpan span = linear_span(p.offsets, at, p.tokens);
+    item.first = static_cast<int32_t>(span.first);
+    item.count = static_cast<int32_t>(span.count);
+  }
+  float* const segment = p.segments + (static_cast<int64_t>(at) * p.heads + r.head) * size;
+  r.from_factor = r.to_factor = 1.f;
+  if constexpr (!Out) {
+    if (item.last) return r;
+    r.to = segment + p.heads * size;
+  } else {
+    // (The places of a sequence in several segments are read by its first before the last writes them.)
+    if (item.index > 0 || (p.state != nullptr && !item.last)) {
+      r.from = segment;
+    } else if (p.state != nullptr) {
+      const int64_t place = linear_place(p.state_slots, item.sequence, p.state_places);
+      if (place >= 0) r.from = p.state + (place * p.heads + r.head) * size;
+      r.from_factor = p.state_factor;
+      r.transposed = p.state_transposed != 0;
+    }
+    if (item.last && p.final != nullptr) {
+      const int64_t place = linear_place(p.final_slots, item.sequence, p.final_places);
+      if (place >= 0) r.to = p.final + (place * p.heads + r.head) * size;
+      r.to_factor = p.final_factor;
+    }
+  }
+  r.first = item.first;
+  r.count = item.count;
+  r.chunks = static_cast<int32_t>((r.count + kChunk - 1) / kChunk);
   return r;
 }
 
@@ -280,7 +339,8 @@ __device__ __forceinline__ int32_t chunk_at(const LinearUnit& u, int32_t x, int3
   return static_cast<int32_t>(u.first + at);
 }
 
-template <int DA, int DC, bool Reverse>
+// Out false: only the state that each unit leaves, from zeros, and without A.
+template <int DA, int DC, bool Reverse, bool Out>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     linear_chunks_kernel(const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_b,
@@ -336,7 +396,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const ptx::WaitCtx ctx{abort_flag, &linear_status_word, p.timeout_ns};
-  const int32_t units = p.sequences * p.heads;
+  const int32_t units = (p.items != nullptr ? *p.item_count : p.sequences) * p.heads;
   const int32_t step = static_cast<int32_t>(gridDim.x);
   // Thread of a warpgroup: the token of the chunk, or the row of the state, that it has, and the TMEM
   // lanes of its warp.
@@ -354,7 +414,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (lane == 0) {
       const uint64_t policy = ptx::policy_evict_first();
       for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-        const LinearUnit unit = linear_unit(p, u);
+        const LinearUnit unit = linear_unit<Out>(p, u);
         const int32_t ha = unit.head / p.a.share, hb = unit.head / p.b.share,
                       hc = unit.head / p.c.share;
 #pragma unroll 1
@@ -372,12 +432,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           for (int j = 0; j < DA / 64; ++j)
             ptx::tma_load_3d(&tm_b, b + j * 16384, b_full + 8 * slot, 64 * j, hb, t, policy);
           // What waits for room below comes into L2 meanwhile.
-          for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_a, 64 * j, ha, t);
+          if (Out)
+            for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_a, 64 * j, ha, t);
           if (one_c)
             for (int j = 0; j < DC / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_c, 64 * j, hc, t);
           // C first unless its only slot is the last to become free.
           for (int turn = 0; turn < 2 && ok; ++turn) {
             if ((turn == 0) == one_c) {
+              if (!Out) continue;
               if (!(ok = ptx::mbar_wait_brief(a_empty, (n & 1u) ^ 1u, ctx, kSiteLinearProducer)))
                 break;
               ptx::mbar_arrive_expect_tx(a_full, L::kTileA);
@@ -410,7 +472,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           none = 0;
           ptx::mbar_wait_tries(c_full + 8 * c_slot(j), c_phase(j), brief, kSiteLinearDrain);
           none = 0;
-          ptx::mbar_wait_tries(a_full, j & 1u, brief, kSiteLinearDrain);
+          if (Out) ptx::mbar_wait_tries(a_full, j & 1u, brief, kSiteLinearDrain);
         }
       }
     }
@@ -425,8 +487,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const uint32_t a_k = ptx::sw128_desc_lo(base + L::kA);  // A along its channels
       const uint32_t s_mn = desc_lo_mn(base + L::kS, DA * 128);
       for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-        const LinearUnit unit = linear_unit(p, u);
-        bool state = unit.from >= 0;
+        const LinearUnit unit = linear_unit<Out>(p, u);
+        bool state = unit.from != nullptr;
 #pragma unroll 1
         for (int32_t x = 0; x < unit.chunks && ok; ++x, ++n) {
           int32_t count;
@@ -434,40 +496,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const uint32_t slot = n & 1u, twice = (n >> 1) & 1u, once = n & 1u;
           const uint32_t b = base + L::kB + slot * L::kTileA;
           const uint32_t c_mn = desc_lo_mn(base + L::kC + c_slot(n) * L::kTileC, 16384);
-          // A B^T.  Its columns hold P of the chunk before until that one's product is done.
-          if (n > 0) ok = ptx::mbar_wait_brief(o_full, once ^ 1u, ctx, kSiteLinearMma);
-          ok = ok && ptx::mbar_wait_brief(a_full, once, ctx, kSiteLinearMma) &&
-               ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearMma);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          const uint32_t b_k = ptx::sw128_desc_lo(b);
-#pragma unroll
-          for (int k = 0; k < DA / 16; ++k)
-            umma_f16_ss(tmem + kColScores, a_k + k_step(k), b_k + k_step(k), kScores, k > 0, issue);
-          umma_commit_if(s_full, issue);
-          // A S into its own columns, once the output before has been read.
-          ok = ptx::mbar_wait_brief(h_ready, once, ctx, kSiteLinearMma);
-          if (n > 0) ok = ok && ptx::mbar_wait_brief(o_free, once ^ 1u, ctx, kSiteLinearMma);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          if (state) {
+          if constexpr (Out) {
+            // A B^T.  Its columns hold P of the chunk before until that one's product is done.
+            if (n > 0) ok = ptx::mbar_wait_brief(o_full, once ^ 1u, ctx, kSiteLinearMma);
+            ok = ok && ptx::mbar_wait_brief(a_full, once, ctx, kSiteLinearMma) &&
+                 ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearMma);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t b_k = ptx::sw128_desc_lo(b);
 #pragma unroll
             for (int k = 0; k < DA / 16; ++k)
-              umma_f16_ss(tmem + kColInter, a_k + k_step(k), s_mn + k * 128, kInter, k > 0, issue);
-          }
-          umma_commit_if(a_empty, issue);
-          // P C.  A partial chunk's rows of C past its end are cleared before b_ready.
-          ok = ptx::mbar_wait_brief(p_ready, once, ctx, kSiteLinearMma) &&
-               ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearMma) &&
-               ptx::mbar_wait_brief(c_ready + 8 * slot, twice, ctx, kSiteLinearMma) &&
-               (count == kChunk || ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma));
-          if (!ok) break;
-          ptx::tc_fence_after();
+              umma_f16_ss(tmem + kColScores, a_k + k_step(k), b_k + k_step(k), kScores, k > 0, issue);
+            umma_commit_if(s_full, issue);
+            // A S into its own columns, once the output before has been read.
+            ok = ptx::mbar_wait_brief(h_ready, once, ctx, kSiteLinearMma);
+            if (n > 0) ok = ok && ptx::mbar_wait_brief(o_free, once ^ 1u, ctx, kSiteLinearMma);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (state) {
 #pragma unroll
-          for (int k = 0; k < kChunk / 16; ++k)
-            umma_f16_ts(tmem + kColIntra, tmem + kColScores + k * 8, c_mn + k * 128, kInter, k > 0,
-                        issue);
-          umma_commit_if(o_full, issue);
+              for (int k = 0; k < DA / 16; ++k)
+                umma_f16_ss(tmem + kColInter, a_k + k_step(k), s_mn + k * 128, kInter, k > 0, issue);
+            }
+            umma_commit_if(a_empty, issue);
+            // P C.  A partial chunk's rows of C past its end are cleared before b_ready.
+            ok = ptx::mbar_wait_brief(p_ready, once, ctx, kSiteLinearMma) &&
+                 ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearMma) &&
+                 ptx::mbar_wait_brief(c_ready + 8 * slot, twice, ctx, kSiteLinearMma) &&
+                 (count == kChunk || ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma));
+            if (!ok) break;
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kChunk / 16; ++k)
+              umma_f16_ts(tmem + kColIntra, tmem + kColScores + k * 8, c_mn + k * 128, kInter, k > 0,
+                          issue);
+            umma_commit_if(o_full, issue);
+          } else {
+            ok = ptx::mbar_wait_brief(h_ready, once, ctx, kSiteLinearMma) &&
+                 ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearMma) &&
+                 ptx::mbar_wait_brief(c_ready + 8 * slot, twice, ctx, kSiteLinearMma);
+            if (!ok) break;
+          }
           // The state's addend, by the parts of left . B.
           if (!(ok = ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma))) break;
           ptx::tc_fence_after();
@@ -500,7 +569,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // ----------------------------------------------------------- infinities and NaN in a box of C
     const uint32_t box = warp - 2;
     for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-      const LinearUnit unit = linear_unit(p, u);
+      const LinearUnit unit = linear_unit<Out>(p, u);
       const uint32_t unit_first = n * kChunk;  // place of the unit's first token in the block's work
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
@@ -522,7 +591,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (__any_sync(0xffffffffu, found != 0u)) {
           // The table is the earlier chunks' outputs' and the unit before's state's until then.
           const uint64_t t0 = ptx::globaltimer();
-          while (ok && !__all_sync(0xffffffffu, lane >= 12 || done[lane] >= n + (lane < 8 ? 0u : 1u)))
+          while (ok && !__all_sync(0xffffffffu, lane >= 12 || (lane < 8 && !Out) ||
+                                              done[lane] >= n + (lane < 8 ? 0u : 1u)))
             if (*abort_flag || ptx::globaltimer() - t0 > ctx.timeout_ns) {
               ptx::record_timeout(ctx, kSiteLinearScan);
               ok = false;
@@ -552,7 +622,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (lane == 0) ptx::mbar_arrive(c_ready + 8 * (n & 1u));
       }
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (Out && warp >= 4 && warp < 8) {
     // ------------------------------------------------------------------------- scores -> P
     const uint32_t w = warp - 4;
     // scale e^(g |m - 32|): with 32 + (this token) - (another of its 32) for m the decay between them, and
@@ -562,7 +632,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const float* own = powers + 32 + lane;
     const float* others = powers + (Reverse ? 32 : 0);
     for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-      const LinearUnit unit = linear_unit(p, u);
+      const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       __syncwarp();
       powers[lane] = p.scale * decay_power(g2, 32 - static_cast<int32_t>(lane));
@@ -624,15 +694,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (lane == 0) ptx::mbar_arrive(p_ready);
       }
     }
-  } else if (warp >= 8 && warp < 16) {
+  } else if (Out && warp >= 8 && warp < 16) {
     // ------------------------------------------------------------------------------ output
     constexpr int kCols = DC / 2;  // of each of the two warps that share TMEM lanes
     const int32_t col0 = static_cast<int32_t>((warp - 8) / 4) * kCols;
     for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-      const LinearUnit unit = linear_unit(p, u);
+      const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       const uint32_t unit_first = n * kChunk;
-      bool state = unit.from >= 0;
+      bool state = unit.from != nullptr;
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
@@ -713,34 +783,45 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else if (warp >= 16 && warp < 20) {
     // --------------------------------------------------------------------------- the state
     const uint32_t mine = lanes + kColState;
-    const int64_t size = static_cast<int64_t>(p.da) * p.dc;
     for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-      const LinearUnit unit = linear_unit(p, u);
+      const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
-      const float* from =
-          unit.from < 0 ? nullptr : p.state + (unit.from * p.heads + unit.head) * size;
       const uint32_t unit_first = n * kChunk;
-      float* to = unit.to < 0 ? nullptr : p.final + (unit.to * p.heads + unit.head) * size;
+      const float* from = unit.from;
+      float* to = unit.to;
       auto starting = [&](int32_t c) {  // column c of row i of the starting state
         return from != nullptr && i < p.da && c < p.dc
-                   ? p.state_factor * from[p.state_transposed ? c * p.da + i : i * p.dc + c]
+                   ? unit.from_factor * from[unit.transposed ? c * p.da + i : i * p.dc + c]
                    : 0.f;
       };
       if (unit.chunks == 0) {
         if (to != nullptr && i < p.da) {
 #pragma unroll 1
-          for (int32_t c = 0; c < p.dc; ++c) to[i * p.dc + c] = p.final_factor * starting(c);
+          for (int32_t c = 0; c < p.dc; ++c) to[i * p.dc + c] = unit.to_factor * starting(c);
         }
         continue;
       }
       if (from != nullptr) {
 #pragma unroll 1
-        for (int32_t col = 0; col < DC; col += 16) {
-          uint32_t s[16];
+        for (int32_t col = 0; col < DC; col += 32) {
+          uint32_t s[32];
+          if (unit.transposed) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) s[k] = __float_as_uint(starting(col + k));
+            for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(starting(col + k));
+          } else {  // 16 bytes at a time (dc is a multiple of 8)
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (i < p.da && col + k < p.dc)
+                v = *reinterpret_cast<const float4*>(from + i * p.dc + col + k);
+              s[k] = __float_as_uint(unit.from_factor * v.x);
+              s[k + 1] = __float_as_uint(unit.from_factor * v.y);
+              s[k + 2] = __float_as_uint(unit.from_factor * v.z);
+              s[k + 3] = __float_as_uint(unit.from_factor * v.w);
+            }
+          }
           __syncwarp();
-          tmem_st_32x32b_x16(mine + col, s);
+          tmem_st_32x32b_x32(mine + col, s);
         }
         tmem_st_wait();
       }
@@ -761,6 +842,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             uint32_t s[16];
             ptx::tmem_ld_32x32b_x16(mine + col, s);
             ptx::tmem_ld_wait();
+            if constexpr (Out) {
 #pragma unroll
             for (int k = 0; k < 2; ++k)
               ptx::st_shared_v4(
@@ -769,6 +851,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                   ptx::pack_bf16x2(__uint_as_float(s[8 * k + 2]), __uint_as_float(s[8 * k + 3])),
                   ptx::pack_bf16x2(__uint_as_float(s[8 * k + 4]), __uint_as_float(s[8 * k + 5])),
                   ptx::pack_bf16x2(__uint_as_float(s[8 * k + 6]), __uint_as_float(s[8 * k + 7])));
+            }
 #pragma unroll
             for (int k = 0; k < 16; k += 2) mul2(s[k], s[k + 1], decay, decay);
             tmem_st_32x32b_x16(mine + col, s);
@@ -802,10 +885,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int k = 0; k < 16; k += 4)
               if (col + k < p.dc)
                 *reinterpret_cast<float4*>(to + i * p.dc + col + k) =
-                    make_float4(p.final_factor * __uint_as_float(s[k]),
-                                p.final_factor * __uint_as_float(s[k + 1]),
-                                p.final_factor * __uint_as_float(s[k + 2]),
-                                p.final_factor * __uint_as_float(s[k + 3]));
+                    make_float4(unit.to_factor * __uint_as_float(s[k]),
+                                unit.to_factor * __uint_as_float(s[k + 1]),
+                                unit.to_factor * __uint_as_float(s[k + 2]),
+                                unit.to_factor * __uint_as_float(s[k + 3]));
           }
         }
       }
@@ -814,7 +897,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else if (warp >= 20) {
     // ----------------------------------------------------------------------------- left . B
     for (int32_t u = blockIdx.x; u < units && ok; u += step) {
-      const LinearUnit unit = linear_unit(p, u);
+      const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
@@ -824,10 +907,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const uint32_t b = base + L::kB + slot * L::kTileA;
         const bool inside = i < count;
         const float left = inside ? decay_power(g2, Reverse ? i + 1 : count - 1 - i) : 0.f;
-        // In place of B, which the scores no longer need; the second part's tile is the chunk
+        // In place of B, once the scores are made; the second part's tile is the chunk
         // before's until its product is done.
         ok = ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearLeft) &&
-             ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearLeft);
+             (!Out || ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearLeft));
         if (ok && n > 0) ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearLeft);
         if (ok && count < kChunk)
           ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearLeft);
@@ -857,20 +940,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           // h = RN(y l1), and y l1 - h, which BF16 holds, + y l2 rounded is the second.
           const uint32_t l1 = bf16_twice(left);
           const uint32_t l2 = bf16_twice(left - bf16_lo(l1));
-#pragma unroll 2
-          for (uint32_t piece = 0; piece < DA / 8; ++piece) {
-            const uint32_t at = tile_offset(i, piece, kChunk);
-            const uint4 v = ld_shared_v4(b + at);
-            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-            uint32_t hi[4], mid[4];
+          const uint32_t mine = static_cast<uint32_t>(i) * 128u + ((static_cast<uint32_t>(i) & 7u) << 4);
+#pragma unroll 1
+          for (uint32_t half = 0; half < DA / 32; ++half) {  // 32 channels (where tile_offset has them)
+            const uint32_t from = (b + (half / 2) * 16384 + mine) ^ ((half & 1u) << 6);
+            const uint32_t to = (base + L::kMid + (half / 2) * 16384 + mine) ^ ((half & 1u) << 6);
+            uint32_t word[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t y = inside ? word[k] : 0u;
-              hi[k] = bf16x2_fma(y, l1, 0x80008000u);
-              mid[k] = bf16x2_fma(y, l2, bf16x2_fma(y, l1, hi[k] ^ 0x80008000u));
+            for (uint32_t piece = 0; piece < 4; ++piece) {
+              const uint4 v = ld_shared_v4(from ^ (piece << 4));
+              word[4 * piece] = v.x;
+              word[4 * piece + 1] = v.y;
+              word[4 * piece + 2] = v.z;
+              word[4 * piece + 3] = v.w;
             }
-            ptx::st_shared_v4(b + at, hi[0], hi[1], hi[2], hi[3]);
-            ptx::st_shared_v4(base + L::kMid + at, mid[0], mid[1], mid[2], mid[3]);
+#pragma unroll
+            for (uint32_t piece = 0; piece < 4; ++piece) {
+              uint32_t hi[4], mid[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t y = inside ? word[4 * piece + k] : 0u;
+                hi[k] = bf16x2_mul(y, l1);
+                mid[k] = bf16x2_fma(y, l2, bf16x2_residual(y, l1, hi[k]));
+              }
+              ptx::st_shared_v4(from ^ (piece << 4), hi[0], hi[1], hi[2], hi[3]);
+              ptx::st_shared_v4(to ^ (piece << 4), mid[0], mid[1], mid[2], mid[3]);
+            }
           }
         }
         if (!inside) {  // other sequences' rows, or none

@@ -432,6 +432,40 @@ def test_linear_attention_pool_of_states():
     attention.linear_attention(q, k, v, decay, offsets=offsets, state=pool, slots=slots)
 
 
+@pytest.mark.parametrize("lengths,h,dk,dv", [([9001], 1, 128, 128), ([6000, 0, 7001, 1], 2, 64, 128),
+                                             ([12000], 3, 128, 40)])
+def test_linear_attention_of_long_sequences(lengths, h, dk, dv):
+    """Few heads and long sequences are worked on in segments, whose states are joined; a pool's
+    states are read before they are written."""
+    q, k, v, decay, offsets = linear_case(3, lengths, h, h, h, h, dk, dv, pad=1)
+    b, g = len(lengths), gen(6)
+    pool = normal(g, b + 2, h, dk, dv, dtype=F32)
+    slots = torch.randperm(b + 2, device="cuda", generator=g)[:b].int()
+    states = [pool[i].clone() for i in slots.tolist()]
+    size = _lib.ctypes.c_int64()
+    p = _lib.LinearProblemC(q.shape[0], b, h, dk, dv, 1.0)
+    _lib.load().cpg_linear_attention_workspace(_lib.ctypes.byref(p), h, h, h, 0,
+                                               _lib.ctypes.byref(size))
+    assert size.value > 0  # they are cut
+    first = attention.linear_attention(q, k, v, decay, scale=0.1, offsets=offsets)[0]
+    check_forward(q[:-1], k[:-1], v[:-1], decay, offsets, 0.1, None, first[:-1])
+    out, _ = attention.linear_attention(q, k, v, decay, scale=0.1, offsets=offsets, state=pool,
+                                        slots=slots, final=pool)
+    # FP32 sums and decays over 100 chunks: 2^-14 of the terms' sizes at most.
+    o, near, far, want, sizes = ref.whole_pass(q, k, v, decay, 0.1, offsets, states)
+    within(out[:-1], o[:-1], (2 ** -8 * near + half(BF) * o.abs() + 2 ** -14 * far)[:-1], "out")
+    within(pool[slots.long()], want, 2 ** -14 * sizes, "final")
+    dy = normal(g, q.shape[0], h, dv)
+    state, dfinal = torch.stack(states), normal(g, b, h, dk, dv, dtype=F32)
+    got = attention.linear_attention_backward(dy, q, k, v, decay, scale=0.1, offsets=offsets,
+                                              state=state, dfinal=dfinal)
+    grads, (ds, dsize) = ref.linear_attention_backward(dy, q, k, v, decay, 0.1, offsets, states,
+                                                       list(dfinal))
+    for name, x, (want, near, far) in zip(("dq", "dk", "dv"), got, grads):
+        within(x, want, 2 ** -8 * near + half(BF) * want.abs() + 2 ** -14 * far, name)
+    within(got[3], ds, 2 ** -14 * dsize, "dstate")
+
+
 def test_linear_attention_nothing_to_do():
     q, k, v, decay, _ = linear_case(3, [4], 2, 2, 2, 2, 64, 64)
     empty = offsets_of([0, 0])
