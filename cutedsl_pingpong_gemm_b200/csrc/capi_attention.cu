@@ -56,7 +56,8 @@ int check_heads(const char* name, const cpg_heads* x, int64_t tokens, int64_t ch
 }
 
 // ------------------------------------------------------------------------- norm and rotation
-constexpr int kGradBlocks = 148 * 4;  // of both parts together
+constexpr int kGradBlocks = 148 * 4;  // of both parts together, at most
+constexpr int64_t kManyThreads = int64_t(148) * 2048 * 4;
 
 // Address bits that some head of x has set (of the lowest ones).
 uint64_t address_bits(const cpg_heads* x, int64_t tokens) {
@@ -159,6 +160,7 @@ cpg::HeadParams head_params(const NormRope& n) {
     }
     h.w = i == 0 ? n.wq : n.wk;
     h.w_f32 = n.dtype_w == CPG_DTYPE_F32 ? 1 : 0;
+    h.w_vec = !misaligned(h.w, 16) ? 1 : 0;
     h.heads = x->heads;
   }
   p.table = n.table;
@@ -188,8 +190,9 @@ int head_vector(const NormRope& n) {
   return static_cast<int>(bits & (~bits + 1)) / eb;
 }
 
-// f(type, vector, lanes, pairs a lane) for the sizes at hand: the fewest lanes that hold a head.
-template <typename T, int V, typename F>
+// f(type, vector, lanes, pairs a lane, heads at a time) for the sizes at hand: the fewest lanes that hold
+// a head, and Many heads at a time where there are more threads than the SMs hold at once.
+template <typename T, int V, int Many, typename F>
 int by_lanes(const NormRope& n, F&& f) {
   using std::integral_constant;
   const int vectors = n.channels / V;
@@ -200,46 +203,52 @@ int by_lanes(const NormRope& n, F&& f) {
   }
   const integral_constant<int, V> v;
   const integral_constant<int, 1> one;
-  if (pairs <= 4) return f(T{}, v, integral_constant<int, 4>{}, one);
-  if (pairs <= 8) return f(T{}, v, integral_constant<int, 8>{}, one);
-  if (pairs <= 16) return f(T{}, v, integral_constant<int, 16>{}, one);
+  auto heads = [&](auto lanes, auto each) {
+    const int64_t rows = n.tokens * (int64_t(n.q->heads) + (n.k != nullptr ? n.k->heads : 0));
+    if (rows * decltype(lanes)::value > kManyThreads)
+      return f(T{}, v, lanes, each, integral_constant<int, V * sizeof(T) == 16 ? Many : 2>{});
+    return f(T{}, v, lanes, each, one);
+  };
+  if (pairs <= 4) return heads(integral_constant<int, 4>{}, one);
+  if (pairs <= 8) return heads(integral_constant<int, 8>{}, one);
+  if (pairs <= 16) return heads(integral_constant<int, 16>{}, one);
   const integral_constant<int, 32> warp;
   // At most kHeadMaxChannels / V / 2 pairs: V = 8 has 16, V = 4 32, V = 2 64, V = 1 128.
   if constexpr (V <= 4) {
-    if (pairs <= 32) return f(T{}, v, warp, one);
+    if (pairs <= 32) return heads(warp, one);
   }
   if constexpr (V <= 2) {
-    if (pairs <= 64) return f(T{}, v, warp, integral_constant<int, 2>{});
+    if (pairs <= 64) return heads(warp, integral_constant<int, 2>{});
   }
   if constexpr (V == 1) {
-    if (pairs <= 128) return f(T{}, v, warp, integral_constant<int, 4>{});
+    if (pairs <= 128) return heads(warp, integral_constant<int, 4>{});
   }
   return fail(CPG_ERR_UNSUPPORTED, "%d channels", n.channels);
 }
 
-template <typename F>
+template <int Many, typename F>
 int by_head(const NormRope& n, F&& f) {
   const int v = head_vector(n);
   if (n.q->dtype == CPG_DTYPE_BF16) {
     using B = __nv_bfloat16;
-    if (v == 8) return by_lanes<B, 8>(n, f);
-    if (v == 4) return by_lanes<B, 4>(n, f);
-    if (v == 2) return by_lanes<B, 2>(n, f);
-    return by_lanes<B, 1>(n, f);
+    if (v == 8) return by_lanes<B, 8, Many>(n, f);
+    if (v == 4) return by_lanes<B, 4, Many>(n, f);
+    if (v == 2) return by_lanes<B, 2, Many>(n, f);
+    return by_lanes<B, 1, Many>(n, f);
   }
-  if (v == 4) return by_lanes<float, 4>(n, f);
-  if (v == 2) return by_lanes<float, 2>(n, f);
-  return by_lanes<float, 1>(n, f);
+  if (v == 4) return by_lanes<float, 4, Many>(n, f);
+  if (v == 2) return by_lanes<float, 2, Many>(n, f);
+  return by_lanes<float, 1, Many>(n, f);
 }
 
-// Blocks of each part in the gradient, in proportion to their heads and at most one per row.
-void grad_blocks(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t* blocks) {
+// Blocks of each part in the gradient, of `all`, in proportion to their heads and at most one per row.
+void grad_blocks(int64_t tokens, int32_t q_heads, int32_t k_heads, int all, int32_t* blocks) {
   const int64_t heads = int64_t(q_heads) + k_heads;
   for (int i = 0; i < 2; ++i) {
     const int64_t h = i == 0 ? q_heads : k_heads;
     blocks[i] = h == 0 ? 0
                        : static_cast<int32_t>(std::max<int64_t>(
-                             1, std::min<int64_t>(tokens * h, kGradBlocks * h / heads)));
+                             1, std::min<int64_t>(tokens * h, all * h / heads)));
   }
 }
 
@@ -537,13 +546,15 @@ int cpg_norm_rope(const cpg_heads* q, const cpg_heads* k, int64_t tokens, int32_
   const int rc = check_norm_rope(n, false);
   if (rc != CPG_OK || tokens == 0) return rc;
   const cpg::HeadParams p = head_params(n);
-  const int64_t rows = tokens * (int64_t(p.part[0].heads) + p.part[1].heads);
-  return by_head(n, [&](auto type, auto v, auto lanes, auto pairs) {
-    constexpr int kRows = cpg::kHeadThreads / decltype(lanes)::value;
+  return by_head<4>(n, [&](auto type, auto v, auto lanes, auto pairs, auto heads) {
+    constexpr int kHeads = decltype(heads)::value;
+    constexpr int kUnits = cpg::kHeadThreads / decltype(lanes)::value;
+    const int64_t units = tokens * ((p.part[0].heads + kHeads - 1) / kHeads +
+                                    (p.part[1].heads + kHeads - 1) / kHeads);
     return launch("head norm kernel", true,
                   &cpg::head_norm_kernel<decltype(type), decltype(v)::value,
-                                         decltype(lanes)::value, decltype(pairs)::value>,
-                  static_cast<unsigned>((rows + kRows - 1) / kRows), cpg::kHeadThreads, 0,
+                                         decltype(lanes)::value, decltype(pairs)::value, kHeads>,
+                  static_cast<unsigned>((units + kUnits - 1) / kUnits), cpg::kHeadThreads, 0,
                   static_cast<cudaStream_t>(stream), 1, p);
   });
 }
@@ -556,7 +567,7 @@ int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, in
   const int rc = check_norm_sizes(tokens, int64_t(q_heads) + k_heads, channels);
   if (rc != CPG_OK) return rc;
   int32_t blocks[2];
-  grad_blocks(tokens, q_heads, k_heads, blocks);
+  grad_blocks(tokens, q_heads, k_heads, kGradBlocks, blocks);
   *bytes = (int64_t(blocks[0]) + blocks[1]) * channels * 4;
   return CPG_OK;
 }
@@ -579,7 +590,11 @@ int cpg_norm_rope_backward(const cpg_heads* dq, const cpg_heads* dk, const cpg_h
   if (dk_weight != nullptr && k == nullptr)
     return fail(CPG_ERR_NULL, "the gradient of k's weight needs k");
   cpg::HeadParams p = head_params(n);
-  grad_blocks(tokens, p.part[0].heads, p.part[1].heads, p.blocks);
+  // As many as are on the SMs at once: two of 16-byte vectors each (8191 tokens x 40 heads x 128, BF16:
+  // 54 us, 60 us with four), four of narrower ones (8192 x 32 x 75: 176 us with two, 98 us).
+  const bool wide = tokens > 0 && head_vector(n) * bytes_of(q->dtype) == 16;
+  grad_blocks(tokens, p.part[0].heads, p.part[1].heads, wide ? kGradBlocks / 2 : kGradBlocks,
+              p.blocks);
   int64_t bytes = 0;
   rc = cpg_norm_rope_workspace(tokens, p.part[0].heads, p.part[1].heads, channels, &bytes);
   if (rc != CPG_OK) return rc;
@@ -588,10 +603,11 @@ int cpg_norm_rope_backward(const cpg_heads* dq, const cpg_heads* dk, const cpg_h
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   p.partial = static_cast<float*>(workspace);
   if (tokens > 0) {
-    rc = by_head(n, [&](auto type, auto v, auto lanes, auto pairs) {
+    rc = by_head<2>(n, [&](auto type, auto v, auto lanes, auto pairs, auto heads) {
       return launch("head norm gradient kernel", true,
                     &cpg::head_norm_grad_kernel<decltype(type), decltype(v)::value,
-                                                decltype(lanes)::value, decltype(pairs)::value>,
+                                                decltype(lanes)::value, decltype(pairs)::value,
+                                                decltype(heads)::value>,
                     static_cast<unsigned>(p.blocks[0] + p.blocks[1]), cpg::kHeadThreads, 0, st, 1,
                     p);
     });

@@ -30,6 +30,7 @@ struct HeadPart {
   int64_t x_token, x_head, dy_token, dy_head, y_token, y_head;
   int32_t heads;
   int32_t w_f32;
+  int32_t w_vec;  // it starts on 16 bytes
 };
 
 struct HeadParams {
@@ -105,23 +106,56 @@ __device__ __forceinline__ void load_angles(const float* p, bool vec, float* f) 
   for (int i = 0; i < N; ++i) f[i] = p[i];
 }
 
-// Turns the pair by its angles (Back: by their negatives).
-template <int V, bool Back>
-__device__ __forceinline__ void turn(const HeadParams& p, const HeadPair& h, int64_t position,
-                                     float* a, float* b) {
+// Cosines and sines of a lane's pair: of its V angles, or, where neighbours are turned, of a's V / 2,
+// then b's.
+template <int V>
+struct HeadTurn {
+  float c[V], s[V];
+};
+
+template <int V>
+__device__ __forceinline__ void load_turn(const HeadParams& p, const HeadPair& h, int64_t position,
+                                          HeadTurn<V>& t) {
   const bool known = position >= 0 && position < p.table_rows;
   const float* cos = p.table + (known ? position : 0) * p.table_ld;
-  const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    t.c[i] = 1.f;
+    t.s[i] = 0.f;
+  }
+  if (p.half == 0) return;
+  if (!known) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.c[i] = __uint_as_float(0x7fc00000u);
+    return;
+  }
   if (h.turned) {
-    float c[V], s[V];
-    load_angles<V>(cos + h.angle, p.table_vec != 0, c);
-    load_angles<V>(cos + p.half + h.angle, p.table_vec != 0, s);
+    load_angles<V>(cos + h.angle, p.table_vec != 0, t.c);
+    load_angles<V>(cos + p.half + h.angle, p.table_vec != 0, t.s);
+  } else if (V > 1 && h.inside) {
+    constexpr int N = V / 2 > 0 ? V / 2 : 1;
+    if (h.a >= 0 && h.a < 2 * p.half) {
+      load_angles<N>(cos + h.a / 2, p.table_vec != 0, t.c);
+      load_angles<N>(cos + p.half + h.a / 2, p.table_vec != 0, t.s);
+    }
+    if (h.b >= 0 && h.b < 2 * p.half) {
+      load_angles<N>(cos + h.b / 2, p.table_vec != 0, t.c + V / 2);
+      load_angles<N>(cos + p.half + h.b / 2, p.table_vec != 0, t.s + V / 2);
+    }
+  }
+}
+
+// Turns the pair by its angles (Back: by their negatives).
+template <int V, bool Back>
+__device__ __forceinline__ void turn(const HeadParams& p, const HeadPair& h, const HeadTurn<V>& t,
+                                     float* a, float* b) {
+  if (h.turned) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float ci = known ? c[i] : nan, si = Back ? -s[i] : s[i];
+      const float s = Back ? -t.s[i] : t.s[i];
       const float x = a[i], y = b[i];
-      a[i] = fmaf(x, ci, -y * si);
-      b[i] = fmaf(y, ci, x * si);
+      a[i] = fmaf(x, t.c[i], -y * s);
+      b[i] = fmaf(y, t.c[i], x * s);
     }
   } else if (V > 1 && h.inside) {
 #pragma unroll
@@ -129,31 +163,24 @@ __device__ __forceinline__ void turn(const HeadParams& p, const HeadPair& h, int
       float* f = v == 0 ? a : b;
       const int32_t at = v == 0 ? h.a : h.b;
       if (at < 0 || at >= 2 * p.half) continue;
-      constexpr int N = V / 2 > 0 ? V / 2 : 1;
-      float c[N], s[N];
-      load_angles<N>(cos + at / 2, p.table_vec != 0, c);
-      load_angles<N>(cos + p.half + at / 2, p.table_vec != 0, s);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
-        const float ci = known ? c[i] : nan, si = Back ? -s[i] : s[i];
+        const int j = v * (V / 2) + i;
+        const float s = Back ? -t.s[j] : t.s[j];
         const float x = f[2 * i], y = f[2 * i + 1];
-        f[2 * i] = fmaf(x, ci, -y * si);
-        f[2 * i + 1] = fmaf(y, ci, x * si);
+        f[2 * i] = fmaf(x, t.c[j], -y * s);
+        f[2 * i + 1] = fmaf(y, t.c[j], x * s);
       }
     }
   }
 }
 
-// Loads may not go through the read-only path: y may be x.
+// V elements as they lie.  Not through the read-only path: y may be x.
 template <typename T, int V>
-__device__ __forceinline__ void load_head(const T* head, int32_t at, float* f) {
+__device__ __forceinline__ typename RowAccess<T, V * static_cast<int>(sizeof(T))>::Data load_head(
+    const T* head, int32_t at) {
   using A = RowAccess<T, V * static_cast<int>(sizeof(T))>;
-  if (at >= 0) {
-    A::unpack(A::template load_all<false>(head + at), f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = 0.f;
-  }
+  return at >= 0 ? A::template load_all<false>(head + at) : A::zero();
 }
 
 template <typename T, int V>
@@ -167,6 +194,21 @@ __device__ __forceinline__ void load_weight(const HeadPart& h, int32_t at, float
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = at >= 0 ? 1.f : 0.f;
   if (h.w == nullptr || at < 0) return;
+  if constexpr (V >= 4) {
+    if (h.w_vec) {  // it starts on 16 bytes, so that every vector does on its size
+      if (h.w_f32) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+          RowAccess<float, 16>::unpack(RowAccess<float, 16>::template load_all<false>(
+                                           static_cast<const float*>(h.w) + at + 4 * i),
+                                       f + 4 * i);
+      } else {
+        using A = RowAccess<__nv_bfloat16, 2 * V>;
+        A::unpack(A::template load_all<false>(static_cast<const __nv_bfloat16*>(h.w) + at), f);
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i)
     f[i] = h.w_f32 ? static_cast<const float*>(h.w)[at + i]
@@ -180,57 +222,82 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-template <typename T, int V, int L, int NP>
-__global__ void __launch_bounds__(kHeadThreads) head_norm_kernel(const HeadParams p) {
+// A group of L lanes takes HB heads of one part of a token: the angles and the weights are loaded
+// once, and all of its heads before the first is used.
+template <typename T, int V, int L, int NP, int HB>
+__global__ void __launch_bounds__(kHeadThreads, 3) head_norm_kernel(const HeadParams p) {
   kernel_begins();
+  using A = RowAccess<T, V * static_cast<int>(sizeof(T))>;
   const int32_t sub = threadIdx.x % L;
-  const uint32_t heads = static_cast<uint32_t>(p.part[0].heads + p.part[1].heads);
-  const uint32_t row = blockIdx.x * (kHeadThreads / L) + threadIdx.x / L;
-  const uint32_t rows = static_cast<uint32_t>(p.tokens) * heads;
-  const bool has = row < rows;  // the others take part in the shuffles
-  const uint32_t token = has ? row / heads : 0u;
-  const uint32_t head = has ? row - token * heads : 0u;
-  const bool key = head >= static_cast<uint32_t>(p.part[0].heads);
+  const uint32_t parts[2] = {(p.part[0].heads + HB - 1u) / HB, (p.part[1].heads + HB - 1u) / HB};
+  const uint32_t per = parts[0] + parts[1];
+  const uint32_t unit = blockIdx.x * (kHeadThreads / L) + threadIdx.x / L;
+  const uint32_t units = static_cast<uint32_t>(p.tokens) * per;
+  const bool has = unit < units;  // the others take part in the shuffles
+  const uint32_t token = has ? unit / per : 0u;
+  const uint32_t place = has ? unit - token * per : 0u;
+  const bool key = place >= parts[0];
   const HeadPart& h = p.part[key ? 1 : 0];
-  const int64_t index = key ? head - p.part[0].heads : head;
-  const T* x = static_cast<const T*>(h.x) + token * h.x_token + index * h.x_head;
-  T* y = static_cast<T*>(h.y) + token * h.y_token + index * h.y_head;
-  float a[NP][V], b[NP][V];
+  const int32_t first = static_cast<int32_t>(key ? place - parts[0] : place) * HB;
+  const int32_t heads = has ? min(h.heads - first, HB) : 0;
+  const T* x = static_cast<const T*>(h.x) + token * h.x_token + first * h.x_head;
+  T* y = static_cast<T*>(h.y) + token * h.y_token + first * h.y_head;
   HeadPair at[NP];
-  float squares = 0.f;
+  typename A::Data raw[HB][NP][2];
 #pragma unroll
-  for (int n = 0; n < NP; ++n) {
-    at[n] = head_pair<V>(p, sub + n * L);
-    load_head<T, V>(x, has ? at[n].a : -1, a[n]);
-    load_head<T, V>(x, has ? at[n].b : -1, b[n]);
-  }
+  for (int n = 0; n < NP; ++n) at[n] = head_pair<V>(p, sub + n * L);
 #pragma unroll
-  for (int n = 0; n < NP; ++n)
+  for (int j = 0; j < HB; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) squares = fmaf(a[n][i], a[n][i], fmaf(b[n][i], b[n][i], squares));
-  const float r = rsqrtf(sum_lanes<L>(squares) / static_cast<float>(p.d) + p.eps);
-  if (!has) return;
+    for (int n = 0; n < NP; ++n) {
+      raw[j][n][0] = load_head<T, V>(x + j * h.x_head, j < heads ? at[n].a : -1);
+      raw[j][n][1] = load_head<T, V>(x + j * h.x_head, j < heads ? at[n].b : -1);
+    }
   const int64_t position = p.positions[token];
+  HeadTurn<V> angles[NP];
+  float wa[NP][V], wb[NP][V];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
-    float w[V];
-    load_weight<V>(h, at[n].a, w);
+    load_turn<V>(p, at[n], position, angles[n]);
+    load_weight<V>(h, at[n].a, wa[n]);
+    load_weight<V>(h, at[n].b, wb[n]);
+  }
+  const float inv_d = 1.f / static_cast<float>(p.d);
 #pragma unroll
-    for (int i = 0; i < V; ++i) a[n][i] *= r * w[i];
-    load_weight<V>(h, at[n].b, w);
+  for (int j = 0; j < HB; ++j) {
+    float a[NP][V], b[NP][V];
+    float squares = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) b[n][i] *= r * w[i];
-    turn<V, false>(p, at[n], position, a[n], b[n]);
-    store_head<T, V>(y, at[n].a, p.d, a[n]);
-    store_head<T, V>(y, at[n].b, p.d, b[n]);
+    for (int n = 0; n < NP; ++n) {
+      A::unpack(raw[j][n][0], a[n]);
+      A::unpack(raw[j][n][1], b[n]);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        squares = fmaf(a[n][i], a[n][i], fmaf(b[n][i], b[n][i], squares));
+    }
+    const float r = rsqrtf(fmaf(sum_lanes<L>(squares), inv_d, p.eps));
+    if (j >= heads) continue;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        a[n][i] *= r * wa[n][i];
+        b[n][i] *= r * wb[n][i];
+      }
+      turn<V, false>(p, at[n], angles[n], a[n], b[n]);
+      store_head<T, V>(y + j * h.y_head, at[n].a, p.d, a[n]);
+      store_head<T, V>(y + j * h.y_head, at[n].b, p.d, b[n]);
+    }
   }
 }
 
-// Gradient.  A block belongs to one part and walks its heads; each lane adds its channels' g n in
-// registers, the block's lanes add theirs in shared memory and head_norm_sum_kernel the blocks'.
-template <typename T, int V, int L, int NP>
-__global__ void __launch_bounds__(kHeadThreads) head_norm_grad_kernel(const HeadParams p) {
+// Gradient.  A block belongs to one part and walks its tokens' heads, HB of a token at a time; each
+// lane adds its channels' g n in registers, the block's lanes add theirs in shared memory and
+// head_norm_sum_kernel the blocks'.
+template <typename T, int V, int L, int NP, int HB>
+__global__ void __launch_bounds__(kHeadThreads, 2) head_norm_grad_kernel(const HeadParams p) {
   kernel_begins();
+  using A = RowAccess<T, V * static_cast<int>(sizeof(T))>;
   constexpr int kGroups = kHeadThreads / L;
   __shared__ float sums[kHeadThreads * 2 * V * NP];  // [kGroups][d]
   const int32_t sub = threadIdx.x % L;
@@ -239,8 +306,8 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_grad_kernel(const Head
   const HeadPart& h = p.part[key ? 1 : 0];
   const uint32_t block = blockIdx.x - (key ? p.blocks[0] : 0);
   const uint32_t blocks = static_cast<uint32_t>(p.blocks[key ? 1 : 0]);
-  const uint32_t heads = static_cast<uint32_t>(h.heads);
-  const uint32_t rows = static_cast<uint32_t>(p.tokens) * heads;
+  const uint32_t per = (static_cast<uint32_t>(h.heads) + HB - 1u) / HB;
+  const uint32_t units = static_cast<uint32_t>(p.tokens) * per;
   HeadPair at[NP];
   float wa[NP][V], wb[NP][V], da[NP][V], db[NP][V];
 #pragma unroll
@@ -252,50 +319,64 @@ __global__ void __launch_bounds__(kHeadThreads) head_norm_grad_kernel(const Head
     for (int i = 0; i < V; ++i) da[n][i] = db[n][i] = 0.f;
   }
   const float inv_d = 1.f / static_cast<float>(p.d);
-  for (uint32_t first = block * kGroups; first < rows; first += blocks * kGroups) {
-    const uint32_t row = first + group;
-    const bool has = row < rows;
-    const uint32_t token = has ? row / heads : 0u;
-    const int64_t index = has ? row - token * heads : 0u;
-    const T* x = static_cast<const T*>(h.x) + token * h.x_token + index * h.x_head;
-    const T* dy = static_cast<const T*>(h.dy) + token * h.dy_token + index * h.dy_head;
-    T* dx = static_cast<T*>(h.y) + token * h.y_token + index * h.y_head;
+  for (uint32_t from = block * kGroups; from < units; from += blocks * kGroups) {
+    const uint32_t unit = from + group;
+    const bool has = unit < units;
+    const uint32_t token = has ? unit / per : 0u;
+    const int32_t first = static_cast<int32_t>(has ? unit - token * per : 0u) * HB;
+    const int32_t heads = has ? min(h.heads - first, HB) : 0;
+    const T* x = static_cast<const T*>(h.x) + token * h.x_token + first * h.x_head;
+    const T* dy = static_cast<const T*>(h.dy) + token * h.dy_token + first * h.dy_head;
+    T* dx = static_cast<T*>(h.y) + token * h.y_token + first * h.y_head;
+    typename A::Data rx[HB][NP][2], rg[HB][NP][2];
+#pragma unroll
+    for (int j = 0; j < HB; ++j)
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        rx[j][n][0] = load_head<T, V>(x + j * h.x_head, j < heads ? at[n].a : -1);
+        rx[j][n][1] = load_head<T, V>(x + j * h.x_head, j < heads ? at[n].b : -1);
+        rg[j][n][0] = load_head<T, V>(dy + j * h.dy_head, j < heads ? at[n].a : -1);
+        rg[j][n][1] = load_head<T, V>(dy + j * h.dy_head, j < heads ? at[n].b : -1);
+      }
+    HeadTurn<V> angles[NP];
     const int64_t position = p.positions[token];
-    float xa[NP][V], xb[NP][V], ga[NP][V], gb[NP][V];
-    float squares = 0.f, dot = 0.f;
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      load_head<T, V>(x, has ? at[n].a : -1, xa[n]);
-      load_head<T, V>(x, has ? at[n].b : -1, xb[n]);
-      load_head<T, V>(dy, has ? at[n].a : -1, ga[n]);
-      load_head<T, V>(dy, has ? at[n].b : -1, gb[n]);
-    }
+    for (int n = 0; n < NP; ++n) load_turn<V>(p, at[n], position, angles[n]);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      if (has) turn<V, true>(p, at[n], position, ga[n], gb[n]);
+    for (int j = 0; j < HB; ++j) {
+      float xa[NP][V], xb[NP][V], ga[NP][V], gb[NP][V];
+      float squares = 0.f, dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        squares = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], squares));
-        dot = fmaf(ga[n][i] * wa[n][i], xa[n][i], fmaf(gb[n][i] * wb[n][i], xb[n][i], dot));
+      for (int n = 0; n < NP; ++n) {
+        A::unpack(rx[j][n][0], xa[n]);
+        A::unpack(rx[j][n][1], xb[n]);
+        A::unpack(rg[j][n][0], ga[n]);
+        A::unpack(rg[j][n][1], gb[n]);
+        if (j < heads) turn<V, true>(p, at[n], angles[n], ga[n], gb[n]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          squares = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], squares));
+          dot = fmaf(ga[n][i] * wa[n][i], xa[n][i], fmaf(gb[n][i] * wb[n][i], xb[n][i], dot));
+        }
       }
-    }
-    squares = sum_lanes<L>(squares);
-    dot = sum_lanes<L>(dot);
-    const float r = rsqrtf(squares * inv_d + p.eps);
-    const float back = dot * inv_d * r * r;  // mean(u n) = r mean(u x), and n = x r
-    if (!has) continue;
+      squares = sum_lanes<L>(squares);
+      dot = sum_lanes<L>(dot);
+      const float r = rsqrtf(fmaf(squares, inv_d, p.eps));
+      const float back = dot * inv_d * r * r;  // mean(u n) = r mean(u x), and n = x r
+      if (j >= heads) continue;
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      float dxa[V], dxb[V];
+      for (int n = 0; n < NP; ++n) {
+        float dxa[V], dxb[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        da[n][i] = fmaf(ga[n][i] * r, xa[n][i], da[n][i]);
-        db[n][i] = fmaf(gb[n][i] * r, xb[n][i], db[n][i]);
-        dxa[i] = r * fmaf(-back, xa[n][i], ga[n][i] * wa[n][i]);
-        dxb[i] = r * fmaf(-back, xb[n][i], gb[n][i] * wb[n][i]);
+        for (int i = 0; i < V; ++i) {
+          da[n][i] = fmaf(ga[n][i] * r, xa[n][i], da[n][i]);
+          db[n][i] = fmaf(gb[n][i] * r, xb[n][i], db[n][i]);
+          dxa[i] = r * fmaf(-back, xa[n][i], ga[n][i] * wa[n][i]);
+          dxb[i] = r * fmaf(-back, xb[n][i], gb[n][i] * wb[n][i]);
+        }
+        store_head<T, V>(dx + j * h.y_head, at[n].a, p.d, dxa);
+        store_head<T, V>(dx + j * h.y_head, at[n].b, p.d, dxb);
       }
-      store_head<T, V>(dx, at[n].a, p.d, dxa);
-      store_head<T, V>(dx, at[n].b, p.d, dxb);
     }
   }
 #pragma unroll
