@@ -101,6 +101,13 @@ def heads(name, t, device=None, tokens=None, channels=None):
         _lib.HeadsC(t.data_ptr() or None, step[0], step[1], size[1], code))
 
 
+def fresh_heads(like, dtype=None):
+    """A contiguous tensor of this shape and its C description."""
+    t = torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+    _, h, d = like.shape
+    return t, ctypes.byref(_lib.HeadsC(t.data_ptr() or None, h * d, d, h, FLOAT_CODES[t.dtype]))
+
+
 def same_heads(name, t, shape, dtype, device):
     """C description of heads of this shape and type."""
     if t is None:

@@ -19,7 +19,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._tensors import FLOAT_CODES, call, error, float_code, heads, matrix, ptr, same_heads, vector
+from ._tensors import (FLOAT_CODES, call, error, float_code, fresh_heads, heads, matrix, ptr,
+                       same_heads, vector)
 
 
 def rope_table(length: int, rotary: int, *, base: float = 10000.0, device="cuda"):
@@ -69,6 +70,18 @@ def _norm_rope_args(q, k, q_weight, k_weight, table, positions, eps, interleaved
                             ptr(positions), 1 if interleaved else 0)
 
 
+def _pair_outputs(out, q, k, q_name, k_name):
+    """Outputs like q and k (k may be None) and their descriptions."""
+    if out is None:
+        q_out, qo = fresh_heads(q)
+        k_out, ko = (None, None) if k is None else fresh_heads(k)
+    else:
+        q_out, k_out = out
+        qo = same_heads(q_name, q_out, q.shape, q.dtype, q.device)
+        ko = None if k is None else same_heads(k_name, k_out, k.shape, k.dtype, q.device)
+    return q_out, k_out, qo, ko
+
+
 def norm_rope(q, k, q_weight, k_weight, table, positions, *, eps: float = 1e-6,
               interleaved: bool = False, out=None):
     """Norm and rotation of every head: ``y = R(x / sqrt(mean(x^2) + eps) * weight)``.
@@ -81,12 +94,7 @@ def norm_rope(q, k, q_weight, k_weight, table, positions, *, eps: float = 1e-6,
     Returns ``(q_out, k_out)``, contiguous unless given as ``out``; ``out`` may be ``(q, k)``."""
     t, d, q_c, k_c, args = _norm_rope_args(q, k, q_weight, k_weight, table, positions, eps,
                                            interleaved)
-    if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=q.device))
-    q_out, k_out = out
-    qo = same_heads("q's output", q_out, q.shape, q.dtype, q.device)
-    ko = None if k is None else same_heads("k's output", k_out, k.shape, k.dtype, q.device)
+    q_out, k_out, qo, ko = _pair_outputs(out, q, k, "q's output", "k's output")
     call(_lib.load().cpg_norm_rope, "norm_rope", q.device, q_c, k_c, *args, qo, ko)
     return q_out, k_out if k is not None else None
 
@@ -102,12 +110,7 @@ def norm_rope_backward(dq, dk, q, k, q_weight, k_weight, table, positions, *, ep
     dev = q.device
     dq_c = same_heads("dq", dq, q.shape, q.dtype, dev)
     dk_c = None if k is None else same_heads("dk", dk, k.shape, k.dtype, dev)
-    if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=dev),
-               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev))
-    dq_in, dk_in = out
-    qo = same_heads("dq_in", dq_in, q.shape, q.dtype, dev)
-    ko = None if k is None else same_heads("dk_in", dk_in, k.shape, k.dtype, dev)
+    dq_in, dk_in, qo, ko = _pair_outputs(out, q, k, "dq_in", "dk_in")
     dwq = None if q_weight is None else torch.empty(d, dtype=torch.float32, device=dev)
     dwk = None if k_weight is None else torch.empty(d, dtype=torch.float32, device=dev)
     lib = _lib.load()
@@ -153,6 +156,17 @@ def _slots(slots, n, device):
     return None if slots is None else vector("slots", slots, (n,), torch.int32, device)
 
 
+def _attention_output(out, v, problem):
+    """``out`` [tokens, heads, dv], or a new one in v's type, and its description."""
+    if out is None:
+        like = v if v.shape[1] == problem.heads else v[:, :1].expand(-1, problem.heads, -1)
+        return fresh_heads(like)
+    if out.dtype not in FLOAT_CODES:
+        raise error(_lib.CPG_ERR_DTYPE, f"out must be BF16 or FP32, got {out.dtype}")
+    shape = (problem.tokens, problem.heads, problem.dv)
+    return out, same_heads("out", out, shape, out.dtype, v.device)
+
+
 def _states(name, s, problem, n, slots, device):
     """A pool of FP32 states [places, heads, dk, dv] (places = n without slots)."""
     if s is None:
@@ -185,12 +199,7 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     b = _sequences(offsets, dev)
     p, problem, q_c, k_c, v_c = _linear_args(q, k, v, log_decay, scale, b)
     _slots(slots, b, dev)
-    shape = (problem.tokens, problem.heads, problem.dv)
-    if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    elif out.dtype not in FLOAT_CODES:
-        raise error(_lib.CPG_ERR_DTYPE, f"out must be BF16 or FP32, got {out.dtype}")
-    o_c = same_heads("out", out, shape, out.dtype, dev)
+    out, o_c = _attention_output(out, v, problem)
     if final is True:
         if slots is not None:
             raise error(_lib.CPG_ERR_UNSUPPORTED, "with slots, final must be a pool to write to")
@@ -225,9 +234,10 @@ def linear_attention_backward(dy, q, k, v, log_decay, *, scale: float = 1.0, off
     y_c = same_heads("dy", dy, (problem.tokens, problem.heads, problem.dv), torch.bfloat16, dev)
     fresh = out is None
     if fresh:
-        out = tuple(torch.empty(x.shape, dtype=torch.bfloat16, device=dev) for x in (q, k, v))
-    outs = [same_heads(name, x, like.shape, torch.bfloat16, dev)
-            for name, x, like in zip(("dq", "dk", "dv"), out, (q, k, v))]
+        out, outs = zip(*(fresh_heads(x) for x in (q, k, v)))
+    else:
+        outs = [same_heads(name, x, like.shape, torch.bfloat16, dev)
+                for name, x, like in zip(("dq", "dk", "dv"), out, (q, k, v))]
     if dstate is None and state is not None:
         dstate = torch.empty((b, problem.heads, problem.dk, problem.dv), dtype=torch.float32,
                              device=dev)
@@ -255,12 +265,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale: float = 1.0, slot
     p, problem, q_c, k_c, v_c = _linear_args(q, k, v, log_decay, scale, 0)
     t = problem.tokens
     _slots(slots, t, dev)
-    shape = (t, problem.heads, problem.dv)
-    if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    elif out.dtype not in FLOAT_CODES:
-        raise error(_lib.CPG_ERR_DTYPE, f"out must be BF16 or FP32, got {out.dtype}")
-    o_c = same_heads("out", out, shape, out.dtype, dev)
+    out, o_c = _attention_output(out, v, problem)
     if state is None:
         raise error(_lib.CPG_ERR_NULL, "state must be given")
     s_c = _states("state", state, problem, t, slots, dev)

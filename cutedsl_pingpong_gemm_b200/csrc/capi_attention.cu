@@ -420,13 +420,16 @@ int device_ready(int* sms) {
 // and 3.5 us where all SMs share the bandwidth.  Cutting sequences costs a pass over B and C for the
 // segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
 // channels 1480 -> XX us.  The lengths are known to the device alone: the mean stands for them.
+// Ragged sequences that stay whole are begun in the order of their lengths (`sorted`) where there is
+// more than one unit per SM.
 struct LinearCut {
   int64_t length, items;
+  bool sorted;
 };
 
 LinearCut linear_cut(const cpg_linear_problem* p) {
   constexpr int64_t kSms = 148, kMostCut = 1024;
-  if (p->sequences == 0 || p->tokens == 0) return {0, 0};
+  if (p->sequences == 0 || p->tokens == 0) return {0, 0, false};
   const int64_t mean = (p->tokens + p->sequences - 1) / p->sequences;
   const int64_t chunks = (mean + cpg::kChunk - 1) / cpg::kChunk;
   const int64_t units = int64_t(p->sequences) * p->heads;
@@ -434,7 +437,9 @@ LinearCut linear_cut(const cpg_linear_problem* p) {
   const double whole = chunks * (units < kSms ? 2.8 : 3.5 * waves);
   double best = whole;
   int64_t cut = 0;
-  if (units > kMostCut) return {0, 0};
+  const bool sorted = units > kSms && p->sequences > 1 && p->sequences <= cpg::kMostSorted;
+  const LinearCut uncut{0, sorted ? p->sequences : 0, sorted};
+  if (units > kMostCut) return uncut;
   for (int64_t length = 2; length < std::min<int64_t>(chunks, 128); ++length) {
     const int64_t segments = (chunks + length - 1) / length;
     const int64_t turns = (segments * units + kSms - 1) / kSms;
@@ -446,20 +451,20 @@ LinearCut linear_cut(const cpg_linear_problem* p) {
       cut = length;
     }
   }
-  if (cut == 0) return {0, 0};
-  return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences};
+  if (cut == 0) return uncut;
+  return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences, false};
 }
 
-// Workspace of a cut pass: the segments' states, the table of segments.
+// Workspace of a pass: the segments' states, the table of segments or sequences.
 struct LinearSpace {
   int64_t items, first, count, bytes;  // offsets in bytes (the states are at 0)
 };
 LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut) {
-  if (cut.length == 0) return {0, 0, 0, 0};
+  if (cut.items == 0) return {0, 0, 0, 0};
   LinearSpace r;
-  r.items = cut.items * p->heads * p->dk * p->dv * 4;
+  r.items = cut.length == 0 ? 0 : cut.items * p->heads * p->dk * p->dv * 4;
   r.first = r.items + cut.items * static_cast<int64_t>(sizeof(cpg::LinearItem));
-  r.count = r.first + (int64_t(p->sequences) + 1) * 4;
+  r.count = r.first + (cut.length == 0 ? 0 : (int64_t(p->sequences) + 1) * 4);
   r.bytes = (r.count + 4 + 15) / 16 * 16;
   return r;
 }
@@ -498,20 +503,25 @@ int run_pass(const cpg_linear_problem* p, cpg::LinearParams r, bool reverse, voi
   r.exact = r.final != nullptr ? 1 : 0;
   r.timeout_ns = kTimeoutNs;
   const LinearCut cut = linear_cut(p);
-  if (cut.length == 0)
-    return run_chunks<true>(r, reverse, int64_t(r.sequences) * r.heads, sms, st);
+  const int64_t units = int64_t(r.sequences) * r.heads;
+  if (cut.items == 0) return run_chunks<true>(r, reverse, units, sms, st);
   const LinearSpace at = linear_space(p, cut);
   char* const bytes = static_cast<char*>(space);
   auto* items = reinterpret_cast<cpg::LinearItem*>(bytes + at.items);
   auto* first = reinterpret_cast<int32_t*>(bytes + at.first);
   auto* count = reinterpret_cast<int32_t*>(bytes + at.count);
+  r.items = items;
+  r.item_count = count;
+  if (cut.length == 0) {
+    rc = launch("sequence order kernel", true, &cpg::linear_order_kernel, 1, 1024, 0, st, 1,
+                r.offsets, r.tokens, r.sequences, items, count);
+    return rc != CPG_OK ? rc : run_chunks<true>(r, reverse, units, sms, st);
+  }
   rc = launch("segment table kernel", true, &cpg::linear_items_kernel, 1, cpg::kItemThreads, 0, st,
               1, r.offsets, r.tokens, r.sequences, static_cast<int32_t>(cut.length),
               reverse ? 1 : 0, items, count, first);
   if (rc != CPG_OK) return rc;
-  r.items = items;
   r.first_item = first;
-  r.item_count = count;
   r.segments = reinterpret_cast<float*>(bytes);
   rc = run_chunks<false>(r, reverse, cut.items * r.heads, sms, st);
   if (rc != CPG_OK) return rc;

@@ -80,6 +80,27 @@ __device__ __forceinline__ int64_t linear_place(const int32_t* slots, int32_t s,
   return at >= 0 && at < places ? at : -1;
 }
 
+// The sequences as one item each, the longest first (equal ones in order).  One block.
+constexpr int kMostSorted = 2048;
+
+__global__ void __launch_bounds__(1024)
+    linear_order_kernel(const int32_t* offsets, int64_t tokens, int32_t sequences,
+                        LinearItem* items, int32_t* item_count) {
+  kernel_begins();
+  __shared__ int32_t counts[kMostSorted];
+  for (int32_t s = threadIdx.x; s < sequences; s += 1024)
+    counts[s] = static_cast<int32_t>(linear_span(offsets, s, tokens).count);
+  __syncthreads();
+  for (int32_t s = threadIdx.x; s < sequences; s += 1024) {
+    const int32_t mine = counts[s];
+    int32_t rank = 0;
+    for (int32_t j = 0; j < sequences; ++j)
+      rank += counts[j] > mine || (counts[j] == mine && j < s) ? 1 : 0;
+    items[rank] = {s, static_cast<int32_t>(linear_span(offsets, s, tokens).first), mine, 0, 1};
+  }
+  if (threadIdx.x == 0) *item_count = sequences;
+}
+
 // The segments of `length` tokens (whole chunks) of every sequence, one after the other in the order of
 // work; an empty sequence has one without tokens.  One block.
 constexpr int kItemThreads = 1024;

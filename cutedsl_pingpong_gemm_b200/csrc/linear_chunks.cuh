@@ -139,9 +139,9 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_16x256b_x8(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], "
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
       "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
           taddr),
@@ -151,6 +151,18 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
       "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -266,6 +278,24 @@ __device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
+// A lane's share of 16 rows x 64 columns of the state in TMEM (the 16x256b layout): rows row and row + 8,
+// columns col, col + 1 and those 8, 16, ... further on.  Eight rows' 32-byte sectors an access, where a
+// row in each lane would touch 32 rows.
+struct StatePart {
+  int32_t row, col;
+  uint32_t tmem;
+};
+template <int DC>
+__device__ __forceinline__ StatePart state_part(uint32_t warp, uint32_t lane, int32_t part) {
+  const int32_t half = part & 1, box = part >> 1;
+  return {static_cast<int32_t>((warp & 3u) * 32 + 16 * half + lane / 4),
+          64 * box + 2 * static_cast<int32_t>(lane & 3u),
+          (static_cast<uint32_t>(16 * half) << 16) + 64 * box};
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // e^(g n) from g / ln 2, 1 for n = 0 whatever g.
 __device__ __forceinline__ float decay_power(float g2, int32_t n) {
   return n == 0 ? 1.f : exp2f(g2 * static_cast<float>(n));
@@ -276,8 +306,7 @@ __device__ __forceinline__ uint32_t tile_offset(uint32_t r, uint32_t piece, uint
   return (piece >> 3) * rows * 128u + r * 128u + (((piece & 7u) ^ (r & 7u)) << 4);
 }
 
-// What a block does: units u = blockIdx.x, + gridDim.x, ... (a sequence's or a segment's tokens of one
-// head) and their chunks.
+// What a block does: units (a sequence's or a segment's tokens of one head) and their chunks.
 struct LinearUnit {
   int32_t head;
   int64_t first, count;
@@ -397,7 +426,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const ptx::WaitCtx ctx{abort_flag, &linear_status_word, p.timeout_ns};
   const int32_t units = (p.items != nullptr ? *p.item_count : p.sequences) * p.heads;
-  const int32_t step = static_cast<int32_t>(gridDim.x);
+  // Units in rounds of one per block, to and fro: in order of their lengths, that evens out the blocks.
+  auto unit_at = [](int32_t round) {
+    const int32_t step = static_cast<int32_t>(gridDim.x), b = static_cast<int32_t>(blockIdx.x);
+    return round * step + (round & 1 ? step - 1 - b : b);
+  };
   // Thread of a warpgroup: the token of the chunk, or the row of the state, that it has, and the TMEM
   // lanes of its warp.
   const int32_t i = static_cast<int32_t>(threadIdx.x & 127u);
@@ -413,7 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // ---------------------------------------------------------------------------- producer
     if (lane == 0) {
       const uint64_t policy = ptx::policy_evict_first();
-      for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
         const LinearUnit unit = linear_unit<Out>(p, u);
         const int32_t ha = unit.head / p.a.share, hb = unit.head / p.b.share,
                       hc = unit.head / p.c.share;
@@ -486,7 +519,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       constexpr uint32_t kState = linear_idesc(DC, true, true);
       const uint32_t a_k = ptx::sw128_desc_lo(base + L::kA);  // A along its channels
       const uint32_t s_mn = desc_lo_mn(base + L::kS, DA * 128);
-      for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+      for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
         const LinearUnit unit = linear_unit<Out>(p, u);
         bool state = unit.from != nullptr;
 #pragma unroll 1
@@ -568,7 +601,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else if (warp < 4) {
     // ----------------------------------------------------------- infinities and NaN in a box of C
     const uint32_t box = warp - 2;
-    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+    for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
       const LinearUnit unit = linear_unit<Out>(p, u);
       const uint32_t unit_first = n * kChunk;  // place of the unit's first token in the block's work
 #pragma unroll 1
@@ -631,7 +664,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     float* powers = reinterpret_cast<float*>(base_ptr + L::kPowers) + 64 * w;
     const float* own = powers + 32 + lane;
     const float* others = powers + (Reverse ? 32 : 0);
-    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+    for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
       const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       __syncwarp();
@@ -698,7 +731,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // ------------------------------------------------------------------------------ output
     constexpr int kCols = DC / 2;  // of each of the two warps that share TMEM lanes
     const int32_t col0 = static_cast<int32_t>((warp - 8) / 4) * kCols;
-    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+    for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
       const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       const uint32_t unit_first = n * kChunk;
@@ -783,7 +816,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else if (warp >= 16 && warp < 20) {
     // --------------------------------------------------------------------------- the state
     const uint32_t mine = lanes + kColState;
-    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+    for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
       const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       const uint32_t unit_first = n * kChunk;
@@ -801,29 +834,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         continue;
       }
-      if (from != nullptr) {
+      if (from != nullptr && unit.transposed) {
 #pragma unroll 1
-        for (int32_t col = 0; col < DC; col += 32) {
-          uint32_t s[32];
-          if (unit.transposed) {
+        for (int32_t col = 0; col < DC; col += 16) {
+          uint32_t s[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(starting(col + k));
-          } else {  // 16 bytes at a time (dc is a multiple of 8)
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (i < p.da && col + k < p.dc)
-                v = *reinterpret_cast<const float4*>(from + i * p.dc + col + k);
-              s[k] = __float_as_uint(unit.from_factor * v.x);
-              s[k + 1] = __float_as_uint(unit.from_factor * v.y);
-              s[k + 2] = __float_as_uint(unit.from_factor * v.z);
-              s[k + 3] = __float_as_uint(unit.from_factor * v.w);
-            }
-          }
+          for (int k = 0; k < 16; ++k) s[k] = __float_as_uint(starting(col + k));
           __syncwarp();
-          tmem_st_32x32b_x32(mine + col, s);
+          tmem_st_32x32b_x16(mine + col, s);
         }
         tmem_st_wait();
+      } else if (from != nullptr) {
+#pragma unroll 1
+        for (int32_t part = 0; part < DC / 32; ++part) {
+          const StatePart at = state_part<DC>(warp, lane, part);
+          const float* tile = from + at.row * p.dc + at.col;
+          uint32_t s[32];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float2 v = make_float2(0.f, 0.f);
+            if (at.row + 8 * (k & 1) < p.da && at.col + 8 * (k / 2) < p.dc)
+              v = *reinterpret_cast<const float2*>(tile + 8 * (k & 1) * p.dc + 8 * (k / 2));
+            s[2 * k] = __float_as_uint(unit.from_factor * v.x);
+            s[2 * k + 1] = __float_as_uint(unit.from_factor * v.y);
+          }
+          __syncwarp();
+          tmem_st_16x256b_x8(mine + at.tmem, s);
+        }
+        tmem_st_wait();
+      }
+      // The next unit's on its way from memory meanwhile.
+      if (const int32_t next = unit_at(r + 1); Out && next < units) {
+        const LinearUnit later = linear_unit<Out>(p, next);
+        if (later.from != nullptr)
+          for (int32_t line = i; line < p.da * p.dc / 32; line += 128)
+            prefetch_l2(later.from + 32 * line);
       }
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
@@ -869,26 +914,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (!ok || !(ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
       ptx::tc_fence_after();
       if (to != nullptr) {
+        const bool spoilt = *last_bad > unit_first;
 #pragma unroll 1
-        for (int32_t col = 0; col < DC; col += 16) {
-          uint32_t s[16];
+        for (int32_t part = 0; part < DC / 32; ++part) {
+          const StatePart at = state_part<DC>(warp, lane, part);
+          float* tile = to + at.row * p.dc + at.col;
+          uint32_t s[32];
           __syncwarp();
-          ptx::tmem_ld_32x32b_x16(mine + col, s);
+          tmem_ld_16x256b_x8(mine + at.tmem, s);
           ptx::tmem_ld_wait();
-          if (*last_bad > unit_first) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (bad[col + k] > unit_first) s[k] = 0x7fc00000u;
-          }
-          if (i < p.da) {
-#pragma unroll
-            for (int k = 0; k < 16; k += 4)
-              if (col + k < p.dc)
-                *reinterpret_cast<float4*>(to + i * p.dc + col + k) =
-                    make_float4(unit.to_factor * __uint_as_float(s[k]),
-                                unit.to_factor * __uint_as_float(s[k + 1]),
-                                unit.to_factor * __uint_as_float(s[k + 2]),
-                                unit.to_factor * __uint_as_float(s[k + 3]));
+          for (int k = 0; k < 16; ++k) {
+            const int32_t col = at.col + 8 * (k / 2);
+            float2 v = make_float2(unit.to_factor * __uint_as_float(s[2 * k]),
+                                   unit.to_factor * __uint_as_float(s[2 * k + 1]));
+            if (spoilt) {
+              if (bad[col] > unit_first) v.x = __uint_as_float(0x7fc00000u);
+              if (bad[col + 1] > unit_first) v.y = __uint_as_float(0x7fc00000u);
+            }
+            if (at.row + 8 * (k & 1) < p.da && col < p.dc)
+              *reinterpret_cast<float2*>(tile + 8 * (k & 1) * p.dc + 8 * (k / 2)) = v;
           }
         }
       }
@@ -896,7 +941,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   } else if (warp >= 20) {
     // ----------------------------------------------------------------------------- left . B
-    for (int32_t u = blockIdx.x; u < units && ok; u += step) {
+    for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
       const LinearUnit unit = linear_unit<Out>(p, u);
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
 #pragma unroll 1
