@@ -257,7 +257,7 @@ int check_linear(const cpg_linear_problem* p) {
   if (p == nullptr) return fail(CPG_ERR_NULL, "the problem is NULL");
   if (p->tokens < 0 || p->tokens > kMaxRows)
     return fail(CPG_ERR_INVALID_SHAPE, "%lld tokens", static_cast<long long>(p->tokens));
-  if (p->sequences < 0 || p->heads < 1 || int64_t(p->sequences) * p->heads > kMaxRows)
+  if (p->sequences < 0 || p->heads < 1 || int64_t(p->sequences) * p->heads > kMaxRows / 4)
     return fail(CPG_ERR_INVALID_SHAPE, "%d sequences x %d heads", p->sequences, p->heads);
   if (p->dk < 8 || p->dk > CPG_LINEAR_MAX_CHANNELS || p->dk % 8 != 0 || p->dv < 8 ||
       p->dv > CPG_LINEAR_MAX_CHANNELS || p->dv % 8 != 0)
@@ -397,10 +397,8 @@ int device_ready(int* sms) {
     auto both = [&](auto da, auto dc) {
       constexpr int kDA = decltype(da)::value, kDC = decltype(dc)::value;
       constexpr uint32_t kBytes = cpg::ChunkLayout<kDA, kDC>::kBytes;
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, false, false>, kBytes);
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, false, true>, kBytes);
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, true, false>, kBytes);
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, true, true>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, false>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, true>, kBytes);
     };
     const std::integral_constant<int, 64> d64;
     const std::integral_constant<int, 128> d128;
@@ -427,15 +425,14 @@ struct LinearCut {
   bool sorted;
 };
 
-LinearCut linear_cut(const cpg_linear_problem* p) {
+LinearCut linear_cut(const cpg_linear_problem* p, int passes) {
   constexpr int64_t kSms = 148, kMostCut = 1024;
   if (p->sequences == 0 || p->tokens == 0) return {0, 0, false};
   const int64_t mean = (p->tokens + p->sequences - 1) / p->sequences;
   const int64_t chunks = (mean + cpg::kChunk - 1) / cpg::kChunk;
-  const int64_t units = int64_t(p->sequences) * p->heads;
+  const int64_t units = int64_t(p->sequences) * p->heads * passes;
   const int64_t waves = (units + kSms - 1) / kSms;
-  const double whole = chunks * (units < kSms ? 2.8 : 3.5 * waves);
-  double best = whole;
+  double best = chunks * (units < kSms ? 2.8 : 3.5 * waves);
   int64_t cut = 0;
   const bool sorted = units > kSms && p->sequences > 1 && p->sequences <= cpg::kMostSorted;
   const LinearCut uncut{0, sorted ? p->sequences : 0, sorted};
@@ -455,90 +452,120 @@ LinearCut linear_cut(const cpg_linear_problem* p) {
   return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences, false};
 }
 
-// Workspace of a pass: the segments' states, the table of segments or sequences.
+// Workspace of passes that run together: the segments' states of each, then the table of segments or
+// sequences in their order and one against it.
 struct LinearSpace {
-  int64_t items, first, count, bytes;  // offsets in bytes (the states are at 0)
+  int64_t states, tables, table;  // bytes of one pass's states, where the tables begin, bytes of one
+  int64_t first, count, bytes;    // offsets within a table, all bytes
 };
-LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut) {
-  if (cut.items == 0) return {0, 0, 0, 0};
+LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut, int passes) {
+  if (cut.items == 0) return {};
   LinearSpace r;
-  r.items = cut.length == 0 ? 0 : cut.items * p->heads * p->dk * p->dv * 4;
-  r.first = r.items + cut.items * static_cast<int64_t>(sizeof(cpg::LinearItem));
+  r.states = cut.length == 0 ? 0 : cut.items * p->heads * p->dk * p->dv * 4;
+  r.tables = r.states * passes;
+  r.first = cut.items * static_cast<int64_t>(sizeof(cpg::LinearItem));
   r.count = r.first + (cut.length == 0 ? 0 : (int64_t(p->sequences) + 1) * 4);
-  r.bytes = (r.count + 4 + 15) / 16 * 16;
+  r.table = (r.count + 4 + 15) / 16 * 16;
+  r.bytes = r.tables + 2 * r.table;
   return r;
 }
 
 template <int DA, int DC, bool Out>
-int run_chunks(const cpg::LinearParams& r, bool reverse, int64_t units, int sms, cudaStream_t st) {
-  CUtensorMap maps[3] = {};
-  const cpg::LinearRows* x[3] = {&r.a, &r.b, &r.c};
-  for (int i = 0; i < 3 && r.tokens > 0; ++i) {
-    const int rc =
-        encode_heads(&maps[i], *x[i], r.tokens, r.heads / x[i]->share, i < 2 ? r.da : r.dc);
-    if (rc != CPG_OK) return rc;
+int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t st) {
+  cpg::LinearMaps maps = {};
+  for (int j = 0; j < b.passes && b.pass[0].tokens > 0; ++j) {
+    const cpg::LinearParams& r = b.pass[j];
+    const cpg::LinearRows* x[3] = {&r.a, &r.b, &r.c};
+    for (int i = 0; i < 3; ++i) {
+      const int rc = encode_heads(&maps.m[j][i], *x[i], r.tokens, r.heads / x[i]->share,
+                                  i < 2 ? r.da : r.dc);
+      if (rc != CPG_OK) return rc;
+    }
   }
-  auto fn = reverse ? &cpg::linear_chunks_kernel<DA, DC, true, Out>
-                    : &cpg::linear_chunks_kernel<DA, DC, false, Out>;
-  return launch("linear attention kernel", true, fn,
+  return launch("linear attention kernel", true, &cpg::linear_chunks_kernel<DA, DC, Out>,
                 static_cast<unsigned>(std::min<int64_t>(units, sms)), cpg::kChunkThreads,
-                cpg::ChunkLayout<DA, DC>::kBytes, st, 1, maps[0], maps[1], maps[2], r);
+                cpg::ChunkLayout<DA, DC>::kBytes, st, 1, maps, b);
 }
 
 template <bool Out>
-int run_chunks(const cpg::LinearParams& r, bool reverse, int64_t units, int sms, cudaStream_t st) {
-  if (r.da > 64)
-    return r.dc > 64 ? run_chunks<128, 128, Out>(r, reverse, units, sms, st)
-                     : run_chunks<128, 64, Out>(r, reverse, units, sms, st);
-  return r.dc > 64 ? run_chunks<64, 128, Out>(r, reverse, units, sms, st)
-                   : run_chunks<64, 64, Out>(r, reverse, units, sms, st);
+int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t st) {
+  if (b.pass[0].da > 64)
+    return b.pass[0].dc > 64 ? run_chunks<128, 128, Out>(b, units, sms, st)
+                             : run_chunks<128, 64, Out>(b, units, sms, st);
+  return b.pass[0].dc > 64 ? run_chunks<64, 128, Out>(b, units, sms, st)
+                           : run_chunks<64, 64, Out>(b, units, sms, st);
 }
 
-int run_pass(const cpg_linear_problem* p, cpg::LinearParams r, bool reverse, void* space,
-             cudaStream_t st) {
-  if (r.sequences == 0) return CPG_OK;
+// Passes of the same kernel (the same widths of 64 or 128 channels).
+int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cudaStream_t st) {
+  if (p->sequences == 0) return CPG_OK;
   int sms = 0;
   int rc = device_ready(&sms);
   if (rc != CPG_OK) return rc;
-  r.exact = r.final != nullptr ? 1 : 0;
-  r.timeout_ns = kTimeoutNs;
-  const LinearCut cut = linear_cut(p);
-  const int64_t units = int64_t(r.sequences) * r.heads;
-  if (cut.items == 0) return run_chunks<true>(r, reverse, units, sms, st);
-  const LinearSpace at = linear_space(p, cut);
-  char* const bytes = static_cast<char*>(space);
-  auto* items = reinterpret_cast<cpg::LinearItem*>(bytes + at.items);
-  auto* first = reinterpret_cast<int32_t*>(bytes + at.first);
-  auto* count = reinterpret_cast<int32_t*>(bytes + at.count);
-  r.items = items;
-  r.item_count = count;
-  if (cut.length == 0) {
-    rc = launch("sequence order kernel", true, &cpg::linear_order_kernel, 1, 1024, 0, st, 1,
-                r.offsets, r.tokens, r.sequences, items, count);
-    return rc != CPG_OK ? rc : run_chunks<true>(r, reverse, units, sms, st);
+  bool ways[2] = {false, false};
+  for (int j = 0; j < b.passes; ++j) {
+    if (b.pass[j].final != nullptr) b.exact = 1;
+    ways[b.pass[j].reverse] = true;
   }
-  rc = launch("segment table kernel", true, &cpg::linear_items_kernel, 1, cpg::kItemThreads, 0, st,
-              1, r.offsets, r.tokens, r.sequences, static_cast<int32_t>(cut.length),
-              reverse ? 1 : 0, items, count, first);
+  b.timeout_ns = kTimeoutNs;
+  const LinearCut cut = linear_cut(p, b.passes);
+  const int64_t heads = int64_t(p->heads) * b.passes;
+  if (cut.items == 0) return run_chunks<true>(b, p->sequences * heads, sms, st);
+  const LinearSpace at = linear_space(p, cut, b.passes);
+  char* const bytes = static_cast<char*>(space);
+  const cpg::LinearParams& any = b.pass[0];
+  for (int way = 0; way < 2; ++way) {
+    // The order of whole sequences is the same either way.
+    if (!(cut.length == 0 ? way == 0 : ways[way])) continue;
+    char* const table = bytes + at.tables + way * at.table;
+    auto* items = reinterpret_cast<cpg::LinearItem*>(table);
+    auto* first = reinterpret_cast<int32_t*>(table + at.first);
+    auto* count = reinterpret_cast<int32_t*>(table + at.count);
+    rc = cut.length == 0
+             ? launch("sequence order kernel", true, &cpg::linear_order_kernel, 1, 1024, 0, st, 1,
+                      any.offsets, any.tokens, any.sequences, items, count)
+             : launch("segment table kernel", true, &cpg::linear_items_kernel, 1,
+                      cpg::kItemThreads, 0, st, 1, any.offsets, any.tokens, any.sequences,
+                      static_cast<int32_t>(cut.length), way, items, count, first);
+    if (rc != CPG_OK) return rc;
+    for (int j = 0; j < b.passes; ++j) {
+      if (cut.length != 0 && b.pass[j].reverse != way) continue;
+      b.pass[j].items = items;
+      b.pass[j].item_count = count;
+      b.pass[j].first_item = first;
+      b.pass[j].segments = reinterpret_cast<float*>(bytes + j * at.states);
+    }
+  }
+  if (cut.length == 0) return run_chunks<true>(b, p->sequences * heads, sms, st);
+  rc = run_chunks<false>(b, cut.items * heads, sms, st);
   if (rc != CPG_OK) return rc;
-  r.first_item = first;
-  r.segments = reinterpret_cast<float*>(bytes);
-  rc = run_chunks<false>(r, reverse, cut.items * r.heads, sms, st);
-  if (rc != CPG_OK) return rc;
-  const unsigned parts = static_cast<unsigned>((r.da * r.dc + 1023) / 1024);
+  const unsigned parts = static_cast<unsigned>((any.da * any.dc + 1023) / 1024);
   rc = launch("segment state kernel", true, &cpg::linear_segments_kernel,
-              static_cast<unsigned>(r.sequences) * r.heads * parts, 256, 0, st, 1, r);
+              static_cast<unsigned>(p->sequences * heads) * parts, 256, 0, st, 1, b);
   if (rc != CPG_OK) return rc;
-  return run_chunks<true>(r, reverse, cut.items * r.heads, sms, st);
+  return run_chunks<true>(b, cut.items * heads, sms, st);
 }
 
-// FP32 sums of a head each, of the widest shared gradient.
-int64_t share_bytes(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
-                    int32_t v_heads) {
-  int64_t d = 0;
-  if (q_heads < p->heads || k_heads < p->heads) d = p->dk;
-  if (v_heads < p->heads) d = std::max<int64_t>(d, p->dv);
-  return p->tokens * p->heads * d * 4;
+// Passes of the gradient that run together: all three, or dq and dk before dv where the widths differ.
+bool same_width(const cpg_linear_problem* p) { return (p->dk > 64) == (p->dv > 64); }
+
+// Workspace: that of the passes, then FP32 sums of a head each for every gradient of shared heads.
+struct BackwardSpace {
+  int64_t grads[3], bytes;  // offsets of q's, k's and v's
+};
+BackwardSpace backward_space(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
+                             int32_t v_heads) {
+  BackwardSpace r;
+  r.bytes = 0;
+  for (int passes = 1; passes <= 3; ++passes)
+    if (same_width(p) ? passes == 3 : passes < 3)
+      r.bytes = std::max(r.bytes, linear_space(p, linear_cut(p, passes), passes).bytes);
+  const int32_t heads[3] = {q_heads, k_heads, v_heads}, channels[3] = {p->dk, p->dk, p->dv};
+  for (int i = 0; i < 3; ++i) {
+    r.grads[i] = r.bytes;
+    if (heads[i] < p->heads) r.bytes += p->tokens * p->heads * channels[i] * 4;
+  }
+  return r;
 }
 
 }  // namespace
@@ -638,8 +665,8 @@ int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads,
   if (rc != CPG_OK) return rc;
   if (q_heads < 1 || k_heads < 1 || v_heads < 1)
     return fail(CPG_ERR_INVALID_SHAPE, "%d, %d and %d heads", q_heads, k_heads, v_heads);
-  *bytes = linear_space(p, linear_cut(p)).bytes +
-           (backward ? share_bytes(p, q_heads, k_heads, v_heads) : 0);
+  *bytes = backward ? backward_space(p, q_heads, k_heads, v_heads).bytes
+                    : linear_space(p, linear_cut(p, 1), 1).bytes;
   return CPG_OK;
 }
 
@@ -665,10 +692,12 @@ int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const 
     return fail(CPG_ERR_NULL, "the workspace must have %lld bytes", static_cast<long long>(bytes));
   if (misaligned(workspace, 16))
     return fail(CPG_ERR_ALIGNMENT, "the workspace must start on 16 bytes");
-  cpg::LinearParams r = linear_params(p, q, k, v, p->dk, p->dv, out, log_decay, offsets);
-  set_state(&r, state, false, 1.f);
-  set_final(&r, final, 1.f);
-  return run_pass(p, r, false, workspace, static_cast<cudaStream_t>(stream));
+  cpg::LinearBatch b = {};
+  b.passes = 1;
+  b.pass[0] = linear_params(p, q, k, v, p->dk, p->dv, out, log_decay, offsets);
+  set_state(&b.pass[0], state, false, 1.f);
+  set_final(&b.pass[0], final, 1.f);
+  return run_passes(p, b, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* dy,
@@ -702,42 +731,55 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
   if (misaligned(workspace, 16))
     return fail(CPG_ERR_ALIGNMENT, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // The gradient of a head that several read: each one's in FP32, then their sum.
-  void* const share_space = static_cast<char*>(workspace) + linear_space(p, linear_cut(p)).bytes;
-  auto pass = [&](const cpg_heads* a, const cpg_heads* b, const cpg_heads* c, int32_t da,
-                  int32_t dc, const cpg_heads* o, bool reverse, const cpg_states* from,
-                  bool transposed, float factor, const cpg_states* to) {
-    const cpg_heads sums{share_space, int64_t(p->heads) * dc, dc, p->heads, CPG_DTYPE_F32};
-    const bool shared = o->heads < p->heads;
-    cpg::LinearParams r =
-        linear_params(p, a, b, c, da, dc, shared ? &sums : o, log_decay, offsets);
-    set_state(&r, from, transposed, factor);
-    set_final(&r, to, p->scale);
-    int e = run_pass(p, r, reverse, workspace, st);
-    if (e != CPG_OK || !shared || p->tokens == 0) return e;
-    const cpg::LinearShareParams s{static_cast<const float*>(share_space),
-                                   static_cast<__nv_bfloat16*>(o->ptr),
-                                   o->token_stride,
-                                   o->head_stride,
+  // dq, dk and dv as passes; the gradient of a head that several read: each one's in FP32 first.
+  const BackwardSpace space = backward_space(p, q->heads, k->heads, v->heads);
+  const cpg_heads* grads[3] = {dq, dk, dv};
+  cpg_heads outs[3];
+  for (int i = 0; i < 3; ++i) {
+    const int32_t d = i < 2 ? p->dk : p->dv;
+    outs[i] = *grads[i];
+    if (grads[i]->heads < p->heads)
+      outs[i] = {static_cast<char*>(workspace) + space.grads[i], int64_t(p->heads) * d, d, p->heads,
+                 CPG_DTYPE_F32};
+  }
+  cpg::LinearBatch b = {};
+  b.pass[0] = linear_params(p, dy, v, k, p->dv, p->dk, &outs[0], log_decay, offsets);
+  set_state(&b.pass[0], state, true, 1.f);
+  b.pass[1] = linear_params(p, v, dy, q, p->dv, p->dk, &outs[1], log_decay, offsets);
+  b.pass[1].reverse = 1;
+  set_state(&b.pass[1], dfinal, true, 1.f / p->scale);
+  b.pass[2] = linear_params(p, k, q, dy, p->dk, p->dv, &outs[2], log_decay, offsets);
+  b.pass[2].reverse = 1;
+  set_state(&b.pass[2], dfinal, false, 1.f / p->scale);
+  set_final(&b.pass[2], dstate, p->scale);
+  b.passes = same_width(p) ? 3 : 2;
+  rc = run_passes(p, b, workspace, st);
+  if (rc == CPG_OK && b.passes == 2) {
+    b.pass[0] = b.pass[2];
+    b.passes = 1;
+    rc = run_passes(p, b, workspace, st);
+  }
+  for (int i = 0; i < 3 && p->tokens > 0; ++i) {
+    if (rc != CPG_OK) return rc;
+    if (grads[i]->heads == p->heads) continue;
+    const int32_t d = i < 2 ? p->dk : p->dv;
+    const cpg::LinearShareParams s{static_cast<const float*>(outs[i].ptr),
+                                   static_cast<__nv_bfloat16*>(grads[i]->ptr),
+                                   grads[i]->token_stride,
+                                   grads[i]->head_stride,
                                    p->tokens,
-                                   o->heads,
-                                   p->heads / o->heads,
-                                   dc,
+                                   grads[i]->heads,
+                                   p->heads / grads[i]->heads,
+                                   d,
                                    offsets,
                                    p->sequences};
-    const int64_t n = p->tokens * o->heads * dc;
-    return launch("shared gradient kernel", true, &cpg::linear_share_kernel,
-                  static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 148 * 8)), 256, 0, st,
-                  1, s);
-  };
-  rc = pass(dy, v, k, p->dv, p->dk, dq, false, state, true, 1.f, nullptr);
-  if (rc == CPG_OK)
-    rc = pass(v, dy, q, p->dv, p->dk, dk, true, dfinal, true, 1.f / p->scale, nullptr);
-  if (rc == CPG_OK)
-    rc = pass(k, q, dy, p->dk, p->dv, dv, true, dfinal, false, 1.f / p->scale, dstate);
+    const int64_t n = p->tokens * grads[i]->heads * d / 8;
+    rc = launch("shared gradient kernel", true, &cpg::linear_share_kernel,
+                static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 148 * 8)), 256, 0, st, 1,
+                s);
+  }
   if (rc != CPG_OK || clear == 0 || offsets == nullptr || p->tokens == 0) return rc;
   cpg::LinearClearParams c = {};
-  const cpg_heads* grads[3] = {dq, dk, dv};
   for (int i = 0; i < 3; ++i) {
     c.p[i] = static_cast<__nv_bfloat16*>(grads[i]->ptr);
     c.token[i] = grads[i]->token_stride;

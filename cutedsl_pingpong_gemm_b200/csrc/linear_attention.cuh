@@ -56,8 +56,15 @@ struct LinearParams {
   const int32_t* first_item;     // [sequences + 1]
   float* segments;         // [items, heads, da, dc]: what the segment before adds to the state, then the
                            // state before each
-  int32_t exact;           // states to FP32 accuracy (they are outputs)
-  uint64_t timeout_ns;     // limit of a wait within the kernel
+  int32_t reverse;
+};
+
+// Passes over the same sequences and heads, side by side in one launch.
+struct LinearBatch {
+  LinearParams pass[3];
+  int32_t passes;
+  int32_t exact;        // states to FP32 accuracy (one is an output)
+  uint64_t timeout_ns;  // limit of a wait within the kernel
 };
 
 struct LinearSpan {
@@ -152,12 +159,15 @@ __global__ void __launch_bounds__(kItemThreads)
 
 // The state before every segment of a sequence that has several: the state before the previous one,
 // decayed by that one's tokens, plus what it adds.  Four neighbouring elements a thread; blockIdx.x:
-// sequence and head, then the elements.
-__global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams p) {
+// pass, sequence and head, then the elements.
+__global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch batch) {
   kernel_begins();
-  const int32_t size = p.da * p.dc;
+  const int32_t size = batch.pass[0].da * batch.pass[0].dc;
   const int32_t parts = (size + 1023) / 1024;
-  const int32_t pair = blockIdx.x / parts;
+  const int32_t each = batch.pass[0].sequences * batch.pass[0].heads;
+  int32_t pair = static_cast<int32_t>(blockIdx.x) / parts;
+  const LinearParams& p = batch.pass[pair / each];
+  pair %= each;
   const int32_t s = pair / p.heads, h = pair % p.heads;
   const int32_t e = (blockIdx.x % parts) * 1024 + static_cast<int32_t>(threadIdx.x) * 4;
   const int32_t first = p.first_item[s], last = p.first_item[s + 1] - 1;
@@ -237,15 +247,29 @@ __global__ void __launch_bounds__(256) linear_share_kernel(const LinearSharePara
     first = min(max(static_cast<int64_t>(p.offsets[0]), int64_t(0)), p.tokens);
     last = min(max(static_cast<int64_t>(p.offsets[p.sequences]), first), p.tokens);
   }
-  const int32_t row = p.heads * p.d;
+  const int32_t row = p.heads * p.d / 8;  // eight neighbouring channels a thread
   const int64_t n = (last - first) * row;
   for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += gridDim.x * int64_t(256)) {
     const int64_t t = first + i / row;
-    const int32_t h = static_cast<int32_t>(i % row) / p.d, x = static_cast<int32_t>(i % row) % p.d;
+    const int32_t e = static_cast<int32_t>(i % row) * 8;
+    const int32_t h = e / p.d, x = e % p.d;
     const float* from = p.partial + (t * p.heads + h) * int64_t(p.share) * p.d + x;
-    float s = 0.f;
-    for (int32_t j = 0; j < p.share; ++j) s += from[static_cast<int64_t>(j) * p.d];
-    p.out[t * p.token + h * p.head + x] = __float2bfloat16_rn(s);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int32_t j = 0; j < p.share; ++j, from += p.d) {
+      const float4 u = reinterpret_cast<const float4*>(from)[0];
+      const float4 v = reinterpret_cast<const float4*>(from)[1];
+      a.x += u.x;
+      a.y += u.y;
+      a.z += u.z;
+      a.w += u.w;
+      b.x += v.x;
+      b.y += v.y;
+      b.z += v.z;
+      b.w += v.w;
+    }
+    ptx::st_global_v4(p.out + t * p.token + h * p.head + x, ptx::pack_bf16x2(a.x, a.y),
+                      ptx::pack_bf16x2(a.z, a.w), ptx::pack_bf16x2(b.x, b.y),
+                      ptx::pack_bf16x2(b.z, b.w));
   }
 }
 

@@ -306,9 +306,15 @@ __device__ __forceinline__ uint32_t tile_offset(uint32_t r, uint32_t piece, uint
   return (piece >> 3) * rows * 128u + r * 128u + (((piece & 7u) ^ (r & 7u)) << 4);
 }
 
-// What a block does: units (a sequence's or a segment's tokens of one head) and their chunks.
+// Tensor maps of A, B and C of every pass.
+struct alignas(64) LinearMaps {
+  CUtensorMap m[3][3];
+};
+
+// What a block does: units (a pass's, a sequence's or a segment's tokens of one head) and their chunks.
 struct LinearUnit {
-  int32_t head;
+  int32_t pass, head;
+  bool reverse;
   int64_t first, count;
   int32_t chunks;
   const float* from;  // starting state, null: zeros
@@ -319,8 +325,12 @@ struct LinearUnit {
 
 // (Out of line: once per unit in each of eight roles.)
 template <bool Out>
-__device__ __noinline__ LinearUnit linear_unit(const LinearParams& p, int32_t u) {
+__device__ __noinline__ LinearUnit linear_unit(const LinearBatch& batch, int32_t each, int32_t u) {
   LinearUnit r = {};
+  r.pass = u / each;
+  u -= r.pass * each;
+  const LinearParams& p = batch.pass[r.pass];
+  r.reverse = p.reverse != 0;
   const int32_t at = u / p.heads;
   const int64_t size = static_cast<int64_t>(p.da) * p.dc;
   r.head = u - at * p.heads;
@@ -360,21 +370,18 @@ __device__ __noinline__ LinearUnit linear_unit(const LinearParams& p, int32_t u)
 }
 
 // The x-th chunk to be done: its first token and how many it has.
-template <bool Reverse>
 __device__ __forceinline__ int32_t chunk_at(const LinearUnit& u, int32_t x, int32_t* count) {
-  const int64_t at = static_cast<int64_t>(Reverse ? u.chunks - 1 - x : x) * kChunk;
+  const int64_t at = static_cast<int64_t>(u.reverse ? u.chunks - 1 - x : x) * kChunk;
   const int64_t left = u.count - at;
   *count = left < kChunk ? static_cast<int32_t>(left) : kChunk;
   return static_cast<int32_t>(u.first + at);
 }
 
 // Out false: only the state that each unit leaves, from zeros, and without A.
-template <int DA, int DC, bool Reverse, bool Out>
+template <int DA, int DC, bool Out>
 __global__ void __launch_bounds__(kChunkThreads, 1)
-    linear_chunks_kernel(const __grid_constant__ CUtensorMap tm_a,
-                         const __grid_constant__ CUtensorMap tm_b,
-                         const __grid_constant__ CUtensorMap tm_c,
-                         const __grid_constant__ LinearParams p) {
+    linear_chunks_kernel(const __grid_constant__ LinearMaps maps,
+                         const __grid_constant__ LinearBatch batch) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
   using L = ChunkLayout<DA, DC>;
   extern __shared__ uint8_t smem_raw[];
@@ -405,11 +412,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     ptx::fence_mbarrier_init_cluster();
     ptx::fence_proxy_async_shared();
   }
-  if (warp == 0 && lane == 0 && p.tokens > 0) {
-    ptx::prefetch_tensormap(&tm_a);
-    ptx::prefetch_tensormap(&tm_b);
-    ptx::prefetch_tensormap(&tm_c);
-  }
+  if (warp == 0 && lane < 3 && batch.pass[0].tokens > 0) ptx::prefetch_tensormap(&maps.m[0][lane]);
   if (warp == 1) {
     ptx::tmem_alloc<1>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     ptx::tmem_relinquish<1>();
@@ -424,8 +427,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const ptx::WaitCtx ctx{abort_flag, &linear_status_word, p.timeout_ns};
-  const int32_t units = (p.items != nullptr ? *p.item_count : p.sequences) * p.heads;
+  const ptx::WaitCtx ctx{abort_flag, &linear_status_word, batch.timeout_ns};
+  const LinearParams& any = batch.pass[0];
+  const int32_t each = (any.items != nullptr ? *any.item_count : any.sequences) * any.heads;
+  const int32_t units = each * batch.passes;
   // Units in rounds of one per block, to and fro: in order of their lengths, that evens out the blocks.
   auto unit_at = [](int32_t round) {
     const int32_t step = static_cast<int32_t>(gridDim.x), b = static_cast<int32_t>(blockIdx.x);
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint32_t n = 0;  // chunks done
   bool ok = true;
   // C's slot of chunk m and the parity of its phases.
-  const bool one_c = L::kShared && p.exact;
+  const bool one_c = L::kShared && batch.exact;
   auto c_slot = [&](uint32_t m) { return one_c ? 0u : m & 1u; };
   auto c_phase = [&](uint32_t m) { return one_c ? m & 1u : (m >> 1) & 1u; };
 
@@ -447,13 +452,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (lane == 0) {
       const uint64_t policy = ptx::policy_evict_first();
       for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-        const LinearUnit unit = linear_unit<Out>(p, u);
+        const LinearUnit unit = linear_unit<Out>(batch, each, u);
+        const LinearParams& p = batch.pass[unit.pass];
+        const CUtensorMap *tm_a = &maps.m[unit.pass][0], *tm_b = &maps.m[unit.pass][1],
+                          *tm_c = &maps.m[unit.pass][2];
         const int32_t ha = unit.head / p.a.share, hb = unit.head / p.b.share,
                       hc = unit.head / p.c.share;
 #pragma unroll 1
         for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
           int32_t count;
-          const int32_t t = chunk_at<Reverse>(unit, x, &count);
+          const int32_t t = chunk_at(unit, x, &count);
           const uint32_t slot = n & 1u;
           const uint32_t b = base + L::kB + slot * L::kTileA;
           const uint32_t c = base + L::kC + c_slot(n) * L::kTileC;
@@ -463,12 +471,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             break;
           ptx::mbar_arrive_expect_tx(b_full + 8 * slot, L::kTileA);
           for (int j = 0; j < DA / 64; ++j)
-            ptx::tma_load_3d(&tm_b, b + j * 16384, b_full + 8 * slot, 64 * j, hb, t, policy);
+            ptx::tma_load_3d(tm_b, b + j * 16384, b_full + 8 * slot, 64 * j, hb, t, policy);
           // What waits for room below comes into L2 meanwhile.
           if (Out)
-            for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_a, 64 * j, ha, t);
+            for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(tm_a, 64 * j, ha, t);
           if (one_c)
-            for (int j = 0; j < DC / 64; ++j) ptx::tma_prefetch_l2_3d(&tm_c, 64 * j, hc, t);
+            for (int j = 0; j < DC / 64; ++j) ptx::tma_prefetch_l2_3d(tm_c, 64 * j, hc, t);
           // C first unless its only slot is the last to become free.
           for (int turn = 0; turn < 2 && ok; ++turn) {
             if ((turn == 0) == one_c) {
@@ -477,14 +485,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 break;
               ptx::mbar_arrive_expect_tx(a_full, L::kTileA);
               for (int j = 0; j < DA / 64; ++j)
-                ptx::tma_load_3d(&tm_a, base + L::kA + j * 16384, a_full, 64 * j, ha, t, policy);
+                ptx::tma_load_3d(tm_a, base + L::kA + j * 16384, a_full, 64 * j, ha, t, policy);
             } else {
               if (!(ok = ptx::mbar_wait_brief(c_empty + 8 * c_slot(n), c_phase(n) ^ 1u, ctx,
                                               kSiteLinearProducer)))
                 break;
               ptx::mbar_arrive_expect_tx(cf, L::kTileC);
               for (int j = 0; j < DC / 64; ++j)
-                ptx::tma_load_3d(&tm_c, c + j * 16384, cf, 64 * j, hc, t, policy);
+                ptx::tma_load_3d(tm_c, c + j * 16384, cf, 64 * j, hc, t, policy);
             }
           }
           if (!ok) {
@@ -520,12 +528,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const uint32_t a_k = ptx::sw128_desc_lo(base + L::kA);  // A along its channels
       const uint32_t s_mn = desc_lo_mn(base + L::kS, DA * 128);
       for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-        const LinearUnit unit = linear_unit<Out>(p, u);
+        const LinearUnit unit = linear_unit<Out>(batch, each, u);
         bool state = unit.from != nullptr;
 #pragma unroll 1
         for (int32_t x = 0; x < unit.chunks && ok; ++x, ++n) {
           int32_t count;
-          chunk_at<Reverse>(unit, x, &count);
+          chunk_at(unit, x, &count);
           const uint32_t slot = n & 1u, twice = (n >> 1) & 1u, once = n & 1u;
           const uint32_t b = base + L::kB + slot * L::kTileA;
           const uint32_t c_mn = desc_lo_mn(base + L::kC + c_slot(n) * L::kTileC, 16384);
@@ -575,7 +583,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           ptx::tc_fence_after();
           uint32_t accumulate = state ? 1u : 0u;
 #pragma unroll 1
-          for (int j = 0; j < (p.exact ? 3 : 2); ++j) {
+          for (int j = 0; j < (batch.exact ? 3 : 2); ++j) {
             const uint32_t part =
                 desc_lo_mn(j == 0 ? b : base + (j == 1 ? L::kMid : L::kLo), 16384);
 #pragma unroll
@@ -602,12 +610,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // ----------------------------------------------------------- infinities and NaN in a box of C
     const uint32_t box = warp - 2;
     for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-      const LinearUnit unit = linear_unit<Out>(p, u);
+      const LinearUnit unit = linear_unit<Out>(batch, each, u);
+      const bool reverse = unit.reverse;
       const uint32_t unit_first = n * kChunk;  // place of the unit's first token in the block's work
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
-        chunk_at<Reverse>(unit, x, &count);
+        chunk_at(unit, x, &count);
         const uint32_t c = base + L::kC + c_slot(n) * L::kTileC + box * 16384;
         if (!(ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearScan)))
           break;
@@ -636,9 +645,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           uint32_t* mine = bad + 64 * box + 2 * lane;  // of the two channels a lane has
 #pragma unroll 1
-          for (int32_t place = Reverse ? kChunk - count : 0; place < (Reverse ? kChunk : count);
+          for (int32_t place = reverse ? kChunk - count : 0; place < (reverse ? kChunk : count);
                ++place) {
-            const int32_t row = Reverse ? kChunk - 1 - place : place;
+            const int32_t row = reverse ? kChunk - 1 - place : place;
             const uint32_t at = c + tile_offset(row, lane / 4, kChunk) + 4 * (lane & 3u);
             const uint32_t v = ptx::ld_shared_u32(at), f = not_finite(v);
             if (f == 0) continue;
@@ -663,10 +672,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // factor an exponent of one sign, so that none is above 1).
     float* powers = reinterpret_cast<float*>(base_ptr + L::kPowers) + 64 * w;
     const float* own = powers + 32 + lane;
-    const float* others = powers + (Reverse ? 32 : 0);
     for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-      const LinearUnit unit = linear_unit<Out>(p, u);
+      const LinearUnit unit = linear_unit<Out>(batch, each, u);
+      const LinearParams& p = batch.pass[unit.pass];
+      const bool reverse = unit.reverse;
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
+      const float* others = powers + (reverse ? 32 : 0);
+      // Which of the warp's tokens each sees.
+      const uint32_t seen = reverse ? 0xffffffffu << lane : 0xffffffffu >> (31u - lane);
       __syncwarp();
       powers[lane] = p.scale * decay_power(g2, 32 - static_cast<int32_t>(lane));
       powers[lane + 32] = p.scale * decay_power(g2, static_cast<int32_t>(lane));
@@ -674,13 +687,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
-        chunk_at<Reverse>(unit, x, &count);
+        chunk_at(unit, x, &count);
         if (!(ok = ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearScores))) break;
         ptx::tc_fence_after();
 #pragma unroll 1
         for (uint32_t blk = 0; blk < 4; ++blk) {
           uint32_t s[32];
-          if (Reverse ? blk < w : blk > w) {
+          if (reverse ? blk < w : blk > w) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) s[k] = 0u;
           } else {
@@ -690,13 +703,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
                 const float f = __uint_as_float(s[k]) * own[-k];
-                const bool seen = Reverse ? static_cast<int32_t>(lane) <= k
-                                          : static_cast<int32_t>(lane) >= k;
-                s[k] = seen ? __float_as_uint(f) : 0u;
+                s[k] = seen & (1u << k) ? __float_as_uint(f) : 0u;
               }
             } else {
               const int32_t first = static_cast<int32_t>(32 * blk);
-              const float r = decay_power(g2, Reverse ? first - i : i - first - 32);
+              const float r = decay_power(g2, reverse ? first - i : i - first - 32);
 #pragma unroll
               for (int k = 0; k < 32; k += 4) {
                 const float4 d = *reinterpret_cast<const float4*>(others + k);
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               }
             }
             // (In order, tokens past the end are later than any whose output is kept.)
-            if (Reverse && count < kChunk) {
+            if (reverse && count < kChunk) {
               const int32_t left = count - static_cast<int32_t>(32 * blk);
 #pragma unroll
               for (int k = 0; k < 32; ++k) s[k] = k < left ? s[k] : 0u;
@@ -732,14 +743,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     constexpr int kCols = DC / 2;  // of each of the two warps that share TMEM lanes
     const int32_t col0 = static_cast<int32_t>((warp - 8) / 4) * kCols;
     for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-      const LinearUnit unit = linear_unit<Out>(p, u);
+      const LinearUnit unit = linear_unit<Out>(batch, each, u);
+      const LinearParams& p = batch.pass[unit.pass];
+      const bool reverse = unit.reverse;
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       const uint32_t unit_first = n * kChunk;
       bool state = unit.from != nullptr;
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
-        const int64_t t = chunk_at<Reverse>(unit, x, &count);
+        const int64_t t = chunk_at(unit, x, &count);
         if (!(ok = ptx::mbar_wait_brief(o_full, n & 1u, ctx, kSiteLinearOutput))) break;
         ptx::tc_fence_after();
         const bool spoilt = *last_bad > unit_first;
@@ -754,7 +767,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int32_t at = token + 8 * r;
-            since[r] = p.scale * decay_power(g2, Reverse ? max(count - 1 - at, 0) : at + 1);
+            since[r] = p.scale * decay_power(g2, reverse ? max(count - 1 - at, 0) : at + 1);
             row[r] = (t + at) * p.o_token + unit.head * p.o_head;
           }
 #pragma unroll 1
@@ -776,7 +789,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const int32_t at = token + 8 * ((j >> 1) & 1);
                 const uint32_t first =
                     bad[col + 8 * (j / 4) + 2 * static_cast<int32_t>(lane & 3u) + (j & 1)];
-                const uint32_t here = n * kChunk + (Reverse ? kChunk - 1 - at : at) + 1;
+                const uint32_t here = n * kChunk + (reverse ? kChunk - 1 - at : at) + 1;
                 if (first > unit_first && here >= first) o[j] = 0x7fc00000u;
               }
             }
@@ -817,7 +830,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // --------------------------------------------------------------------------- the state
     const uint32_t mine = lanes + kColState;
     for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-      const LinearUnit unit = linear_unit<Out>(p, u);
+      const LinearUnit unit = linear_unit<Out>(batch, each, u);
+      const LinearParams& p = batch.pass[unit.pass];
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
       const uint32_t unit_first = n * kChunk;
       const float* from = unit.from;
@@ -865,7 +879,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       // The next unit's on its way from memory meanwhile.
       if (const int32_t next = unit_at(r + 1); Out && next < units) {
-        const LinearUnit later = linear_unit<Out>(p, next);
+        const LinearUnit later = linear_unit<Out>(batch, each, next);
         if (later.from != nullptr)
           for (int32_t line = i; line < p.da * p.dc / 32; line += 128)
             prefetch_l2(later.from + 32 * line);
@@ -873,7 +887,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
-        chunk_at<Reverse>(unit, x, &count);
+        chunk_at(unit, x, &count);
         const float decay = decay_power(g2, count);
         // The chunk before is done with the state and its copy (at a unit's first chunk: waited for
         // at the end of the last one).
@@ -942,16 +956,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else if (warp >= 20) {
     // ----------------------------------------------------------------------------- left . B
     for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
-      const LinearUnit unit = linear_unit<Out>(p, u);
+      const LinearUnit unit = linear_unit<Out>(batch, each, u);
+      const LinearParams& p = batch.pass[unit.pass];
+      const bool reverse = unit.reverse;
       const float g2 = p.log_decay[unit.head] * 1.4426950408889634f;
 #pragma unroll 1
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
-        chunk_at<Reverse>(unit, x, &count);
+        chunk_at(unit, x, &count);
         const uint32_t slot = n & 1u, twice = (n >> 1) & 1u;
         const uint32_t b = base + L::kB + slot * L::kTileA;
         const bool inside = i < count;
-        const float left = inside ? decay_power(g2, Reverse ? i + 1 : count - 1 - i) : 0.f;
+        const float left = inside ? decay_power(g2, reverse ? i + 1 : count - 1 - i) : 0.f;
         // In place of B, once the scores are made; the second part's tile is the chunk
         // before's until its product is done.
         ok = ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearLeft) &&
@@ -960,7 +976,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (ok && count < kChunk)
           ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearLeft);
         if (!ok) break;
-        if (p.exact) {
+        if (batch.exact) {
 #pragma unroll 1
           for (uint32_t piece = 0; piece < DA / 8; ++piece) {
             const uint32_t at = tile_offset(i, piece, kChunk);
