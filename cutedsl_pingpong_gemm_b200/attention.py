@@ -194,7 +194,7 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     Returns ``(out, final)``: ``out`` [T, H, dv] BF16 (FP32 if it is given so).
     Products are taken of BF16 values: the decayed scores and the state before each 128 tokens are
     rounded to BF16 for them, all sums and the states kept are FP32.  An infinity or a NaN in ``v``
-    may spoil its channel in the 127 outputs before it, as well as those after it."""
+    makes its channel NaN from its token on, and no output before it."""
     dev = q.device
     b = _sequences(offsets, dev)
     p, problem, q_c, k_c, v_c = _linear_args(q, k, v, log_decay, scale, b)
@@ -253,6 +253,15 @@ def linear_attention_backward(dy, q, k, v, log_decay, *, scale: float = 1.0, off
          ptr(log_decay), ptr(offsets), s_c, f_c, *outs, d_c, 1 if fresh else 0, ptr(work),
          size.value)
     return (*out, dstate)
+
+
+def status(device=None) -> int:
+    """0, or the code of the first wait within a linear attention kernel that ever ran out (10 s) on
+    this CUDA device (None: the current one).  Synchronises."""
+    code = ctypes.c_int32()
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().cpg_attention_status(ctypes.byref(code)), "status")
+    return code.value
 
 
 def linear_attention_step(q, k, v, log_decay, state, *, scale: float = 1.0, slots=None, out=None):

@@ -264,8 +264,8 @@ int check_linear(const cpg_linear_problem* p) {
     return fail(CPG_ERR_INVALID_SHAPE,
                 "dk = %d, dv = %d must be multiples of 8 from 8 to %d", p->dk, p->dv,
                 CPG_LINEAR_MAX_CHANNELS);
-  if (!std::isfinite(p->scale) || p->scale == 0.f)
-    return fail(CPG_ERR_INVALID_CONFIG, "scale must be finite and not 0");
+  if (!std::isfinite(p->scale) || !std::isfinite(1.f / p->scale))
+    return fail(CPG_ERR_INVALID_CONFIG, "scale and 1 / scale must be finite");
   return CPG_OK;
 }
 

@@ -514,6 +514,119 @@ def test_linear_attention_keeps_sequences_and_times_apart():
     assert torch.equal(got[278:350, 0], want[278:350, 0])  # a NaN key spoils no earlier output
 
 
+def test_linear_attention_backward_keeps_times_apart():
+    """A NaN in an operand reaches the gradients that are made of it and no others."""
+    q, k, v, decay, _ = linear_case(3, [300], 2, 2, 2, 2, 64, 64)
+    dy = normal(gen(5), 300, 2, 64)
+    f = attention.linear_attention_backward
+    want = f(dy, q, k, v, decay)[:3]
+    t = 200
+    # Which rows of head 0 of (dq, dk, dv) a NaN at token t makes NaN, at least in one channel.
+    later, earlier = set(range(t, 300)), set(range(t + 1))
+    reach = {"q": (set(), earlier, earlier), "k": (later, set(), {t}), "v": (later, {t}, set()),
+             "dy": ({t}, earlier, earlier)}
+    for name, rows in reach.items():
+        x = {"q": q, "k": k, "v": v, "dy": dy}
+        x[name] = x[name].clone()
+        x[name][t, 0, 5] = float("nan")
+        got = f(x["dy"], x["q"], x["k"], x["v"], decay)[:3]
+        for g, w, spoilt in zip(got, want, rows):
+            assert torch.equal(g[:, 1], w[:, 1])
+            keep = torch.tensor([i not in spoilt for i in range(300)])
+            assert torch.equal(g[keep, 0], w[keep, 0]), name
+            assert g[~keep, 0].isnan().any(dim=1).all(), name
+
+
+def test_linear_attention_infinities_in_several_places():
+    """Bad values in neighbouring chunks, in both boxes of channels and in two sequences of a block;
+    each channel is NaN from its first on, in the final state too."""
+    lengths = [300] * 3
+    q, k, v, decay, offsets = linear_case(4, lengths, 100, 100, 100, 100, 64, 128)
+    v = v.clone()
+    bad = [(10, 3, 7), (140, 3, 7), (290, 3, 100), (300, 3, 64), (301, 50, 0), (899, 99, 127)]
+    for t, h, c in bad:
+        v[t, h, c] = float("inf") if t % 2 else float("nan")
+    clean = torch.where(v.isfinite(), v, 0.0).bfloat16()
+    want, wf = attention.linear_attention(q, k, clean, decay, offsets=offsets, final=True)
+    got, gf = attention.linear_attention(q, k, v, decay, offsets=offsets, final=True)
+    for t, h, c in bad:
+        end = (t // 300 + 1) * 300
+        want[t:end, h, c] = float("nan")
+        wf[t // 300, h, :, c] = float("nan")
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(gf.isnan(), wf.isnan())
+    assert torch.equal(got[~got.isnan()], want[~want.isnan()])
+    assert torch.equal(gf[~gf.isnan()], wf[~wf.isnan()])
+
+
+def test_linear_attention_of_many_short_sequences():
+    lengths = [i % 4 for i in range(3000)]
+    q, k, v, decay, offsets = linear_case(4, lengths, 2, 2, 2, 2, 16, 16)
+    out, final = attention.linear_attention(q, k, v, decay, offsets=offsets, final=True)
+    check_forward(q, k, v, decay, offsets, 1.0, None, out, final)
+    some = offsets[:1501]  # few enough to be sorted by their lengths
+    part, ends = attention.linear_attention(q, k, v, decay, offsets=some, final=True)
+    n = int(some[-1])
+    assert torch.equal(part[:n], out[:n]) and torch.equal(ends, final[:1500])
+
+
+def test_rows_and_states_past_2_31_elements():
+    """Tokens 2^30 elements apart, and a pool of states of more than 2^31."""
+    wide = torch.empty(2 ** 31 + 4096, dtype=BF, device="cuda")
+    far = lambda h, d, at: wide.as_strided((3, h, d), (2 ** 30, d, 1), at)  # noqa: E731
+    g = gen(2)
+    q, k, v, out = (far(2, 64, 256 * i) for i in range(4))
+    near = [normal(g, 3, 2, 64) for _ in range(3)]
+    for x, y in zip((q, k, v), near):
+        x.copy_(y)
+    decay = torch.tensor([-0.1, -1.0], device="cuda")
+    attention.linear_attention(q, k, v, decay, out=out)
+    assert torch.equal(out, attention.linear_attention(*near, decay)[0])
+    dy = normal(g, 3, 2, 64)
+    got = attention.linear_attention_backward(dy, q, k, v, decay, out=(q, k, out))
+    want = attention.linear_attention_backward(dy, *near, decay)
+    assert torch.equal(out, want[2])
+    for x, y in zip((q, k), near):
+        x.copy_(y)
+    w = torch.ones(64, device="cuda")
+    table, pos = attention.rope_table(8, 64), torch.arange(3, device="cuda").int()
+    attention.norm_rope(q, k, w, w, table, pos, out=(q, k))
+    for x, y in zip((q, k), attention.norm_rope(*near[:2], w, w, table, pos)):
+        assert torch.equal(x, y)
+    del wide, q, k, v, out, got
+    places = 2 ** 31 // (32 * 128 * 128) + 2
+    pool = torch.empty(places, 32, 128, 128, device="cuda")
+    q, k, v = (normal(g, 2, 32, 128) for _ in range(3))
+    decay = -torch.rand(32, device="cuda", generator=g)
+    slots = torch.tensor([places - 1, 0], dtype=torch.int32, device="cuda")
+    small = normal(g, 2, 32, 128, 128, dtype=F32)
+    for f in (lambda s, slots: attention.linear_attention_step(q, k, v, decay, s, slots=slots),
+              lambda s, slots: attention.linear_attention(
+                  q, k, v, decay, offsets=torch.arange(3, device="cuda").int(), state=s, slots=slots,
+                  final=s)[0]):
+        pool[slots.long()] = small
+        mine = small.clone()
+        y = f(pool, slots)
+        assert torch.equal(y, f(mine, torch.arange(2, device="cuda").int()))
+        assert torch.equal(pool[slots.long()], mine)
+
+
+def test_calls_on_two_streams():
+    """The same operators at once on two streams, each with its own inputs."""
+    cases = [linear_case(s, [700, 900], 8, 8, 8, 8, 128, 128) for s in (1, 2)]
+    want = [attention.linear_attention(*c[:4], offsets=c[4], final=True) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [None, None]
+    for _ in range(5):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i] = attention.linear_attention(*c[:4], offsets=c[4], final=True)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert attention.status() == 0
+
+
 STEP = [(1, 1, 1, 1, 1, 8, 8), (4, 32, 32, 32, 32, 128, 128), (3, 2, 1, 4, 4, 64, 128),
         (7, 2, 2, 2, 2, 128, 40), (65, 1, 1, 2, 2, 72, 64), (300, 3, 3, 3, 3, 16, 24)]
 

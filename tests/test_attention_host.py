@@ -170,10 +170,11 @@ def test_linear_attention_refusals(lib):
         for bad in (dict(t=-1), dict(t=BIG), dict(h=0), dict(dk=0), dict(dk=7), dict(dk=12),
                     dict(dk=136), dict(dv=4), dict(dv=256), dict(b=-1)):
             assert f(p=problem(**bad)) == S, bad
-        for bad in (0.0, float("nan"), float("inf")):
+        for bad in (0.0, float("nan"), float("inf"), 1e-39):
             assert f(p=problem(scale=bad)) == C
         assert f(q=heads(dtype=F32)) == D and f(v=heads(dtype=I8)) == D
         assert f(q=heads(h=3)) == S and f(k=heads(h=16)) == S and f(v=heads(h=0)) == S
+        assert f(q=heads(ts=0)) == U and f(v=heads(hs=0)) == U  # give a shared head once
         assert f(q=heads(p=None)) == N and f(q=heads(p=4104)) == A
         assert f(k=heads(ts=68)) == A and f(v=heads(hs=12)) == A and f(out=heads(h=4)) == S
         assert f(st=states(p=None, places=9)) == N and f(st=states(p=4100, places=9)) == A
