@@ -526,7 +526,8 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
                       any.offsets, any.tokens, any.sequences, items, count)
              : launch("segment table kernel", true, &cpg::linear_items_kernel, 1,
                       cpg::kItemThreads, 0, st, 1, any.offsets, any.tokens, any.sequences,
-                      static_cast<int32_t>(cut.length), way, items, count, first);
+                      static_cast<int32_t>(cut.length), way, static_cast<int32_t>(cut.items), items,
+                      count, first);
     if (rc != CPG_OK) return rc;
     for (int j = 0; j < b.passes; ++j) {
       if (cut.length != 0 && b.pass[j].reverse != way) continue;

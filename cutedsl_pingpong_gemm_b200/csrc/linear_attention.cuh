@@ -109,51 +109,54 @@ __global__ void __launch_bounds__(1024)
 }
 
 // The segments of `length` tokens (whole chunks) of every sequence, one after the other in the order of
-// work; an empty sequence has one without tokens.  One block.
+// work; an empty sequence has one without tokens.  Offsets that decrease could make more than the table
+// has room for (`most`): those past it are left out.  One block.
 constexpr int kItemThreads = 1024;
 
 __global__ void __launch_bounds__(kItemThreads)
     linear_items_kernel(const int32_t* offsets, int64_t tokens, int32_t sequences, int32_t length,
-                        int32_t reverse, LinearItem* items, int32_t* item_count,
+                        int32_t reverse, int32_t most, LinearItem* items, int32_t* item_count,
                         int32_t* first_item) {
   kernel_begins();
-  __shared__ int32_t sums[kItemThreads / 32];
+  __shared__ int64_t sums[kItemThreads / 32];
   const int32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int32_t base = 0;
+  int64_t base = 0;
   for (int32_t from = 0; from < sequences; from += kItemThreads) {
     const int32_t s = from + static_cast<int32_t>(threadIdx.x);
     LinearSpan span = {0, 0};
     if (s < sequences) span = linear_span(offsets, s, tokens);
     int32_t n = s < sequences ? static_cast<int32_t>((span.count + length - 1) / length) : 0;
     if (s < sequences && n == 0) n = 1;
-    int32_t before = n;  // inclusive sum within the warp
+    int64_t before = n;  // inclusive sum within the warp
     for (int o = 1; o < 32; o *= 2) {
-      const int32_t v = __shfl_up_sync(0xffffffffu, before, o);
+      const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += v;
     }
     __syncthreads();
     if (lane == 31) sums[warp] = before;
     __syncthreads();
-    int32_t all = 0;
+    int64_t all = 0;
     for (int w = 0; w < kItemThreads / 32; ++w) {
       if (w == warp) before += all;
       all += sums[w];
     }
     if (s < sequences) {
-      const int32_t at = base + before - n;
+      const int32_t at = static_cast<int32_t>(min(base + before - n, static_cast<int64_t>(most)));
       first_item[s] = at;
-      for (int32_t k = 0; k < n; ++k) {
+      for (int32_t k = 0; k < min(n, most - at); ++k) {
         const int64_t first = static_cast<int64_t>(reverse ? n - 1 - k : k) * length;
         const int64_t left = span.count - first;
         items[at + k] = {s, static_cast<int32_t>(span.first + first),
-                         static_cast<int32_t>(left < length ? left : length), k, k == n - 1};
+                         static_cast<int32_t>(left < length ? left : length), k,
+                         k == n - 1 || at + k == most - 1};
       }
     }
     base += all;
   }
   if (threadIdx.x == 0) {
-    *item_count = base;
-    first_item[sequences] = base;
+    const int32_t all = static_cast<int32_t>(min(base, static_cast<int64_t>(most)));
+    *item_count = all;
+    first_item[sequences] = all;
   }
 }
 

@@ -6,6 +6,8 @@ attention rounds scores and chunk states to BF16 (2^-8 of `near`, the sum of the
 them), then the output (H |o|); the sums of products of up to 128 tokens and channels, and the
 states' two BF16 parts, keep 2^-15 of the terms' sizes `far`.  States: three BF16 parts of every
 addend and FP32 sums of at most a few hundred terms, 2^-17 of their sizes."""
+import ctypes
+
 import pytest
 import torch
 
@@ -498,6 +500,30 @@ def test_linear_attention_offsets_beyond_the_rows():
         assert torch.equal(final[b], end[0])
         if b == 2:
             assert torch.equal(out[140:200], one[50:])
+
+
+def test_linear_attention_offsets_that_decrease_stay_in_their_workspace():
+    """Offsets that go back and forth name more segments than the rows have; those past the
+    workspace are left out, and nothing behind it or in front of it changes."""
+    h, n = 2, 64
+    lib = _lib.load()
+    for t, sequences in ((8192, 3), (65536, 9)):
+        q, k, v, decay, _ = linear_case(3, [t], h, h, h, h, 64, 64)
+        offsets = torch.tensor([0, t] * ((sequences + 1) // 2), dtype=torch.int32, device="cuda")
+        p, problem, q_c, k_c, v_c = attention._linear_args(q, k, v, decay, 1.0, sequences)
+        size = ctypes.c_int64()
+        _lib.check(lib.cpg_linear_attention_workspace(p, h, h, h, 0, ctypes.byref(size)))
+        assert size.value > sequences * h * 64 * 64 * 4  # the sequences are cut
+        work = torch.full((n + size.value + n,), 7, dtype=torch.uint8, device="cuda")
+        out, o_c = attention._attention_output(None, v, problem)
+        final = torch.zeros(sequences, h, 64, 64, device="cuda")
+        f_c = attention._states("final", final, problem, sequences, None, q.device)
+        _lib.check(lib.cpg_linear_attention(
+            p, q_c, k_c, v_c, decay.data_ptr(), offsets.data_ptr(), None, f_c, o_c,
+            work.data_ptr() + n, size.value, torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert (work[:n] == 7).all() and (work[n + size.value:] == 7).all()
+        assert attention.status() == 0
 
 
 def test_linear_attention_keeps_sequences_and_times_apart():
