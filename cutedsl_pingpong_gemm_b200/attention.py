@@ -182,7 +182,8 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T``, ``o_t = scale * S_t^T q_t`` (S in FP32).
 
     ``q``, ``k`` [T, Hq, dk] and [T, Hk, dk], ``v`` [T, Hv, dv], BF16; ``log_decay`` FP32 [H], at
-    most 0; Hq, Hk and Hv divide H, and head h reads head h // (H // Hx) of each.  dk and dv are
+    most 0 (-inf: no state is kept); Hq, Hk and Hv divide H (at most 2^20), and head h reads head
+    h // (H // Hx) of each.  dk and dv are
     multiples of 8 up to 128, addresses and strides multiples of 16 bytes.
     ``offsets`` int32 [B + 1], read on the device: sequence b is the rows
     ``offsets[b] <= t < offsets[b + 1]`` (None: one sequence of all rows); rows outside are not

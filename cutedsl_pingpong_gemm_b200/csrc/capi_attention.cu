@@ -26,6 +26,7 @@ using cpg_capi::misaligned;
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
+constexpr int32_t kMaxLinearHeads = 1 << 20;
 constexpr int64_t kMaxStride = int64_t(1) << 38;  // elements; tensor maps take 2^40 bytes
 
 // Heads [tokens, heads, channels] with elements aligned to `bytes`; `written`: no two overlap.
@@ -257,7 +258,9 @@ int check_linear(const cpg_linear_problem* p) {
   if (p == nullptr) return fail(CPG_ERR_NULL, "the problem is NULL");
   if (p->tokens < 0 || p->tokens > kMaxRows)
     return fail(CPG_ERR_INVALID_SHAPE, "%lld tokens", static_cast<long long>(p->tokens));
-  if (p->sequences < 0 || p->heads < 1 || int64_t(p->sequences) * p->heads > kMaxRows / 4)
+  // (Heads: a token's channels of all of them are counted in 32 bits, a workspace's bytes in 64.)
+  if (p->sequences < 0 || p->heads < 1 || p->heads > kMaxLinearHeads ||
+      int64_t(p->sequences) * p->heads > kMaxRows / 4)
     return fail(CPG_ERR_INVALID_SHAPE, "%d sequences x %d heads", p->sequences, p->heads);
   if (p->dk < 8 || p->dk > CPG_LINEAR_MAX_CHANNELS || p->dk % 8 != 0 || p->dv < 8 ||
       p->dv > CPG_LINEAR_MAX_CHANNELS || p->dv % 8 != 0)

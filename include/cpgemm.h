@@ -432,7 +432,8 @@ int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, in
  * there are), NULL for one sequence of all tokens.  Rows outside are neither read nor written.
  * q, k, v BF16, their heads divide `heads` (head h reads head h / (heads / x.heads)); dk and dv
  * multiples of 8 up to CPG_LINEAR_MAX_CHANNELS; rows and strides multiples of 16 bytes.
- * log_decay FP32 [heads], at most 0.  scale and 1 / scale finite. */
+ * log_decay FP32 [heads], at most 0 (-infinity: no state is kept).  At most 2^20 heads.  scale and
+ * 1 / scale finite. */
 typedef struct cpg_linear_problem {
   int64_t tokens;
   int32_t sequences;

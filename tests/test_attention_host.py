@@ -206,6 +206,19 @@ def test_linear_attention_refusals(lib):
     assert lib.cpg_linear_attention_workspace(problem(), 0, 8, 8, 0, ctypes.byref(size)) == S
 
 
+def test_linear_attention_refuses_heads_that_its_counts_do_not_hold(lib):
+    """2^24 heads x 128 channels are 2^31 elements of a token; a workspace's bytes fit 64 bits."""
+    size = ctypes.c_int64(-1)
+    for h in (BIG - 1, 1 << 24, (1 << 20) + 1):
+        p = problem(t=4, h=h, dk=128, dv=128)
+        assert lib.cpg_linear_attention_workspace(p, 1, 1, 1, 1, ctypes.byref(size)) == S
+        assert lib.cpg_linear_attention(p, heads(h=1), heads(h=1), heads(h=1), ADDRESS, None, None,
+                                        None, heads(h=h, hs=128, ts=h * 128), None, 0, None) == S
+    most = problem(t=BIG - 1, h=1 << 20, dk=128, dv=128)
+    assert lib.cpg_linear_attention_workspace(most, 1, 1, 1, 1, ctypes.byref(size)) == _lib.CPG_OK
+    assert size.value >= 3 * (BIG - 1) * (1 << 20) * 128 * 4
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros(4, 2, 8, dtype=torch.bfloat16)
     g = torch.zeros(2)
