@@ -800,7 +800,9 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
 
 int cpg_attention_status(int32_t* status) {
   if (status == nullptr) return fail(CPG_ERR_NULL, "status is NULL");
-  const cudaError_t e = cudaMemcpyFromSymbol(status, cpg::linear_status_word, sizeof(*status));
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
+  e = cudaMemcpyFromSymbol(status, cpg::linear_status_word, sizeof(*status));
   return e == cudaSuccess ? CPG_OK : cuda_fail(e, "cudaMemcpyFromSymbol");
 }
 
