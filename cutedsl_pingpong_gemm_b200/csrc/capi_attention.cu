@@ -420,7 +420,7 @@ int device_ready(int* sms) {
 // be.  A unit (a sequence or segment of one head) is a chain of chunks of one SM, 2.8 us each alone
 // and 3.5 us where all SMs share the bandwidth.  Cutting sequences costs a pass over B and C for the
 // segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
-// channels 1480 -> XX us.  The lengths are known to the device alone: the mean stands for them.
+// channels 1470 -> 350 us.  The lengths are known to the device alone: the mean stands for them.
 // Ragged sequences that stay whole are begun in the order of their lengths (`sorted`) where there is
 // more than one unit per SM.
 struct LinearCut {
@@ -464,7 +464,7 @@ struct LinearSpace {
 LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut, int passes) {
   if (cut.items == 0) return {};
   LinearSpace r;
-  r.states = cut.length == 0 ? 0 : cut.items * p->heads * p->dk * p->dv * 4;
+  r.states = cut.length == 0 ? 0 : (cut.items + p->sequences) * p->heads * p->dk * p->dv * 4;
   r.tables = r.states * passes;
   r.first = cut.items * static_cast<int64_t>(sizeof(cpg::LinearItem));
   r.count = r.first + (cut.length == 0 ? 0 : (int64_t(p->sequences) + 1) * 4);
@@ -537,7 +537,9 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
       b.pass[j].items = items;
       b.pass[j].item_count = count;
       b.pass[j].first_item = first;
+      if (cut.length == 0) continue;
       b.pass[j].segments = reinterpret_cast<float*>(bytes + j * at.states);
+      b.pass[j].most_items = static_cast<int32_t>(cut.items);
     }
   }
   if (cut.length == 0) return run_chunks<true>(b, p->sequences * heads, sms, st);
@@ -547,6 +549,9 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   rc = launch("segment state kernel", true, &cpg::linear_segments_kernel,
               static_cast<unsigned>(p->sequences * heads) * parts, 256, 0, st, 1, b);
   if (rc != CPG_OK) return rc;
+  // The final states are made: this pass's need no third part and C has both slots (65536 tokens x 16
+  // heads of 128 channels with the final states, in a long loop: 470 us, 494 with them made here).
+  b.exact = 0;
   return run_chunks<true>(b, cut.items * heads, sms, st);
 }
 

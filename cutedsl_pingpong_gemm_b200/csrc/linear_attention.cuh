@@ -54,8 +54,10 @@ struct LinearParams {
   const LinearItem* items;       // null: a unit is a whole sequence
   const int32_t* item_count;
   const int32_t* first_item;     // [sequences + 1]
-  float* segments;         // [items, heads, da, dc]: what the segment before adds to the state, then the
-                           // state before each
+  // null: sequences stay whole.  [items, heads, da, dc]: what the segment before adds to the state, then
+  // the state before each; then [sequences, heads, da, dc]: what the last segment adds, if that is wanted.
+  float* segments;
+  int32_t most_items;
   int32_t reverse;
 };
 
@@ -160,8 +162,9 @@ __global__ void __launch_bounds__(kItemThreads)
   }
 }
 
-// The state before every segment of a sequence that has several: the state before the previous one,
-// decayed by that one's tokens, plus what it adds.  Four neighbouring elements a thread; blockIdx.x:
+// The state before every segment of a sequence: the state before the previous one, decayed by that
+// one's tokens, plus what it adds; after the last one that is the final state.  (The starting states
+// are copied: the final ones may take their places.)  Four neighbouring elements a thread; blockIdx.x:
 // pass, sequence and head, then the elements.
 __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch batch) {
   kernel_begins();
@@ -174,10 +177,11 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch 
   const int32_t s = pair / p.heads, h = pair % p.heads;
   const int32_t e = (blockIdx.x % parts) * 1024 + static_cast<int32_t>(threadIdx.x) * 4;
   const int32_t first = p.first_item[s], last = p.first_item[s + 1] - 1;
-  if (e >= size || first >= last) return;
+  if (e >= size || first > last) return;
   const float g2 = p.log_decay[h] * 1.4426950408889634f;
   const int64_t step = static_cast<int64_t>(p.heads) * size;
-  float* x = p.segments + first * step + static_cast<int64_t>(h) * size + e;
+  const int64_t own = static_cast<int64_t>(h) * size + e;
+  float* x = p.segments + first * step + own;
   float4 state = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.state != nullptr) {
     const int64_t place = linear_place(p.state_slots, s, p.state_places);
@@ -193,18 +197,28 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch 
     }
     *reinterpret_cast<float4*>(x) = state;
   }
-#pragma unroll 4
-  for (int32_t at = first; at < last; ++at) {
-    x += step;
-    const int32_t n = p.items[at].count;
-    const float decay = exp2f(g2 * static_cast<float>(n));
-    const float4 v = *reinterpret_cast<const float4*>(x);
+  auto follow = [&](int32_t item, const float* adds) {
+    const int32_t n = p.items[item].count;
+    const float decay = n == 0 ? 1.f : exp2f(g2 * static_cast<float>(n));
+    const float4 v = *reinterpret_cast<const float4*>(adds);
     state.x = fmaf(state.x, decay, v.x);
     state.y = fmaf(state.y, decay, v.y);
     state.z = fmaf(state.z, decay, v.z);
     state.w = fmaf(state.w, decay, v.w);
+  };
+#pragma unroll 4
+  for (int32_t at = first; at < last; ++at) {
+    x += step;
+    follow(at, x);
     *reinterpret_cast<float4*>(x) = state;
   }
+  if (p.final == nullptr) return;
+  const int64_t place = linear_place(p.final_slots, s, p.final_places);
+  if (place < 0) return;
+  follow(last, p.segments + (static_cast<int64_t>(p.most_items) + s) * step + own);
+  const float f = p.final_factor;
+  *reinterpret_cast<float4*>(p.final + place * step + own) =
+      make_float4(f * state.x, f * state.y, f * state.z, f * state.w);
 }
 
 // Rows of a [tokens, heads, d] outside the sequences, set to zero.

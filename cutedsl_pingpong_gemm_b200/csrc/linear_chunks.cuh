@@ -342,22 +342,27 @@ __device__ __noinline__ LinearUnit linear_unit(const LinearBatch& batch, int32_t
     item.first = static_cast<int32_t>(span.first);
     item.count = static_cast<int32_t>(span.count);
   }
+  const bool cut = p.segments != nullptr;
   float* const segment = p.segments + (static_cast<int64_t>(at) * p.heads + r.head) * size;
   r.from_factor = r.to_factor = 1.f;
   if constexpr (!Out) {
-    if (item.last) return r;
-    r.to = segment + p.heads * size;
+    if (!item.last)
+      r.to = segment + p.heads * size;
+    else if (p.final != nullptr)
+      r.to = p.segments +
+             ((static_cast<int64_t>(p.most_items) + item.sequence) * p.heads + r.head) * size;
+    else
+      return r;
+  } else if (cut) {  // (linear_segments_kernel has written the final state, maybe over the starting one)
+    if (item.index > 0 || p.state != nullptr) r.from = segment;
   } else {
-    // (The places of a sequence in several segments are read by its first before the last writes them.)
-    if (item.index > 0 || (p.state != nullptr && !item.last)) {
-      r.from = segment;
-    } else if (p.state != nullptr) {
+    if (p.state != nullptr) {
       const int64_t place = linear_place(p.state_slots, item.sequence, p.state_places);
       if (place >= 0) r.from = p.state + (place * p.heads + r.head) * size;
       r.from_factor = p.state_factor;
       r.transposed = p.state_transposed != 0;
     }
-    if (item.last && p.final != nullptr) {
+    if (p.final != nullptr) {
       const int64_t place = linear_place(p.final_slots, item.sequence, p.final_places);
       if (place >= 0) r.to = p.final + (place * p.heads + r.head) * size;
       r.to_factor = p.final_factor;
