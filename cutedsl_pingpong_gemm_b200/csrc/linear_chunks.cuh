@@ -846,10 +846,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                    ? unit.from_factor * from[unit.transposed ? c * p.da + i : i * p.dc + c]
                    : 0.f;
       };
-      if (unit.chunks == 0) {
-        if (to != nullptr && i < p.da) {
-#pragma unroll 1
-          for (int32_t c = 0; c < p.dc; ++c) to[i * p.dc + c] = unit.to_factor * starting(c);
+      if (unit.chunks == 0) {  // the final state is the starting one
+        const float factor = unit.from_factor * unit.to_factor;
+        const int32_t size = p.da * p.dc;
+        if (to == nullptr || (to == from && factor == 1.f && !unit.transposed)) continue;
+        for (int32_t e0 = 4 * i; e0 < size; e0 += 4 * 128 * 4) {  // four loads in flight
+          float4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int32_t e = e0 + 4 * 128 * k;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (from == nullptr || e >= size) continue;
+            if (!unit.transposed) {
+              v[k] = *reinterpret_cast<const float4*>(from + e);
+            } else {
+              const float* at = from + e % p.dc * p.da + e / p.dc;
+              v[k] = make_float4(at[0], at[p.da], at[2 * p.da], at[3 * p.da]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (e0 + 4 * 128 * k < size)
+              *reinterpret_cast<float4*>(to + e0 + 4 * 128 * k) =
+                  make_float4(factor * v[k].x, factor * v[k].y, factor * v[k].z, factor * v[k].w);
         }
         continue;
       }

@@ -489,6 +489,22 @@ def test_linear_attention_nothing_to_do():
     assert not any(x.any() for x in got[:3])
 
 
+@pytest.mark.parametrize("dk,dv", [(8, 8), (24, 128), (128, 40), (128, 128)])
+def test_linear_attention_empty_sequences_hand_their_states_on(dk, dv):
+    """Their final states are the starting ones, bit for bit, in place too; gradients likewise."""
+    q, k, v, decay, offsets = linear_case(3, [0, 9, 0, 140, 0], 2, 2, 2, 2, dk, dv)
+    state = normal(gen(4), 5, 2, dk, dv, dtype=F32)
+    _, final = attention.linear_attention(q, k, v, decay, scale=0.3, offsets=offsets, state=state,
+                                          final=True)
+    pool = state.clone()
+    attention.linear_attention(q, k, v, decay, scale=0.3, offsets=offsets, state=pool, final=pool)
+    assert torch.equal(pool, final) and torch.equal(final[::2], state[::2])
+    dy = normal(gen(5), *v.shape)
+    dstate = attention.linear_attention_backward(dy, q, k, v, decay, offsets=offsets, state=state,
+                                                 dfinal=state)[3]
+    assert torch.equal(dstate[::2], state[::2])
+
+
 def test_linear_attention_offsets_beyond_the_rows():
     """Offsets are cut to the rows there are; a sequence that would end before it starts is empty."""
     q, k, v, decay, _ = linear_case(3, [300], 2, 2, 2, 2, 64, 64)
