@@ -192,7 +192,8 @@ int head_vector(const NormRope& n) {
 }
 
 // f(type, vector, lanes, pairs a lane, heads at a time) for the sizes at hand: the fewest lanes that hold
-// a head, and Many heads at a time where there are more threads than the SMs hold at once.
+// a head, and Many heads at a time where there are more threads than the SMs hold at once (16384 tokens
+// x 40 heads x 128, BF16: 67 us, one at a time 90; few threads would leave SMs idle).
 template <typename T, int V, int Many, typename F>
 int by_lanes(const NormRope& n, F&& f) {
   using std::integral_constant;
@@ -422,7 +423,7 @@ int device_ready(int* sms) {
 // segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
 // channels 1470 -> 350 us.  The lengths are known to the device alone: the mean stands for them.
 // Ragged sequences that stay whole are begun in the order of their lengths (`sorted`) where there is
-// more than one unit per SM.
+// more than one unit per SM: a long one begun last would run alone.
 struct LinearCut {
   int64_t length, items;
   bool sorted;

@@ -291,8 +291,9 @@ __global__ void __launch_bounds__(256) linear_share_kernel(const LinearSharePara
 }
 
 // One token of each of many sequences: S <- e^g S + k v^T in place, o = scale * S^T q.
-// Bound by HBM: every state is read and written once.  A block takes `cols` columns of a state;
-// a lane four neighbouring ones of every (32 * warps / lanes)-th row, whose loads are independent.
+// Bound by HBM: every state is read and written once (256 tokens x 64 heads x 128 x 128: 369 us, 0.90 of
+// the copy rate).  A block has one state, a lane four neighbouring columns of every (1024 / dv)-th row,
+// whose loads are independent.
 struct LinearStepParams {
   LinearRows q, k, v;
   void* o;

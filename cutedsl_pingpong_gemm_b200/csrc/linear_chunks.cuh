@@ -3,10 +3,16 @@
 // before it,
 //   scores = A B^T,   P = scores . w (0 where j is later than i),
 //   O = scale * (P C + e^(g (i + 1)) (A S)),   S <- e^(g 128) S + (left . B)^T C
-// (left: the decay from a token to the chunk's end).  Four products of 128 x 128 x 128 per chunk of
-// four 32 KiB tiles read or written: 128 flop per byte, so HBM is the bound as long as the products of a
-// chunk, which depend on one another, take less time than its tiles: 3.0 us when 148 blocks share the
-// measured bandwidth.
+// (left: the decay from a token to the chunk's end).  Four products of 128 x 128 x 128, the last in two
+// or three parts, per chunk of four 32 KiB tiles read or written: 160 flop per byte, so HBM would be the
+// bound, 3.0 us a chunk when 148 blocks share the measured bandwidth.  The work of a chunk is a chain,
+// scores (760 cycles) -> P (2400) -> P C (1050) -> the state (1050) -> its copy, of which the tiles'
+// loads, left . B, the next scores and the output run beside: 5300 cycles a chunk of 128 channels, 4100 of
+// 64, 2.7 us at 1965 MHz (8 sequences of 2048 tokens x 64 heads x 128: 226 us after a rest, HBM 164).  In
+// long loops the power limit holds the clock at 1.45 GHz and the same takes 288 us.
+// Measured level or slower, and not kept: P by eight warps, A in TMEM, the output by way of shared memory
+// and TMA, P C begun on the first half of P (0-2 %, more spills), the moves of states shared with the warps
+// of left . B; one part of left . B instead of two would save 3 %.
 //
 // One block per SM walks (sequence, head) pairs with 768 threads:
 //   warp 0       TMA producer: tiles of A, B and C, 128 tokens x 64 channels a box, 128-byte swizzle.
@@ -323,7 +329,7 @@ struct LinearUnit {
   bool transposed;    // from
 };
 
-// (Out of line: once per unit in each of eight roles.)
+// (Out of line: once per unit in each role.)
 template <bool Out>
 __device__ __noinline__ LinearUnit linear_unit(const LinearBatch& batch, int32_t each, int32_t u) {
   LinearUnit r = {};

@@ -10,6 +10,8 @@ Contents:
 * ``tile_scheduler_ref`` -- restatement of ``SimpleTileScheduler`` (tile_scheduler.py:20-183).
 * ``gemm_ref``           -- fp32 CPU matmul ``D = A @ B.T`` (gemm_base.py:590) and the
   tolerance checks stated by the project spec.
+* ``moe_ref``, ``attention_ref`` -- 64-bit definitions of the expert operators, of the norm with
+  rotation and of linear attention, with the sizes of their terms for the tests' tolerances.
 
 Pinning: ``fast_math_ref`` and ``tile_scheduler_ref`` are checked bit-exact against golden
 vectors produced by executing the reference's own Python code under CuTe-DSL
