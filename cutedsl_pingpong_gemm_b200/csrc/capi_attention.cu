@@ -15,6 +15,7 @@
 #include "linear_attention.cuh"
 #include "linear_chunks.cuh"
 
+using cpg::Work;
 using cpg_capi::bytes_of;
 using cpg_capi::cuda_fail;
 using cpg_capi::encode_fn;
@@ -401,8 +402,9 @@ int device_ready(int* sms) {
     auto both = [&](auto da, auto dc) {
       constexpr int kDA = decltype(da)::value, kDC = decltype(dc)::value;
       constexpr uint32_t kBytes = cpg::ChunkLayout<kDA, kDC>::kBytes;
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, false>, kBytes);
-      raise(&cpg::linear_chunks_kernel<kDA, kDC, true>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kStates>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kOutput>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kFine>, kBytes);
     };
     const std::integral_constant<int, 64> d64;
     const std::integral_constant<int, 128> d128;
@@ -474,7 +476,7 @@ LinearSpace linear_space(const cpg_linear_problem* p, const LinearCut& cut, int 
   return r;
 }
 
-template <int DA, int DC, bool Out>
+template <int DA, int DC, Work W>
 int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t st) {
   cpg::LinearMaps maps = {};
   for (int j = 0; j < b.passes && b.pass[0].tokens > 0; ++j) {
@@ -486,18 +488,18 @@ int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t s
       if (rc != CPG_OK) return rc;
     }
   }
-  return launch("linear attention kernel", true, &cpg::linear_chunks_kernel<DA, DC, Out>,
+  return launch("linear attention kernel", true, &cpg::linear_chunks_kernel<DA, DC, W>,
                 static_cast<unsigned>(std::min<int64_t>(units, sms)), cpg::kChunkThreads,
                 cpg::ChunkLayout<DA, DC>::kBytes, st, 1, maps, b);
 }
 
-template <bool Out>
+template <Work W>
 int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t st) {
   if (b.pass[0].da > 64)
-    return b.pass[0].dc > 64 ? run_chunks<128, 128, Out>(b, units, sms, st)
-                             : run_chunks<128, 64, Out>(b, units, sms, st);
-  return b.pass[0].dc > 64 ? run_chunks<64, 128, Out>(b, units, sms, st)
-                           : run_chunks<64, 64, Out>(b, units, sms, st);
+    return b.pass[0].dc > 64 ? run_chunks<128, 128, W>(b, units, sms, st)
+                             : run_chunks<128, 64, W>(b, units, sms, st);
+  return b.pass[0].dc > 64 ? run_chunks<64, 128, W>(b, units, sms, st)
+                           : run_chunks<64, 64, W>(b, units, sms, st);
 }
 
 // Passes of the same kernel (the same widths of 64 or 128 channels).
@@ -514,7 +516,12 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   b.timeout_ns = kTimeoutNs;
   const LinearCut cut = linear_cut(p, b.passes);
   const int64_t heads = int64_t(p->heads) * b.passes;
-  if (cut.items == 0) return run_chunks<true>(b, p->sequences * heads, sms, st);
+  auto run_out = [&](int64_t units) {
+    if ((p->tokens / cpg::kChunk + p->sequences) * heads <= sms)  // (why: at the kernel)
+      return run_chunks<Work::kFine>(b, units, sms, st);
+    return run_chunks<Work::kOutput>(b, units, sms, st);
+  };
+  if (cut.items == 0) return run_out(p->sequences * heads);
   const LinearSpace at = linear_space(p, cut, b.passes);
   char* const bytes = static_cast<char*>(space);
   const cpg::LinearParams& any = b.pass[0];
@@ -543,8 +550,8 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
       b.pass[j].most_items = static_cast<int32_t>(cut.items);
     }
   }
-  if (cut.length == 0) return run_chunks<true>(b, p->sequences * heads, sms, st);
-  rc = run_chunks<false>(b, cut.items * heads, sms, st);
+  if (cut.length == 0) return run_out(p->sequences * heads);
+  rc = run_chunks<Work::kStates>(b, cut.items * heads, sms, st);
   if (rc != CPG_OK) return rc;
   const unsigned parts = static_cast<unsigned>((any.da * any.dc + 1023) / 1024);
   rc = launch("segment state kernel", true, &cpg::linear_segments_kernel,
@@ -553,7 +560,7 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   // The final states are made: this pass's need no third part and C has both slots (65536 tokens x 16
   // heads of 128 channels with the final states, in a long loop: 470 us, 494 with them made here).
   b.exact = 0;
-  return run_chunks<true>(b, cut.items * heads, sms, st);
+  return run_out(cut.items * heads);
 }
 
 // Passes of the gradient that run together: all three, or dq and dk before dv where the widths differ.

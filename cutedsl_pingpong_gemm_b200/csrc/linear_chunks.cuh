@@ -22,7 +22,10 @@
 //   warps 8-15   the output.
 //   warps 16-19  the state: its BF16 copy in shared memory for A S, and its decay in TMEM.
 //   warps 20-23  left . B.
-// Roundings: P and the copy of S are BF16, as operands have to be; the state itself stays FP32.  left . B
+// Roundings: P and the copy of S are BF16, as operands have to be; the state itself stays FP32.  Where the
+// chunks are not more than the SMs (kFine) P is two BF16 parts, its sum to 2^-17: few scores' roundings do
+// not average out (a token's output could be 2^-8 off), and the time is small beside a launch's (4096
+// tokens of one head 39 us, 37 with one part; 37 tokens of 16 heads no difference).  left . B
 // is split into BF16 parts whose sum it is to 2^-17 (two products), or, where the state is an output
 // (`exact`), to 2^-25 (three), so that a state keeps FP32 accuracy.
 // An infinity or NaN in C would spoil its channel in all of the chunk's outputs, the earlier ones too
@@ -388,13 +391,17 @@ __device__ __forceinline__ int32_t chunk_at(const LinearUnit& u, int32_t x, int3
   return static_cast<int32_t>(u.first + at);
 }
 
-// Out false: only the state that each unit leaves, from zeros, and without A.
-template <int DA, int DC, bool Out>
+// Work::kStates: only the state that each unit leaves, from zeros, and without A.  kFine: see above (a
+// variant of its own: decided at run time, it takes registers that the others want, 2-11 %).
+enum class Work { kStates, kOutput, kFine };
+
+template <int DA, int DC, Work W>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     linear_chunks_kernel(const __grid_constant__ LinearMaps maps,
                          const __grid_constant__ LinearBatch batch) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
   using L = ChunkLayout<DA, DC>;
+  constexpr bool Out = W != Work::kStates, kFine = W == Work::kFine;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -578,10 +585,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                  (count == kChunk || ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma));
             if (!ok) break;
             ptx::tc_fence_after();
+            if constexpr (!kFine) {
 #pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(tmem + kColIntra, tmem + kColScores + k * 8, c_mn + k * 128, kInter, k > 0,
-                          issue);
+              for (int k = 0; k < kChunk / 16; ++k)
+                umma_f16_ts(tmem + kColIntra, tmem + kColScores + k * 8, c_mn + k * 128, kInter, k > 0,
+                            issue);
+            } else {
+#pragma unroll 1
+              for (int k = 0; k < kChunk / 8; ++k)  // both parts of 16 tokens
+                umma_f16_ts(tmem + kColIntra, tmem + kColScores + 32 * (k >> 2) + 8 * (k & 3),
+                            c_mn + ((k >> 2) * 2 + (k & 1)) * 128, kInter, k > 0, issue);
+            }
             umma_commit_if(o_full, issue);
           } else {
             ok = ptx::mbar_wait_brief(h_ready, once, ctx, kSiteLinearMma) &&
@@ -734,14 +748,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
               for (int k = 0; k < 32; ++k) s[k] = k < left ? s[k] : 0u;
             }
+            if constexpr (kFine) {  // the second part, over the second half of this block's scores
+              uint32_t low[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              s[k] = ptx::pack_bf16x2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+              for (int k = 0; k < 16; ++k) {
+                const float x = __uint_as_float(s[2 * k]), y = __uint_as_float(s[2 * k + 1]);
+                s[k] = ptx::pack_bf16x2(x, y);
+                low[k] = ptx::pack_bf16x2(x - bf16_lo(s[k]), y - bf16_hi(s[k]));
+              }
+              tmem_st_32x32b_x16(lanes + kColScores + 32 * blk + 16, low);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                s[k] = ptx::pack_bf16x2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+            }
           }
           // Over scores that this lane has read: those of blocks up to this one.
           const uint32_t packed[16] = {s[0], s[1], s[2],  s[3],  s[4],  s[5],  s[6],  s[7],
                                        s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15]};
-          tmem_st_32x32b_x16(lanes + kColScores + 16 * blk, packed);
+          tmem_st_32x32b_x16(lanes + kColScores + (kFine ? 32 : 16) * blk, packed);
+          if (kFine && (reverse ? blk < w : blk > w))
+            tmem_st_32x32b_x16(lanes + kColScores + 32 * blk + 16, packed);  // zeros too
         }
         tmem_st_wait();
         ptx::tc_fence_before();

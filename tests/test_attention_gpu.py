@@ -401,6 +401,37 @@ def test_linear_attention_decays(decay):
     within(got[3], ds, 2 ** -17 * size)
 
 
+@pytest.mark.parametrize("lengths,h,dk,dv,dtype", [
+    ([1], 1, 8, 8, BF), ([2], 1, 64, 64, BF), ([5], 2, 128, 64, F32), ([1, 1, 1], 2, 64, 128, BF),
+    ([37], 3, 72, 40, BF), ([128], 1, 128, 128, F32), ([129, 3], 2, 128, 128, BF)])
+def test_linear_attention_of_few_chunks(lengths, h, dk, dv, dtype):
+    """Without a starting state and up to one chunk a sequence, only the output is rounded to BF16:
+    scores are two BF16 parts, their sum to 2^-17 (half a step of the second, which is below 2^-8 of
+    the score), and the sums of their products stay within 2^-15 of far.
+    (Tokens of a second chunk also read a BF16 state.)"""
+    q, k, v, decay, offsets = linear_case(11, lengths, h, h, h, h, dk, dv)
+    out = torch.empty(*v.shape, dtype=dtype, device="cuda")
+    attention.linear_attention(q, k, v, decay, scale=dk ** -0.5, offsets=offsets, out=out)
+    o, near, far, _, _ = ref.whole_pass(q, k, v, decay, dk ** -0.5, offsets)
+    tol = half(dtype) * o.abs() + 2 ** -15 * far
+    first = 0
+    for n in lengths:
+        tol[first + 128:first + n] += 2 ** -8 * near[first + 128:first + n]
+        first += n
+    within(out, o, tol)
+    # Against the order of the tokens, a gradient: dk = pass(v, dy, q) from behind.
+    dy = normal(gen(12), *v.shape)
+    dk_got = attention.linear_attention_backward(dy, q, k, v, decay, scale=dk ** -0.5,
+                                                 offsets=offsets)[1]
+    o, near, far, _, _ = ref.whole_pass(v, dy, q, decay, dk ** -0.5, offsets, reverse=True)
+    tol = half(BF) * o.abs() + 2 ** -15 * far
+    first = 0
+    for n in lengths:  # (chunks are counted from the sequence's first token; the last has no state)
+        tol[first:first + (n - 1) // 128 * 128] += 2 ** -8 * near[first:first + (n - 1) // 128 * 128]
+        first += n
+    within(dk_got, o, tol)
+
+
 def test_linear_attention_one_sequence_without_offsets():
     q, k, v, decay, offsets = linear_case(3, [333], 2, 2, 2, 2, 64, 128)
     a = attention.linear_attention(q, k, v, decay, offsets=offsets, final=True)
