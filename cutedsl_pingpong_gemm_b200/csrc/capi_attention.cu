@@ -495,14 +495,19 @@ int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t s
 
 template <Work W>
 int run_chunks(const cpg::LinearBatch& b, int64_t units, int sms, cudaStream_t st) {
-  if (b.pass[0].da > 64)
-    return b.pass[0].dc > 64 ? run_chunks<128, 128, W>(b, units, sms, st)
-                             : run_chunks<128, 64, W>(b, units, sms, st);
-  return b.pass[0].dc > 64 ? run_chunks<64, 128, W>(b, units, sms, st)
-                           : run_chunks<64, 64, W>(b, units, sms, st);
+  bool wide_a = false, wide_c = false;
+  for (int j = 0; j < b.passes; ++j) {
+    wide_a |= b.pass[j].da > 64;
+    wide_c |= b.pass[j].dc > 64;
+  }
+  if (wide_a)
+    return wide_c ? run_chunks<128, 128, W>(b, units, sms, st)
+                  : run_chunks<128, 64, W>(b, units, sms, st);
+  return wide_c ? run_chunks<64, 128, W>(b, units, sms, st)
+                : run_chunks<64, 64, W>(b, units, sms, st);
 }
 
-// Passes of the same kernel (the same widths of 64 or 128 channels).
+// Passes over the same sequences and heads in one launch, in the kernel that is wide enough for all.
 int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cudaStream_t st) {
   if (p->sequences == 0) return CPG_OK;
   int sms = 0;
@@ -563,8 +568,15 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   return run_out(cut.items * heads);
 }
 
-// Passes of the gradient that run together: all three, or dq and dk before dv where the widths differ.
-bool same_width(const cpg_linear_problem* p) { return (p->dk > 64) == (p->dv > 64); }
+// Whether all three passes of the gradient run together, or dq and dk before dv.  Where dk and dv are not
+// both up to 64 or above, together means 128 channels for all, which pays where launches and the last
+// blocks' tails count (dk = 64, dv = 128 in a graph: 37 tokens x 16 heads 25 -> 17 us, 5 sequences of 820
+// 105 -> 92) and costs where the chunks do (8 sequences of 2048 x 32 heads 335 -> 370 us).
+bool one_launch(const cpg_linear_problem* p) {
+  if ((p->dk > 64) == (p->dv > 64)) return true;
+  return p->tokens <= int64_t(8) * cpg::kChunk * p->sequences &&
+         int64_t(p->sequences) * p->heads * 3 <= 2 * 148;
+}
 
 // Workspace: that of the passes, then FP32 sums of a head each for every gradient of shared heads.
 struct BackwardSpace {
@@ -575,7 +587,7 @@ BackwardSpace backward_space(const cpg_linear_problem* p, int32_t q_heads, int32
   BackwardSpace r;
   r.bytes = 0;
   for (int passes = 1; passes <= 3; ++passes)
-    if (same_width(p) ? passes == 3 : passes < 3)
+    if (one_launch(p) ? passes == 3 : passes < 3)
       r.bytes = std::max(r.bytes, linear_space(p, linear_cut(p, passes), passes).bytes);
   const int32_t heads[3] = {q_heads, k_heads, v_heads}, channels[3] = {p->dk, p->dk, p->dv};
   for (int i = 0; i < 3; ++i) {
@@ -769,7 +781,7 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
   b.pass[2].reverse = 1;
   set_state(&b.pass[2], dfinal, false, 1.f / p->scale);
   set_final(&b.pass[2], dstate, p->scale);
-  b.passes = same_width(p) ? 3 : 2;
+  b.passes = one_launch(p) ? 3 : 2;
   rc = run_passes(p, b, workspace, st);
   if (rc == CPG_OK && b.passes == 2) {
     b.pass[0] = b.pass[2];

@@ -337,6 +337,22 @@ def test_linear_attention_backward(lengths, hq, hk, hv, h, dk, dv, layout, state
     assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("lengths,dk,dv", [([1200, 1101], 64, 128), ([1200, 1101], 128, 40),
+                                           ([1000, 9], 64, 128), ([1000, 9], 128, 40)])
+def test_linear_attention_backward_of_two_widths(lengths, dk, dv):
+    """dq and dk with dv, or before it."""
+    q, k, v, decay, offsets = linear_case(6, lengths, 1, 2, 2, 2, dk, dv)
+    dy = normal(gen(5), *v.shape)
+    state = normal(gen(7), len(lengths), 2, dk, dv, dtype=F32)
+    got = attention.linear_attention_backward(dy, q, k, v, decay, scale=0.2, offsets=offsets,
+                                              state=state, dfinal=state)
+    grads, (ds, size) = ref.linear_attention_backward(dy, q, k, v, decay, 0.2, offsets, list(state),
+                                                      list(state))
+    for x, (want, near, far) in zip(got, grads):
+        within(x, want, 2 ** -8 * near + half(BF) * want.abs() + 2 ** -15 * far)
+    within(got[3], ds, 2 ** -17 * size)
+
+
 def test_linear_attention_backward_outputs():
     q, k, v, decay, offsets = linear_case(1, [70, 200], 2, 2, 2, 2, 64, 64, pad=3, first=2)
     dy = normal(gen(2), 275, 2, 64)
