@@ -405,6 +405,7 @@ int device_ready(int* sms) {
       raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kStates>, kBytes);
       raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kOutput>, kBytes);
       raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kFine>, kBytes);
+      raise(&cpg::linear_chunks_kernel<kDA, kDC, Work::kExact>, kBytes);
     };
     const std::integral_constant<int, 64> d64;
     const std::integral_constant<int, 128> d128;
@@ -524,7 +525,8 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   auto run_out = [&](int64_t units) {
     if ((p->tokens / cpg::kChunk + p->sequences) * heads <= sms)  // (why: at the kernel)
       return run_chunks<Work::kFine>(b, units, sms, st);
-    return run_chunks<Work::kOutput>(b, units, sms, st);
+    return b.exact ? run_chunks<Work::kExact>(b, units, sms, st)
+                   : run_chunks<Work::kOutput>(b, units, sms, st);
   };
   if (cut.items == 0) return run_out(p->sequences * heads);
   const LinearSpace at = linear_space(p, cut, b.passes);

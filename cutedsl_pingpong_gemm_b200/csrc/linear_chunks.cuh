@@ -27,7 +27,10 @@
 // not average out (a token's output could be 2^-8 off), and the time is small beside a launch's (4096
 // tokens of one head 39 us, 37 with one part; 37 tokens of 16 heads no difference).  left . B
 // is split into BF16 parts whose sum it is to 2^-17 (two products), or, where the state is an output
-// (`exact`), to 2^-25 (three), so that a state keeps FP32 accuracy.
+// (kExact), to 2^-25 (three).  The tensor cores cut off a sum's last bits every 16 tokens: 24 times a
+// chunk at the state's size would leave it 1e-6 off.  The two small parts are summed apart then, in P's
+// columns, and added in FP32: 2e-7, as with FP32 throughout (8 sequences of 2048 x 64 heads x 128 with
+// final states in a loop: 350 us, 321 in one sum, 277 without final states).
 // An infinity or NaN in C would spoil its channel in all of the chunk's outputs, the earlier ones too
 // (0 times it is NaN).  It is replaced by 0, and its channel is NaN from its token on in what is
 // written.
@@ -74,7 +77,7 @@ struct ChunkLayout {
   static constexpr uint32_t kLo = kShared ? kC + kTileC : kC + 2 * kTileC;
   static constexpr uint32_t kS = kLo + kTileA;
   static constexpr uint32_t kBars = kS + (kTileS > 16384u ? kTileS : 16384u);
-  static constexpr uint32_t kNumBars = 20;
+  static constexpr uint32_t kNumBars = 22;
   static constexpr uint32_t kSlot = kBars + kNumBars * 8;
   static constexpr uint32_t kPowers = kSlot + 16;      // 64 for each warp of the scores
   static_assert(kPowers % 16 == 0, "read four at a time");
@@ -391,9 +394,10 @@ __device__ __forceinline__ int32_t chunk_at(const LinearUnit& u, int32_t x, int3
   return static_cast<int32_t>(u.first + at);
 }
 
-// Work::kStates: only the state that each unit leaves, from zeros, and without A.  kFine: see above (a
-// variant of its own: decided at run time, it takes registers that the others want, 2-11 %).
-enum class Work { kStates, kOutput, kFine };
+// Work::kStates: only the state that each unit leaves, from zeros, and without A.  kFine: see above, kExact:
+// outputs with states to FP32 accuracy (variants of their own: decided at run time, they take registers
+// that kOutput wants, 2-11 %; the others ask batch.exact).
+enum class Work { kStates, kOutput, kFine, kExact };
 
 template <int DA, int DC, Work W>
 __global__ void __launch_bounds__(kChunkThreads, 1)
@@ -402,6 +406,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
   using L = ChunkLayout<DA, DC>;
   constexpr bool Out = W != Work::kStates, kFine = W == Work::kFine;
+  const bool exact = W == Work::kOutput ? false : W == Work::kExact ? true : batch.exact != 0;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                  b_empty = bars + 48, c_empty = bars + 64, s_full = bars + 80, p_ready = bars + 88,
                  o_full = bars + 96, o_free = bars + 104, h_ready = bars + 112,
                  b_ready = bars + 120, h_full = bars + 128, c_ready = bars + 136,
-                 drain = bars + 152;
+                 drain = bars + 152, small_free = bars + 160;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + L::kSlot);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(base_ptr + L::kSlot + 4);
   const uint32_t warp = threadIdx.x >> 5;
@@ -422,7 +427,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (uint32_t i = 0; i < L::kNumBars; ++i) {
       const uint32_t bar = bars + 8 * i;
       ptx::mbar_init(bar, bar == o_free ? 8
-                          : bar == p_ready || bar == h_ready || bar == b_ready ? 4
+                          : bar == p_ready || bar == h_ready || bar == b_ready || bar == small_free ? 4
                           : bar == c_ready || bar == c_ready + 8 ? 2
                                                                  : 1);
     }
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint32_t n = 0;  // chunks done
   bool ok = true;
   // C's slot of chunk m and the parity of its phases.
-  const bool one_c = L::kShared && batch.exact;
+  const bool one_c = L::kShared && exact;
   auto c_slot = [&](uint32_t m) { return one_c ? 0u : m & 1u; };
   auto c_phase = [&](uint32_t m) { return one_c ? m & 1u : (m >> 1) & 1u; };
 
@@ -556,8 +561,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const uint32_t b = base + L::kB + slot * L::kTileA;
           const uint32_t c_mn = desc_lo_mn(base + L::kC + c_slot(n) * L::kTileC, 16384);
           if constexpr (Out) {
-            // A B^T.  Its columns hold P of the chunk before until that one's product is done.
+            // A B^T.  Its columns hold P of the chunk before until that one's product is done, and then
+            // the small parts of the state's addend until they have been added.
             if (n > 0) ok = ptx::mbar_wait_brief(o_full, once ^ 1u, ctx, kSiteLinearMma);
+            if (n > 0 && exact)
+              ok = ok && ptx::mbar_wait_brief(small_free, once ^ 1u, ctx, kSiteLinearMma);
             ok = ok && ptx::mbar_wait_brief(a_full, once, ctx, kSiteLinearMma) &&
                  ptx::mbar_wait_brief(b_full + 8 * slot, twice, ctx, kSiteLinearMma);
             if (!ok) break;
@@ -606,18 +614,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           // The state's addend, by the parts of left . B.
           if (!(ok = ptx::mbar_wait_brief(b_ready, once, ctx, kSiteLinearMma))) break;
           ptx::tc_fence_after();
-          uint32_t accumulate = state ? 1u : 0u;
+          uint32_t accumulate = state ? 1u : 0u, sum = kColState;
 #pragma unroll 1
-          for (int j = 0; j < (batch.exact ? 3 : 2); ++j) {
+          for (int j = 0; j < (exact ? 3 : 2); ++j) {
+            if (exact && j == 1) {  // over P
+              if (Out && !(ok = ptx::mbar_wait_brief(o_full, once, ctx, kSiteLinearMma))) break;
+              ptx::tc_fence_after();
+              accumulate = 0u;
+              sum = kColScores;
+            }
             const uint32_t part =
                 desc_lo_mn(j == 0 ? b : base + (j == 1 ? L::kMid : L::kLo), 16384);
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k) {
-              umma_f16_ss(tmem + kColState, part + k * 128, c_mn + k * 128, kState, accumulate,
-                          issue);
+              umma_f16_ss(tmem + sum, part + k * 128, c_mn + k * 128, kState, accumulate, issue);
               accumulate = 1u;
             }
           }
+          if (!ok) break;
           umma_commit_if(b_empty + 8 * slot, issue);
           umma_commit_if(c_empty + 8 * c_slot(n), issue);
           umma_commit_if(h_full, issue);
@@ -957,6 +971,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           for (int32_t col = 0; col < DC; col += 16) {
             uint32_t s[16];
             ptx::tmem_ld_32x32b_x16(mine + col, s);
+            if (exact && x > 0) {
+              uint32_t small[16];
+              ptx::tmem_ld_32x32b_x16(lanes + kColScores + col, small);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) add2(s[k], s[k + 1], 1.f, small[k], small[k + 1]);
+            }
             ptx::tmem_ld_wait();
             if constexpr (Out) {
 #pragma unroll
@@ -979,6 +1000,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         __syncwarp();
         if (lane == 0) {
           ptx::mbar_arrive(h_ready);
+          if (exact && x > 0) ptx::mbar_arrive(small_free);
           done[warp - 8] = n + 1;
         }
       }
@@ -987,15 +1009,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (to != nullptr) {
         const bool spoilt = *last_bad > unit_first;
 #pragma unroll 1
-        for (int32_t part = 0; part < DC / 32; ++part) {
-          const StatePart at = state_part<DC>(warp, lane, part);
+        for (int32_t part = 0; part < DC / 16; ++part) {  // half a part: 32 columns
+          StatePart at = state_part<DC>(warp, lane, part / 2);
+          at.col += 32 * (part & 1);
+          at.tmem += 32 * (part & 1);
           float* tile = to + at.row * p.dc + at.col;
-          uint32_t s[32];
+          uint32_t s[16];
           __syncwarp();
-          tmem_ld_16x256b_x8(mine + at.tmem, s);
+          tmem_ld_16x256b_x4(mine + at.tmem, s);
+          if (exact) {
+            uint32_t small[16];
+            tmem_ld_16x256b_x4(lanes + kColScores + at.tmem, small);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) add2(s[k], s[k + 1], 1.f, small[k], small[k + 1]);
+          }
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
+          for (int k = 0; k < 8; ++k) {
             const int32_t col = at.col + 8 * (k / 2);
             float2 v = make_float2(unit.to_factor * __uint_as_float(s[2 * k]),
                                    unit.to_factor * __uint_as_float(s[2 * k + 1]));
@@ -1009,6 +1040,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
       ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && exact) ptx::mbar_arrive(small_free);
     }
   } else if (warp >= 20) {
     // ----------------------------------------------------------------------------- left . B
@@ -1033,7 +1066,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (ok && count < kChunk)
           ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearLeft);
         if (!ok) break;
-        if (batch.exact) {
+        if (exact) {
 #pragma unroll 1
           for (uint32_t piece = 0; piece < DA / 8; ++piece) {
             const uint32_t at = tile_offset(i, piece, kChunk);
