@@ -193,10 +193,10 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     pools [places, H, dk, dv] and sequence b is at ``slots[b]``; one outside the pool starts from
     zeros and is not written.  ``final`` may be ``state``; no two sequences may share a place there.
     Returns ``(out, final)``: ``out`` [T, H, dv] BF16 (FP32 if it is given so).
-    Products are taken of BF16 values: the decayed scores (in short calls two parts of each) and the
-    state before each 128 tokens are rounded to BF16 for them, all sums and the states kept are
-    FP32.  An infinity or a NaN in ``v`` makes its channel NaN from its token on, and no output
-    before it."""
+    Products are taken of BF16 values: the decayed scores (two parts of each in calls of few chunks
+    of 128 tokens or of sequences of up to four tokens) and the state before each 128 tokens are
+    rounded to BF16 for them, all sums and the states kept are FP32.  An infinity or a NaN in ``v``
+    makes its channel NaN from its token on, and no output before it."""
     dev = q.device
     b = _sequences(offsets, dev)
     p, problem, q_c, k_c, v_c = _linear_args(q, k, v, log_decay, scale, b)

@@ -523,7 +523,8 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
   const LinearCut cut = linear_cut(p, b.passes);
   const int64_t heads = int64_t(p->heads) * b.passes;
   auto run_out = [&](int64_t units) {
-    if ((p->tokens / cpg::kChunk + p->sequences) * heads <= sms)  // (why: at the kernel)
+    if ((p->tokens / cpg::kChunk + p->sequences) * heads <= sms ||
+        p->tokens <= int64_t(4) * p->sequences)  // (why: at the kernel)
       return run_chunks<Work::kFine>(b, units, sms, st);
     return b.exact ? run_chunks<Work::kExact>(b, units, sms, st)
                    : run_chunks<Work::kOutput>(b, units, sms, st);

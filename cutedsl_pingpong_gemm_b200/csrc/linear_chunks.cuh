@@ -23,9 +23,10 @@
 //   warps 16-19  the state: its BF16 copy in shared memory for A S, and its decay in TMEM.
 //   warps 20-23  left . B.
 // Roundings: P and the copy of S are BF16, as operands have to be; the state itself stays FP32.  Where the
-// chunks are not more than the SMs (kFine) P is two BF16 parts, its sum to 2^-17: few scores' roundings do
-// not average out (a token's output could be 2^-8 off), and the time is small beside a launch's (4096
-// tokens of one head 39 us, 37 with one part; 37 tokens of 16 heads no difference).  left . B
+// chunks are not more than the SMs, or sequences have four tokens or fewer on average (kFine), P is two
+// BF16 parts, its sum to 2^-17: few scores' roundings do not average out (a token's output could be 2^-8
+// off).  The time is small beside a launch's (4096 tokens of one head 39 us, 37 with one part; 37 tokens
+// of 16 heads no difference), but not with many short sequences (64 of 4 tokens x 32 heads 84 us, 66).  left . B
 // is split into BF16 parts whose sum it is to 2^-17 (two products), or, where the state is an output
 // (kExact), to 2^-25 (three).  The tensor cores cut off a sum's last bits every 16 tokens: 24 times a
 // chunk at the state's size would leave it 1e-6 off.  The two small parts are summed apart then, in P's

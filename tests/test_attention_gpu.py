@@ -419,7 +419,7 @@ def test_linear_attention_decays(decay):
 
 @pytest.mark.parametrize("lengths,h,dk,dv,dtype", [
     ([1], 1, 8, 8, BF), ([2], 1, 64, 64, BF), ([5], 2, 128, 64, F32), ([1, 1, 1], 2, 64, 128, BF),
-    ([37], 3, 72, 40, BF), ([128], 1, 128, 128, F32), ([129, 3], 2, 128, 128, BF)])
+    ([1, 2, 1, 3] * 20, 4, 64, 64, BF), ([37], 3, 72, 40, BF), ([128], 1, 128, 128, F32), ([129, 3], 2, 128, 128, BF)])
 def test_linear_attention_of_few_chunks(lengths, h, dk, dv, dtype):
     """Without a starting state and up to one chunk a sequence, only the output is rounded to BF16:
     scores are two BF16 parts, their sum to 2^-17 (half a step of the second, which is below 2^-8 of
