@@ -856,6 +856,33 @@ def test_streams_and_graphs():
     del graphs
 
 
+def test_graph_of_segments_advances_a_pool_in_place():
+    """Captured with the sequences cut into segments, states read from and written to one pool:
+    each replay goes on from the last one's states, as eager calls do, bit for bit."""
+    q, k, v, decay, offsets = linear_case(8, [5000, 0, 3000], 2, 2, 2, 2, 64, 128)
+    slots = torch.tensor([3, 0, 1], dtype=torch.int32, device="cuda")
+    first = normal(gen(2), 5, 2, 64, 128, dtype=F32)
+    wants, pool = [], first.clone()
+    for _ in range(3):
+        out, _ = attention.linear_attention(q, k, v, decay, scale=0.1, offsets=offsets, state=pool,
+                                            slots=slots, final=pool)
+        wants.append((out, pool.clone()))
+    assert torch.equal(wants[2][1][[0, 2, 4]], first[[0, 2, 4]])
+    check_forward(q, k, v, decay, offsets, 0.1, [first[3], first[0], first[1]], wants[0][0],
+                  wants[0][1][[3, 0, 1]])
+    pool = first.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = attention.linear_attention(q, k, v, decay, scale=0.1, offsets=offsets, state=pool,
+                                            slots=slots, final=pool)
+    assert torch.equal(pool, first)
+    for want in wants:
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(pool, want[1])
+    del graph
+
+
 def test_layer_of_products_and_attention():
     """Projection, norm with rotation, linear attention, output projection, as a layer runs them,
     with every step against the 64-bit form of the values it was given, and its gradient."""
