@@ -39,6 +39,7 @@ ROUTE_SCORINGS = {"softmax": 0, "sigmoid": 1}
 ROUTE_GROUP_SCORES = {"max": 0, "top2": 1}
 
 CPG_INJECT_SKIP_LOADS = 1
+CPG_INJECT_SKIP_VALUES = 2
 CPG_SPLIT_K_STREAM = -1
 CPG_SPLIT_K_HYBRID = -2
 CPG_SPLIT_K_DECODE = -3
@@ -51,7 +52,7 @@ CPG_ACT_GELU_TANH = 4
 ACTIVATIONS = {None: CPG_ACT_NONE, "none": CPG_ACT_NONE, "relu": CPG_ACT_RELU,
                "silu": CPG_ACT_SILU, "gelu": CPG_ACT_GELU, "gelu_tanh": CPG_ACT_GELU_TANH}
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 
 class CpgError(RuntimeError):
@@ -216,6 +217,8 @@ SIGNATURES = {
     "cpg_linear_attention_workspace": (ctypes.c_int, [_P(LinearProblemC), _i32, _i32, _i32, _i32,
                                                       _P(_i64)]),
     "cpg_attention_status": (ctypes.c_int, [_P(_i32)]),
+    "cpg_attention_set_timeout_ms": (ctypes.c_int, [_i32]),
+    "cpg_attention_set_fault_injection": (ctypes.c_int, [_i32]),
     "cpg_linear_attention_step": (ctypes.c_int, [_P(LinearProblemC), _H, _H, _H, _vp, _S, _H,
                                                  _vp]),
     "cpg_cast_f32_bf16": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),

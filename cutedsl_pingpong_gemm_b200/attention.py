@@ -258,12 +258,23 @@ def linear_attention_backward(dy, q, k, v, log_decay, *, scale: float = 1.0, off
 
 
 def status(device=None) -> int:
-    """0, or the code of the first wait within a linear attention kernel that ever ran out (10 s) on
-    this CUDA device (None: the current one).  Synchronises."""
+    """0, or the code of the first wait within a linear attention kernel that ever ran out on this
+    CUDA device (None: the current one); the outputs of that call are not valid.  Synchronises."""
     code = ctypes.c_int32()
     with torch.cuda.device(device):
         _lib.check(_lib.load().cpg_attention_status(ctypes.byref(code)), "status")
     return code.value
+
+
+def set_timeout_ms(ms: int) -> None:
+    """Limit of every wait within the linear attention kernels that this process launches from now on
+    (10 s, or CPG_WAIT_TIMEOUT_MS from the environment)."""
+    _lib.check(_lib.load().cpg_attention_set_timeout_ms(int(ms)), "set_timeout_ms")
+
+
+def set_fault_injection(flags: int) -> None:
+    """Test hook (see cpg_attention_set_fault_injection): 1 = no loads, 2 = none of v's tiles."""
+    _lib.check(_lib.load().cpg_attention_set_fault_injection(int(flags)), "set_fault_injection")
 
 
 def linear_attention_step(q, k, v, log_decay, state, *, scale: float = 1.0, slots=None, out=None):

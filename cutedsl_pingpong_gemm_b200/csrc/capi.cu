@@ -367,7 +367,7 @@ struct cpg_gemm {
 
 extern "C" {
 
-int cpg_abi_version(void) { return 17; }
+int cpg_abi_version(void) { return 18; }
 
 const char* cpg_strerror(int code) {
   switch (code) {

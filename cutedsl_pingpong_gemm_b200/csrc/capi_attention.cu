@@ -3,7 +3,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <mutex>
 #include <type_traits>
@@ -25,6 +27,10 @@ using cpg_capi::launch;
 using cpg_capi::misaligned;
 
 namespace {
+
+static_assert(cpg::kLinearSkipLoads == CPG_INJECT_SKIP_LOADS &&
+                  cpg::kLinearSkipValues == CPG_INJECT_SKIP_VALUES,
+              "the flags go to the kernel as they are");
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
 constexpr int32_t kMaxLinearHeads = 1 << 20;
@@ -378,7 +384,20 @@ int encode_heads(CUtensorMap* m, const cpg::LinearRows& x, int64_t tokens, int32
   return CPG_OK;
 }
 
-constexpr uint64_t kTimeoutNs = 10000000000ull;
+// Limit of the kernels' waits in ms (0: not yet read from the environment), and the loads that the
+// producers leave out.
+std::atomic<int32_t> g_timeout_ms{0}, g_inject{0};
+
+uint64_t timeout_ns() {
+  int32_t ms = g_timeout_ms.load();
+  if (ms == 0) {
+    const char* env = std::getenv("CPG_WAIT_TIMEOUT_MS");
+    int32_t first = env != nullptr ? std::atoi(env) : 0;
+    if (first <= 0) first = 10000;
+    if (g_timeout_ms.compare_exchange_strong(ms, first)) ms = first;
+  }
+  return static_cast<uint64_t>(ms) * 1000000ull;
+}
 
 // SMs of the current device; also raises the shared-memory limit of the chunk kernels there, once.
 int device_ready(int* sms) {
@@ -519,7 +538,8 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
     if (b.pass[j].final != nullptr) b.exact = 1;
     ways[b.pass[j].reverse] = true;
   }
-  b.timeout_ns = kTimeoutNs;
+  b.timeout_ns = timeout_ns();
+  b.inject = g_inject.load();
   const LinearCut cut = linear_cut(p, b.passes);
   const int64_t heads = int64_t(p->heads) * b.passes;
   auto run_out = [&](int64_t units) {
@@ -832,6 +852,19 @@ int cpg_attention_status(int32_t* status) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
   e = cudaMemcpyFromSymbol(status, cpg::linear_status_word, sizeof(*status));
   return e == cudaSuccess ? CPG_OK : cuda_fail(e, "cudaMemcpyFromSymbol");
+}
+
+int cpg_attention_set_timeout_ms(int32_t timeout_ms) {
+  if (timeout_ms <= 0) return fail(CPG_ERR_INVALID_SHAPE, "timeout must be positive");
+  g_timeout_ms.store(timeout_ms);
+  return CPG_OK;
+}
+
+int cpg_attention_set_fault_injection(int32_t flags) {
+  if ((flags & ~(CPG_INJECT_SKIP_LOADS | CPG_INJECT_SKIP_VALUES)) != 0)
+    return fail(CPG_ERR_INVALID_CONFIG, "unknown fault-injection flags %d", flags);
+  g_inject.store(flags);
+  return CPG_OK;
 }
 
 int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, const cpg_heads* k,

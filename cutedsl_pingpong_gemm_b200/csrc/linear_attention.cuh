@@ -66,6 +66,7 @@ struct LinearBatch {
   LinearParams pass[3];
   int32_t passes;
   int32_t exact;        // states to FP32 accuracy (one is an output)
+  int32_t inject;       // test hook: loads that the producer leaves out
   uint64_t timeout_ns;  // limit of a wait within the kernel
 };
 

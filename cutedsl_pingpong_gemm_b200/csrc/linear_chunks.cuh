@@ -58,6 +58,9 @@ enum : int32_t {
 
 constexpr uint64_t kLinearDrainNs = 100000000;
 
+// Host-selected, for testing the bounded waits: the producer loads nothing, or no tile of C.
+constexpr int32_t kLinearSkipLoads = 1, kLinearSkipValues = 2;
+
 // First error of any launch on this device (0: none).
 __device__ int32_t linear_status_word;
 
@@ -324,6 +327,17 @@ struct alignas(64) LinearMaps {
   CUtensorMap m[3][3];
 };
 
+// A wait of a role whose warps go on together (.sync.aligned accesses to TMEM, votes, __syncwarp): one
+// result for all lanes.  Each lane waits for itself, and where some gave up and others did not, those that
+// go on would wait in vain for the rest.  (Two votes a wait where the first try fails; the MMA issuer, on
+// which the products wait, has no such instructions and goes without.  Level with no votes at all, votes
+// there too 0 to 2 %.)
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const ptx::WaitCtx& ctx,
+                                          int32_t site) {
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, ptx::mbar_wait_tries(bar, parity, ctx, site));
+}
+
 // What a block does: units (a pass's, a sequence's or a segment's tokens of one head) and their chunks.
 struct LinearUnit {
   int32_t pass, head;
@@ -475,6 +489,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // ---------------------------------------------------------------------------- producer
     if (lane == 0) {
       const uint64_t policy = ptx::policy_evict_first();
+      const bool skip_all = batch.inject & kLinearSkipLoads;
+      const bool skip_c = batch.inject & (kLinearSkipLoads | kLinearSkipValues);
+      uint32_t end_a = 0, end_b = 0, end_c = 0;  // one past the last chunk whose tile is on its way
       for (int32_t r = 0, u = unit_at(0); u < units && ok; u = unit_at(++r)) {
         const LinearUnit unit = linear_unit<Out>(batch, each, u);
         const LinearParams& p = batch.pass[unit.pass];
@@ -493,9 +510,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (!(ok = ptx::mbar_wait_brief(b_empty + 8 * slot, ((n >> 1) & 1u) ^ 1u, ctx,
                                           kSiteLinearProducer)))
             break;
+          if (skip_all) continue;
           ptx::mbar_arrive_expect_tx(b_full + 8 * slot, L::kTileA);
           for (int j = 0; j < DA / 64; ++j)
             ptx::tma_load_3d(tm_b, b + j * 16384, b_full + 8 * slot, 64 * j, hb, t, policy);
+          end_b = n + 1;
           // What waits for room below comes into L2 meanwhile.
           if (Out)
             for (int j = 0; j < DA / 64; ++j) ptx::tma_prefetch_l2_3d(tm_a, 64 * j, ha, t);
@@ -510,41 +529,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               ptx::mbar_arrive_expect_tx(a_full, L::kTileA);
               for (int j = 0; j < DA / 64; ++j)
                 ptx::tma_load_3d(tm_a, base + L::kA + j * 16384, a_full, 64 * j, ha, t, policy);
+              end_a = n + 1;
             } else {
               if (!(ok = ptx::mbar_wait_brief(c_empty + 8 * c_slot(n), c_phase(n) ^ 1u, ctx,
                                               kSiteLinearProducer)))
                 break;
+              if (skip_c) continue;
               ptx::mbar_arrive_expect_tx(cf, L::kTileC);
               for (int j = 0; j < DC / 64; ++j)
                 ptx::tma_load_3d(tm_c, c + j * 16384, cf, 64 * j, hc, t, policy);
+              end_c = n + 1;
             }
           }
-          if (!ok) {
-            ++n;
-            break;
-          }
+          if (!ok) break;
         }
       }
-      if (!ok) {
-        // Copies in flight land before the block ends.  (Where the waits above all succeeded, the
-        // consumers have waited for every one.)
-        volatile int32_t none = 0;
-        const ptx::WaitCtx brief{&none, nullptr, kLinearDrainNs};
+      // The copies land before the block ends, whichever role has given up: the last in every slot, as a
+      // slot is filled again only after the copy before has.
+      volatile int32_t none = 0;
+      const ptx::WaitCtx brief{&none, nullptr, kLinearDrainNs};
+      auto landed = [&](uint32_t bar, uint32_t parity) {
+        none = 0;
+        ptx::mbar_wait_brief(bar, parity, brief, kSiteLinearDrain);
+      };
 #pragma unroll 1
-        for (uint32_t j = n > 2 ? n - 2 : 0; j < n; ++j) {
-          none = 0;
-          ptx::mbar_wait_tries(b_full + 8 * (j & 1u), (j >> 1) & 1u, brief, kSiteLinearDrain);
-          none = 0;
-          ptx::mbar_wait_tries(c_full + 8 * c_slot(j), c_phase(j), brief, kSiteLinearDrain);
-          none = 0;
-          if (Out) ptx::mbar_wait_tries(a_full, j & 1u, brief, kSiteLinearDrain);
-        }
-      }
+      for (uint32_t j = end_b > 2 ? end_b - 2 : 0; j < end_b; ++j)
+        landed(b_full + 8 * (j & 1u), (j >> 1) & 1u);
+      const uint32_t slots_c = one_c ? 1 : 2;
+#pragma unroll 1
+      for (uint32_t j = end_c > slots_c ? end_c - slots_c : 0; j < end_c; ++j)
+        landed(c_full + 8 * c_slot(j), c_phase(j));
+      if (end_a > 0) landed(a_full, (end_a - 1) & 1u);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------------------- MMA issuer
     {
+      // (Each lane waits, and may give up, for itself: the issuing lane alone makes products, and the others
+      // do not take part in anything before the end.)
       const uint32_t issue = elect_one();
       constexpr uint32_t kScores = linear_idesc(kChunk, false, false);
       constexpr uint32_t kInter = linear_idesc(DC, false, true);
@@ -639,11 +661,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           state = true;
         }
       }
-      if (!ok) {  // products in flight end before TMEM is freed
-        volatile int32_t none = 0;
-        umma_commit_if(drain, issue);
-        ptx::mbar_wait_tries(drain, 0, {&none, nullptr, kLinearDrainNs}, kSiteLinearDrain);
-      }
+      // The products end before TMEM is freed, whichever role has given up.
+      volatile int32_t none = 0;
+      umma_commit_if(drain, issue);
+      ptx::mbar_wait_brief(drain, 0, {&none, nullptr, kLinearDrainNs}, kSiteLinearDrain);
     }
     __syncwarp();
   } else if (warp < 4) {
@@ -658,7 +679,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         int32_t count;
         chunk_at(unit, x, &count);
         const uint32_t c = base + L::kC + c_slot(n) * L::kTileC + box * 16384;
-        if (!(ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearScan)))
+        if (!(ok = wait_warp(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearScan)))
           break;
         uint32_t found = 0;
         if (box < DC / 64) {
@@ -674,15 +695,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           // The table is the earlier chunks' outputs' and the unit before's state's until then.
           const uint64_t t0 = ptx::globaltimer();
           while (ok && !__all_sync(0xffffffffu, lane >= 12 || (lane < 8 && !Out) ||
-                                              done[lane] >= n + (lane < 8 ? 0u : 1u)))
-            if (*abort_flag || ptx::globaltimer() - t0 > ctx.timeout_ns) {
-              ptx::record_timeout(ctx, kSiteLinearScan);
-              ok = false;
-            }
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
+                                              done[lane] >= n + (lane < 8 ? 0u : 1u))) {
+            const bool late = ptx::globaltimer() - t0 > ctx.timeout_ns;
+            if (late) ptx::record_timeout(ctx, kSiteLinearScan);
+            ok = !__any_sync(0xffffffffu, late || *abort_flag != 0);
           }
+          if (!ok) break;
           uint32_t* mine = bad + 64 * box + 2 * lane;  // of the two channels a lane has
 #pragma unroll 1
           for (int32_t place = reverse ? kChunk - count : 0; place < (reverse ? kChunk : count);
@@ -728,7 +746,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
         chunk_at(unit, x, &count);
-        if (!(ok = ptx::mbar_wait_brief(s_full, n & 1u, ctx, kSiteLinearScores))) break;
+        if (!(ok = wait_warp(s_full, n & 1u, ctx, kSiteLinearScores))) break;
         ptx::tc_fence_after();
 #pragma unroll 1
         for (uint32_t blk = 0; blk < 4; ++blk) {
@@ -806,7 +824,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       for (int32_t x = 0; x < unit.chunks; ++x, ++n) {
         int32_t count;
         const int64_t t = chunk_at(unit, x, &count);
-        if (!(ok = ptx::mbar_wait_brief(o_full, n & 1u, ctx, kSiteLinearOutput))) break;
+        if (!(ok = wait_warp(o_full, n & 1u, ctx, kSiteLinearOutput))) break;
         ptx::tc_fence_after();
         const bool spoilt = *last_bad > unit_first;
         // 16 tokens x 32 channels at a time: a lane has neighbouring pairs of channels of two tokens,
@@ -964,7 +982,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // The chunk before is done with the state and its copy (at a unit's first chunk: waited for
         // at the end of the last one).
         if (x > 0) {
-          if (!(ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
+          if (!(ok = wait_warp(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
           ptx::tc_fence_after();
         }
         if ((warp & 3u) * 32 < DA && (x > 0 || from != nullptr)) {
@@ -1005,7 +1023,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           done[warp - 8] = n + 1;
         }
       }
-      if (!ok || !(ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
+      if (!ok || !(ok = wait_warp(h_full, (n - 1) & 1u, ctx, kSiteLinearState))) break;
       ptx::tc_fence_after();
       if (to != nullptr) {
         const bool spoilt = *last_bad > unit_first;
@@ -1066,7 +1084,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (ok && n > 0) ok = ptx::mbar_wait_brief(h_full, (n - 1) & 1u, ctx, kSiteLinearLeft);
         if (ok && count < kChunk)
           ok = ptx::mbar_wait_brief(c_full + 8 * c_slot(n), c_phase(n), ctx, kSiteLinearLeft);
-        if (!ok) break;
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;  // (together, as wait_warp)
         if (exact) {
 #pragma unroll 1
           for (uint32_t piece = 0; piece < DA / 8; ++piece) {
@@ -1132,7 +1150,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
   }
-  // Every product has completed: the state's of the last chunk is waited for above.
+  // Every copy has landed and every product has completed (waited for by the roles that began them).
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc<1>(tmem, 512);

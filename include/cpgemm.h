@@ -473,9 +473,22 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
 int cpg_linear_attention_workspace(const cpg_linear_problem* p, int32_t q_heads, int32_t k_heads,
                                    int32_t v_heads, int32_t backward, int64_t* bytes);
 
-/* Synchronises and reads the current device's word of the linear attention kernels: 0, or the code of
- * the first wait that ever ran out there (10 s; the outputs of that launch are not valid). */
+/* Synchronises and reads the current device's word of the linear attention kernels: 0, or the code
+ * (0x100 | wait site) of the first wait that ever ran out there; the outputs of that launch are not
+ * valid. */
 int cpg_attention_status(int32_t* status);
+
+/* Limit of every wait within the linear attention kernels launched (or captured) from now on, in
+ * milliseconds; of the process (default CPG_WAIT_TIMEOUT_MS from the environment, or 10000). */
+int cpg_attention_set_timeout_ms(int32_t timeout_ms);
+
+/* Test hook for those waits, of the process: the kernels launched from now on load nothing
+ * (CPG_INJECT_SKIP_LOADS), or all but the tiles of v (CPG_INJECT_SKIP_VALUES; in the gradient those of
+ * k, q and dy that are in its place), so that waits run out their limit.  The kernels record the
+ * wait site, stop every role, wait for their copies and products in flight, free TMEM and return.  0
+ * restores normal operation. */
+#define CPG_INJECT_SKIP_VALUES 2
+int cpg_attention_set_fault_injection(int32_t flags);
 
 /* One token of each of p->tokens sequences: q, k, v and out [tokens, heads, channels], the states
  * updated in place.  Tokens whose slot is outside [0, places) are padding: their out is 0. */
