@@ -216,6 +216,7 @@ SIGNATURES = {
                                                      _S, _S, _H, _H, _H, _S, _i32, _vp, _i64, _vp]),
     "cpg_linear_attention_workspace": (ctypes.c_int, [_P(LinearProblemC), _i32, _i32, _i32, _i32,
                                                       _P(_i64)]),
+    "cpg_linear_attention_clear": (ctypes.c_int, [_P(LinearProblemC), _H, _vp, _vp]),
     "cpg_attention_status": (ctypes.c_int, [_P(_i32)]),
     "cpg_attention_set_timeout_ms": (ctypes.c_int, [_i32]),
     "cpg_attention_set_fault_injection": (ctypes.c_int, [_i32]),

@@ -186,8 +186,8 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     h // (H // Hx) of each.  dk and dv are
     multiples of 8 up to 128, addresses and strides multiples of 16 bytes.
     ``offsets`` int32 [B + 1], read on the device: sequence b is the rows
-    ``offsets[b] <= t < offsets[b + 1]`` (None: one sequence of all rows); rows outside are not
-    written (undefined without a given ``out``).
+    ``offsets[b] <= t < offsets[b + 1]`` (None: one sequence of all rows); rows outside are 0
+    in an ``out`` that it allocates and left as they were in one that is given.
     ``state`` FP32 [B, H, dk, dv]: where the sequences start (None: zeros); ``final``: True, or a
     tensor like it, gets the states after their last tokens.  With ``slots`` (int32 [B]) both are
     pools [places, H, dk, dv] and sequence b is at ``slots[b]``; one outside the pool starts from
@@ -201,6 +201,7 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     b = _sequences(offsets, dev)
     p, problem, q_c, k_c, v_c = _linear_args(q, k, v, log_decay, scale, b)
     _slots(slots, b, dev)
+    fresh = out is None
     out, o_c = _attention_output(out, v, problem)
     if final is True:
         if slots is not None:
@@ -218,6 +219,8 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     work = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
     call(lib.cpg_linear_attention, "linear_attention", dev, p, q_c, k_c, v_c, ptr(log_decay),
          ptr(offsets), s_c, f_c, o_c, ptr(work), size.value)
+    if fresh and offsets is not None:
+        call(lib.cpg_linear_attention_clear, "linear_attention", dev, p, o_c, ptr(offsets))
     return out, final
 
 

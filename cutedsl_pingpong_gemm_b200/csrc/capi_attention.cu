@@ -620,6 +620,25 @@ BackwardSpace backward_space(const cpg_linear_problem* p, int32_t q_heads, int32
   return r;
 }
 
+// Clearing of rows outside the sequences.
+void add_cleared(cpg::LinearClearParams* c, int i, const cpg_heads* x, int32_t d) {
+  const int eb = bytes_of(x->dtype);
+  c->p[i] = static_cast<char*>(x->ptr);
+  c->token[i] = x->token_stride * eb;
+  c->head[i] = x->head_stride * eb;
+  c->heads[i] = x->heads;
+  c->pieces[i] = d * eb / 16;
+}
+
+int run_clear(cpg::LinearClearParams c, const cpg_linear_problem* p, const int32_t* offsets,
+              cudaStream_t st) {
+  c.offsets = offsets;
+  c.tokens = p->tokens;
+  c.sequences = p->sequences;
+  return launch("clear kernel", true, &cpg::linear_clear_kernel,
+                static_cast<unsigned>(std::min<int64_t>(p->tokens, 148)), 256, 0, st, 1, c);
+}
+
 }  // namespace
 
 extern "C" {
@@ -832,18 +851,21 @@ int cpg_linear_attention_backward(const cpg_linear_problem* p, const cpg_heads* 
   }
   if (rc != CPG_OK || clear == 0 || offsets == nullptr || p->tokens == 0) return rc;
   cpg::LinearClearParams c = {};
-  for (int i = 0; i < 3; ++i) {
-    c.p[i] = static_cast<__nv_bfloat16*>(grads[i]->ptr);
-    c.token[i] = grads[i]->token_stride;
-    c.head[i] = grads[i]->head_stride;
-    c.heads[i] = grads[i]->heads;
-    c.d[i] = i < 2 ? p->dk : p->dv;
-  }
-  c.offsets = offsets;
-  c.tokens = p->tokens;
-  c.sequences = p->sequences;
-  return launch("clear kernel", true, &cpg::linear_clear_kernel,
-                static_cast<unsigned>(std::min<int64_t>(p->tokens, 148)), 256, 0, st, 1, c);
+  for (int i = 0; i < 3; ++i) add_cleared(&c, i, grads[i], i < 2 ? p->dk : p->dv);
+  return run_clear(c, p, offsets, st);
+}
+
+int cpg_linear_attention_clear(const cpg_linear_problem* p, const cpg_heads* out,
+                               const int32_t* offsets, void* stream) {
+  int rc = check_linear(p);
+  if (rc == CPG_OK) rc = check_operand("out", p, out, p->dv, true, true);
+  if (rc != CPG_OK) return rc;
+  if (offsets == nullptr) return fail(CPG_ERR_NULL, "offsets is NULL");
+  if (misaligned(offsets, 4)) return fail(CPG_ERR_ALIGNMENT, "offsets must be aligned to 4 bytes");
+  if (p->tokens == 0) return CPG_OK;
+  cpg::LinearClearParams c = {};
+  add_cleared(&c, 0, out, p->dv);
+  return run_clear(c, p, offsets, static_cast<cudaStream_t>(stream));
 }
 
 int cpg_attention_status(int32_t* status) {

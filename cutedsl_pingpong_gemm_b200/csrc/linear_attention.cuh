@@ -222,11 +222,11 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch 
       make_float4(f * state.x, f * state.y, f * state.z, f * state.w);
 }
 
-// Rows of a [tokens, heads, d] outside the sequences, set to zero.
+// Rows of up to three [tokens, heads, d] outside the sequences, set to zero, 16 bytes at a time.
 struct LinearClearParams {
-  __nv_bfloat16* p[3];
-  int64_t token[3], head[3];
-  int32_t heads[3], d[3];
+  char* p[3];
+  int64_t token[3], head[3];    // strides in bytes
+  int32_t heads[3], pieces[3];  // 16-byte pieces of a head
   const int32_t* offsets;
   int64_t tokens;
   int32_t sequences;
@@ -242,8 +242,9 @@ __global__ void __launch_bounds__(256) linear_clear_kernel(const LinearClearPara
     const int64_t t = r < first ? r : last + r - first;
 #pragma unroll
     for (int n = 0; n < 3; ++n)
-      for (int32_t i = threadIdx.x; i < p.heads[n] * p.d[n]; i += blockDim.x)
-        p.p[n][t * p.token[n] + i / p.d[n] * p.head[n] + i % p.d[n]] = __float2bfloat16_rn(0.f);
+      for (int32_t i = threadIdx.x; i < p.heads[n] * p.pieces[n]; i += blockDim.x)
+        ptx::st_global_v4(p.p[n] + t * p.token[n] + i / p.pieces[n] * p.head[n] + i % p.pieces[n] * 16,
+                          0u, 0u, 0u, 0u);
   }
 }
 

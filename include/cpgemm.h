@@ -459,6 +459,11 @@ int cpg_linear_attention(const cpg_linear_problem* p, const cpg_heads* q, const 
                          const cpg_states* state, const cpg_states* final, const cpg_heads* out,
                          void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Sets the rows of out (of the problem above) that are outside the sequences to zero, for callers that
+ * hand on all of its rows.  offsets must not be NULL. */
+int cpg_linear_attention_clear(const cpg_linear_problem* p, const cpg_heads* out,
+                               const int32_t* offsets, void* stream);
+
 /* Gradients of q, k and v (BF16, summed in FP32 over the heads that share one) from dy, the
  * gradient of out (BF16 [tokens, heads, dv]), and dfinal, that of the final states (NULL: zeros);
  * dstate (NULL: not wanted) gets that of the starting states.  clear != 0: rows outside the
