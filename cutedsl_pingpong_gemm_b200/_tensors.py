@@ -101,11 +101,13 @@ def heads(name, t, device=None, tokens=None, channels=None):
         _lib.HeadsC(t.data_ptr() or None, step[0], step[1], size[1], code))
 
 
-def fresh_heads(like, dtype=None):
-    """A contiguous tensor of this shape and its C description."""
-    t = torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
-    _, h, d = like.shape
-    return t, ctypes.byref(_lib.HeadsC(t.data_ptr() or None, h * d, d, h, FLOAT_CODES[t.dtype]))
+def fresh_heads(like, heads=None):
+    """A contiguous tensor of this shape and type (with another number of heads) and its C
+    description."""
+    t, h, d = like.shape
+    h = h if heads is None else heads
+    x = torch.empty((t, h, d), dtype=like.dtype, device=like.device)
+    return x, ctypes.byref(_lib.HeadsC(x.data_ptr() or None, h * d, d, h, FLOAT_CODES[x.dtype]))
 
 
 def same_heads(name, t, shape, dtype, device):

@@ -159,8 +159,7 @@ def _slots(slots, n, device):
 def _attention_output(out, v, problem):
     """``out`` [tokens, heads, dv], or a new one in v's type, and its description."""
     if out is None:
-        like = v if v.shape[1] == problem.heads else v[:, :1].expand(-1, problem.heads, -1)
-        return fresh_heads(like)
+        return fresh_heads(v, heads=problem.heads)
     if out.dtype not in FLOAT_CODES:
         raise error(_lib.CPG_ERR_DTYPE, f"out must be BF16 or FP32, got {out.dtype}")
     shape = (problem.tokens, problem.heads, problem.dv)

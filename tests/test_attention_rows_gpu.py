@@ -73,3 +73,23 @@ def test_clear_refusals(lib):
     assert clear(dtype=_lib.CPG_DTYPE_I8) == D
     assert lib.cpg_linear_attention_clear(None, None, 4096, None) == N
     assert clear(t=0, p=None) == _lib.CPG_OK
+
+
+@pytest.mark.gpu
+def test_tensors_without_heads_are_refused():
+    """With the framework's own error, before an output is made."""
+    q, decay = normal(1, 9, 2, 64), torch.zeros(2, device="cuda")
+    state = torch.zeros(9, 2, 64, 64, device="cuda")
+    none = q[:, :0]
+    for a, b, c in ((none, q, q), (q, none, q), (q, q, none)):
+        for call in (lambda: attention.linear_attention(a, b, c, decay),
+                     lambda: attention.linear_attention_step(a, b, c, decay, state),
+                     lambda: attention.linear_attention_backward(q, a, b, c, decay)):
+            with pytest.raises(_lib.CpgError) as e:
+                call()
+            assert e.value.code == _lib.CPG_ERR_INVALID_SHAPE
+    with pytest.raises(_lib.CpgError):
+        attention.linear_attention(q, q, q, decay[:0])
+    pos = torch.zeros(9, dtype=torch.int32, device="cuda")
+    with pytest.raises(_lib.CpgError):
+        attention.norm_rope(none, q, None, None, None, pos)
