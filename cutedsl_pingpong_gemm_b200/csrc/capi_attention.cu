@@ -222,7 +222,7 @@ int by_lanes(const NormRope& n, F&& f) {
   if (pairs <= 8) return heads(integral_constant<int, 8>{}, one);
   if (pairs <= 16) return heads(integral_constant<int, 16>{}, one);
   const integral_constant<int, 32> warp;
-  // At most kHeadMaxChannels / V / 2 pairs: V = 8 has 16, V = 4 32, V = 2 64, V = 1 128.
+  // At most CPG_HEAD_MAX_CHANNELS / V / 2 pairs: V = 8 has 16, V = 4 32, V = 2 64, V = 1 128.
   if constexpr (V <= 4) {
     if (pairs <= 32) return heads(warp, one);
   }
@@ -444,16 +444,15 @@ int device_ready(int* sms) {
 // and 3.5 us where all SMs share the bandwidth.  Cutting sequences costs a pass over B and C for the
 // segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
 // channels 1470 -> 350 us.  The lengths are known to the device alone: the mean stands for them.
-// Ragged sequences that stay whole are begun in the order of their lengths (`sorted`) where there is
+// Ragged sequences that stay whole are items too, begun in the order of their lengths, where there is
 // more than one unit per SM: a long one begun last would run alone.
 struct LinearCut {
   int64_t length, items;
-  bool sorted;
 };
 
 LinearCut linear_cut(const cpg_linear_problem* p, int passes) {
   constexpr int64_t kSms = 148, kMostCut = 1024;
-  if (p->sequences == 0 || p->tokens == 0) return {0, 0, false};
+  if (p->sequences == 0 || p->tokens == 0) return {0, 0};
   const int64_t mean = (p->tokens + p->sequences - 1) / p->sequences;
   const int64_t chunks = (mean + cpg::kChunk - 1) / cpg::kChunk;
   const int64_t units = int64_t(p->sequences) * p->heads * passes;
@@ -461,7 +460,7 @@ LinearCut linear_cut(const cpg_linear_problem* p, int passes) {
   double best = chunks * (units < kSms ? 2.8 : 3.5 * waves);
   int64_t cut = 0;
   const bool sorted = units > kSms && p->sequences > 1 && p->sequences <= cpg::kMostSorted;
-  const LinearCut uncut{0, sorted ? p->sequences : 0, sorted};
+  const LinearCut uncut{0, sorted ? p->sequences : 0};
   if (units > kMostCut) return uncut;
   for (int64_t length = 2; length < std::min<int64_t>(chunks, 128); ++length) {
     const int64_t segments = (chunks + length - 1) / length;
@@ -475,7 +474,7 @@ LinearCut linear_cut(const cpg_linear_problem* p, int passes) {
     }
   }
   if (cut == 0) return uncut;
-  return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences, false};
+  return {cut * cpg::kChunk, p->tokens / (cut * cpg::kChunk) + p->sequences};
 }
 
 // Workspace of passes that run together: the segments' states of each, then the table of segments or
@@ -922,7 +921,6 @@ int cpg_linear_attention_step(const cpg_linear_problem* p, const cpg_heads* q, c
                                 state->ptr,
                                 state->slots,
                                 state->places,
-                                static_cast<int32_t>(p->tokens),
                                 p->heads,
                                 p->dk,
                                 p->dv,

@@ -23,7 +23,6 @@
 namespace cpg {
 
 constexpr int kHeadThreads = 256;
-constexpr int kHeadMaxChannels = 256;
 
 struct HeadPart {
   const void* x;

@@ -15,8 +15,6 @@
 
 namespace cpg {
 
-constexpr int kLinearMaxChannels = 128;
-
 struct LinearRows {
   const __nv_bfloat16* p;
   int64_t token, head;  // strides in elements
@@ -305,7 +303,7 @@ struct LinearStepParams {
   float* state;  // [places, heads, dk, dv]
   const int32_t* slots;
   int64_t places;
-  int32_t batch, heads, dk, dv;
+  int32_t heads, dk, dv;
   float scale;
 };
 

@@ -301,7 +301,6 @@ struct StatePart {
   int32_t row, col;
   uint32_t tmem;
 };
-template <int DC>
 __device__ __forceinline__ StatePart state_part(uint32_t warp, uint32_t lane, int32_t part) {
   const int32_t half = part & 1, box = part >> 1;
   return {static_cast<int32_t>((warp & 3u) * 32 + 16 * half + lane / 4),
@@ -912,23 +911,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                    ? unit.from_factor * from[unit.transposed ? c * p.da + i : i * p.dc + c]
                    : 0.f;
       };
-      if (unit.chunks == 0) {  // the final state is the starting one
+      if (unit.chunks == 0) {  // the final state is the starting one (no pass has both one and a transposed one)
         const float factor = unit.from_factor * unit.to_factor;
         const int32_t size = p.da * p.dc;
-        if (to == nullptr || (to == from && factor == 1.f && !unit.transposed)) continue;
+        if (to == nullptr || (to == from && factor == 1.f)) continue;
         for (int32_t e0 = 4 * i; e0 < size; e0 += 4 * 128 * 4) {  // four loads in flight
           float4 v[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int32_t e = e0 + 4 * 128 * k;
             v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (from == nullptr || e >= size) continue;
-            if (!unit.transposed) {
-              v[k] = *reinterpret_cast<const float4*>(from + e);
-            } else {
-              const float* at = from + e % p.dc * p.da + e / p.dc;
-              v[k] = make_float4(at[0], at[p.da], at[2 * p.da], at[3 * p.da]);
-            }
+            if (from != nullptr && e < size) v[k] = *reinterpret_cast<const float4*>(from + e);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -951,7 +944,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       } else if (from != nullptr) {
 #pragma unroll 1
         for (int32_t part = 0; part < DC / 32; ++part) {
-          const StatePart at = state_part<DC>(warp, lane, part);
+          const StatePart at = state_part(warp, lane, part);
           const float* tile = from + at.row * p.dc + at.col;
           uint32_t s[32];
 #pragma unroll
@@ -1029,7 +1022,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool spoilt = *last_bad > unit_first;
 #pragma unroll 1
         for (int32_t part = 0; part < DC / 16; ++part) {  // half a part: 32 columns
-          StatePart at = state_part<DC>(warp, lane, part / 2);
+          StatePart at = state_part(warp, lane, part / 2);
           at.col += 32 * (part & 1);
           at.tmem += 32 * (part & 1);
           float* tile = to + at.row * p.dc + at.col;
