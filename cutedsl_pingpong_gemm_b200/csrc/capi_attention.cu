@@ -64,7 +64,10 @@ int check_heads(const char* name, const cpg_heads* x, int64_t tokens, int64_t ch
 }
 
 // ------------------------------------------------------------------------- norm and rotation
-constexpr int kGradBlocks = 148 * 4;  // of both parts together, at most
+// Blocks of the gradient, of both parts together, at most.  Two an SM are on it at once whatever the
+// vectors; with four a second round follows (8191 tokens x 40 heads x 128, BF16: 55 us, 60 with four; 8192
+// x 32 x 20 in BF16 23 and 25, x 75 in FP32 110 and 118, in BF16 180 and 174).
+constexpr int kGradBlocks = 148 * 2;
 constexpr int64_t kManyThreads = int64_t(148) * 2048 * 4;
 
 // Address bits that some head of x has set (of the lowest ones).
@@ -250,14 +253,14 @@ int by_head(const NormRope& n, F&& f) {
   return by_lanes<float, 1, Many>(n, f);
 }
 
-// Blocks of each part in the gradient, of `all`, in proportion to their heads and at most one per row.
-void grad_blocks(int64_t tokens, int32_t q_heads, int32_t k_heads, int all, int32_t* blocks) {
+// Blocks of each part in the gradient, in proportion to their heads and at most one per row.
+void grad_blocks(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t* blocks) {
   const int64_t heads = int64_t(q_heads) + k_heads;
   for (int i = 0; i < 2; ++i) {
     const int64_t h = i == 0 ? q_heads : k_heads;
     blocks[i] = h == 0 ? 0
                        : static_cast<int32_t>(std::max<int64_t>(
-                             1, std::min<int64_t>(tokens * h, all * h / heads)));
+                             1, std::min<int64_t>(tokens * h, kGradBlocks * h / heads)));
   }
 }
 
@@ -674,7 +677,7 @@ int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, in
   const int rc = check_norm_sizes(tokens, int64_t(q_heads) + k_heads, channels);
   if (rc != CPG_OK) return rc;
   int32_t blocks[2];
-  grad_blocks(tokens, q_heads, k_heads, kGradBlocks, blocks);
+  grad_blocks(tokens, q_heads, k_heads, blocks);
   *bytes = (int64_t(blocks[0]) + blocks[1]) * channels * 4;
   return CPG_OK;
 }
@@ -697,11 +700,7 @@ int cpg_norm_rope_backward(const cpg_heads* dq, const cpg_heads* dk, const cpg_h
   if (dk_weight != nullptr && k == nullptr)
     return fail(CPG_ERR_NULL, "the gradient of k's weight needs k");
   cpg::HeadParams p = head_params(n);
-  // As many as are on the SMs at once: two of 16-byte vectors each (8191 tokens x 40 heads x 128, BF16:
-  // 54 us, 60 us with four), four of narrower ones (8192 x 32 x 75: 176 us with two, 98 us).
-  const bool wide = tokens > 0 && head_vector(n) * bytes_of(q->dtype) == 16;
-  grad_blocks(tokens, p.part[0].heads, p.part[1].heads, wide ? kGradBlocks / 2 : kGradBlocks,
-              p.blocks);
+  grad_blocks(tokens, p.part[0].heads, p.part[1].heads, p.blocks);
   int64_t bytes = 0;
   rc = cpg_norm_rope_workspace(tokens, p.part[0].heads, p.part[1].heads, channels, &bytes);
   if (rc != CPG_OK) return rc;
