@@ -185,8 +185,9 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, offsets=None, st
     h // (H // Hx) of each.  dk and dv are
     multiples of 8 up to 128, addresses and strides multiples of 16 bytes.
     ``offsets`` int32 [B + 1], read on the device: sequence b is the rows
-    ``offsets[b] <= t < offsets[b + 1]`` (None: one sequence of all rows); rows outside are 0
-    in an ``out`` that it allocates and left as they were in one that is given.
+    ``offsets[b] <= t < offsets[b + 1]`` (None: one sequence of all rows), cut to the rows that
+    there are and empty where it would end before it starts; no two may overlap.  Rows outside are
+    0 in an ``out`` that is allocated here and left as they were in one that is given.
     ``state`` FP32 [B, H, dk, dv]: where the sequences start (None: zeros); ``final``: True, or a
     tensor like it, gets the states after their last tokens.  With ``slots`` (int32 [B]) both are
     pools [places, H, dk, dv] and sequence b is at ``slots[b]``; one outside the pool starts from

@@ -220,6 +220,19 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearBatch 
       make_float4(f * state.x, f * state.y, f * state.z, f * state.w);
 }
 
+// Offsets from the first up to the last pass every row between them on their way; where they also decrease,
+// a sequence may lie outside.  Whether they do (asked by a whole block), and whether a row is in one.
+__device__ __forceinline__ bool linear_decreases(const int32_t* offsets, int32_t sequences) {
+  bool down = false;
+  for (int32_t s = threadIdx.x; s < sequences; s += blockDim.x) down |= offsets[s] > offsets[s + 1];
+  return __syncthreads_or(down);
+}
+__device__ __forceinline__ bool linear_inside(const int32_t* offsets, int32_t sequences, int64_t t) {
+  for (int32_t s = 0; s < sequences; ++s)
+    if (offsets[s] <= t && t < offsets[s + 1]) return true;
+  return false;
+}
+
 // Rows of up to three [tokens, heads, d] outside the sequences, set to zero, 16 bytes at a time.
 struct LinearClearParams {
   char* p[3];
@@ -236,8 +249,11 @@ __global__ void __launch_bounds__(256) linear_clear_kernel(const LinearClearPara
   const int64_t last =
       min(max(static_cast<int64_t>(p.offsets[p.sequences]), first), p.tokens);
   const int64_t rows = first + p.tokens - last;
+  if (rows == 0) return;
+  const bool down = linear_decreases(p.offsets, p.sequences);
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const int64_t t = r < first ? r : last + r - first;
+    if (down && linear_inside(p.offsets, p.sequences, t)) continue;
 #pragma unroll
     for (int n = 0; n < 3; ++n)
       for (int32_t i = threadIdx.x; i < p.heads[n] * p.pieces[n]; i += blockDim.x)
@@ -265,10 +281,7 @@ __global__ void __launch_bounds__(256) linear_share_kernel(const LinearSharePara
     last = min(max(static_cast<int64_t>(p.offsets[p.sequences]), first), p.tokens);
   }
   const int32_t row = p.heads * p.d / 8;  // eight neighbouring channels a thread
-  const int64_t n = (last - first) * row;
-  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += gridDim.x * int64_t(256)) {
-    const int64_t t = first + i / row;
-    const int32_t e = static_cast<int32_t>(i % row) * 8;
+  auto add = [&](int64_t t, int32_t e) {
     const int32_t h = e / p.d, x = e % p.d;
     const float* from = p.partial + (t * p.heads + h) * int64_t(p.share) * p.d + x;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -287,6 +300,16 @@ __global__ void __launch_bounds__(256) linear_share_kernel(const LinearSharePara
     ptx::st_global_v4(p.out + t * p.token + h * p.head + x, ptx::pack_bf16x2(a.x, a.y),
                       ptx::pack_bf16x2(a.z, a.w), ptx::pack_bf16x2(b.x, b.y),
                       ptx::pack_bf16x2(b.z, b.w));
+  };
+  const int64_t n = (last - first) * row;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += gridDim.x * int64_t(256))
+    add(first + i / row, static_cast<int32_t>(i % row) * 8);
+  const int64_t rows = first + p.tokens - last;
+  if (rows == 0 || !linear_decreases(p.offsets, p.sequences)) return;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int64_t t = r < first ? r : last + r - first;
+    if (!linear_inside(p.offsets, p.sequences, t)) continue;
+    for (int32_t i = threadIdx.x; i < row; i += 256) add(t, i * 8);
   }
 }
 

@@ -428,8 +428,8 @@ int cpg_norm_rope_workspace(int64_t tokens, int32_t q_heads, int32_t k_heads, in
 
 /* Linear attention with a decay per head, over sequences packed along the tokens:
  *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t    (S [dk, dv], FP32)
- * offsets: int32 [sequences + 1], token rows of every sequence (not decreasing; cut to the tokens
- * there are), NULL for one sequence of all tokens.  Rows outside are neither read nor written.
+ * offsets: int32 [sequences + 1], token rows of every sequence (cut to the tokens there are; a
+ * sequence that would end before it starts is empty; none overlap), NULL for one sequence of all tokens.  Rows outside are neither read nor written.
  * q, k, v BF16, their heads divide `heads` (head h reads head h / (heads / x.heads)); dk and dv
  * multiples of 8 up to CPG_LINEAR_MAX_CHANNELS; rows and strides multiples of 16 bytes.
  * log_decay FP32 [heads], at most 0 (-infinity: no state is kept).  At most 2^20 heads.  scale and

@@ -93,3 +93,29 @@ def test_tensors_without_heads_are_refused():
     pos = torch.zeros(9, dtype=torch.int32, device="cuda")
     with pytest.raises(_lib.CpgError):
         attention.norm_rope(none, q, None, None, None, pos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets", [[0, 140, 90], [50, 100, 0, 30], [60, 20, 190, 40], [5, 3],
+                                     [-4, 70, 2 ** 31 - 1, 10]])
+@pytest.mark.parametrize("share", [1, 2])
+def test_rows_of_a_sequence_stay_where_offsets_decrease(offsets, share):
+    """A sequence that would end before it starts is empty; clearing what is outside leaves the rows of
+    the others, wherever they lie."""
+    t, h = 200, 2
+    q, k, v, dy = (normal(i, t, h if i == 3 else h // share, 64) for i in range(4))
+    decay = torch.tensor([-0.1, -0.02], device="cuda")
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    held = torch.full((t, h, 64), 7.0, dtype=BF, device="cuda")
+    want, _ = attention.linear_attention(q, k, v, decay, offsets=off, out=held)
+    out, _ = attention.linear_attention(q, k, v, decay, offsets=off)
+    wants = [torch.full(q.shape, 7.0, dtype=BF, device="cuda") for _ in range(3)]
+    attention.linear_attention_backward(dy, q, k, v, decay, offsets=off, out=tuple(wants))
+    grads = attention.linear_attention_backward(dy, q, k, v, decay, offsets=off)
+    inside = torch.zeros(t, dtype=torch.bool)
+    for a, b in zip(offsets, offsets[1:]):
+        inside[max(a, 0):max(b, 0)] = True
+    assert 0 < int(inside.sum()) < t or offsets == [5, 3] or offsets[0] < 0
+    for x, y in ((out, want), *zip(grads, wants)):
+        assert torch.equal(x[inside], y[inside]) and not x[~inside].any()
+        assert (y[~inside] == 7).all()
