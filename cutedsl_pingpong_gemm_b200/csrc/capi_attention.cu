@@ -203,7 +203,7 @@ int head_vector(const NormRope& n) {
 
 // f(type, vector, lanes, pairs a lane, heads at a time) for the sizes at hand: the fewest lanes that hold
 // a head, and Many heads at a time where there are more threads than the SMs hold at once (16384 tokens
-// x 40 heads x 128, BF16: 67 us, one at a time 90; few threads would leave SMs idle).
+// x 40 heads x 128, BF16: 68 us, one at a time 90; few threads would leave SMs idle).
 template <typename T, int V, int Many, typename F>
 int by_lanes(const NormRope& n, F&& f) {
   using std::integral_constant;
@@ -446,7 +446,7 @@ int device_ready(int* sms) {
 // be.  A unit (a sequence or segment of one head) is a chain of chunks of one SM, 2.8 us each alone
 // and 3.5 us where all SMs share the bandwidth.  Cutting sequences costs a pass over B and C for the
 // segments' states (2 us a chunk) and their joining, but fills the SMs: 65536 tokens x 16 heads of 128
-// channels 1470 -> 350 us.  The lengths are known to the device alone: the mean stands for them.
+// channels 1470 -> 340 to 400 us.  The lengths are known to the device alone: the mean stands for them.
 // Ragged sequences that stay whole are items too, begun in the order of their lengths, where there is
 // more than one unit per SM: a long one begun last would run alone.
 struct LinearCut {
@@ -595,8 +595,9 @@ int run_passes(const cpg_linear_problem* p, cpg::LinearBatch b, void* space, cud
 
 // Whether all three passes of the gradient run together, or dq and dk before dv.  Where dk and dv are not
 // both up to 64 or above, together means 128 channels for all, which pays where launches and the last
-// blocks' tails count (dk = 64, dv = 128 in a graph: 37 tokens x 16 heads 25 -> 17 us, 5 sequences of 820
-// 105 -> 92) and costs where the chunks do (8 sequences of 2048 x 32 heads 335 -> 370 us).
+// blocks' tails count (dk = 64, dv = 128 x 16 heads in a graph: 37 tokens 18 -> 10 us, 2 sequences of 1024
+// 57 -> 32, 5 of 820 75 -> 56) and costs where the chunks do (8 of 1024 92 -> 98 us, of 2048 x 32 heads 347 ->
+// 379).
 bool one_launch(const cpg_linear_problem* p) {
   if ((p->dk > 64) == (p->dv > 64)) return true;
   return p->tokens <= int64_t(8) * cpg::kChunk * p->sequences &&

@@ -6,9 +6,9 @@
 // n = x r:
 //   dx = r (u - n mean(u n)),   dw = sum over tokens and heads of g n.
 // Bound by HBM: a head is read once (its gradient: x and dy) and written once.  16384 tokens x 32 heads x
-// 128, FP32: 84 us, its gradient 130, 0.97 and 0.95 of the copy rate; with BF16 the instructions for twice
-// the elements a byte show: 16384 x 40 x 128 67 us (0.77), the gradient of 8191 54 us (0.72).  Narrow
-// vectors are bound by instructions: 8192 x 32 x 75 BF16 69 us (0.18).
+// 128, FP32: 87 us, its gradient 133, 0.95 and 0.93 of the copy rate; with BF16 the instructions for twice
+// the elements a byte show: 16384 x 40 x 128 68 us (0.75), the gradient of 8191 54 us (0.71).  Narrow
+// vectors are bound by instructions: 8192 x 32 x 75 BF16 69 us (0.18), its gradient 177 us (0.10).
 //
 // A head is split into vectors of V elements, the widest its alignment allows.  A lane takes two
 // vectors at a time, those whose channels are turned into one another (channels i and i + half, or
@@ -226,7 +226,7 @@ __device__ __forceinline__ float sum_lanes(float v) {
 
 // A group of L lanes takes HB heads of one part of a token: the angles and the weights are loaded
 // once, and all of its heads before the first is used.  (Three blocks an SM although four heads of
-// 16-byte vectors then spill 150 bytes: 67 us for 16384 x 40 x 128 in BF16, 73 with two.  Weights
+// 16-byte vectors then spill 150 bytes: 68 us for 16384 x 40 x 128 in BF16, 73 with two.  Weights
 // multiplied into the angles, or two FP32 operations an instruction: 66 and 80 us, their gradients 111
 // and 114, not 96, for more registers.)
 template <typename T, int V, int L, int NP, int HB>

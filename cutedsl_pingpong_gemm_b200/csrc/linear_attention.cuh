@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) linear_share_kernel(const LinearSharePara
 }
 
 // One token of each of many sequences: S <- e^g S + k v^T in place, o = scale * S^T q.
-// Bound by HBM: every state is read and written once (256 tokens x 64 heads x 128 x 128: 369 us, 0.90 of
+// Bound by HBM: every state is read and written once (256 tokens x 64 heads x 128 x 128: 367 us, 0.90 of
 // the copy rate).  A block has one state, a lane four neighbouring columns of every (1024 / dv)-th row,
 // whose loads are independent.
 struct LinearStepParams {

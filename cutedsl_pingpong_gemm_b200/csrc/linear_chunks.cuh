@@ -8,8 +8,10 @@
 // bound, 3.0 us a chunk when 148 blocks share the measured bandwidth.  The work of a chunk is a chain,
 // scores (760 cycles) -> P (2400) -> P C (1050) -> the state (1050) -> its copy, of which the tiles'
 // loads, left . B, the next scores and the output run beside: 5300 cycles a chunk of 128 channels, 4100 of
-// 64, 2.7 us at 1965 MHz (8 sequences of 2048 tokens x 64 heads x 128: 226 us after a rest, HBM 164).  In
-// long loops the power limit holds the clock at 1.43 to 1.5 GHz and the same takes 276 to 293 us.
+// 64, 2.7 us at 1965 MHz (8 sequences of 2048 tokens x 64 heads x 128: 226 to 240 us after a rest, HBM 164).
+// In long loops the power limit holds the clock at 1.43 to 1.5 GHz and the same takes 276 to 293 us.  (The
+// state's product reads nothing of P: it stands in the chain only because it is issued after P C.  The other
+// order has not been tried.)
 // Measured level or slower, and not kept: P by eight warps, A in TMEM, the output by way of shared memory
 // and TMA, P C begun on the first half of P (0-2 %, more spills), the moves of states shared with the warps
 // of left . B; one part of left . B instead of two would save 3 %.
